@@ -1,0 +1,29 @@
+// The cache in 4 bits: what its bytes mean.
+//
+// A row is a token's key or value of one key/value head, hd numbers.  It is cut into groups of 32 neighbouring ones; with
+// lo = min(x, 0) and hi = max(x, 0) over a group its step is s = (hi - lo) / 15, rounded to 4 significant bits, its zero
+// point z = rint(-lo / s) in 0..15, a number's code c = rint(x / s) + z, kept in 0..15, and the number that it stands for
+// (c - z) s.  c - z has 4 bits and s has 4, so that number is exact in bfloat16 and in 32 bits: whoever reads the cache, in
+// whatever type and order, reads the same numbers.  (A step with the 8 bits of a bfloat16 would be off by 0.2 % instead of
+// 2 % on average; the codes' own rounding is 14 times larger than either, and z would have needed bytes of its own.)
+// A group of zeros, or whose step would lie under 2^-126, has step 0 and stands for zeros.  A group that holds a number that
+// is not finite stands for NaN: what sees the token is NaN and nothing is lost silently.
+//
+// A page of 64 tokens and one head: 64 rows of key codes (hd / 2 bytes, the lower half of a byte first), 64 rows of the
+// keys' words (hd / 32 of 16 bits: the bits of s as a bfloat16, whose lowest 4 are zero, with z in them), then the values' codes
+// and words.  With hd = 128 that is 9,216 bytes where bfloat16 takes 32,768.
+#pragma once
+
+#include "common.cuh"
+
+#define KV4_PAGE 64
+#define KV4_GROUP 32
+#define KV4_MAX_DIM 256
+
+__host__ __device__ constexpr int kv4_code_bytes(int hd) { return KV4_PAGE * hd / 2; }
+__host__ __device__ constexpr int kv4_half_bytes(int hd) { return KV4_PAGE * (hd / 2 + hd / 16); }     // keys, or values
+__host__ __device__ constexpr int kv4_page_bytes(int hd) { return 2 * kv4_half_bytes(hd); }
+
+__device__ __forceinline__ float kv4_step(uint32_t word) { return __uint_as_float((word & 0xfff0u) << 16); }
+__device__ __forceinline__ float kv4_zero(uint32_t word) { return (float)(word & 15u); }
+__device__ __forceinline__ bool kv4_is_nan(uint32_t word) { return (word & 0x7f80u) == 0x7f80u; }

@@ -1,0 +1,207 @@
+// The write into the cache in 4 bits, and its pages back as bfloat16 or 32-bit numbers.
+#include "kv4.cuh"
+
+// The code of a number of a group with step s > 0 and zero point z.  The quotient's rounding to 32 bits can put a number on the
+// wrong side of the border between two codes; x - (c + 1/2) s in 64 bits tells (ties go to the even quotient, as rint has it).
+__device__ __forceinline__ int kv4_code(double x, float s, float z) {
+    float c = rintf((float)x / s);
+    const double r = fma(-(double)c, (double)s, x), half = 0.5 * (double)s;
+    if (r > half || (r == half && ((int)c & 1))) c += 1.f;
+    else if (r < -half || (r == -half && ((int)c & 1))) c -= 1.f;
+    return (int)fminf(fmaxf(c + z, 0.f), 15.f);
+}
+
+// Step and zero point of a group from its lowest and highest number (0 among them): the word, and both as floats.
+__device__ __forceinline__ uint32_t kv4_word(double lo, double hi, bool finite, float& s, float& z) {
+    const double t = (hi - lo) / 15.0;
+    const long long up = __double_as_longlong(t) + (1ll << 48);                         // to 4 significant bits: 3 of the 52 behind the point stay
+    const double step = __longlong_as_double(up & ~((1ll << 49) - 1));
+    s = z = 0.f;
+    if (!finite || !(step < 3.0e38)) return 0x7fc0u;
+    if (step < 1.1754943508222875e-38) return 0u;
+    s = (float)step;
+    z = (float)fmin(rint(-lo / step), 15.0);
+    return (__float_as_uint(s) >> 16) | (uint32_t)z;
+}
+
+// One warp a (token, head): queries, then key heads, then value heads, in the order of the fused projection's columns.  Keys
+// and values go through 64 bits: the norm, the rotation and the choice of the codes are the formula's whatever the order of
+// the sums, and a code is a choice, not a number that could be off by a little.  Queries are made in 32 bits, as for the cache in
+// 16 bits.
+#define KS_WARPS 4
+template <typename TQ>
+__global__ void __launch_bounds__(KS_WARPS * 32)
+kv4_store_kernel(const float* __restrict__ qkv, const float* __restrict__ q_weight, const float* __restrict__ k_weight,
+                 const float* __restrict__ cos_t, const float* __restrict__ sin_t, const int* __restrict__ slot_map,
+                 TQ* __restrict__ q_out, unsigned char* __restrict__ pool, long long n_rows, int Hq, int Hkv, int hd, int rot,
+                 float eps, int store_kv) {
+    pdl_wait();
+    pdl_launch_dependents();
+    __shared__ double rows[KS_WARPS][KV4_MAX_DIM];
+    const int t = blockIdx.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int head = blockIdx.y * KS_WARPS + warp, n_heads = Hq + 2 * Hkv;
+    if (head >= n_heads) return;
+    const bool is_q = head < Hq, is_k = !is_q && head < Hq + Hkv;
+    const float* src = qkv + ((size_t)t * n_heads + head) * hd;
+    const int half = rot >> 1;
+    const float* c = cos_t + (size_t)t * half;
+    const float* sn = sin_t + (size_t)t * half;
+    if (is_q) {
+        float scale = 1.f;
+        if (q_weight) {
+            float ss = 0.f;
+            for (int i = lane; i < hd; i += 32) ss += src[i] * src[i];
+            scale = 1.f / sqrtf(warp_sum(ss) / (float)hd + eps);
+        }
+        TQ* dst = q_out + ((size_t)t * Hq + head) * hd;
+        for (int i = lane; i < half; i += 32) {
+            float a = src[i] * scale, b = src[i + half] * scale;
+            if (q_weight) { a *= q_weight[i]; b *= q_weight[i + half]; }
+            dst[i] = from_f32<TQ>(a * c[i] - b * sn[i]);
+            dst[i + half] = from_f32<TQ>(a * sn[i] + b * c[i]);
+        }
+        for (int i = rot + lane; i < hd; i += 32) dst[i] = from_f32<TQ>(q_weight ? src[i] * scale * q_weight[i] : src[i]);
+        return;
+    }
+    const long long slot = slot_map[t];
+    if (!store_kv || slot < 0 || slot >= n_rows) return;            // a token that has no place (behind the last sequence)
+    double* row = rows[warp];
+    if (is_k) {
+        double scale = 1.0;
+        if (k_weight) {
+            double ss = 0.0;
+            for (int i = lane; i < hd; i += 32) ss += (double)src[i] * src[i];
+#pragma unroll
+            for (int o = 16; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+            scale = 1.0 / sqrt(ss / hd + (double)eps);
+        }
+        for (int i = lane; i < half; i += 32) {
+            double a = src[i] * scale, b = src[i + half] * scale;
+            if (k_weight) { a *= k_weight[i]; b *= k_weight[i + half]; }
+            row[i] = a * c[i] - b * sn[i];
+            row[i + half] = a * sn[i] + b * c[i];
+        }
+        for (int i = rot + lane; i < hd; i += 32) row[i] = k_weight ? src[i] * scale * k_weight[i] : (double)src[i];
+    } else {
+        for (int i = lane; i < hd; i += 32) row[i] = src[i];
+    }
+    __syncwarp();
+    const int kvh = is_k ? head - Hq : head - Hq - Hkv, at = (int)(slot % KV4_PAGE);
+    unsigned char* base = pool + ((size_t)(slot / KV4_PAGE) * Hkv + kvh) * kv4_page_bytes(hd) + (is_k ? 0 : kv4_half_bytes(hd));
+    for (int g = 0; g < hd / KV4_GROUP; ++g) {
+        const double x = row[g * KV4_GROUP + lane];
+        const bool finite = __all_sync(0xffffffffu, fabs(x) <= 3.4028234663852886e38);
+        double lo = fmin(x, 0.0), hi = fmax(x, 0.0);
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) {
+            lo = fmin(lo, __shfl_xor_sync(0xffffffffu, lo, o));
+            hi = fmax(hi, __shfl_xor_sync(0xffffffffu, hi, o));
+        }
+        float s, z;
+        const uint32_t word = kv4_word(lo, hi, finite, s, z);
+        const int code = s > 0.f ? kv4_code(x, s, z) : 0;
+        const int next = __shfl_down_sync(0xffffffffu, code, 1);
+        if (!(lane & 1)) base[(size_t)at * (hd / 2) + (g * KV4_GROUP + lane) / 2] = (unsigned char)(code | (next << 4));
+        if (lane == 0) reinterpret_cast<uint16_t*>(base + kv4_code_bytes(hd))[at * (hd / KV4_GROUP) + g] = (uint16_t)word;
+    }
+}
+
+extern "C" int qwb_kv4_store(const float* qkv, const float* q_weight, const float* k_weight, const float* cos_t, const float* sin_t,
+                             const int* slot_map, void* q_out, int q_dtype, unsigned char* pool, int n_pages, int T, int Hq,
+                             int Hkv, int hd, int rot, float eps, int store_kv, cudaStream_t stream) {
+    if (T <= 0) return 0;
+    if (Hq <= 0 || Hkv <= 0 || hd <= 0 || hd % KV4_GROUP || hd > KV4_MAX_DIM || rot < 0 || rot > hd || (rot & 1) || n_pages <= 0)
+        return qwb_fail(QWB_ERR_ARG, "kv4_store: bad sizes Hq=%d Hkv=%d hd=%d rot=%d pages=%d", Hq, Hkv, hd, rot, n_pages);
+    dim3 grid(T, (Hq + 2 * Hkv + KS_WARPS - 1) / KS_WARPS);
+    if (grid.y > 65535) return qwb_fail(QWB_ERR_ARG, "kv4_store: too many heads (%d)", Hq + 2 * Hkv);
+    if (q_dtype == QWB_DT_F32)
+        qwb_launch(kv4_store_kernel<float>, grid, KS_WARPS * 32, 0, stream, qkv, q_weight, k_weight, cos_t, sin_t, slot_map, (float*)q_out, pool,
+                   (long long)n_pages * KV4_PAGE, Hq, Hkv, hd, rot, eps, store_kv);
+    else if (q_dtype == QWB_DT_BF16)
+        qwb_launch(kv4_store_kernel<bf16>, grid, KS_WARPS * 32, 0, stream, qkv, q_weight, k_weight, cos_t, sin_t, slot_map, (bf16*)q_out, pool,
+                   (long long)n_pages * KV4_PAGE, Hq, Hkv, hd, rot, eps, store_kv);
+    else
+        return qwb_fail(QWB_ERR_ARG, "kv4_store: unknown dtype %d", q_dtype);
+    return qwb_check_launch("kv4_store");
+}
+
+// Pages of a step's sequences, one after the other, as plain pages [P, Hkv, 64, hd] of keys and of values; rows behind a
+// sequence's last token are zeros.  A block takes a (page, head), a thread 8 numbers at a time (one 32-bit word of codes).
+// `marked`: a token one of whose values is not finite has values of zero and keys of NaN here, so that a kernel that multiplies
+// what a query does not see by 0 gives NaN to the queries that see it only.
+// Blocks of the first head also write the table that names these pages: [B, width], page_start[b] + j.
+template <typename T>
+__global__ void __launch_bounds__(256)
+kv4_read_kernel(const unsigned char* __restrict__ pool, const int* __restrict__ pages, const int* __restrict__ page_start,
+                const int* __restrict__ seq_len, T* __restrict__ k_out, T* __restrict__ v_out, int* __restrict__ table, int P, int B,
+                int width, int pool_pages, int Hkv, int hd, int marked) {
+    pdl_wait();
+    pdl_launch_dependents();
+    const int entry = blockIdx.x, head = blockIdx.y;
+    // the sequence that holds this entry: the last one that begins at or before it
+    int lo = 0, hi = B;
+    while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (page_start[mid] <= entry) lo = mid; else hi = mid;
+    }
+    const int j = entry - page_start[lo];
+    if (head == 0 && threadIdx.x == 0 && j >= 0 && j < width && entry < page_start[lo + 1]) table[(size_t)lo * width + j] = entry;
+    const long long page = pages[entry];
+    int live = entry < page_start[lo + 1] ? min(max(seq_len[lo] - j * KV4_PAGE, 0), KV4_PAGE) : 0;
+    if (j < 0 || page < 0 || page >= pool_pages) live = 0;
+    const int words = hd / 8, groups = hd / KV4_GROUP;
+    const unsigned char* base = pool + ((size_t)(live ? page : 0) * Hkv + head) * kv4_page_bytes(hd);
+    const size_t out0 = ((size_t)entry * Hkv + head) * KV4_PAGE * hd;
+    const uint16_t* v_words = reinterpret_cast<const uint16_t*>(base + kv4_half_bytes(hd) + kv4_code_bytes(hd));
+    for (int i = threadIdx.x; i < 2 * KV4_PAGE * words; i += blockDim.x) {
+        const bool is_v = i >= KV4_PAGE * words;
+        const int at = is_v ? i - KV4_PAGE * words : i, row = at / words, w = at - row * words;
+        const unsigned char* part = base + (is_v ? kv4_half_bytes(hd) : 0);
+        float y[8];
+        if (row < live) {
+            const uint32_t codes = reinterpret_cast<const uint32_t*>(part)[at];
+            const uint32_t word = reinterpret_cast<const uint16_t*>(part + kv4_code_bytes(hd))[row * groups + w / 4];
+            float s = kv4_step(word);
+            const float z = kv4_zero(word);
+            if (marked) {
+                bool bad = false;
+                for (int g = 0; g < groups; ++g) bad |= kv4_is_nan(v_words[row * groups + g]);
+                if (bad) s = is_v ? 0.f : __uint_as_float(0x7fffffffu);
+            }
+#pragma unroll
+            for (int n = 0; n < 8; ++n) y[n] = ((float)((codes >> (4 * n)) & 15u) - z) * s;
+        } else {
+#pragma unroll
+            for (int n = 0; n < 8; ++n) y[n] = 0.f;
+        }
+        T* dst = (is_v ? v_out : k_out) + out0 + (size_t)at * 8;
+        if constexpr (sizeof(T) == 4) {
+            reinterpret_cast<float4*>(dst)[0] = make_float4(y[0], y[1], y[2], y[3]);
+            reinterpret_cast<float4*>(dst)[1] = make_float4(y[4], y[5], y[6], y[7]);
+        } else {
+            __nv_bfloat162 p[4];
+#pragma unroll
+            for (int n = 0; n < 4; ++n) p[n] = __floats2bfloat162_rn(y[2 * n], y[2 * n + 1]);
+            *reinterpret_cast<uint4*>(dst) = *reinterpret_cast<uint4*>(p);
+        }
+    }
+}
+
+extern "C" int qwb_kv4_read(const unsigned char* pool, const int* pages, const int* page_start, const int* seq_len, void* k_out,
+                            void* v_out, int dtype, int* table, int P, int B, int width, int pool_pages, int Hkv, int hd,
+                            int marked, cudaStream_t stream) {
+    if (P <= 0) return 0;
+    if (B <= 0 || width <= 0 || Hkv <= 0 || Hkv > 65535 || hd <= 0 || hd % KV4_GROUP || hd > KV4_MAX_DIM || pool_pages <= 0)
+        return qwb_fail(QWB_ERR_ARG, "kv4_read: bad sizes B=%d width=%d Hkv=%d hd=%d pages=%d", B, width, Hkv, hd, pool_pages);
+    if ((uintptr_t)pool % 16 || (uintptr_t)k_out % 16 || (uintptr_t)v_out % 16)
+        return qwb_fail(QWB_ERR_ARG, "kv4_read: pool and outputs must start at a multiple of 16 bytes");
+    if (dtype == QWB_DT_F32)
+        qwb_launch(kv4_read_kernel<float>, dim3(P, Hkv), 256, 0, stream, pool, pages, page_start, seq_len, (float*)k_out, (float*)v_out, table, P, B,
+                   width, pool_pages, Hkv, hd, marked);
+    else if (dtype == QWB_DT_BF16)
+        qwb_launch(kv4_read_kernel<bf16>, dim3(P, Hkv), 256, 0, stream, pool, pages, page_start, seq_len, (bf16*)k_out, (bf16*)v_out, table, P, B,
+                   width, pool_pages, Hkv, hd, marked);
+    else
+        return qwb_fail(QWB_ERR_ARG, "kv4_read: unknown dtype %d", dtype);
+    return qwb_check_launch("kv4_read");
+}

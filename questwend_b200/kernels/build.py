@@ -30,7 +30,7 @@ EXTRA_FLAGS: dict[str, list[str]] = {}
 NVCC_FLAGS += os.environ.get("QWB200_NVCC_FLAGS", "").split()      # more flags (-D switches) for experiments; part of the stamp
 MODULES = ("elementwise", "layernorm", "rope_kv", "attention", "attention_mma", "attention_tc", "attention_streams", "attention_latent", "attention_latent_mma",
            "attention_pool", "attention_maps", "attention_bias", "recurrent", "recurrent_chunks", "rglru", "mlstm", "moe",
-           "gemm_small", "gemm_stream", "gemm_ring", "gemm_tc", "sampling")
+           "gemm_small", "gemm_stream", "gemm_ring", "gemm_tc", "sampling", "step_tables", "kv4_cache", "attention_kv4", "logprobs")
 
 _lock = threading.Lock()
 _loaded: dict[str, ctypes.CDLL] = {}

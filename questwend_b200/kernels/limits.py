@@ -90,3 +90,12 @@ def shaped_attention_refusal(dim: int, vdim: int) -> str | None:
         if n <= 0 or n > SHAPED_ATTN_MAX_DIM:
             return f"the attention with shaped scores takes {what} sizes up to {SHAPED_ATTN_MAX_DIM}, not {n}"
     return None
+
+KV4_GROUP = 32              # csrc/kv4.cuh: numbers of a row of the 4-bit cache that share a step
+
+
+def kv4_refusal(head_dim: int) -> str | None:
+    """None if keys and values of this size can be held in 4 bits, else why not."""
+    if head_dim <= 0 or head_dim % KV4_GROUP or head_dim > MAX_HEAD_DIM:
+        return f"a cache in 4 bits holds heads of a multiple of {KV4_GROUP} numbers up to {MAX_HEAD_DIM}, not {head_dim}"
+    return None

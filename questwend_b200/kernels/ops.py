@@ -10,10 +10,12 @@ from __future__ import annotations
 import ctypes
 import math
 import operator
+from typing import NamedTuple
 
 import torch
 
 from .build import host_calls, host_calls_built, load_module
+from .limits import KV4_GROUP, kv4_refusal
 
 DT_F32, DT_BF16 = 0, 1
 PAGE_SIZE = 64          # tokens per cache page
@@ -82,6 +84,14 @@ def _need(t: torch.Tensor, name: str, dtype=None, ndim=None):
         raise KernelError(f"{name}: must be {dtype}, got {t.dtype}")
     if ndim is not None and t.dim() != ndim:
         raise KernelError(f"{name}: must have {ndim} dimensions, got {t.dim()}")
+
+
+def _here(what: str, *tensors) -> None:
+    """Refuse tensors of another device than the current one: the launch would run here on memory that lies there."""
+    here = torch.cuda.current_device()
+    for t in tensors:
+        if t is not None and t.get_device() != here:
+            raise KernelError(f"{what}: a tensor on {t.device}, while the current device is cuda:{here} (use torch.cuda.device)")
 
 
 def _column_gate(what: str, gate: torch.Tensor | None, col0: int, T: int, H: int):
@@ -2077,3 +2087,198 @@ def decode_advance(sampled, token_ids, tok_pos, pos0, seq_len, step_counter=None
     window = recent.shape[1] if recent is not None else 0
     _call("elementwise", "qwb_decode_advance", _ptr(sampled), _ptr(token_ids), _ptr(tok_pos), _ptr(pos0),
           _ptr(seq_len), _ptr(step_counter), _ptr(recent), _ptr(n_seen), _i(window), _i(B), _stream())
+
+
+# ----------------------------------------------------------------------------- a step's tables
+class StepTables(NamedTuple):
+    """Which rows of a paged cache a step's tokens are and see (``step_tables``).  All int32.  A step with padding may have more
+    tokens than its sequences bring: those behind the last sequence's have -1 in ``tok_seq``, ``tok_pos`` and ``slot_map``."""
+    cu_seqlens: torch.Tensor        # [B + 1] where each sequence's tokens begin in the packed order
+    seq_len: torch.Tensor           # [B] tokens that each sequence holds after the step
+    tok_seq: torch.Tensor           # [T] batch row of each token
+    tok_pos: torch.Tensor           # [T] its position in its sequence
+    page_table: torch.Tensor        # [B, width] pages of each sequence, in order; 0 behind the last one
+    slot_map: torch.Tensor          # [T] its row of the pool, page * 64 + place in the page; -1: no place (nothing is written)
+    pos0: torch.Tensor              # [B] tokens held before the step (as given)
+    pages: torch.Tensor | None = None           # all sequences' pages, one after the other (as given), and ...
+    page_start: torch.Tensor | None = None      # [B + 1] ... where each sequence's begin
+
+
+STEP_TABLES_MAX_SEQS = 8192     # csrc/step_tables.cu: ST_MAX_SEQS
+
+
+def step_tables(pages: torch.Tensor, page_start: torch.Tensor, pos0: torch.Tensor, n_new: torch.Tensor, n_tokens: int, table_width: int,
+                tokens: bool = True) -> StepTables:
+    """The tables of a step from its sequences' lengths, made on the device in one launch.  int32: ``pages`` [P] the sequences'
+    page ids, one sequence after the other, ``page_start`` [B + 1] where each one's begin, ``pos0`` [B] what each holds, ``n_new``
+    [B] what it brings (0: nothing).  ``n_tokens`` is the sum of ``n_new``, or more (a padded step); ``table_width`` the columns of the page
+    table (0: none is made), pages beyond it are left out.  A token for which its sequence has no page has slot -1.  ``tokens`` False:
+    the page table alone (another group of the same step); the tensors of the tokens are then None.  Reads nothing on the host, so it
+    can be captured into a graph; page ids are below 2^25, so that rows are whole numbers of 32 bits."""
+    for name, t in (("pages", pages), ("page_start", page_start), ("pos0", pos0), ("n_new", n_new)):
+        _need(t, name, torch.int32, 1)
+    _here("step_tables", pages, page_start, pos0, n_new)
+    B, T, W = pos0.numel(), int(n_tokens), int(table_width)
+    if B < 1 or B > STEP_TABLES_MAX_SEQS or n_new.numel() != B or page_start.numel() != B + 1:
+        raise KernelError(f"step_tables: {B} lengths (1 to {STEP_TABLES_MAX_SEQS}), {n_new.numel()} counts and {page_start.numel()} page "
+                          f"starts do not belong together")
+    if T < 0 or W < 0 or T >= 2 ** 31 or W >= 2 ** 31:
+        raise KernelError(f"step_tables: {T} tokens, a table of {W} columns")
+    dev = pos0.device
+    table = _empty((B, W), dtype=torch.int32, device=dev)
+    cu = seq_len = tok_seq = tok_pos = slot = None
+    if tokens:      # one piece of memory: a tensor made anew takes the host longer than a view
+        cu, seq_len, tok_seq, tok_pos, slot = _empty((2 * B + 1 + 3 * T,), dtype=torch.int32, device=dev).split((B + 1, B, T, T, T))
+    _call("step_tables", "qwb_step_tables", _ptr(pages), _ptr(page_start), _ptr(pos0), _ptr(n_new), _ptr(cu), _ptr(seq_len), _ptr(tok_seq),
+          _ptr(tok_pos), _ptr(slot), _ptr(table), _i(pages.numel()), _i(B), _i(T), _i(W), _i(PAGE_SIZE), _i(1 if tokens else 0), _stream())
+    return StepTables(cu, seq_len, tok_seq, tok_pos, table, slot, pos0, pages, page_start)
+
+
+# ----------------------------------------------------------------------------- the cache in 4 bits
+def kv4_page_bytes(head_dim: int) -> int:
+    """Bytes of a page (64 tokens, keys and values) of one head in the 4-bit cache; a pool is uint8 [pages, Hkv, this many]."""
+    refusal = kv4_refusal(head_dim)
+    if refusal:
+        raise KernelError(f"kv4: {refusal}")
+    return 2 * PAGE_SIZE * (head_dim // 2 + 2 * (head_dim // KV4_GROUP))
+
+
+def _kv4_pool(what: str, pool: torch.Tensor, head_dim: int) -> None:
+    _need(pool, "pool", torch.uint8, 3)
+    if pool.shape[2] != kv4_page_bytes(head_dim):
+        raise KernelError(f"{what}: a pool of {tuple(pool.shape)} does not hold heads of {head_dim} ({kv4_page_bytes(head_dim)} bytes a page)")
+    if pool.data_ptr() % 16:
+        raise KernelError(f"{what}: the pool must start at a multiple of 16 bytes")
+
+
+def kv4_store(qkv: torch.Tensor, q_weight, k_weight, cos, sin, slot_map: torch.Tensor, pool: torch.Tensor, n_heads: int, n_kv_heads: int,
+              head_dim: int, rotary_dim: int, eps: float, q_dtype: torch.dtype, store_kv: bool = True) -> torch.Tensor:
+    """``qk_norm_rope_store`` for the cache in 4 bits: per-head norm (``q_weight`` / ``k_weight`` or None), rotation of the first
+    ``rotary_dim`` numbers, and the write.  ``qkv`` float32 [T, (Hq + 2 Hkv) * hd]; ``slot_map`` int32 [T] each token's row of the pool (below 0 or
+    beyond the pool: nothing is written; a row may be named once).  Returns the queries [T, Hq, hd] in ``q_dtype``.
+
+    32 neighbouring numbers of a key or value share a step s of 4 significant bits and a zero point z; each is held as a code c of
+    0..15 and stands for (c - z) s, the nearest of the 16 such numbers.  Keys are normed, turned and rounded to codes in 64 bits.  A group
+    with a number that is not finite stands for NaN."""
+    _need(qkv, "qkv", torch.float32, 2)
+    _kv4_pool("kv4_store", pool, head_dim)
+    _need(slot_map, "slot_map", torch.int32, 1)
+    T = qkv.shape[0]
+    if qkv.shape[1] != (n_heads + 2 * n_kv_heads) * head_dim or slot_map.numel() != T or pool.shape[1] != n_kv_heads:
+        raise KernelError(f"kv4_store: qkv {tuple(qkv.shape)} and {slot_map.numel()} slots for {n_heads} + 2 x {n_kv_heads} heads of {head_dim} and a "
+                          f"pool of {pool.shape[1]} heads")
+    for name, t in (("q_weight", q_weight), ("k_weight", k_weight)):
+        if t is not None:
+            _need(t, name, torch.float32, 1)
+            if t.numel() != head_dim:
+                raise KernelError(f"kv4_store: {name} has {t.numel()} entries for heads of {head_dim}")
+    if rotary_dim < 0 or rotary_dim > head_dim or rotary_dim % 2:
+        raise KernelError(f"kv4_store: rotary size {rotary_dim} for heads of {head_dim}")
+    if rotary_dim:
+        _need(cos, "cos", torch.float32, 2)
+        _need(sin, "sin", torch.float32, 2)
+        if tuple(cos.shape) != (T, rotary_dim // 2) or sin.shape != cos.shape:
+            raise KernelError(f"kv4_store: cos/sin {tuple(cos.shape)} do not fit {T} tokens and rotary size {rotary_dim}")
+    else:
+        cos = sin = None
+    _here("kv4_store", qkv, q_weight, k_weight, cos, sin, slot_map, pool)
+    q_out = _empty((T, n_heads, head_dim), dtype=q_dtype, device=qkv.device)
+    _call("kv4_cache", "qwb_kv4_store", _ptr(qkv), _ptr(q_weight), _ptr(k_weight), _ptr(cos), _ptr(sin), _ptr(slot_map), _ptr(q_out), _i(_dt(q_dtype)),
+          _ptr(pool), _i(pool.shape[0]), _i(T), _i(n_heads), _i(n_kv_heads), _i(head_dim), _i(rotary_dim), _f(eps),
+          _i(1 if store_kv else 0), _stream())
+    return q_out
+
+
+def kv4_read(pool: torch.Tensor, pages: torch.Tensor, page_start: torch.Tensor, seq_len: torch.Tensor, max_len: int, head_dim: int,
+             dtype: torch.dtype, marked: bool = False) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """What the 4-bit cache holds for a step's sequences, as plain pages: keys and values [P, Hkv, 64, hd] in ``dtype`` of the P
+    entries of ``pages`` (``StepTables``), zeros behind a sequence's last token, and the page table [B, pages of ``max_len``] that names
+    them (0 where a sequence has no page).  Both types hold the numbers exactly.  ``marked``: a token with a value that is not finite has
+    values of 0 and keys of NaN instead (what a kernel needs that multiplies unseen values by 0)."""
+    _kv4_pool("kv4_read", pool, head_dim)
+    for name, t in (("pages", pages), ("page_start", page_start), ("seq_len", seq_len)):
+        _need(t, name, torch.int32, 1)
+    P, B, Hkv = pages.numel(), seq_len.numel(), pool.shape[1]
+    if B < 1 or page_start.numel() != B + 1 or max_len < 1:
+        raise KernelError(f"kv4_read: {page_start.numel()} page starts for {B} sequences of up to {max_len} tokens")
+    _here("kv4_read", pool, pages, page_start, seq_len)
+    width = -(-max_len // PAGE_SIZE)
+    k = _empty((P, Hkv, PAGE_SIZE, head_dim), dtype=dtype, device=pool.device)
+    v = _empty((P, Hkv, PAGE_SIZE, head_dim), dtype=dtype, device=pool.device)
+    table = torch.zeros((B, width), dtype=torch.int32, device=pool.device)
+    _call("kv4_cache", "qwb_kv4_read", _ptr(pool), _ptr(pages), _ptr(page_start), _ptr(seq_len), _ptr(k), _ptr(v), _i(_dt(dtype)), _ptr(table),
+          _i(P), _i(B), _i(width), _i(pool.shape[0]), _i(Hkv), _i(head_dim), _i(1 if marked else 0), _stream())
+    return k, v, table
+
+
+def kv4_attention(q: torch.Tensor, pool: torch.Tensor, tables: StepTables, max_new: int, max_len: int, scale: float, window: int = 0,
+                  impl: str = "auto") -> torch.Tensor:
+    """Causal attention of a step's tokens over the cache in 4 bits (their own rows written before).  ``q`` [T, Hq, hd] float32
+    or bfloat16; ``max_new`` and ``max_len`` bound what a sequence brings and holds; with ``window`` > 0 a query sees the last ``window``
+    keys, its own among them.  Returns [T, Hq * hd] in q's type, zeros for a token of no sequence.  ``impl``: "auto" or "plain"."""
+    _need(q, "q", ndim=3)
+    T, Hq, hd = q.shape
+    _kv4_pool("kv4_attention", pool, hd)
+    table, tok_seq, tok_pos, cu, pos0 = tables.page_table, tables.tok_seq, tables.tok_pos, tables.cu_seqlens, tables.pos0
+    _need(table, "page_table", torch.int32, 2)
+    for name, t in (("tok_seq", tok_seq), ("tok_pos", tok_pos), ("cu_seqlens", cu), ("pos0", pos0)):
+        _need(t, name, torch.int32, 1)
+    B, Hkv = pos0.numel(), pool.shape[1]
+    if tok_seq.numel() != T or tok_pos.numel() != T or cu.numel() != B + 1 or table.shape[0] < B or Hq % Hkv:
+        raise KernelError(f"kv4_attention: tables of {tok_seq.numel()} tokens, {cu.numel() - 1} and {B} sequences for queries {tuple(q.shape)} over "
+                          f"{Hkv} heads")
+    if max_new < 1 or max_len < 1 or table.shape[1] < 1 or window < 0:
+        raise KernelError(f"kv4_attention: up to {max_new} new tokens of sequences of up to {max_len}, window {window}, a page table of "
+                          f"{table.shape[1]} columns")
+    max_len = min(max_len, table.shape[1] * PAGE_SIZE)
+    if impl not in ("auto", "plain"):
+        raise KernelError(f"kv4_attention: unknown form '{impl}'")
+    _here("kv4_attention", q, pool, table, tok_seq, tok_pos, cu, pos0)
+    out = _empty((T, Hq * hd), dtype=q.dtype, device=q.device)
+    _call("attention_kv4", "qwb_kv4_attn_plain", _ptr(q), _ptr(pool), _ptr(table), _ptr(tok_seq), _ptr(tok_pos), _ptr(out), _i(_dt(q.dtype)), _i(T),
+          _i(B), _i(pool.shape[0]), _i(Hq), _i(Hkv), _i(hd), _i(table.shape[1]), _f(scale), _i(window), _stream())
+    return out
+
+
+# ----------------------------------------------------------------------------- log probabilities
+class TokenLogprobs(NamedTuple):
+    logprob: torch.Tensor           # [R] float32: of each row's token
+    entropy: torch.Tensor           # [R] float32: of each row's distribution, in nats
+    top_ids: torch.Tensor           # [R, top] int32: the most probable tokens, the first the most
+    top_logprobs: torch.Tensor      # [R, top] float32
+
+
+LOGPROBS_MAX_TOP = 64           # csrc/logprobs.cu: LP_MAX_TOP
+LOGPROBS_MAX_ROWS = 65535
+
+
+def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top: int = 0, out: TokenLogprobs | None = None) -> TokenLogprobs:
+    """Per row of float32 ``logits`` [R, V] the log probability of the row's token (int32 ``tokens`` [R]), the entropy, and the
+    ``top`` most probable tokens with theirs; of equally probable ones the lower id comes first.  A logit of -infinity is a token of probability 0.
+    A row with a NaN, with +infinity or with nothing but -infinity has no distribution: its numbers are NaN (a NaN logit is not among the
+    alternatives; where fewer than ``top`` remain the id is -1).  A token outside 0..V-1 has log probability NaN.  ``out``: tensors of
+    an earlier call of the same sizes to write into."""
+    _need(logits, "logits", torch.float32, 2)
+    _need(tokens, "tokens", torch.int32, 1)
+    R, V = logits.shape
+    if tokens.numel() != R or R > LOGPROBS_MAX_ROWS:
+        raise KernelError(f"token_logprobs: {tokens.numel()} tokens for {R} rows (at most {LOGPROBS_MAX_ROWS})")
+    if not 0 <= top <= min(V, LOGPROBS_MAX_TOP) or V < 1:
+        raise KernelError(f"token_logprobs: 0 to {LOGPROBS_MAX_TOP} alternatives of a vocabulary of at least as many: {top} of {V}")
+    dev = logits.device
+    if out is None:
+        out = TokenLogprobs(_empty((R,), dtype=torch.float32, device=dev), _empty((R,), dtype=torch.float32, device=dev),
+                            _empty((R, top), dtype=torch.int32, device=dev), _empty((R, top), dtype=torch.float32, device=dev))
+    else:
+        for name, t, dtype, shape in (("logprob", out.logprob, torch.float32, (R,)), ("entropy", out.entropy, torch.float32, (R,)),
+                                      ("top_ids", out.top_ids, torch.int32, (R, top)), ("top_logprobs", out.top_logprobs, torch.float32, (R, top))):
+            _need(t, name, dtype, len(shape))
+            if tuple(t.shape) != shape:
+                raise KernelError(f"token_logprobs: {name} of {tuple(t.shape)} for {R} rows and {top} alternatives")
+    _here("token_logprobs", logits, tokens, *out)
+    if R:
+        segments = _lookup("logprobs", "qwb_logprobs_segments")[1](V)
+        scratch = _empty((R * segments * (3 + 2 * top),), dtype=torch.float32, device=dev)
+        _call("logprobs", "qwb_logprobs", _ptr(logits), _ptr(tokens), _ptr(out.logprob), _ptr(out.entropy), _ptr(out.top_ids), _ptr(out.top_logprobs),
+              _ptr(scratch), _i(R), _i(V), _i(top), _stream(), kernels=2)
+    return out
