@@ -17,7 +17,7 @@ state for layers that have it (:115-116, 493-494), zeroed at start (:614-630).  
 * A mixer may ask for several kinds of rows (its ``kv_spec`` is then a tuple): each lands in a group of its own.  A
   spec with ``stride`` s > 1 holds one row for every s tokens (a row per complete block of s tokens), so a sequence of
   n tokens holds n // s rows there and its group's pool is that much smaller; a spec with ``value_dim`` has values of
-  another size than its keys.
+  another size than its keys; one with ``bits`` 4 holds keys and values in 4 bits, ``[units, pages, Hkv, bytes of a page]``.
 * The pools are zeroed once, when they are made.  Nothing is zeroed when a page or
   slot is handed out again: kernels never use what lies beyond a sequence's length
   (the tensor-core kernels multiply it by probability 0, so it must be finite: it is
@@ -33,7 +33,7 @@ from dataclasses import dataclass
 import numpy as np
 import torch
 
-from ..kernels.ops import PAGE_SIZE
+from ..kernels.ops import PAGE_SIZE, kv4_page_bytes
 from ..parts.base import KVSpec, StateSpec, UnitCache
 
 
@@ -95,8 +95,8 @@ class _KVGroup:
     spec: KVSpec
     units: list            # schedule indices that own storage here
     pool: FreeList
-    k: torch.Tensor        # [units, pages, Hkv, PAGE_SIZE, hd]
-    v: torch.Tensor | None # None for a spec without separate values
+    k: torch.Tensor        # [units, pages, Hkv, PAGE_SIZE, hd]; in 4 bits uint8 [units, pages, Hkv, bytes of a page]
+    v: torch.Tensor | None # None for a spec without separate values, and in 4 bits
     pages: dict            # slot -> list of page ids, in order
 
 
@@ -149,8 +149,15 @@ class CacheManager:
             shape = (len(members), n_pages, spec.n_kv_heads, PAGE_SIZE, spec.head_dim)
             # zeroed once (the reference zeroes its cache too, core/runtime.cpp:614-630): a page's unused tail is
             # multiplied by probability 0 in the tensor-core kernels and must hold finite numbers
-            k = torch.zeros(shape, dtype=dtype, device=self.device)
-            v = torch.zeros((*shape[:-1], spec.v_dim), dtype=dtype, device=self.device) if spec.values else None
+            if spec.bits == 4:
+                if not spec.values or spec.v_dim != spec.head_dim or spec.stride > 1:
+                    raise CacheError(f"a cache in 4 bits holds a key and a value of one size per token, not {spec}")
+                k, v = torch.zeros((*shape[:3], kv4_page_bytes(spec.head_dim)), dtype=torch.uint8, device=self.device), None
+            elif spec.bits:
+                raise CacheError(f"the cache holds numbers in the engine's dtype or in 4 bits, not in {spec.bits}")
+            else:
+                k = torch.zeros(shape, dtype=dtype, device=self.device)
+                v = torch.zeros((*shape[:-1], spec.v_dim), dtype=dtype, device=self.device) if spec.values else None
             self._groups.append(_KVGroup(spec, members, FreeList(n_pages, "page"), k, v, {}))
             for j, u in enumerate(members):
                 self._unit_group.setdefault(u, []).append((gid, j))
@@ -272,6 +279,11 @@ class CacheManager:
             del g.pages[slot][keep:]
 
     # ------------------------------------------------------------------ page tables
+    def page_lists(self, gid: int, slots) -> list:
+        """The pages that each of these slots holds in a group, in order."""
+        pages = self._groups[gid].pages
+        return [pages[s] for s in slots]
+
     def page_table_host(self, gid: int, slots) -> np.ndarray:
         """[len(slots), table_width] int32; entries beyond a sequence's pages are 0 and never read."""
         g = self._groups[gid]

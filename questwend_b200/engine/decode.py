@@ -41,8 +41,9 @@ def length_bucket(n_tokens: int) -> int:
 class DecodeRunner:
     """Fixed buffers and graphs for decode steps of ``batch`` sequences with one sampling setup."""
 
-    def __init__(self, engine, batch: int, sampling: SamplingParams, use_graph: bool = True):
+    def __init__(self, engine, batch: int, sampling: SamplingParams, use_graph: bool = True, logprobs: int | None = None):
         self.engine = engine
+        self.logprobs = logprobs
         self.B = B = batch
         self.sampling = sampling
         self.use_graph = use_graph
@@ -69,6 +70,16 @@ class DecodeRunner:
                        for g in range(cache.n_groups())}
         self.tables_host = {g: torch.zeros((B, cache.table_width), dtype=torch.int32).pin_memory()
                             for g in range(cache.n_groups())}
+        # groups in 4 bits: the rows that the step's tokens are written to come from the tables above, taken as lists of all their
+        # columns (``ops.step_tables``, in the step)
+        self.table_start = torch.arange(B + 1, dtype=torch.int32, device=dev) * cache.table_width
+        self.ones = torch.ones((B,), dtype=torch.int32, device=dev)
+        self.groups4 = [g for g in range(cache.n_groups()) if cache.group_spec(g).bits == 4]
+        if logprobs is not None:        # log probability, entropy and alternatives of a step's tokens in one piece, one copy to the host
+            self.scores_flat = torch.zeros((B * (2 + 2 * logprobs),), dtype=torch.float32, device=dev)
+            lp, entropy, ids, lps = self.scores_flat.split((B, B, B * logprobs, B * logprobs))
+            self.scores = ops.TokenLogprobs(lp, entropy, ids.view(torch.int32).view(B, logprobs), lps.view(B, logprobs))
+            self.scores_host = torch.zeros_like(self.scores_flat, device="cpu").pin_memory()
         self.state_host = torch.zeros((N_SCALARS + N_ROWS * B,), dtype=torch.int32).pin_memory()
         self._state_np = self.state_host.numpy()
         self.tokens_host = torch.zeros((B,), dtype=torch.int32).pin_memory()
@@ -129,18 +140,27 @@ class DecodeRunner:
 
     # ------------------------------------------------------------------ one step
     def _context(self, max_len_bucket: int) -> StepContext:
+        tables = {}
+        for g in self.groups4:
+            made = ops.step_tables(self.tables[g].view(-1), self.table_start, self.pos0, self.ones, self.B, 0)
+            tables[g] = made._replace(page_table=self.tables[g], pages=None, page_start=None)
         return StepContext(n_tokens=self.B, n_seqs=self.B, token_ids=self.token_ids, tok_seq=self.tok_seq,
                            tok_pos=self.tok_pos, cu_seqlens=self.cu_seqlens, pos0=self.pos0, seq_len=self.seq_len,
                            slots=self.slot_ids, max_new=1, max_len=max_len_bucket, single_token=True,
-                           page_tables=self.tables, host_slots=None)
+                           page_tables=self.tables, host_slots=None, tables=tables)
 
     def _forward_and_sample(self, max_len_bucket: int) -> None:
         eng, p = self.engine, self.sampling
         logits = eng.model.forward(self._context(max_len_bucket), eng.unit_caches, self.rows)
+        as_they_are = logits
+        if self.logprobs is not None and p.penalized:       # the sampler changes the logits by the penalties
+            as_they_are = logits.clone()
         ops.sample(logits, p.temperature, top_k=p.top_k, top_p=p.top_p, seed=0, seed_from=self.seed_word,
                    sequence_index=self.seq_index, step=0, step_add=self.step_counter, recent=self.recent,
                    repeat_penalty=p.repeat_penalty, presence_penalty=p.presence_penalty,
                    frequency_penalty=p.frequency_penalty, out=self.sampled)
+        if self.logprobs is not None:
+            ops.token_logprobs(as_they_are, self.sampled, top=self.logprobs, out=self.scores)
 
     def _advance(self) -> None:
         ops.decode_advance(self.sampled, self.token_ids, self.tok_pos, self.pos0, self.seq_len,
@@ -168,7 +188,7 @@ class DecodeRunner:
                 self._forward_and_sample(bucket)
                 self._advance()
                 if host_copies:
-                    self.sampled_host.copy_(self.sampled, non_blocking=True)
+                    self._copy_out()
         finally:
             if collect_again:
                 gc.enable()
@@ -230,7 +250,7 @@ class DecodeRunner:
                 self.launches_per_step = ops.LAUNCHES[0] - before
                 self._plain_steps[self._bucket] = self._plain_steps.get(self._bucket, 0) + 1
                 if host_copies:
-                    self.sampled_host.copy_(self.sampled, non_blocking=True)
+                    self._copy_out()
             if prof:
                 prof.launched()
         self._sampled_on_host = host_copies
@@ -241,6 +261,17 @@ class DecodeRunner:
     def read_sampled(self) -> list:
         """The ids sampled by the last step, on the host (waits for the step; copies first if the step did not)."""
         if not self._sampled_on_host:
-            self.sampled_host.copy_(self.sampled, non_blocking=True)
+            self._copy_out()
         torch.cuda.current_stream().synchronize()
         return self._sampled_np.tolist()
+
+    def _copy_out(self) -> None:
+        self.sampled_host.copy_(self.sampled, non_blocking=True)
+        if self.logprobs is not None:
+            self.scores_host.copy_(self.scores_flat, non_blocking=True)
+
+    def host_scores(self) -> ops.TokenLogprobs:
+        """The log probabilities of the ids that ``read_sampled`` gave last, on the host (overwritten by the next step)."""
+        B, n = self.B, self.logprobs
+        lp, entropy, ids, lps = self.scores_host.split((B, B, B * n, B * n))
+        return ops.TokenLogprobs(lp, entropy, ids.view(torch.int32).view(B, n), lps.view(B, n))

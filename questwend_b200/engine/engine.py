@@ -24,7 +24,7 @@ from ..config.registry import get_architecture, load_config
 from ..kernels import build as kernel_build
 from ..kernels import ops
 from ..kernels.ops import PAGE_SIZE, fill_int32
-from ..parts.base import Runtime, StepContext
+from ..parts.base import KVSpec, Runtime, StepContext
 from ..parts.linear import require_true_fp32
 from ..weights.loader import load_tensors
 from ..weights.random_init import random_tensors
@@ -74,11 +74,11 @@ def build_step_context(cache: CacheManager, entries: list, vocab_size: int, devi
     T = sum(n_new)
     pos0 = [cache.length(s) for s in slots]
 
-    # one packed int32 buffer, one copy to the device
+    # what only the host knows, as one int32 array: the tokens, each sequence's length, count and slot, the places wanted
     n_want = sum(len(e.want) for e in entries)
-    offs = np.cumsum([0, T, T, T, B + 1, B, B, B, n_want])
+    offs = np.cumsum([0, T, B, B, B, n_want]).tolist()
     buf = np.empty(offs[-1], dtype=np.int32)
-    ids, tok_seq, tok_pos, cu, p0, slen, slot_a, want = (buf[offs[i]:offs[i + 1]] for i in range(8))
+    ids, p0, counts, slot_a, want = (buf[offs[i]:offs[i + 1]] for i in range(5))
     t = 0
     w = 0
     for b, e in enumerate(entries):
@@ -88,33 +88,71 @@ def build_step_context(cache: CacheManager, entries: list, vocab_size: int, devi
                 ids[t:t + n] = e.tokens
             except (TypeError, ValueError, OverflowError):
                 raise EngineError(f"slot {e.slot}: token ids must be integers") from None
-        tok_seq[t:t + n] = b
-        tok_pos[t:t + n] = np.arange(pos0[b], pos0[b] + n)
-        cu[b] = t
         for i in e.want:
             if not 0 <= i < n:
                 raise EngineError(f"slot {e.slot}: wanted place {i} is outside this step's {n} tokens")
             want[w] = t + i
             w += 1
         t += n
-    cu[B] = T
     if T and (ids.min() < 0 or ids.max() >= vocab_size):
         bad = int(ids[(ids < 0) | (ids >= vocab_size)][0])
         raise EngineError(f"token id {bad} is outside the vocabulary of {vocab_size}")
     p0[:] = pos0
-    slen[:] = [p + n for p, n in zip(pos0, n_new)]
+    counts[:] = n_new
     slot_a[:] = slots
-    cache.reserve({s: p + n for s, p, n in zip(slots, pos0, n_new)})     # after every check: a refused step holds nothing
-    dev = torch.from_numpy(buf).to(device)
-    parts = [dev[offs[i]:offs[i + 1]] for i in range(8)]
-    tables = {}
-    for gid in range(cache.n_groups()):
-        tables[gid] = torch.from_numpy(cache.page_table_host(gid, slots)).to(device)
-    ctx = StepContext(n_tokens=T, n_seqs=B, token_ids=parts[0], tok_seq=parts[1], tok_pos=parts[2],
-                      cu_seqlens=parts[3], pos0=parts[4], seq_len=parts[5], slots=parts[6],
-                      max_new=max(n_new), min_new=min(n_new), max_len=int(max(slen)), single_token=all(n == 1 for n in n_new),
-                      page_tables=tables, host_slots=slots, all_start=all(p == 0 for p in pos0))
-    return ctx, parts[7]
+    slen = [p + n for p, n in zip(pos0, n_new)]
+    cache.reserve(dict(zip(slots, slen)))     # after every check: a refused step holds nothing
+    # behind it each cache group's pages, one sequence after the other, and where each one's begin: one copy to the device,
+    # which makes everything else (``ops.step_tables``: a launch a group)
+    group_pages, ends = [], [offs[-1]]
+    for gid in range(max(1, cache.n_groups())):
+        lists = cache.page_lists(gid, slots) if cache.n_groups() else [[] for _ in slots]
+        start = np.zeros(B + 1, dtype=np.int32)
+        np.cumsum([len(p) for p in lists], out=start[1:])
+        flat = np.empty(int(start[B]), dtype=np.int32)
+        for b, p in enumerate(lists):
+            if not fill_int32(flat[start[b]:start[b + 1]], p):
+                flat[start[b]:start[b + 1]] = p
+        group_pages += [start, flat]
+        ends += [ends[-1] + B + 1, ends[-1] + B + 1 + len(flat)]
+    dev = torch.from_numpy(np.concatenate([buf, *group_pages])).to(device)
+    parts = [dev[offs[i]:offs[i + 1]] for i in range(5)]
+    tables, first = {}, None
+    for gid in range(max(1, cache.n_groups())):
+        start, flat = dev[ends[2 * gid]:ends[2 * gid + 1]], dev[ends[2 * gid + 1]:ends[2 * gid + 2]]
+        of_tokens = first is None or cache.group_spec(gid).bits == 4
+        with torch.cuda.device(dev.device):
+            made = ops.step_tables(flat, start, parts[1], parts[2], T, cache.table_width if cache.n_groups() else 0, tokens=of_tokens)
+        first = first or made
+        if cache.n_groups():
+            tables[gid] = made
+    ctx = StepContext(n_tokens=T, n_seqs=B, token_ids=parts[0], tok_seq=first.tok_seq, tok_pos=first.tok_pos,
+                      cu_seqlens=first.cu_seqlens, pos0=parts[1], seq_len=first.seq_len, slots=parts[3],
+                      max_new=max(n_new), min_new=min(n_new), max_len=max(slen), single_token=all(n == 1 for n in n_new),
+                      page_tables={gid: t.page_table for gid, t in tables.items()}, host_slots=slots,
+                      all_start=all(p == 0 for p in pos0), tables=tables)
+    return ctx, parts[4]
+
+
+def require_cache_bits(plan, cache_bits: int) -> None:
+    """Refuse a cache in fewer bits that a mixer of this plan does not keep, before a weight is read."""
+    if cache_bits == 0:
+        return
+    if cache_bits != 4:
+        raise EngineError(f"cache_bits: keys and values are cached in the engine's dtype (0) or in 4 bits (4), not in {cache_bits}")
+    try:
+        model = Model(plan, Runtime(torch.device("cpu"), torch.bfloat16, cache_bits))
+    except ValueError as e:
+        raise EngineError(f"cache_bits=4: {e}") from None
+    found = 0
+    for run, (kv, _, _) in zip(plan.schedule, model.cache_units()):
+        for spec in () if kv is None else (kv,) if isinstance(kv, KVSpec) else kv:
+            found += 1
+            if spec.bits != cache_bits:
+                raise EngineError(f"cache_bits=4: layer {run.layer}'s mixer '{plan.layers[run.layer].mixer.kind}' keeps its cache in the "
+                                  f"engine's dtype only")
+    if not found:
+        raise EngineError("cache_bits=4: this model caches no keys and values")
 
 
 class Engine:
@@ -123,20 +161,25 @@ class Engine:
     max_tokens   the most tokens live sequences hold together (each rounded up to pages of 64)
     max_seq_len  the longest single sequence (default: max_tokens, capped by the model's trained length)
     max_batch    the most sequences alive at once (default: as many as could each hold one page, up to 256)
+    cache_bits   4: keys and values are cached in 4 bits, a step for 32 of them (3.6 times as many tokens in the same memory as in
+                 bfloat16; the cache's numbers are then off by 2 % of a row's size, so logits differ from those of a cache in the
+                 engine's dtype); grouped-query attention only.  0: in the engine's dtype
     """
 
     def __init__(self, config: ModelConfig, weights: dict, dtype: torch.dtype, device: torch.device,
-                 max_tokens: int, max_seq_len: int | None = None, max_batch: int | None = None):
+                 max_tokens: int, max_seq_len: int | None = None, max_batch: int | None = None, cache_bits: int = 0):
         self.config = config
         self.dtype = dtype
+        self.cache_bits = cache_bits
         self.device = device
         if dtype == torch.float32:
             require_true_fp32()
         arch = get_architecture(config.architecture)
         self.plan = arch.plan(config)
-        self.runtime = Runtime(device, dtype)
+        require_cache_bits(self.plan, cache_bits)
+        self.runtime = Runtime(device, dtype, cache_bits)
         self.model = Model(self.plan, self.runtime)
-        kernel_build.compile_modules(self.model.kernel_modules())
+        kernel_build.compile_modules(["step_tables", *self.model.kernel_modules()])
         self.model.bind(weights)
         self.vocab_size = self.plan.vocab_size
         if max_seq_len is None:
@@ -162,6 +205,7 @@ class Engine:
         dtype = DTYPES[dtype]
         config = load_config(model_dir)
         plan = get_architecture(config.architecture).plan(config)
+        require_cache_bits(plan, kw.get("cache_bits", 0))
         weights = load_tensors(model_dir, plan.manifest(), dtype, device)
         return cls(config, weights, dtype, device, **kw)
 
@@ -172,6 +216,7 @@ class Engine:
         _require_cuda(device)
         dtype = DTYPES[dtype]
         plan = get_architecture(config.architecture).plan(config)
+        require_cache_bits(plan, kw.get("cache_bits", 0))
         weights = random_tensors(plan.manifest(), seed, dtype, device=device, vector_dtype=torch.float32)
         return cls(config, weights, dtype, device, **kw)
 
@@ -206,25 +251,27 @@ class Engine:
         with torch.cuda.device(self.device):
             ops.gemm_tc_check(self.device)
 
-    def decode_runner(self, batch: int, sampling, use_graph: bool = True):
+    def decode_runner(self, batch: int, sampling, use_graph: bool = True, logprobs: int | None = None):
         """The fixed buffers and CUDA graphs for decode steps of ``batch`` sequences (made once, kept).  The sampling
-        options without the seed key it: the seed lives on the device and is given with ``bind``."""
+        options without the seed key it: the seed lives on the device and is given with ``bind``.  ``logprobs``: also the sampled
+        tokens' log probabilities, with so many alternatives each."""
         import dataclasses
         from .decode import DecodeRunner
         sampling = dataclasses.replace(sampling, seed=0)
-        key = (batch, sampling, use_graph)
+        key = (batch, sampling, use_graph, logprobs)
         runner = self._runners.get(key)
         if runner is None:
             if len(self._runners) >= 16:             # graphs hold memory: drop the oldest
                 self._runners.pop(next(iter(self._runners)))
-            runner = self._runners[key] = DecodeRunner(self, batch, sampling, use_graph)
+            runner = self._runners[key] = DecodeRunner(self, batch, sampling, use_graph, logprobs)
         return runner
 
     # ------------------------------------------------------------------ facts
     def describe(self) -> dict:
         n_params = sum(int(np.prod(t.shape)) for t in self.model.tensors() if not (t.optional or t.ignored))
         return {"architecture": self.config.architecture, "dtype": str(self.dtype).replace("torch.", ""),
-                "parameters": n_params, "cache_bytes": self.cache.bytes_held(),
+                "parameters": n_params, "cache_bits": self.cache_bits or 8 * torch.empty((), dtype=self.dtype).element_size(),
+                "cache_bytes": self.cache.bytes_held(),
                 "max_tokens": self.cache.max_tokens, "max_seq_len": self.cache.max_seq_len,
                 "max_batch": self.max_batch, "page_size": PAGE_SIZE, "layers": len(self.plan.layers),
                 "schedule": len(self.plan.schedule), "cache_groups": self.cache.n_groups()}

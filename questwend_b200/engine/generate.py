@@ -14,11 +14,15 @@ device, so they can be followed with any object that has ``open_sequences``,
 """
 from __future__ import annotations
 
+import operator
 import os
 import time
 from dataclasses import dataclass, field
 
+import torch
+
 from ..cache.manager import pages_for
+from ..kernels import ops
 from ..sampling.params import GREEDY, SamplingParams
 from ..sampling.sampler import DeviceSampler, PenaltyWindow
 from .engine import StepEntry
@@ -28,11 +32,27 @@ FINISH_LENGTH = "length"      # max_new_tokens were emitted
 FINISH_CONTEXT = "context"    # the sequence reached the longest length the cache allows
 
 
+@dataclass(frozen=True)
+class TokenScore:
+    """How probable a token was where it stands, by the model's logits as they are (no penalties, temperature or cuts)."""
+    token: int
+    logprob: float
+    entropy: float                # of the whole distribution, in nats
+    top: tuple = ()               # the most probable tokens: (id, log probability), the first the most
+
+
+def _scores_of(tokens, r: ops.TokenLogprobs) -> list[TokenScore]:
+    ids, lps = r.top_ids.tolist(), r.top_logprobs.tolist()
+    return [TokenScore(int(t), lp, h, tuple(zip(i, l))) for t, lp, h, i, l in
+            zip(tokens, r.logprob.tolist(), r.entropy.tolist(), ids, lps)]
+
+
 @dataclass
 class GenerationResult:
     tokens: list = field(default_factory=list)
     finish_reason: str = ""
     prompt_tokens: int = 0
+    scores: list = field(default_factory=list)    # a TokenScore for each token, if ``generate`` was asked for log probabilities
 
 
 @dataclass
@@ -120,12 +140,24 @@ class StepProfile:
         self._last_end = self.clock()
 
 
+def _sample(sampler, logits, active, step, windows, logprobs):
+    """The sampler's ids for these rows and (``logprobs`` not None) their scores by the logits as they are before it."""
+    if logprobs is None:
+        return sampler(logits, active, step, windows), []
+    as_they_are = logits.clone()                # a sampler may change its logits
+    ids = sampler(logits, active, step, windows)
+    tokens = torch.tensor([int(t) for t in ids], dtype=torch.int32, device=logits.device)
+    with torch.cuda.device(logits.device):
+        return ids, _scores_of(ids, ops.token_logprobs(as_they_are, tokens, top=logprobs))
+
+
 class _PlainStepper:
     """Decode steps through ``engine.step`` and a sampler callable."""
 
-    def __init__(self, engine, sampler, slot_of, windows, profile=None):
+    def __init__(self, engine, sampler, slot_of, windows, profile=None, logprobs=None):
         self.engine, self.sampler, self.slot_of, self.windows = engine, sampler, slot_of, windows
         self.profile = profile
+        self.logprobs, self.scores = logprobs, []
 
     def run(self, active, tokens, step):
         prof = self.profile
@@ -137,7 +169,7 @@ class _PlainStepper:
         logits = self.engine.step(entries)
         if prof:
             prof.launched()
-        ids = self.sampler(logits, active, step, [self.windows[i] for i in active])
+        ids, self.scores = _sample(self.sampler, logits, active, step, [self.windows[i] for i in active], self.logprobs)
         if prof:
             prof.end(step, len(active), "plain")
         return ids
@@ -146,8 +178,9 @@ class _PlainStepper:
 class _GraphStepper:
     """Decode steps replayed from CUDA graphs (``DecodeRunner``); rebinds when the batch changes."""
 
-    def __init__(self, engine, sampling, seed, slot_of, windows, profile=None):
+    def __init__(self, engine, sampling, seed, slot_of, windows, profile=None, logprobs=None):
         self.engine, self.sampling, self.seed = engine, sampling, seed
+        self.logprobs, self.scores = logprobs, []
         self.slot_of, self.windows = slot_of, windows
         self.bound = None
         self.runner = None
@@ -158,7 +191,8 @@ class _GraphStepper:
         if prof:
             prof.begin()
         if self.bound != active:
-            self.runner = self.engine.decode_runner(len(active), self.sampling)
+            more = {} if self.logprobs is None else {"logprobs": self.logprobs}
+            self.runner = self.engine.decode_runner(len(active), self.sampling, **more)
             self.runner.bind([self.slot_of[i] for i in active], tokens, active, step,
                              [self.windows[i] for i in active], seed=self.seed)
             self.bound = list(active)
@@ -166,6 +200,8 @@ class _GraphStepper:
             self.runner.profile = prof
         self.runner.step(host_tokens=tokens)
         ids = self.runner.read_sampled()
+        if self.logprobs is not None:
+            self.scores = _scores_of(ids, self.runner.host_scores())
         if prof:
             self.runner.profile = None
             prof.end(step, len(active), self.runner.last_step_how)
@@ -174,7 +210,7 @@ class _GraphStepper:
 
 def generate(engine, prompts, max_new_tokens: int = 128, sampling: SamplingParams = GREEDY,
              stop_ids=None, ignore_eos: bool = False, sampler=None, stats: GenerationStats | None = None,
-             clock=time.perf_counter, use_graph: bool = True, profile=None) -> list[GenerationResult]:
+             clock=time.perf_counter, use_graph: bool = True, profile=None, logprobs: int | None = None) -> list[GenerationResult]:
     """Generate for every prompt (a list of token ids each).
 
     stop_ids    tokens that end a sequence; default: the model's own (``eos_token_id``)
@@ -183,7 +219,11 @@ def generate(engine, prompts, max_new_tokens: int = 128, sampling: SamplingParam
     use_graph   replay decode steps from CUDA graphs (needs the default sampler)
     profile     a ``StepProfile``, or True for one that prints to stderr: a line per decode step that says where its
                 time went (also switched on by the environment variable QWB200_PROF=1)
+    logprobs    each result's ``scores``: every token's log probability, the entropy of its distribution and so many (0: none)
+                of the most probable tokens, by the model's logits before penalties, temperature and cuts
     """
+    if logprobs is not None and not 0 <= logprobs <= min(ops.LOGPROBS_MAX_TOP, getattr(engine, "vocab_size", ops.LOGPROBS_MAX_TOP)):
+        raise ValueError(f"logprobs: 0 to {ops.LOGPROBS_MAX_TOP} alternatives and no more than the vocabulary holds, not {logprobs}")
     if profile is None and os.environ.get("QWB200_PROF", "0") not in ("", "0"):
         profile = True
     if profile is True:
@@ -217,26 +257,28 @@ def generate(engine, prompts, max_new_tokens: int = 128, sampling: SamplingParam
         windows = {i: PenaltyWindow(sampling, prompts[i]) for i in batch}
         length = {i: len(prompts[i]) for i in batch}
         active = list(batch)
-        stepper = (_GraphStepper(engine, sampling, sampler.seed, slot_of, windows, profile) if graph_path
-                   else _PlainStepper(engine, sampler, slot_of, windows, profile))
+        stepper = (_GraphStepper(engine, sampling, sampler.seed, slot_of, windows, profile, logprobs) if graph_path
+                   else _PlainStepper(engine, sampler, slot_of, windows, profile, logprobs))
         try:
             t0 = clock()
             want_last = max_new_tokens > 0
             logits = engine.step([StepEntry(slot_of[i], prompts[i], [len(prompts[i]) - 1] if want_last else [])
                                   for i in active])
-            ids = sampler(logits, active, 0, [windows[i] for i in active]) if want_last else []
+            ids, scores = _sample(sampler, logits, active, 0, [windows[i] for i in active], logprobs) if want_last else ([], [])
             stats.prefill_seconds += clock() - t0
             stats.prompt_tokens += sum(len(prompts[i]) for i in active)
             step = 1
             while want_last and active:
                 going, done = [], []
-                for i, tok in zip(active, ids):
+                for n, (i, tok) in enumerate(zip(active, ids)):
                     tok = int(tok)
                     if tok in stops:                         # not emitted, not counted
                         results[i].finish_reason = FINISH_STOP
                         done.append(i)
                         continue
                     results[i].tokens.append(tok)
+                    if logprobs is not None:
+                        results[i].scores.append(scores[n])
                     windows[i].accept(tok)
                     stats.generated_tokens += 1
                     if len(results[i].tokens) >= max_new_tokens:
@@ -254,6 +296,7 @@ def generate(engine, prompts, max_new_tokens: int = 128, sampling: SamplingParam
                     break
                 t0 = clock()
                 ids = stepper.run(active, [results[i].tokens[-1] for i in active], step)
+                scores = stepper.scores
                 took = clock() - t0
                 stats.decode_seconds += took
                 stats.step_seconds.append(took)
@@ -269,4 +312,54 @@ def generate(engine, prompts, max_new_tokens: int = 128, sampling: SamplingParam
         for i in batch:
             if not results[i].finish_reason:
                 results[i].finish_reason = FINISH_LENGTH
+    return results
+
+
+SCORE_ROWS = 2048           # rows of logits that one step of ``score`` makes (at 151,936 tokens 1.2 GB)
+
+
+def score(engine, sequences, top: int = 0, max_rows: int = SCORE_ROWS) -> list[list[TokenScore]]:
+    """How probable each token of these sequences (lists of token ids) is behind the ones before it: for a sequence of n tokens
+    n - 1 ``TokenScore``, for its second token and on, each with the ``top`` most probable tokens.  Sequences run together while
+    they have ``max_rows`` tokens in all, a longer one in pieces of as many."""
+    if not 0 <= top <= min(ops.LOGPROBS_MAX_TOP, engine.vocab_size):
+        raise ValueError(f"top: 0 to {ops.LOGPROBS_MAX_TOP} alternatives and no more than the vocabulary holds, not {top}")
+    if not 1 <= max_rows <= ops.LOGPROBS_MAX_ROWS:
+        raise ValueError(f"max_rows: 1 to {ops.LOGPROBS_MAX_ROWS}, not {max_rows}")
+    sequences = [[operator.index(t) for t in s] for s in sequences]
+    for i, s in enumerate(sequences):
+        if not s:
+            raise ValueError(f"sequence {i} is empty")
+        if len(s) - 1 > engine.cache.max_seq_len:
+            raise ValueError(f"sequence {i} has {len(s)} tokens; the longest sequence allowed is {engine.cache.max_seq_len} and the one behind")
+        bad = [t for t in s if not 0 <= t < engine.vocab_size]
+        if bad:
+            raise ValueError(f"sequence {i}: {bad[0]} is not a token id below {engine.vocab_size}")
+    results: list[list[TokenScore]] = [[] for _ in sequences]
+    todo = [i for i, s in enumerate(sequences) if len(s) > 1]
+    pages = min(engine.cache.free_pages(), default=0) if engine.cache.n_groups() else pages_for(engine.cache.max_tokens)
+    while todo:
+        batch, rows, held = [], 0, 0
+        for i in todo:                                  # in their order, as many as fit a step and the cache
+            n = len(sequences[i]) - 1
+            if batch and (rows + n > max_rows or held + pages_for(n) > pages or len(batch) >= min(engine.max_batch, engine.cache.slots.n_free)):
+                break
+            batch.append(i)
+            rows, held = rows + n, held + pages_for(n)
+        todo = todo[len(batch):]
+        slots = engine.open_sequences(len(batch))
+        try:
+            at = 0
+            while at < max(len(sequences[i]) - 1 for i in batch):       # more than one round only for a sequence on its own
+                pieces = [sequences[i][at:min(at + max_rows, len(sequences[i]) - 1)] for i in batch]
+                logits = engine.step([StepEntry(s, p, list(range(len(p)))) for s, p in zip(slots, pieces)])
+                behind = [t for i, p in zip(batch, pieces) for t in sequences[i][at + 1:at + 1 + len(p)]]
+                with torch.cuda.device(logits.device):
+                    found = _scores_of(behind, ops.token_logprobs(logits, torch.tensor(behind, dtype=torch.int32, device=logits.device), top=top))
+                for i, p in zip(batch, pieces):
+                    results[i] += found[:len(p)]
+                    found = found[len(p):]
+                at += max_rows
+        finally:
+            engine.close_sequences(slots)
     return results

@@ -9,7 +9,7 @@ import math
 import torch
 
 from ..kernels import ops
-from ..kernels.limits import (conv_taps_refusal, head_dim_refusal, maps_attention_refusal, pool_attention_refusal,
+from ..kernels.limits import (conv_taps_refusal, head_dim_refusal, kv4_refusal, maps_attention_refusal, pool_attention_refusal,
                               shaped_attention_refusal)
 from ..weights.manifest import MATRIX, NORM_WEIGHT, VECTOR, TensorSpec
 from .base import KVSpec, Mixer, StateSpec, take_weight
@@ -26,7 +26,9 @@ DECODE_SPLIT_TOKENS = 256     # keys per run of the plain decode kernel; fixed, 
 
 class GroupedQueryAttention(Mixer):
     """params: hidden_size, n_heads, n_kv_heads, head_dim, qk_norm (bool), norm_eps, window (0: none),
-    scale (default 1/sqrt(head_dim)), names (optional overrides of the tensor names)."""
+    scale (default 1/sqrt(head_dim)), names (optional overrides of the tensor names).
+    With ``Runtime.cache_bits`` 4 keys and values are cached in 4 bits and attention reads them from there, the step's own too:
+    a prompt's logits do not depend on the pieces that it comes in."""
 
     NAMES = {"q": "q_proj.weight", "k": "k_proj.weight", "v": "v_proj.weight", "o": "o_proj.weight",
              "q_norm": "q_norm.weight", "k_norm": "k_norm.weight"}
@@ -50,6 +52,9 @@ class GroupedQueryAttention(Mixer):
         refusal = head_dim_refusal(self.head_dim)           # now, and not at the first step with the weights loaded
         if refusal:
             raise ValueError(f"grouped-query attention '{self.prefix}': parameter 'head_dim': {refusal}")
+        self.cache_bits = getattr(runtime, "cache_bits", 0)
+        if self.cache_bits and kv4_refusal(self.head_dim):
+            raise ValueError(f"grouped-query attention '{self.prefix}': {kv4_refusal(self.head_dim)}")
         if self.rotary_dim > self.head_dim:
             raise ValueError(f"rotary size {self.rotary_dim} exceeds the head size {self.head_dim}")
         self.w_qkv = self.w_o = self.q_norm_w = self.k_norm_w = None
@@ -77,7 +82,11 @@ class GroupedQueryAttention(Mixer):
 
     def kernel_modules(self):
         mods = ["rope_kv", *linear_modules(self.runtime.dtype)]
-        if ops.mma_attention_fits(self.runtime.dtype, self.head_dim, ops.PAGE_SIZE):
+        if self.cache_bits:
+            mods += ["kv4_cache", "attention_kv4"]
+            if ops.tc_attention_fits(self.runtime.dtype, self.head_dim, ops.PAGE_SIZE, self.n_heads // self.n_kv_heads):
+                mods.append("attention_tc")
+        elif ops.mma_attention_fits(self.runtime.dtype, self.head_dim, ops.PAGE_SIZE):
             mods.append("attention_mma")
             if ops.tc_attention_fits(self.runtime.dtype, self.head_dim, ops.PAGE_SIZE, self.n_heads // self.n_kv_heads):
                 mods.append("attention_tc")
@@ -86,7 +95,7 @@ class GroupedQueryAttention(Mixer):
         return tuple(mods)
 
     def kv_spec(self):
-        return KVSpec(self.n_kv_heads, self.head_dim, self.window)
+        return KVSpec(self.n_kv_heads, self.head_dim, self.window, bits=self.cache_bits)
 
     adds_to_residual = True
 
@@ -96,7 +105,12 @@ class GroupedQueryAttention(Mixer):
         if self.position is not None:
             cos, sin = self.position.prepare(ctx)
         table = ctx.page_tables[cache.group_id]
-        if (ctx.single_token and ctx.n_seqs <= FUSED_DECODE_MAX_BATCH and self.rotary_dim in (0, self.head_dim)
+        if self.cache_bits:
+            tables = ctx.tables[cache.group_id]
+            q = ops.kv4_store(qkv, self.q_norm_w, self.k_norm_w, cos, sin, tables.slot_map, cache.k_pool, self.n_heads, self.n_kv_heads,
+                              self.head_dim, self.rotary_dim, self.eps, self.runtime.dtype, store_kv=cache.writable)
+            att = ops.kv4_attention(q, cache.k_pool, tables, ctx.max_new, ctx.max_len, self.scale, window=self.window)
+        elif (ctx.single_token and ctx.n_seqs <= FUSED_DECODE_MAX_BATCH and self.rotary_dim in (0, self.head_dim)
                 and ops.mma_attention_fits(cache.k_pool.dtype, self.head_dim, cache.k_pool.shape[2])):
             # one token for each of a few sequences on the tensor-core path: norm, rotation and cache write happen inside
             # the attention kernel

@@ -44,10 +44,17 @@ class KVSpec:
     value_dim: int = 0          # size of a value row where it differs from a key row's (0: the same)
     stride: int = 1             # one cached row for every ``stride`` tokens of the sequence (a row per complete block of
                                 # tokens: pooled keys and values); a sequence of n tokens holds n // stride rows
+    bits: int = 0               # 0: in the engine's dtype.  4: keys and values in 4 bits with a step for 32 of them; the unit's
+                                # ``k_pool`` is then uint8 [n_pages, Hkv, bytes of a page], with the values in it, its ``v_pool`` None
 
     @property
     def v_dim(self) -> int:
         return self.value_dim or self.head_dim
+
+    def token_bytes(self, itemsize: int) -> int:
+        """Bytes of a cached row of all heads, keys and values, where the engine's dtype takes ``itemsize`` a number."""
+        numbers = self.n_kv_heads * (self.head_dim + (self.v_dim if self.values else 0))
+        return numbers * 9 // 16 if self.bits == 4 else numbers * itemsize       # 4 bits each and 16 for every 32
 
 
 @dataclass(frozen=True)
@@ -63,6 +70,7 @@ class Runtime:
     """Where and how a model computes."""
     device: torch.device
     dtype: torch.dtype          # torch.bfloat16 or torch.float32: matrices, cache and matrix-product inputs
+    cache_bits: int = 0         # 4: keys and values are cached in 4 bits, by the mixers that can (``KVSpec.bits``); 0: in ``dtype``
 
 
 @dataclass
@@ -87,6 +95,8 @@ class StepContext:
     shared: dict = field(default_factory=dict)   # per-step values shared between layers (rotation tables)
     min_new: int = 1            # no sequence brings fewer new tokens
     all_start: bool = False     # every sequence of the step starts at its position 0 (whole prompts): known on the host
+    tables: dict = field(default_factory=dict)  # cache group id -> ``ops.StepTables``: the page table above, the tokens' rows of the
+                                # pool and the pages one after the other (groups in 4 bits; others where the step's context made them)
 
 
 class UnitCache:
