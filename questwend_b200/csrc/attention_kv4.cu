@@ -1,5 +1,23 @@
 // Attention over the cache in 4 bits (kv4.cuh), causal, grouped heads, with an optional window.
 //
+// Few new tokens a sequence, bfloat16, heads of 64 or 128 (kv4_attn_rows_kernel): a decode step.  What it has to do is read the
+// cache, 144 bytes a token and head of 128, for 4 x 128 multiply-adds a query head: on mma.sync, whose products are far from the limit
+// here (a group of 4 heads fills half of the 8 columns), so that the time is loads and the way from codes to bfloat16.
+//   * A block takes a key/value head and a run of a sequence's pages; its four warps take 16 keys of every page each, with their
+//     own copies (cp.async into a ring of their own), maxima, sums and outputs, and meet at the run's end in shared memory.  Nothing in
+//     between waits for another warp.
+//   * The 16-row operand of both products is the cache's, the 8 columns are (token, query head) pairs:
+//     S^T = K Q^T and O^T = V^T P^T, so that 4 query heads take half of an mma and not a quarter.
+//   * Which number of a row sits where in an mma's inner dimension is free as long as both operands agree.  A lane therefore takes
+//     32 neighbouring numbers of a key (one 16-byte load, one group, one step), and of a value its 16 numbers of 4 keys; codes come out
+//     of a 32-bit word two at a time, in the places where their shifts leave them.
+//   * A code c becomes the bfloat16 128 + c by one and-or (its 7 bits behind the point hold c), 128 + z is taken off and s
+//     multiplied: both exact.
+//   * The scores' columns are the next product's inner dimension: P^T's operand is two 8 x 8 transpositions (movmatrix).
+//   * A run's softmax is relative to a reference that is raised, and O rescaled, only where a score passes it by 2^8: most tiles vote once
+//     and exchange no maxima.
+// Runs are cut by the sequence's own length (kv4_runs), never by what else is in the batch; a second kernel joins them.
+//
 // The plain kernel: any head size that is a multiple of 32, queries in 32 bits or bfloat16.  A block takes a (token, query head),
 // its four warps every fourth key; a lane holds the numbers lane, lane + 32, ... of the query, of the sums and of a key, so a
 // group of 32 is a step of the loop over them.  Each warp keeps a running maximum, sum and output; they meet in shared memory.
@@ -30,7 +48,7 @@ kv4_attn_plain_kernel(const T* __restrict__ q, const unsigned char* __restrict__
         for (int j = first + warp; j <= pos; j += KP_WARPS) {
             if (j / KV4_PAGE >= table_width) break;
             const long long page = page_table[(size_t)b * table_width + j / KV4_PAGE];
-            if (page < 0 || page >= pool_pages) break;
+            if (page < 0 || page >= pool_pages) continue;
             const int row = j % KV4_PAGE;
             const unsigned char* k = pool + ((size_t)page * Hkv + kvh) * kv4_page_bytes(hd);
             const unsigned char* v = k + kv4_half_bytes(hd);
@@ -90,4 +108,450 @@ extern "C" int qwb_kv4_attn_plain(const void* q, const unsigned char* pool, cons
     else
         return qwb_fail(QWB_ERR_ARG, "kv4_attention: unknown dtype %d", dtype);
     return qwb_check_launch("kv4_attention");
+}
+
+// ----------------------------------------------------------------------------- few new tokens: mma.sync
+#define KD_WARPS 4
+#define KD_KEYS 16              // keys of a warp's tile: the mma's 16 rows
+#define KD_STAGES 4             // tiles of a warp's ring
+#define KD_RUNS 16              // a sequence's pages are cut into about so many runs ...
+#define KD_RUN_PAGES 8          // ... of at most this many pages
+#define KD_RAISE 8.f            // a run's reference is raised where a score passes it by 2^8
+
+// The pages that a sequence's new tokens see, and how they are cut.
+struct Kv4Runs { int first, count, per_run, runs; };
+__host__ __device__ __forceinline__ Kv4Runs kv4_runs(int pos0, int len, int window, int table_width) {
+    Kv4Runs r;
+    const int low = window > 0 && pos0 - window + 1 > 0 ? pos0 - window + 1 : 0;
+    r.first = low / KV4_PAGE;
+    const int last = (len - 1) / KV4_PAGE < table_width - 1 ? (len - 1) / KV4_PAGE : table_width - 1;
+    r.count = len > 0 && last >= r.first ? last - r.first + 1 : 0;
+    const int even = (r.count + KD_RUNS - 1) / KD_RUNS;
+    r.per_run = even < 1 ? 1 : (even > KD_RUN_PAGES ? KD_RUN_PAGES : even);
+    r.runs = (r.count + r.per_run - 1) / r.per_run;
+    return r;
+}
+
+__device__ __forceinline__ void kd_copy16(void* dst, const void* src) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"((uint32_t)__cvta_generic_to_shared(dst)), "l"(src) : "memory");
+}
+__device__ __forceinline__ void kd_mma(float* c, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                 : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t kd_transpose(uint32_t x) {
+    uint32_t y;
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+    return y;
+}
+__device__ __forceinline__ uint32_t kd_pack(float lo, float hi) {
+    __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
+    return *reinterpret_cast<uint32_t*>(&v);
+}
+__device__ __forceinline__ float kd_exp2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+// Two codes, in the lowest four bits of each half of `codes`, as the bfloat16 numbers (c - z) s; zero: 128 + z twice, step: s twice.
+__device__ __forceinline__ uint32_t kd_numbers(uint32_t codes, uint32_t zero, uint32_t step) {
+    uint32_t e = (codes & 0x000f000fu) | 0x43004300u;
+    __nv_bfloat162 v = __hmul2(__hsub2(*reinterpret_cast<__nv_bfloat162*>(&e), *reinterpret_cast<__nv_bfloat162*>(&zero)),
+                               *reinterpret_cast<__nv_bfloat162*>(&step));
+    return *reinterpret_cast<uint32_t*>(&v);
+}
+
+template <int HD>
+struct KdTile {                                             // a warp's 16 keys of a page and head
+    static constexpr int CODES = KD_KEYS * HD / 2, WORDS = KD_KEYS * HD / 16, HALF = CODES + WORDS, BYTES = 2 * HALF;
+};
+template <int HD, int NT>
+struct KdSmem {
+    static constexpr int RING = KD_WARPS * KD_STAGES * KdTile<HD>::BYTES;
+    static constexpr int COL = HD + 4;                      // floats of a column of outputs: two columns are 8 banks apart
+    static constexpr int JOIN = KD_WARPS * 8 * NT * (COL + 2) * 4;
+    static constexpr int BYTES = RING > JOIN ? RING : JOIN;
+};
+
+// NT: tiles of 8 columns of a block.  part: [rows, max_runs, HD] outputs, then [rows, max_runs, 2] maxima (of scores times log2 e) and sums
+// of the runs of sequences that have more than one; a row is (token, query head).
+template <int HD, int NT>
+__global__ void __launch_bounds__(KD_WARPS * 32, NT == 1 ? 4 : 3)
+kv4_attn_rows_kernel(const bf16* __restrict__ q, const unsigned char* __restrict__ pool, const int* __restrict__ page_table,
+                     const int* __restrict__ cu_seqlens, const int* __restrict__ pos0, bf16* __restrict__ out, float* __restrict__ part_o,
+                     float* __restrict__ part_ml, int T, int B, int pool_pages, int Hq, int Hkv, int table_width, float scale_log2, int window,
+                     int tiles, int max_runs) {
+    pdl_wait();
+    pdl_launch_dependents();
+    using Tile = KdTile<HD>;
+    using Smem = KdSmem<HD, NT>;
+    extern __shared__ __align__(128) unsigned char smem[];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, r = lane >> 2, c = lane & 3;
+    const int tile = blockIdx.x % tiles, run = blockIdx.x / tiles, kvh = blockIdx.y, b = blockIdx.z;
+    const int G = Hq / Hkv;
+    if (blockIdx.x == 0 && kvh == 0 && b == 0) {            // tokens behind the last sequence's: zeros
+        for (long long i = (long long)max(cu_seqlens[B], 0) * Hq * HD + threadIdx.x; i < (long long)T * Hq * HD; i += KD_WARPS * 32) out[i] = from_f32<bf16>(0.f);
+    }
+    const int t0 = cu_seqlens[b], n_new = min(cu_seqlens[b + 1], T) - t0;
+    const int col0 = tile * 8 * NT, cols = n_new * G;
+    if (t0 < 0 || n_new <= 0 || col0 >= cols) return;
+    const int p0 = pos0[b], len = p0 + n_new;
+    const Kv4Runs cut = kv4_runs(p0, len, window, table_width);
+    const int runs = min(cut.runs, max_runs);               // a sequence beyond max_len: cut off there, never written beyond the scratch
+    if (run >= runs && run > 0) return;
+    const int first_page = cut.first + run * cut.per_run, n_pages = min(cut.per_run, cut.count - run * cut.per_run);
+    const int* table = page_table + (size_t)b * table_width + first_page;
+    int my_page = -1;                                       // lane i: the run's i-th page
+    if (lane < n_pages) my_page = table[lane];
+    if (my_page >= pool_pages) my_page = -1;
+
+    // this block's columns: their last and first key; the queries, in the order in which a lane holds the keys' numbers
+    int last_key[NT][2], first_key[NT][2];
+    uint32_t qf[NT][HD / 16][2];
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+            const int col = min(col0 + n * 8 + 2 * c + e, cols - 1);
+            last_key[n][e] = p0 + col / G;
+            first_key[n][e] = window > 0 ? p0 + col / G - window + 1 : 0;
+        }
+        const int col = col0 + n * 8 + r;
+        const bool live = col < cols;
+        const bf16* src = q + ((size_t)(t0 + (live ? col / G : 0)) * Hq + kvh * G + (live ? col % G : 0)) * HD + c * (HD / 4);
+#pragma unroll
+        for (int w = 0; w < HD / 32; ++w) {
+            uint4 v = make_uint4(0, 0, 0, 0);
+            if (live) v = *reinterpret_cast<const uint4*>(src + 8 * w);
+            qf[n][2 * w][0] = __byte_perm(v.x, v.z, 0x5410);            // numbers 0 and 4, 1 and 5, 2 and 6, 3 and 7 of 8
+            qf[n][2 * w][1] = __byte_perm(v.x, v.z, 0x7632);
+            qf[n][2 * w + 1][0] = __byte_perm(v.y, v.w, 0x5410);
+            qf[n][2 * w + 1][1] = __byte_perm(v.y, v.w, 0x7632);
+        }
+    }
+    const int see_all_from = window > 0 ? p0 + min(col0 + 8 * NT, cols) / G - window + 1 : 0;    // keys below may be hidden from a column,
+    const int see_all_to = p0 + col0 / G;                                                       // keys above as well
+
+    unsigned char* ring = smem + (size_t)warp * KD_STAGES * Tile::BYTES;
+    auto ask = [&](int i) {                                 // the warp's 16 keys of the run's i-th page
+        const int page = __shfl_sync(0xffffffffu, my_page, i & 31);
+        if (i < n_pages && page >= 0) {
+            unsigned char* dst = ring + (i % KD_STAGES) * Tile::BYTES;
+            const unsigned char* src = pool + ((size_t)page * Hkv + kvh) * kv4_page_bytes(HD) + warp * Tile::CODES;
+            constexpr int WORDS_AT = kv4_code_bytes(HD);
+#pragma unroll
+            for (int o = 0; o < Tile::CODES; o += 512) {
+                kd_copy16(dst + o + lane * 16, src + o + lane * 16);
+                kd_copy16(dst + Tile::HALF + o + lane * 16, src + kv4_half_bytes(HD) + o + lane * 16);
+            }
+            constexpr int PIECES = Tile::WORDS / 16;
+            if (lane < 2 * PIECES) {
+                const int half = lane / PIECES, at = (lane % PIECES) * 16;
+                kd_copy16(dst + half * Tile::HALF + Tile::CODES + at, src + half * kv4_half_bytes(HD) + WORDS_AT - warp * Tile::CODES + warp * Tile::WORDS + at);
+            }
+        }
+        asm volatile("cp.async.commit_group;" ::: "memory");
+    };
+
+    float o[NT][HD / 16][4], m[NT][2], l[NT][2];
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+#pragma unroll
+        for (int i = 0; i < HD / 16; ++i) o[n][i][0] = o[n][i][1] = o[n][i][2] = o[n][i][3] = 0.f;
+        m[n][0] = m[n][1] = -INFINITY;
+        l[n][0] = l[n][1] = 0.f;
+    }
+#pragma unroll
+    for (int i = 0; i < KD_STAGES - 1; ++i) ask(i);
+    // row r of a tile is key `key_r` of the 16, row r + 8 the key 8 behind it: of the keys that one load takes from shared memory then
+    // never two lie in the same banks
+    const int key_r = (r & 1) ? 4 + ((r >> 1) ^ 1) : r >> 1;
+    const int vk0 = c, vk1 = 4 + (c ^ 1);                   // a lane's four keys of a value tile: rows 2c, 2c + 1 and the ones 8 behind
+
+    for (int i = 0; i < n_pages; ++i) {
+        ask(i + KD_STAGES - 1);
+        asm volatile("cp.async.wait_group %0;" ::"n"(KD_STAGES - 1) : "memory");
+        __syncwarp();
+        const unsigned char* kt = ring + (i % KD_STAGES) * Tile::BYTES;
+        const unsigned char* vt = kt + Tile::HALF;
+        const uint16_t* kw = reinterpret_cast<const uint16_t*>(kt + Tile::CODES);
+        const uint16_t* vw = reinterpret_cast<const uint16_t*>(vt + Tile::CODES);
+        const int base = (first_page + i) * KV4_PAGE + warp * KD_KEYS;
+        const bool there = __shfl_sync(0xffffffffu, my_page, i) >= 0;
+        if (there && base < len) {
+            // S^T = K Q^T
+            float s[NT][4];
+#pragma unroll
+            for (int n = 0; n < NT; ++n) s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.f;
+            constexpr int LW = HD / 32;                     // 32-bit words of codes of a lane's numbers of a key
+            uint32_t ka[LW], kb[LW], za, sa, zb, sb;
+            {
+                const unsigned char* pa = kt + key_r * (HD / 2) + c * (HD / 8);
+                const unsigned char* pb = pa + 8 * (HD / 2);
+                if constexpr (LW == 4) {
+                    const uint4 va = *reinterpret_cast<const uint4*>(pa), vb = *reinterpret_cast<const uint4*>(pb);
+                    ka[0] = va.x; ka[1] = va.y; ka[2] = va.z; ka[3] = va.w;
+                    kb[0] = vb.x; kb[1] = vb.y; kb[2] = vb.z; kb[3] = vb.w;
+                } else {
+                    const uint2 va = *reinterpret_cast<const uint2*>(pa), vb = *reinterpret_cast<const uint2*>(pb);
+                    ka[0] = va.x; ka[1] = va.y;
+                    kb[0] = vb.x; kb[1] = vb.y;
+                }
+                const int g = c * (HD / 4) / KV4_GROUP;
+                const uint32_t wa = kw[key_r * (HD / KV4_GROUP) + g] * 0x10001u, wb = kw[(key_r + 8) * (HD / KV4_GROUP) + g] * 0x10001u;
+                za = (wa & 0x000f000fu) | 0x43004300u;
+                sa = wa & 0xfff0fff0u;
+                zb = (wb & 0x000f000fu) | 0x43004300u;
+                sb = wb & 0xfff0fff0u;
+            }
+#pragma unroll
+            for (int k = 0; k < HD / 16; ++k) {
+                const int sh = 8 * (k & 1);
+                const uint32_t a0 = kd_numbers(ka[k / 2] >> sh, za, sa), a1 = kd_numbers(kb[k / 2] >> sh, zb, sb);
+                const uint32_t a2 = kd_numbers(ka[k / 2] >> (sh + 4), za, sa), a3 = kd_numbers(kb[k / 2] >> (sh + 4), zb, sb);
+#pragma unroll
+                for (int n = 0; n < NT; ++n) kd_mma(s[n], a0, a1, a2, a3, qf[n][k][0], qf[n][k][1]);
+            }
+            const bool part_hidden = base + KD_KEYS - 1 > see_all_to || base < see_all_from;        // the same for the warp
+            uint32_t w0 = vw[vk0 * (HD / KV4_GROUP) + r * (HD / 8) / KV4_GROUP], w1 = vw[vk1 * (HD / KV4_GROUP) + r * (HD / 8) / KV4_GROUP];
+            uint32_t w2 = vw[(vk0 + 8) * (HD / KV4_GROUP) + r * (HD / 8) / KV4_GROUP], w3 = vw[(vk1 + 8) * (HD / KV4_GROUP) + r * (HD / 8) / KV4_GROUP];
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) s[n][e] *= scale_log2;
+            if (part_hidden) {
+                // a hidden key counts for nothing whatever it holds: its weight is 0, and a value that is not finite is taken as 0 here and
+                // gives those that see it a score of NaN instead
+                bool bad[2] = {false, false};
+#pragma unroll
+                for (int g = 0; g < HD / KV4_GROUP; ++g) {
+                    bad[0] |= kv4_is_nan(vw[key_r * (HD / KV4_GROUP) + g]);
+                    bad[1] |= kv4_is_nan(vw[(key_r + 8) * (HD / KV4_GROUP) + g]);
+                }
+#pragma unroll
+                for (int n = 0; n < NT; ++n)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const int key = base + key_r + (e >> 1) * 8;
+                        if (bad[e >> 1]) s[n][e] = __uint_as_float(0x7fffffffu);
+                        if (key > last_key[n][e & 1] || key < first_key[n][e & 1]) s[n][e] = -INFINITY;
+                    }
+                if (base + vk0 >= len || kv4_is_nan(w0)) w0 = 0;
+                if (base + vk1 >= len || kv4_is_nan(w1)) w1 = 0;
+                if (base + vk0 + 8 >= len || kv4_is_nan(w2)) w2 = 0;
+                if (base + vk1 + 8 >= len || kv4_is_nan(w3)) w3 = 0;
+            }
+            // P = 2^(S - reference)
+            bool over = false;
+#pragma unroll
+            for (int n = 0; n < NT; ++n) over |= fmaxf(s[n][0], s[n][2]) > m[n][0] + KD_RAISE || fmaxf(s[n][1], s[n][3]) > m[n][1] + KD_RAISE;
+            if (__any_sync(0xffffffffu, over)) {
+#pragma unroll
+                for (int n = 0; n < NT; ++n) {
+                    float f[2];
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        float top = fmaxf(s[n][e], s[n][e + 2]);
+                        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 4));
+                        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
+                        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
+                        const float up = fmaxf(m[n][e], top);
+                        f[e] = up == m[n][e] ? 1.f : exp2f(m[n][e] - up);
+                        m[n][e] = up;
+                        l[n][e] *= f[e];
+                    }
+#pragma unroll
+                    for (int k = 0; k < HD / 16; ++k) {
+                        o[n][k][0] *= f[0];
+                        o[n][k][1] *= f[1];
+                        o[n][k][2] *= f[0];
+                        o[n][k][3] *= f[1];
+                    }
+                }
+            }
+            uint32_t pb[NT][2];
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+                const float r0 = m[n][0] == -INFINITY ? 0.f : m[n][0], r1 = m[n][1] == -INFINITY ? 0.f : m[n][1];
+                const uint32_t lo = kd_pack(kd_exp2(s[n][0] - r0), kd_exp2(s[n][1] - r1)), hi = kd_pack(kd_exp2(s[n][2] - r0), kd_exp2(s[n][3] - r1));
+                // the sum of the weights as they are rounded for the product
+                l[n][0] += __uint_as_float(lo << 16) + __uint_as_float(hi << 16);
+                l[n][1] += __uint_as_float(lo & 0xffff0000u) + __uint_as_float(hi & 0xffff0000u);
+                pb[n][0] = kd_transpose(lo);
+                pb[n][1] = kd_transpose(hi);
+            }
+            // O^T += V^T P^T
+            const uint32_t w01 = __byte_perm(w0, w1, 0x5410), w23 = __byte_perm(w2, w3, 0x5410);
+            const uint32_t z01 = (w01 & 0x000f000fu) | 0x43004300u, s01 = w01 & 0xfff0fff0u;
+            const uint32_t z23 = (w23 & 0x000f000fu) | 0x43004300u, s23 = w23 & 0xfff0fff0u;
+            constexpr int VW = HD / 64;                     // words of codes of a lane's numbers of a value
+            uint32_t v0[VW], v1[VW], v2[VW], v3[VW];
+            const unsigned char* pv = vt + r * (HD / 16);
+            if constexpr (VW == 2) {
+                const uint2 x0 = *reinterpret_cast<const uint2*>(pv + vk0 * (HD / 2)), x1 = *reinterpret_cast<const uint2*>(pv + vk1 * (HD / 2));
+                const uint2 x2 = *reinterpret_cast<const uint2*>(pv + (vk0 + 8) * (HD / 2)), x3 = *reinterpret_cast<const uint2*>(pv + (vk1 + 8) * (HD / 2));
+                v0[0] = x0.x; v0[1] = x0.y; v1[0] = x1.x; v1[1] = x1.y; v2[0] = x2.x; v2[1] = x2.y; v3[0] = x3.x; v3[1] = x3.y;
+            } else {
+                v0[0] = *reinterpret_cast<const uint32_t*>(pv + vk0 * (HD / 2));
+                v1[0] = *reinterpret_cast<const uint32_t*>(pv + vk1 * (HD / 2));
+                v2[0] = *reinterpret_cast<const uint32_t*>(pv + (vk0 + 8) * (HD / 2));
+                v3[0] = *reinterpret_cast<const uint32_t*>(pv + (vk1 + 8) * (HD / 2));
+            }
+#pragma unroll
+            for (int w = 0; w < VW; ++w) {
+                const uint32_t lo01 = __byte_perm(v0[w], v1[w], 0x5410), hi01 = __byte_perm(v0[w], v1[w], 0x7632);
+                const uint32_t lo23 = __byte_perm(v2[w], v3[w], 0x5410), hi23 = __byte_perm(v2[w], v3[w], 0x7632);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const uint32_t a0 = kd_numbers(lo01 >> (4 * j), z01, s01), a1 = kd_numbers(hi01 >> (4 * j), z01, s01);
+                    const uint32_t a2 = kd_numbers(lo23 >> (4 * j), z23, s23), a3 = kd_numbers(hi23 >> (4 * j), z23, s23);
+#pragma unroll
+                    for (int n = 0; n < NT; ++n) kd_mma(o[n][4 * w + j], a0, a1, a2, a3, pb[n][0], pb[n][1]);
+                }
+            }
+        }
+        __syncwarp();                                       // the slot is asked for again
+    }
+    asm volatile("cp.async.wait_all;" ::: "memory");
+    __syncthreads();                                        // the ring's memory holds the warps' results from here on
+
+    // outputs of a column in the order [mma][upper or lower 8 rows][row]: number row * HD / 8 + 8 (mma / 4) + 4 half + mma % 4
+    float* join_o = reinterpret_cast<float*>(smem);
+    float* join_ml = join_o + KD_WARPS * 8 * NT * Smem::COL;
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+            float sum = l[n][e];
+            sum += __shfl_xor_sync(0xffffffffu, sum, 4);
+            sum += __shfl_xor_sync(0xffffffffu, sum, 8);
+            sum += __shfl_xor_sync(0xffffffffu, sum, 16);
+            const int col = n * 8 + 2 * c + e;
+            float* dst = join_o + (warp * 8 * NT + col) * Smem::COL + r;
+#pragma unroll
+            for (int k = 0; k < HD / 16; ++k) {
+                dst[16 * k] = o[n][k][e];
+                dst[16 * k + 8] = o[n][k][e + 2];
+            }
+            if (r == 0) {
+                join_ml[(warp * 8 * NT + col) * 2] = m[n][e];
+                join_ml[(warp * 8 * NT + col) * 2 + 1] = sum;
+            }
+        }
+    }
+    __syncthreads();
+    for (int x = threadIdx.x; x < 8 * NT * HD; x += KD_WARPS * 32) {
+        const int col = x / HD, at = x % HD;
+        if (col0 + col >= cols) break;
+        float top = -INFINITY, total = 0.f, y = 0.f;
+#pragma unroll
+        for (int w = 0; w < KD_WARPS; ++w) top = fmaxf(top, join_ml[(w * 8 * NT + col) * 2]);
+#pragma unroll
+        for (int w = 0; w < KD_WARPS; ++w) {
+            const float mw = join_ml[(w * 8 * NT + col) * 2], lw = join_ml[(w * 8 * NT + col) * 2 + 1];
+            if (lw != 0.f) {
+                const float f = mw == top ? 1.f : exp2f(mw - top);
+                total += f * lw;
+                y += f * join_o[(w * 8 * NT + col) * Smem::COL + at];
+            }
+        }
+        const int t = t0 + (col0 + col) / G, h = kvh * G + (col0 + col) % G;
+        const size_t row = (size_t)t * Hq + h;
+        if (runs <= 1) {
+            const int mma = at / 16, half = (at >> 3) & 1, d = (at & 7) * (HD / 8) + 8 * (mma >> 2) + 4 * half + (mma & 3);
+            out[row * HD + d] = from_f32<bf16>(total == 0.f ? 0.f : y / total);
+        } else {
+            part_o[(row * max_runs + run) * HD + at] = y;
+            if (at == 0) {
+                part_ml[(row * max_runs + run) * 2] = top;
+                part_ml[(row * max_runs + run) * 2 + 1] = total;
+            }
+        }
+    }
+}
+
+// Joins the runs of a row (a warp each).
+template <int HD>
+__global__ void __launch_bounds__(128)
+kv4_attn_join_kernel(const float* __restrict__ part_o, const float* __restrict__ part_ml, const int* __restrict__ cu_seqlens,
+                     const int* __restrict__ pos0, const int* __restrict__ tok_seq, bf16* __restrict__ out, int rows, int B, int Hq, int table_width,
+                     int window, int max_runs) {
+    pdl_wait();
+    pdl_launch_dependents();
+    const int lane = threadIdx.x & 31, row = blockIdx.x * 4 + (threadIdx.x >> 5);
+    if (row >= rows) return;
+    const int b = tok_seq[row / Hq];
+    if (b < 0 || b >= B) return;
+    const int p0 = pos0[b], len = p0 + min(cu_seqlens[b + 1], rows / Hq) - cu_seqlens[b];
+    const int runs = min(kv4_runs(p0, len, window, table_width).runs, max_runs);
+    if (runs <= 1) return;
+    const float* ml = part_ml + (size_t)row * max_runs * 2;
+    float top = -INFINITY;
+    for (int i = lane; i < runs; i += 32) top = fmaxf(top, ml[2 * i]);
+    top = warp_max(top);
+    constexpr int E = HD / 32;
+    float y[E] = {}, total = 0.f;
+    for (int i = 0; i < runs; ++i) {
+        const float lw = ml[2 * i + 1];
+        if (lw == 0.f) continue;
+        const float mw = ml[2 * i], f = mw == top ? 1.f : exp2f(mw - top);
+        total += f * lw;
+        const float* src = part_o + ((size_t)row * max_runs + i) * HD;
+#pragma unroll
+        for (int e = 0; e < E; ++e) y[e] += f * src[e * 32 + lane];
+    }
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+        const int at = e * 32 + lane, mma = at / 16, half = (at >> 3) & 1, d = (at & 7) * (HD / 8) + 8 * (mma >> 2) + 4 * half + (mma & 3);
+        out[(size_t)row * HD + d] = from_f32<bf16>(total == 0.f ? 0.f : y[e] / total);
+    }
+}
+
+// The most runs of a sequence of up to max_len tokens of which it brings up to max_new.
+extern "C" int qwb_kv4_max_runs(int max_len, int max_new, int window, int table_width) {
+    long long pages = ((long long)max_len + KV4_PAGE - 1) / KV4_PAGE;
+    if (window > 0 && ((long long)window + max_new) / KV4_PAGE + 2 < pages) pages = ((long long)window + max_new) / KV4_PAGE + 2;
+    if (pages > table_width) pages = table_width;
+    if (pages <= KD_RUNS) return pages < 1 ? 1 : (int)pages;
+    const long long even = (pages + KD_RUN_PAGES - 1) / KD_RUN_PAGES;
+    return (int)(even > KD_RUNS ? even : KD_RUNS);
+}
+
+template <int HD, int NT>
+static int kv4_launch_rows(const bf16* q, const unsigned char* pool, const int* page_table, const int* cu, const int* pos0, const int* tok_seq, bf16* out,
+                           float* scratch, int T, int B, int pool_pages, int max_new, int Hq, int Hkv, int table_width, float scale, int window, int max_runs,
+                           cudaStream_t stream) {
+    using Smem = KdSmem<HD, NT>;
+    auto kernel = kv4_attn_rows_kernel<HD, NT>;
+    static_assert(Smem::BYTES <= 48 * 1024, "more needs an attribute of the kernel");
+    const long long tiles = ((long long)max_new * (Hq / Hkv) + 8 * NT - 1) / (8 * NT);
+    if (tiles * max_runs > 2147483647ll || Hkv > 65535 || B > 65535)
+        return qwb_fail(QWB_ERR_ARG, "kv4_attention: %d sequences of up to %d new tokens, %d heads: too many blocks", B, max_new, Hkv);
+    const long long rows = (long long)T * Hq;
+    if (rows > 2147483647ll) return qwb_fail(QWB_ERR_ARG, "kv4_attention: %lld rows of queries", rows);
+    float* part_ml = scratch ? scratch + (size_t)rows * max_runs * HD : nullptr;
+    qwb_launch(kernel, dim3((unsigned)(tiles * max_runs), Hkv, B), KD_WARPS * 32, Smem::BYTES, stream, q, pool, page_table, cu, pos0, out, scratch, part_ml, T, B,
+               pool_pages, Hq, Hkv, table_width, scale * 1.4426950408889634f, window, (int)tiles, max_runs);
+    if (max_runs > 1)
+        qwb_launch(kv4_attn_join_kernel<HD>, dim3((unsigned)((rows + 3) / 4)), 128, 0, stream, scratch, part_ml, cu, pos0, tok_seq, out, (int)rows, B, Hq, table_width,
+                   window, max_runs);
+    return qwb_check_launch("kv4_attention");
+}
+
+// scratch: T * Hq * max_runs * (hd + 2) floats where max_runs (qwb_kv4_max_runs) is above 1
+extern "C" int qwb_kv4_attn_rows(const void* q, const unsigned char* pool, const int* page_table, const int* cu, const int* pos0, const int* tok_seq,
+                                 void* out, float* scratch, int T, int B, int pool_pages, int max_new, int Hq, int Hkv, int hd, int table_width, float scale,
+                                 int window, int max_runs, cudaStream_t stream) {
+    if (T <= 0) return 0;
+    if (Hkv <= 0 || Hq <= 0 || Hq % Hkv || (hd != 64 && hd != 128) || table_width <= 0 || window < 0 || max_new <= 0 || max_runs <= 0 || B <= 0)
+        return qwb_fail(QWB_ERR_ARG, "kv4_attention: heads of 64 or 128 only: Hq=%d Hkv=%d hd=%d width=%d window=%d", Hq, Hkv, hd, table_width, window);
+    if (max_runs > 1 && !scratch) return qwb_fail(QWB_ERR_ARG, "kv4_attention: no scratch for %d runs", max_runs);
+    if ((uintptr_t)q % 16 || (uintptr_t)pool % 16) return qwb_fail(QWB_ERR_ARG, "kv4_attention: q and the pool must start at a multiple of 16 bytes");
+    const bool two = (long long)max_new * (Hq / Hkv) > 8;
+#define KV4_ROWS(HD, NT) kv4_launch_rows<HD, NT>((const bf16*)q, pool, page_table, cu, pos0, tok_seq, (bf16*)out, scratch, T, B, pool_pages, max_new, Hq, Hkv, \
+                                                 table_width, scale, window, max_runs, stream)
+    if (hd == 128) return two ? KV4_ROWS(128, 2) : KV4_ROWS(128, 1);
+    return two ? KV4_ROWS(64, 2) : KV4_ROWS(64, 1);
+#undef KV4_ROWS
 }

@@ -129,15 +129,22 @@ extern "C" int qwb_kv4_store(const float* qkv, const float* q_weight, const floa
 // sequence's last token are zeros.  A block takes a (page, head), a thread 8 numbers at a time (one 32-bit word of codes).
 // `marked`: a token one of whose values is not finite has values of zero and keys of NaN here, so that a kernel that multiplies
 // what a query does not see by 0 gives NaN to the queries that see it only.
-// Blocks of the first head also write the table that names these pages: [B, width], page_start[b] + j.
+// Blocks of the first head also write the table that names these pages: [B, width], page_start[b] + j; and with `rows_out` the blocks
+// set rows of `row_bytes` (a multiple of 16) behind row `rows_used` of `rows` there to zero (what no sequence of a padded step writes).
 template <typename T>
 __global__ void __launch_bounds__(256)
 kv4_read_kernel(const unsigned char* __restrict__ pool, const int* __restrict__ pages, const int* __restrict__ page_start,
                 const int* __restrict__ seq_len, T* __restrict__ k_out, T* __restrict__ v_out, int* __restrict__ table, int P, int B,
-                int width, int pool_pages, int Hkv, int hd, int marked) {
+                int width, int pool_pages, int Hkv, int hd, int marked, uint4* __restrict__ rows_out, const int* __restrict__ rows_used,
+                int rows, int row_bytes) {
     pdl_wait();
     pdl_launch_dependents();
     const int entry = blockIdx.x, head = blockIdx.y;
+    if (rows_out) {
+        const long long end = (long long)rows * (row_bytes / 16), step = (long long)gridDim.x * gridDim.y * blockDim.x;
+        for (long long i = (long long)max(*rows_used, 0) * (row_bytes / 16) + ((long long)head * gridDim.x + entry) * blockDim.x + threadIdx.x; i < end; i += step)
+            rows_out[i] = make_uint4(0, 0, 0, 0);
+    }
     // the sequence that holds this entry: the last one that begins at or before it
     int lo = 0, hi = B;
     while (hi - lo > 1) {
@@ -189,18 +196,20 @@ kv4_read_kernel(const unsigned char* __restrict__ pool, const int* __restrict__ 
 
 extern "C" int qwb_kv4_read(const unsigned char* pool, const int* pages, const int* page_start, const int* seq_len, void* k_out,
                             void* v_out, int dtype, int* table, int P, int B, int width, int pool_pages, int Hkv, int hd,
-                            int marked, cudaStream_t stream) {
+                            int marked, void* rows_out, const int* rows_used, int rows, int row_bytes, cudaStream_t stream) {
     if (P <= 0) return 0;
     if (B <= 0 || width <= 0 || Hkv <= 0 || Hkv > 65535 || hd <= 0 || hd % KV4_GROUP || hd > KV4_MAX_DIM || pool_pages <= 0)
         return qwb_fail(QWB_ERR_ARG, "kv4_read: bad sizes B=%d width=%d Hkv=%d hd=%d pages=%d", B, width, Hkv, hd, pool_pages);
     if ((uintptr_t)pool % 16 || (uintptr_t)k_out % 16 || (uintptr_t)v_out % 16)
         return qwb_fail(QWB_ERR_ARG, "kv4_read: pool and outputs must start at a multiple of 16 bytes");
+    if (rows_out && ((uintptr_t)rows_out % 16 || row_bytes % 16 || !rows_used))
+        return qwb_fail(QWB_ERR_ARG, "kv4_read: rows of %d bytes", row_bytes);
     if (dtype == QWB_DT_F32)
         qwb_launch(kv4_read_kernel<float>, dim3(P, Hkv), 256, 0, stream, pool, pages, page_start, seq_len, (float*)k_out, (float*)v_out, table, P, B,
-                   width, pool_pages, Hkv, hd, marked);
+                   width, pool_pages, Hkv, hd, marked, (uint4*)rows_out, rows_used, rows, row_bytes);
     else if (dtype == QWB_DT_BF16)
         qwb_launch(kv4_read_kernel<bf16>, dim3(P, Hkv), 256, 0, stream, pool, pages, page_start, seq_len, (bf16*)k_out, (bf16*)v_out, table, P, B,
-                   width, pool_pages, Hkv, hd, marked);
+                   width, pool_pages, Hkv, hd, marked, (uint4*)rows_out, rows_used, rows, row_bytes);
     else
         return qwb_fail(QWB_ERR_ARG, "kv4_read: unknown dtype %d", dtype);
     return qwb_check_launch("kv4_read");

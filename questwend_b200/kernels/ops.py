@@ -2190,11 +2190,12 @@ def kv4_store(qkv: torch.Tensor, q_weight, k_weight, cos, sin, slot_map: torch.T
 
 
 def kv4_read(pool: torch.Tensor, pages: torch.Tensor, page_start: torch.Tensor, seq_len: torch.Tensor, max_len: int, head_dim: int,
-             dtype: torch.dtype, marked: bool = False) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+             dtype: torch.dtype, marked: bool = False, rest: tuple | None = None) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
     """What the 4-bit cache holds for a step's sequences, as plain pages: keys and values [P, Hkv, 64, hd] in ``dtype`` of the P
     entries of ``pages`` (``StepTables``), zeros behind a sequence's last token, and the page table [B, pages of ``max_len``] that names
     them (0 where a sequence has no page).  Both types hold the numbers exactly.  ``marked``: a token with a value that is not finite has
-    values of 0 and keys of NaN instead (what a kernel needs that multiplies unseen values by 0)."""
+    values of 0 and keys of NaN instead (what a kernel needs that multiplies unseen values by 0).  ``rest`` (rows [n, bytes a multiple of
+    16], one int32 on the device): the rows from that number on are set to zero."""
     _kv4_pool("kv4_read", pool, head_dim)
     for name, t in (("pages", pages), ("page_start", page_start), ("seq_len", seq_len)):
         _need(t, name, torch.int32, 1)
@@ -2202,20 +2203,33 @@ def kv4_read(pool: torch.Tensor, pages: torch.Tensor, page_start: torch.Tensor, 
     if B < 1 or page_start.numel() != B + 1 or max_len < 1:
         raise KernelError(f"kv4_read: {page_start.numel()} page starts for {B} sequences of up to {max_len} tokens")
     _here("kv4_read", pool, pages, page_start, seq_len)
+    rows, used = rest if rest is not None else (None, None)
+    if rest is not None:
+        _need(rows, "rest", ndim=2)
+        _need(used, "rest", torch.int32)
+        _here("kv4_read", rows, used)
     width = -(-max_len // PAGE_SIZE)
     k = _empty((P, Hkv, PAGE_SIZE, head_dim), dtype=dtype, device=pool.device)
     v = _empty((P, Hkv, PAGE_SIZE, head_dim), dtype=dtype, device=pool.device)
     table = torch.zeros((B, width), dtype=torch.int32, device=pool.device)
     _call("kv4_cache", "qwb_kv4_read", _ptr(pool), _ptr(pages), _ptr(page_start), _ptr(seq_len), _ptr(k), _ptr(v), _i(_dt(dtype)), _ptr(table),
-          _i(P), _i(B), _i(width), _i(pool.shape[0]), _i(Hkv), _i(head_dim), _i(1 if marked else 0), _stream())
+          _i(P), _i(B), _i(width), _i(pool.shape[0]), _i(Hkv), _i(head_dim), _i(1 if marked else 0), _ptr(rows), _ptr(used),
+          _i(0 if rows is None else rows.shape[0]), _i(0 if rows is None else rows.shape[1] * rows.element_size()), _stream())
     return k, v, table
+
+
+KV4_ROWS_MAX_COLUMNS = 64       # new tokens of a sequence times query heads of a group up to which a prompt's pieces go as rows
 
 
 def kv4_attention(q: torch.Tensor, pool: torch.Tensor, tables: StepTables, max_new: int, max_len: int, scale: float, window: int = 0,
                   impl: str = "auto") -> torch.Tensor:
     """Causal attention of a step's tokens over the cache in 4 bits (their own rows written before).  ``q`` [T, Hq, hd] float32
     or bfloat16; ``max_new`` and ``max_len`` bound what a sequence brings and holds; with ``window`` > 0 a query sees the last ``window``
-    keys, its own among them.  Returns [T, Hq * hd] in q's type, zeros for a token of no sequence.  ``impl``: "auto" or "plain"."""
+    keys, its own among them.  Returns [T, Hq * hd] in q's type, zeros for a token of no sequence.
+
+    ``impl``: "rows" (bfloat16, heads of 64 or 128: codes to tensor-core fragments, a sequence's keys cut into runs; for few new tokens), "read"
+    (the same sizes, groups of up to 64 heads, ``tables.pages`` given: the step's pages as bfloat16 once, then the tcgen05 prompt kernel), "plain"
+    (every size and type), or "auto": the fastest that takes the case."""
     _need(q, "q", ndim=3)
     T, Hq, hd = q.shape
     _kv4_pool("kv4_attention", pool, hd)
@@ -2231,10 +2245,31 @@ def kv4_attention(q: torch.Tensor, pool: torch.Tensor, tables: StepTables, max_n
         raise KernelError(f"kv4_attention: up to {max_new} new tokens of sequences of up to {max_len}, window {window}, a page table of "
                           f"{table.shape[1]} columns")
     max_len = min(max_len, table.shape[1] * PAGE_SIZE)
-    if impl not in ("auto", "plain"):
+    if impl not in ("auto", "plain", "rows", "read"):
         raise KernelError(f"kv4_attention: unknown form '{impl}'")
     _here("kv4_attention", q, pool, table, tok_seq, tok_pos, cu, pos0)
+    group = Hq // Hkv
+    fits = q.dtype == torch.bfloat16 and hd in (64, 128)
+    reads = fits and group <= 64 and tables.pages is not None and tables.page_start is not None
+    if impl == "auto":
+        impl = "plain" if not fits else "read" if reads and max_new * group > KV4_ROWS_MAX_COLUMNS else "rows"
+    if (impl == "rows" and not fits) or (impl == "read" and not reads):
+        raise KernelError(f"kv4_attention: form '{impl}' does not take {q.dtype} queries of {hd}, groups of {group}"
+                          f"{'' if reads else ' (or has no list of pages)'}")
     out = _empty((T, Hq * hd), dtype=q.dtype, device=q.device)
+    if impl == "rows":
+        max_runs = _lookup("attention_kv4", "qwb_kv4_max_runs")[1](max_len, max_new, window, table.shape[1])
+        scratch = _empty((T * Hq * max_runs * (hd + 2),), dtype=torch.float32, device=q.device) if max_runs > 1 else None
+        _call("attention_kv4", "qwb_kv4_attn_rows", _ptr(q), _ptr(pool), _ptr(table), _ptr(cu), _ptr(pos0), _ptr(tok_seq), _ptr(out), _ptr(scratch), _i(T),
+              _i(B), _i(pool.shape[0]), _i(max_new), _i(Hq), _i(Hkv), _i(hd), _i(table.shape[1]), _f(scale), _i(window), _i(max_runs), _stream(),
+              kernels=2 if max_runs > 1 else 1)
+        return out
+    if impl == "read":
+        k, v, compact = kv4_read(pool, tables.pages, tables.page_start, tables.seq_len, max_len, hd, q.dtype, marked=True, rest=(out, cu[B:]))
+        _call("attention_tc", "qwb_attn_tc_prefill", _ptr(q), _ptr(k), _ptr(v), _ptr(compact), _ptr(cu), _ptr(pos0), _ptr(out), _i(B), _i(T), _i(max_new),
+              _i(k.shape[0]), _i(Hq), _i(Hkv), _i(hd), _i(hd), _i(PAGE_SIZE), _i(compact.shape[1]), _f(scale), _i(window), _i(0), _ptr(None), _ptr(None),
+              _ptr(gemm_tc_error_word(q.device)), _stream())
+        return out
     _call("attention_kv4", "qwb_kv4_attn_plain", _ptr(q), _ptr(pool), _ptr(table), _ptr(tok_seq), _ptr(tok_pos), _ptr(out), _i(_dt(q.dtype)), _i(T),
           _i(B), _i(pool.shape[0]), _i(Hq), _i(Hkv), _i(hd), _i(table.shape[1]), _f(scale), _i(window), _stream())
     return out

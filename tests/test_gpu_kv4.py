@@ -200,18 +200,25 @@ def tolerance(dtype, hd, mass, big, out, n_keys):
     return (u + 2.0 ** -21 + 2 * (hd + 2) * 2.0 ** -23 * big + n_keys * 2.0 ** -23) * mass + (u + 2.0 ** -23) * np.abs(out) + n_keys * 2.0 ** -122
 
 
-def _check(pool, tables, seqs, q, pos0, n_new, max_len, scale, window, impl="auto", **kw):
-    got = ops.kv4_attention(q, pool, tables, max(n_new), max_len, scale, window=window, impl=impl, **kw)
-    assert got.dtype == q.dtype and tuple(got.shape) == (q.shape[0], q.shape[1] * q.shape[2])
-    got, t = f64(got).reshape(q.shape), 0
-    qd = f64(q)
+def forms(q):
+    return ["auto", "plain", "rows", "read"] if q.dtype == BF and q.shape[2] in (64, 128) else ["auto"]
+
+
+def _check(pool, tables, seqs, q, pos0, n_new, max_len, scale, window):
+    qd, t, want = f64(q), 0, []
     for b, n in enumerate(n_new):
-        out, mass, big = pk.attention(qd[t:t + n], *seqs[b], [pos0[b] + i for i in range(n)], scale, window)
-        lim = tolerance(q.dtype, q.shape[2], mass, big, out, min(pos0[b] + n, window or 1 << 30))
-        bad = np.abs(got[t:t + n] - out) > lim
-        assert not bad.any(), (b, np.abs(got[t:t + n] - out).max(), (np.abs(got[t:t + n] - out) / np.maximum(lim, 1e-30)).max(), np.argwhere(bad)[:5])
+        want.append((t, n, *pk.attention(qd[t:t + n], *seqs[b], [pos0[b] + i for i in range(n)], scale, window)))
         t += n
-    assert (got[t:] == 0).all()
+    for impl in forms(q):
+        got = ops.kv4_attention(q, pool, tables, max(n_new), max_len, scale, window=window, impl=impl)
+        assert got.dtype == q.dtype and tuple(got.shape) == (q.shape[0], q.shape[1] * q.shape[2])
+        got = f64(got).reshape(q.shape)
+        for b, (at, n, out, mass, big) in enumerate(want):
+            lim = tolerance(q.dtype, q.shape[2], mass, big, out, min(pos0[b] + n, window or 1 << 30))
+            bad = ~(np.abs(got[at:at + n] - out) <= lim)
+            assert not bad.any(), (impl, b, np.abs(got[at:at + n] - out).max(), (np.abs(got[at:at + n] - out) / np.maximum(lim, 1e-30)).max(),
+                                   np.argwhere(bad)[:5].tolist())
+        assert (got[t:] == 0).all(), impl
 
 
 SIZES = [(4, 1, 128), (8, 2, 64), (3, 3, 128), (2, 1, 64), (16, 2, 128), (10, 2, 128), (12, 1, 64), (32, 1, 128)]
@@ -284,17 +291,18 @@ def test_a_token_that_is_not_finite_reaches_those_that_see_it_only(dtype, n_new)
     pool, order, start, seqs, rng = _cache(7, [L], 2, hd)
     t = _tables(order, start, [L - n_new], [n_new])
     q = torch.from_numpy(rng.standard_normal((n_new, 4, hd))).to(dtype).to(DEV)
-    clean = ops.kv4_attention(q, pool, t, n_new, L, 0.1).view(n_new, 4, hd)
+    clean = {f: ops.kv4_attention(q, pool, t, n_new, L, 0.1, impl=f).view(n_new, 4, hd) for f in forms(q)}
     at = L - 2
     page, row = order[at // 64], at % 64
     for part in (0, 1):                                  # a key's word, a value's word, of head 1
         broken = pool.clone()
         word = part * 64 * (hd // 2 + hd // 16) + 64 * hd // 2 + row * (hd // 16)
         broken[page, 1, word:word + 2] = torch.tensor([0xC0, 0x7F], dtype=torch.uint8, device=DEV)
-        got = ops.kv4_attention(q, broken, t, n_new, L, 0.1).view(n_new, 4, hd)
-        assert torch.equal(got[:, :2], clean[:, :2])                                     # the other head's queries
-        assert torch.equal(got[:-2, 2:], clean[:-2, 2:])                                 # tokens before it
-        assert got[-2:, 2:, :32].isnan().all()
+        for f in forms(q):
+            got = ops.kv4_attention(q, broken, t, n_new, L, 0.1, impl=f).view(n_new, 4, hd)
+            assert torch.equal(got[:, :2], clean[f][:, :2]), f                            # the other head's queries
+            assert torch.equal(got[:-2, 2:], clean[f][:-2, 2:]), f                        # tokens before it
+            assert got[-2:, 2:, :32].isnan().all(), f
 
 
 def test_attention_does_not_depend_on_the_batch():
@@ -309,12 +317,56 @@ def test_attention_does_not_depend_on_the_batch():
         assert torch.equal(whole[b:b + 1], alone)
 
 
+@pytest.mark.parametrize("impl", ["plain", "rows"])
+def test_lengths_beyond_what_was_said_are_cut_off(impl):
+    """More tokens on the device than ``max_len``, or than the page table holds, pages that the pool does not have: what is not there is not
+    seen, and nothing beyond the scratch is written."""
+    pool, order, start, seqs, rng = _cache(11, [900], 1, 128)
+    q = torch.from_numpy(rng.standard_normal((1, 4, 128))).to(BF).to(DEV)
+    t = _tables(order, start, [899], [1])
+    whole = ops.kv4_attention(q, pool, t, 1, 900, 0.1, impl=impl)
+    assert ops.kv4_attention(q, pool, t, 1, 64, 0.1, impl=impl).isfinite().all()
+    narrow = t._replace(page_table=t.page_table[:, :3].contiguous())
+    first = ops.kv4_attention(q, pool, narrow, 1, 900, 0.1, impl=impl)
+    ref = pk.attention(f64(q), *(x[:192] for x in seqs[0]), [191], 0.1)
+    assert (np.abs(f64(first).reshape(1, 4, 128) - ref[0]) <= tolerance(BF, 128, ref[1], ref[2], ref[0], 192)).all()
+    wrong = t.page_table.clone()
+    wrong[0, 3:] = pool.shape[0]
+    wrong[0, 4] = -5
+    gone = ops.kv4_attention(q, pool, t._replace(page_table=wrong), 1, 900, 0.1, impl=impl)
+    assert (f64(gone).reshape(1, 4, 128) - ref[0] <= tolerance(BF, 128, ref[1], ref[2], ref[0], 192)).all()
+    assert torch.equal(whole, ops.kv4_attention(q, pool, t, 1, 900, 0.1, impl=impl))
+
+
+def test_a_replayed_graph_and_another_stream():
+    lens = [500, 130]
+    pool, order, start, seqs, rng = _cache(12, lens, 2, 128)
+    q = torch.from_numpy(rng.standard_normal((2, 8, 128))).to(BF).to(DEV)
+    pos0, starts, pages = ints([300, 100]), ints(start), ints(order)
+    want = [ops.kv4_attention(q, pool, ops.step_tables(pages, starts, p, ints([1, 1]), 2, 8), 1, 512, 0.1) for p in (pos0, pos0 + 29)]
+    ones = ints([1, 1])
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        assert torch.equal(ops.kv4_attention(q, pool, ops.step_tables(pages, starts, pos0, ones, 2, 8), 1, 512, 0.1), want[0])
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = ops.kv4_attention(q, pool, ops.step_tables(pages, starts, pos0, ones, 2, 8)._replace(pages=None), 1, 512, 0.1)
+    graph.replay()
+    assert torch.equal(out, want[0])
+    pos0 += 29
+    graph.replay()
+    assert torch.equal(out, want[1])
+
+
 def test_attention_refusals():
     pool, order, start, _, _ = _cache(1, [70], 2, 64)
     t = _tables(order, start, [69], [1])
     q = torch.zeros(1, 4, 64, device=DEV)
     for args, kw in [((q, pool, t, 0, 70, 1.0), {}), ((q, pool, t, 1, 0, 1.0), {}), ((q, pool, t, 1, 70, 1.0), {"window": -1}),
-                     ((q, pool, t, 1, 70, 1.0), {"impl": "none"}), ((torch.zeros(1, 3, 64, device=DEV), pool, t, 1, 70, 1.0), {}),
+                     ((q, pool, t, 1, 70, 1.0), {"impl": "none"}), ((q, pool, t, 1, 70, 1.0), {"impl": "rows"}), ((q, pool, t, 1, 70, 1.0), {"impl": "read"}),
+                     ((q.bfloat16(), pool, t._replace(pages=None), 1, 70, 1.0), {"impl": "read"}), ((torch.zeros(1, 3, 64, device=DEV), pool, t, 1, 70, 1.0), {}),
                      ((torch.zeros(2, 4, 64, device=DEV), pool, t, 1, 70, 1.0), {}), ((torch.zeros(1, 4, 128, device=DEV), pool, t, 1, 70, 1.0), {}),
                      ((q, pool.clone().view(-1)[:9216].view(2, 1, 4608), t._replace(pos0=ints([1, 2])), 1, 70, 1.0), {})]:
         with pytest.raises(KernelError, match="kv4"):
