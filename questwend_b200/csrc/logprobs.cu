@@ -3,17 +3,26 @@
 //
 //     lp(t) = x_t - m - ln S,   S = sum exp(x - m),   H = ln S - U / S,   U = sum exp(x - m) (x - m),   m = max x
 //
-// A block takes a segment of a row, LP_SEG logits, and holds it in registers: the segment's maximum, sums and largest logits come
-// from there, and memory is read once.  A segment leaves (m, S, U) and its `top` largest as a sorted list; a second kernel joins a
-// row's segments (sums relative to the largest m, lists by merging).  Segments are cut by the row alone, so a row's result
-// does not depend on how many rows there are.
+// A block takes a segment of a row, LP_SEG logits, a thread 64 of them in pieces of 16 with the next piece's loads on their way;
+// it keeps a reference (a largest logit so far, or up to 8 below it), S and U relative to that, and its largest logit.  Logits are
+// bounded by memory as long as a logit costs few instructions: maximum, difference, exp2 of a product, two sums are 7.
+// A segment leaves (m, S, U) and each thread's largest logit, a 64th of what it read; a second kernel joins a row's sums and finds its
+// `top` largest from these maxima, with a look at the few threads' logits that can be among them.  (A sorted list from every
+// segment, found in its block while the others wait at the memory, took 407 us for 2,048 rows of 151,936 logits and a top of 20, where
+// the sums alone take 183.)  Segments are cut by the row alone, so a row's result does not depend on how many rows there are.
 // Of equal logits the one with the lower id is larger.  A NaN is no candidate for the list and makes the row's numbers NaN.
 #include "common.cuh"
 
+#include <limits.h>
+
 #define LP_THREADS 256
-#define LP_PER_THREAD 32
+#define LP_PIECE 16             // logits of a thread at a time
+#define LP_PER_THREAD 64
 #define LP_SEG (LP_THREADS * LP_PER_THREAD)
 #define LP_MAX_TOP 64
+#define LP_LINK_ROWS 16         // up to so many rows the joining kernel starts under the tail of the one before it
+#define LP_HELD 8              // maxima of a thread of the joining kernel that it keeps in registers: 131,072 logits' worth
+#define LP_GATHER 1024          // candidates of a row that shared memory holds
 
 // Larger logits first, of equal ones the lower id (id < 0: nothing).
 __device__ __forceinline__ bool lp_before(float a, int ia, float b, int ib) { return ib < 0 ? ia >= 0 : (ia >= 0 && (a > b || (a == b && ia < ib))); }
@@ -27,133 +36,256 @@ __device__ __forceinline__ void lp_warp_best(float& v, int& i) {
     }
 }
 
-__global__ void __launch_bounds__(LP_THREADS)
-lp_segments_kernel(const float* __restrict__ logits, float* __restrict__ sums, float* __restrict__ best, int* __restrict__ best_id, int V,
-                   int segs, int top) {
+// Numbers in their order as whole ones (-0 and 0 are one; no NaN).
+__device__ __forceinline__ int lp_key(float x) {
+    const int b = __float_as_int(x + 0.f);
+    return b < 0 ? b ^ 0x7fffffff : b;
+}
+
+// VEC: rows begin at a multiple of 16 bytes and hold a multiple of 4 logits.  A thread then holds 4 neighbouring logits of every 1,024.
+template <bool VEC>
+__device__ __forceinline__ int lp_index(int e, int tid) { return VEC ? (e >> 2) * (4 * LP_THREADS) + 4 * tid + (e & 3) : e * LP_THREADS + tid; }
+
+__device__ __forceinline__ float lp_exp(float d) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(d * 1.4426950408889634f));
+    return y;
+}
+// Sums relative to `from` as sums relative to `to`, which is not below it.  The clamp: nothing times -infinity is nothing.
+__device__ __forceinline__ void lp_raise(float& S, float& U, float from, float to) {
+    const float d = from - to, f = lp_exp(d);
+    U = (U + S * fmaxf(d, -1e30f)) * f;
+    S *= f;
+}
+#define LP_LOWEST -3.4028234663852886e38f       // a reference when there is none: -infinity itself would leave -infinity minus -infinity
+
+template <bool VEC>
+__global__ void __launch_bounds__(LP_THREADS, 4)
+lp_segments_kernel(const float* __restrict__ logits, float* __restrict__ sums, float* __restrict__ maxima, int V, int segs) {
     pdl_wait();
     pdl_launch_dependents();
-    __shared__ float scratch[32], win_v[LP_THREADS / 32];
-    __shared__ int win_i[LP_THREADS / 32];
+    constexpr int WARPS = LP_THREADS / 32;
+    __shared__ float warp_m[WARPS], warp_s[WARPS], warp_u[WARPS];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const long long row = blockIdx.y;
-    const int seg = blockIdx.x, first = seg * LP_SEG;
-    const float* x = logits + row * V;
-    float v[LP_PER_THREAD];
-    float m = -INFINITY;
+    const int seg = blockIdx.x, first = seg * LP_SEG, here = min(V - first, LP_SEG);
+    const float* x = logits + row * V + first;
+    const bool whole = VEC && here == LP_SEG;
+    auto load = [&](float (&v)[LP_PIECE], int e0) {
+        if (whole) {
 #pragma unroll
-    for (int e = 0; e < LP_PER_THREAD; ++e) {
-        const int i = first + e * LP_THREADS + tid;
-        v[e] = i < V ? x[i] : -INFINITY;
-        m = fmaxf(m, v[e]);
-    }
-    m = warp_max(m);
-    if (lane == 0) scratch[warp] = m;
-    __syncthreads();
-    for (int w = 0; w < LP_THREADS / 32; ++w) m = fmaxf(m, scratch[w]);
-    float S = 0.f, U = 0.f;
+            for (int e = 0; e < LP_PIECE; e += 4) {
+                const float4 y = *reinterpret_cast<const float4*>(x + lp_index<VEC>(e0 + e, tid));
+                v[e] = y.x; v[e + 1] = y.y; v[e + 2] = y.z; v[e + 3] = y.w;
+            }
+        } else {
 #pragma unroll
-    for (int e = 0; e < LP_PER_THREAD; ++e) {
-        const float d = v[e] - m, p = v[e] == -INFINITY ? 0.f : __expf(d);
-        S += p;
-        if (p > 0.f) U += p * d;
+            for (int e = 0; e < LP_PIECE; ++e) v[e] = lp_index<VEC>(e0 + e, tid) < here ? x[lp_index<VEC>(e0 + e, tid)] : -INFINITY;
+        }
+    };
+    float mine = -INFINITY, ref = LP_LOWEST, S = 0.f, U = 0.f, v[2][LP_PIECE];
+    load(v[0], 0);
+#pragma unroll
+    for (int p = 0; p < LP_PER_THREAD / LP_PIECE; ++p) {
+        if (p + 1 < LP_PER_THREAD / LP_PIECE) load(v[(p + 1) & 1], (p + 1) * LP_PIECE);
+        const float (&y)[LP_PIECE] = v[p & 1];
+#pragma unroll
+        for (int e = 0; e < LP_PIECE; ++e) mine = fmaxf(mine, y[e]);
+        if (mine > ref + 8.f) {
+            lp_raise(S, U, ref, mine);
+            ref = mine;
+        }
+        float s0 = 0.f, s1 = 0.f, u0 = 0.f, u1 = 0.f;
+#pragma unroll
+        for (int e = 0; e < LP_PIECE; e += 2) {
+            const float d0 = y[e] - ref, d1 = y[e + 1] - ref, p0 = lp_exp(d0), p1 = lp_exp(d1);
+            s0 += p0;
+            s1 += p1;
+            u0 = fmaf(p0, fmaxf(d0, -1e30f), u0);                   // 0 times -infinity is 0 here
+            u1 = fmaf(p1, fmaxf(d1, -1e30f), u1);
+        }
+        S += s0 + s1;
+        U += u0 + u1;
     }
-    S = block_sum(S, scratch);
-    U = block_sum(U, scratch);
     const long long at = row * segs + seg;
+    if (maxima) maxima[at * LP_THREADS + tid] = mine;
+    const float most = warp_max(mine);
+    if (lane == 0) warp_m[warp] = most;
+    __syncthreads();
+    float m = ref;                                                  // the lowest number where there is nothing but -infinity
+#pragma unroll
+    for (int w = 0; w < WARPS; ++w) m = fmaxf(m, warp_m[w]);
+    lp_raise(S, U, ref, m);
+    S = warp_sum(S);
+    U = warp_sum(U);
+    if (lane == 0) { warp_s[warp] = S; warp_u[warp] = U; }
+    __syncthreads();
     if (tid == 0) {
+        m = LP_LOWEST;
+        S = U = 0.f;
+        for (int w = 0; w < WARPS; ++w) {
+            m = fmaxf(m, warp_m[w]);
+            S += warp_s[w];
+            U += warp_u[w];
+        }
         sums[at * 3] = m;
         sums[at * 3 + 1] = S;
         sums[at * 3 + 2] = U;
     }
-    // the `top` largest, one after the other: everyone's largest that is behind the last one found
+}
+
+// A block a row.  The `top` largest: a thread takes its share of the maxima; each warp's (top / warps, rounded up)-th largest of its
+// threads' largest, and the lowest of these, the bar, is at most the row's top-th largest logit, and few maxima are at or above it
+// (with random logits about twice `top`).  Their threads' 64 logits are read again and what is at or above the bar gathered
+// in shared memory; each one's rank is how many stand before it.  Where more are there than fit (equal logits, orders that put
+// the largest into few threads) the list is found one by one.
+template <bool VEC>
+__global__ void __launch_bounds__(LP_THREADS, 8)
+lp_join_kernel(const float* __restrict__ logits, const int* __restrict__ tokens, const float* sums, const float* maxima,
+               float* __restrict__ logprob, float* __restrict__ entropy, int* __restrict__ top_ids, float* __restrict__ top_lps, int V, int segs,
+               int top) {
+    pdl_wait();
+    pdl_launch_dependents();
+    constexpr int WARPS = LP_THREADS / 32;
+    __shared__ float warp_t[WARPS], found_v[LP_GATHER];
+    __shared__ int found_i[LP_GATHER], holders[LP_GATHER], picked[LP_GATHER], n_found, n_holders, n_picked;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const long long row = blockIdx.x;
+    const float* x = logits + row * V;
+    const float* mine = sums + row * segs * 3;
+    const float* at_most = maxima + row * segs * LP_THREADS;
+    float held[LP_HELD];                    // this thread's share of the maxima, the first of them in registers
+#pragma unroll
+    for (int j = 0; j < LP_HELD; ++j) held[j] = top && j < segs ? __ldcg(at_most + j * LP_THREADS + tid) : -INFINITY;
+    // every warp has the sums: the same additions in the same order
+    float m = LP_LOWEST;
+    for (int s = lane; s < segs; s += 32) m = fmaxf(m, __ldcg(mine + s * 3));
+    m = warp_max(m);
+    float S = 0.f, U = 0.f;
+    for (int s = lane; s < segs; s += 32) {
+        float Ss = __ldcg(mine + s * 3 + 1), Us = __ldcg(mine + s * 3 + 2);
+        lp_raise(Ss, Us, __ldcg(mine + s * 3), m);
+        S += Ss;
+        U += Us;
+    }
+    S = warp_sum(S);
+    U = warp_sum(U);
+    const float lnS = logf(S);
+    if (tid == 0) {
+        const int t = tokens[row];
+        logprob[row] = (t >= 0 && t < V) ? (x[t] - m) - lnS : __uint_as_float(0x7fffffffu);
+        entropy[row] = lnS - U / S;
+        n_found = n_holders = n_picked = 0;
+    }
+    if (!top) return;
+    float largest = -INFINITY;
+#pragma unroll
+    for (int j = 0; j < LP_HELD; ++j) largest = fmaxf(largest, held[j]);
+    for (int j = LP_HELD; j < segs; ++j) largest = fmaxf(largest, __ldcg(at_most + j * LP_THREADS + tid));
+    int left = lp_key(largest), kth = __reduce_max_sync(0xffffffffu, left);
+    for (int k = 1; k < (top + WARPS - 1) / WARPS; ++k) {                               // take the warp's largest out, look again
+        const unsigned at = __ballot_sync(0xffffffffu, left == kth);
+        if (lane == __ffs(at) - 1) left = INT_MIN;
+        kth = __reduce_max_sync(0xffffffffu, left);
+    }
+    if (lane == 0) warp_t[warp] = kth == INT_MIN ? -INFINITY : __int_as_float(kth < 0 ? kth ^ 0x7fffffff : kth);
+    __syncthreads();
+    float bar = warp_t[0];
+#pragma unroll
+    for (int w = 1; w < WARPS; ++w) bar = fminf(bar, warp_t[w]);
+    if (largest >= bar) {
+        auto hold = [&](int j, float y) {
+            const int at = atomicAdd(&n_holders, 1);
+            if (at < LP_GATHER) {
+                holders[at] = j;
+                found_v[at] = y;
+            }
+        };
+#pragma unroll
+        for (int j = 0; j < LP_HELD; ++j)
+            if (j < segs && held[j] >= bar) hold(j * LP_THREADS + tid, held[j]);
+        for (int j = LP_HELD; j < segs; ++j) {
+            const float y = __ldcg(at_most + j * LP_THREADS + tid);
+            if (y >= bar) hold(j * LP_THREADS + tid, y);
+        }
+    }
+    __syncthreads();
+    // the top-th largest of the maxima found is a higher bar, with about half as many at or above it
+    const int n_held = min(n_holders, LP_GATHER);
+    for (int i = tid; i < n_held; i += LP_THREADS) {
+        const float a = found_v[i];
+        int above = 0, same = 0;
+        for (int j = 0; j < n_held; ++j) {
+            above += found_v[j] > a;
+            same += found_v[j] == a;
+        }
+        if (above < top && top <= above + same) warp_t[0] = a;          // whoever writes, writes the same number
+    }
+    __syncthreads();
+    if (n_holders <= LP_GATHER) bar = warp_t[0];
+    for (int i = tid; i < n_held; i += LP_THREADS)
+        if (found_v[i] >= bar) picked[atomicAdd(&n_picked, 1)] = holders[i];
+    __syncthreads();
+    // 64 logits of each, all threads side by side
+    const int looks = n_picked * LP_PER_THREAD;
+#pragma unroll 4
+    for (int j = tid; j < looks; j += LP_THREADS) {
+        const int who = picked[j / LP_PER_THREAD], i = who / LP_THREADS * LP_SEG + lp_index<VEC>(j % LP_PER_THREAD, who % LP_THREADS);
+        const float y = i < V ? x[i] : -INFINITY;
+        if (y >= bar && i < V) {
+            const int at = atomicAdd(&n_found, 1);
+            if (at < LP_GATHER) {
+                found_v[at] = y;
+                found_i[at] = i;
+            }
+        }
+    }
+    __syncthreads();
+    const int n = n_found;
+    auto leave = [&](int rank, float a, int ia) {
+        top_ids[row * top + rank] = ia;
+        top_lps[row * top + rank] = ia < 0 ? __uint_as_float(0x7fffffffu) : (a - m) - lnS;
+    };
+    if (n <= LP_GATHER && n_holders <= LP_GATHER) {
+        for (int i = tid; i < n; i += LP_THREADS) {
+            const float a = found_v[i];
+            const int ia = found_i[i];
+            int rank = 0;
+            for (int j = 0; j < n; ++j) rank += lp_before(found_v[j], found_i[j], a, ia);
+            if (rank < top) leave(rank, a, ia);
+        }
+        for (int i = n + tid; i < top; i += LP_THREADS) leave(i, -INFINITY, -1);
+        return;
+    }
+    // one after the other: everyone's largest that is behind the last one found
     float last = INFINITY;
     int last_i = -1;
     for (int k = 0; k < top; ++k) {
         float bv = -INFINITY;
         int bi = -1;
-#pragma unroll
-        for (int e = 0; e < LP_PER_THREAD; ++e) {
-            const int i = first + e * LP_THREADS + tid;
-            const bool open = i < V && v[e] == v[e] && (last_i < 0 || lp_before(last, last_i, v[e], i));
-            if (open && lp_before(v[e], i, bv, bi)) { bv = v[e]; bi = i; }
+        for (int i = tid; i < V; i += LP_THREADS) {
+            const float y = x[i];
+            const bool open = y == y && (last_i < 0 || lp_before(last, last_i, y, i));
+            if (open && lp_before(y, i, bv, bi)) { bv = y; bi = i; }
         }
         lp_warp_best(bv, bi);
         __syncthreads();
-        if (lane == 0) { win_v[warp] = bv; win_i[warp] = bi; }
+        if (lane == 0) { found_v[warp] = bv; found_i[warp] = bi; }
         __syncthreads();
-        bv = win_v[0];
-        bi = win_i[0];
-        for (int w = 1; w < LP_THREADS / 32; ++w)
-            if (lp_before(win_v[w], win_i[w], bv, bi)) { bv = win_v[w]; bi = win_i[w]; }
-        if (tid == 0) { best[at * top + k] = bv; best_id[at * top + k] = bi; }
-        if (bi < 0) {
-            for (int r = k + 1 + tid; r < top; r += LP_THREADS) { best[at * top + r] = -INFINITY; best_id[at * top + r] = -1; }
-            break;
-        }
+        bv = found_v[0];
+        bi = found_i[0];
+        for (int w = 1; w < WARPS; ++w)
+            if (lp_before(found_v[w], found_i[w], bv, bi)) { bv = found_v[w]; bi = found_i[w]; }
+        if (tid == 0) leave(k, bv, bi);
         last = bv;
         last_i = bi;
     }
 }
 
-// One warp a row joins its segments.
-__global__ void __launch_bounds__(128)
-lp_join_kernel(const float* __restrict__ logits, const int* __restrict__ tokens, const float* __restrict__ sums, const float* __restrict__ best,
-               const int* __restrict__ best_id, float* __restrict__ logprob, float* __restrict__ entropy, int* __restrict__ top_ids,
-               float* __restrict__ top_lps, int rows, int V, int segs, int top) {
-    pdl_wait();
-    pdl_launch_dependents();
-    const int lane = threadIdx.x & 31;
-    const long long row = (long long)blockIdx.x * 4 + (threadIdx.x >> 5);
-    if (row >= rows) return;
-    const float* mine = sums + row * segs * 3;
-    float m = -INFINITY;
-    for (int s = lane; s < segs; s += 32) m = fmaxf(m, mine[s * 3]);
-    m = warp_max(m);
-    float S = 0.f, U = 0.f;
-    for (int s = lane; s < segs; s += 32) {
-        const float ms = mine[s * 3], Ss = mine[s * 3 + 1], Us = mine[s * 3 + 2];
-        if (Ss != 0.f) {                                    // a segment of nothing but -infinity adds nothing
-            const float f = expf(ms - m);
-            S += Ss * f;
-            U += (Us + Ss * (ms - m)) * f;
-        }
-    }
-    S = warp_sum(S);
-    U = warp_sum(U);
-    const float lnS = logf(S);
-    if (lane == 0) {
-        const int t = tokens[row];
-        logprob[row] = (t >= 0 && t < V) ? (logits[row * V + t] - m) - lnS : __uint_as_float(0x7fffffffu);
-        entropy[row] = lnS - U / S;
-    }
-    float last = INFINITY;
-    int last_i = -1;
-    for (int k = 0; k < top; ++k) {
-        float bv = -INFINITY;
-        int bi = -1;
-        for (int s = lane; s < segs; s += 32) {
-            const float* lv = best + (row * segs + s) * top;
-            const int* li = best_id + (row * segs + s) * top;
-            for (int r = 0; r < top; ++r) {                 // the first of the list that is behind the last one found
-                if (li[r] < 0) break;
-                if (last_i < 0 || lp_before(last, last_i, lv[r], li[r])) {
-                    if (lp_before(lv[r], li[r], bv, bi)) { bv = lv[r]; bi = li[r]; }
-                    break;
-                }
-            }
-        }
-        lp_warp_best(bv, bi);
-        if (lane == 0) {
-            top_ids[row * top + k] = bi;
-            top_lps[row * top + k] = bi < 0 ? __uint_as_float(0x7fffffffu) : (bv - m) - lnS;
-        }
-        if (bi >= 0) { last = bv; last_i = bi; }
-    }
-}
-
+// Segments of a row.
 extern "C" int qwb_logprobs_segments(int V) { return (int)(((long long)V + LP_SEG - 1) / LP_SEG); }
 
-// scratch: rows x segments x (3 + top) floats, then rows x segments x top ints
+// scratch: rows x segments x 3 floats, and with top > 0 LP_THREADS more for each
 extern "C" int qwb_logprobs(const float* logits, const int* tokens, float* logprob, float* entropy, int* top_ids, float* top_lps, float* scratch,
                             int rows, int V, int top, cudaStream_t stream) {
     if (rows <= 0) return 0;
@@ -161,10 +293,10 @@ extern "C" int qwb_logprobs(const float* logits, const int* tokens, float* logpr
         return qwb_fail(QWB_ERR_ARG, "token_logprobs: 0 to %d alternatives of a vocabulary of at least as many: top=%d V=%d", LP_MAX_TOP, top, V);
     if (rows > 65535) return qwb_fail(QWB_ERR_ARG, "token_logprobs: at most 65535 rows in a call, not %d", rows);
     const int segs = qwb_logprobs_segments(V);
-    float* best = scratch + (size_t)rows * segs * 3;
-    int* best_id = reinterpret_cast<int*>(best + (size_t)rows * segs * top);
-    qwb_launch(lp_segments_kernel, dim3(segs, rows), LP_THREADS, 0, stream, logits, scratch, best, best_id, V, segs, top);
-    qwb_launch(lp_join_kernel, dim3((rows + 3) / 4), 128, 0, stream, logits, tokens, scratch, best, best_id, logprob, entropy, top_ids, top_lps, rows, V,
-               segs, top);
+    float* maxima = top ? scratch + (size_t)rows * segs * 3 : nullptr;
+    const bool vec = V % 4 == 0 && (uintptr_t)logits % 16 == 0;
+    qwb_launch(vec ? lp_segments_kernel<true> : lp_segments_kernel<false>, dim3(segs, rows), LP_THREADS, 0, stream, logits, scratch, maxima, V, segs);
+    qwb_launch_link(rows, LP_LINK_ROWS, vec ? lp_join_kernel<true> : lp_join_kernel<false>, dim3(rows), LP_THREADS, 0, stream, logits, tokens, scratch, maxima, logprob, entropy,
+               top_ids, top_lps, V, segs, top);
     return qwb_check_launch("token_logprobs");
 }

@@ -2313,7 +2313,7 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top: int = 0, out
     _here("token_logprobs", logits, tokens, *out)
     if R:
         segments = _lookup("logprobs", "qwb_logprobs_segments")[1](V)
-        scratch = _empty((R * segments * (3 + 2 * top),), dtype=torch.float32, device=dev)
+        scratch = _empty((R * segments * (259 if top else 3),), dtype=torch.float32, device=dev)
         _call("logprobs", "qwb_logprobs", _ptr(logits), _ptr(tokens), _ptr(out.logprob), _ptr(out.entropy), _ptr(out.top_ids), _ptr(out.top_logprobs),
               _ptr(scratch), _i(R), _i(V), _i(top), _stream(), kernels=2)
     return out

@@ -17,9 +17,9 @@ U = 2.0 ** -23
 def check(x, tokens, top):
     r = ops.token_logprobs(torch.from_numpy(x).to(DEV), torch.tensor(tokens, dtype=torch.int32, device=DEV), top=top)
     lp, H, ids, lps, mean, square = pk.logprobs(x, tokens, top)
-    # ln S: an exponential is off by (2 + 1.173 |d|) units of 2^-23 (its stated bound), a sum of at most 32 + 5 + 8 terms one after the
-    # other and then 1 / 32 of the segments + 5 by half a unit each; then the differences x - m and (x - m) - ln S, and ln's own unit
-    lnS = (2 + 1.2 * mean + (50 + x.shape[1] / 8192 / 32) / 2) * U
+    # ln S: an exponential is off by (2 + 1.173 |d|) units of 2^-23 (its stated bound), a sum of at most 16 + 5 + 8 terms one after the
+    # other, five changes of the reference (an exponential, a product) and then 1 / 32 of the segments + 5 by half a unit each; then the differences x - m and (x - m) - ln S, and ln's own unit
+    lnS = (2 + 1.2 * mean + (70 + x.shape[1] / 8192 / 32) / 2) * U
 
     def near(got, ref, lim):
         got = got.cpu().numpy().astype(np.float64)
@@ -29,7 +29,7 @@ def check(x, tokens, top):
     d = lambda v: np.abs(v) * U * 2 + U * 32                                            # |v| + |ln S| below 2 |v| + 32
     assert near(r.logprob, lp, lnS + d(lp))
     # U / S: the same errors on terms of |d|, and d's own rounding
-    assert near(r.entropy, H, lnS + (2 * mean + 1.2 * square + mean * (52 + x.shape[1] / 8192 / 32)) * U + U * 32)
+    assert near(r.entropy, H, lnS + (2 * mean + 1.2 * square + mean * (72 + x.shape[1] / 8192 / 32)) * U + U * 32)
     assert r.top_ids.dtype == torch.int32 and r.top_ids.cpu().numpy().tolist() == ids.tolist()
     if top:
         assert near(r.top_logprobs, lps, lnS[:, None] + d(lps))
@@ -67,16 +67,18 @@ def test_ties_and_orders(V, order):
 
 def test_large_and_masked_logits():
     rng = np.random.default_rng(3)
-    x = (rng.standard_normal((6, 12000)) * 2).astype(np.float32)
+    x = (rng.standard_normal((8, 20000)) * 2).astype(np.float32)
     x[0] += 3e4
     x[1] *= 100
     x[2, 100:] = -np.inf                                    # most tokens cannot be
-    x[3, :9000] = -np.inf                                   # a whole segment
+    x[3, :17000] = -np.inf                                  # a whole segment
     x[4, 1:] = -np.inf                                      # one token left
-    x[5] = np.where(rng.random(12000) < 0.5, np.finfo(np.float32).min, x[5])          # masked by the type's lowest value
-    r = check(x, [5, 7, 3, 9500, 0, int(np.argmax(x[5]))], 30)
+    x[5] = np.where(rng.random(20000) < 0.5, np.finfo(np.float32).min, x[5])          # masked by the type's lowest value
+    x[6] = np.finfo(np.float32).min                         # all of them: as good as each other
+    x[7] = np.where(rng.random(20000) < 0.5, 3e38, -3e38)
+    r = check(x, [5, 7, 3, 17500, 0, int(np.argmax(x[5])), 3, int(np.argmax(x[7]))], 30)
     assert float(r.logprob[4]) == 0.0 and float(r.entropy[4]) == 0.0
-    got = ops.token_logprobs(torch.from_numpy(x).to(DEV), torch.tensor([0, 0, 500, 5, 9, 0], dtype=torch.int32, device=DEV))
+    got = ops.token_logprobs(torch.from_numpy(x).to(DEV), torch.tensor([0, 0, 500, 5, 9, 0, 0, 0], dtype=torch.int32, device=DEV))
     assert got.logprob[2:5].tolist() == [-math.inf] * 3
 
 
