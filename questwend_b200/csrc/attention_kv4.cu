@@ -3,7 +3,7 @@
 // Few new tokens a sequence, bfloat16, heads of 64 or 128 (kv4_attn_rows_kernel): a decode step.  What it has to do is read the
 // cache, 144 bytes a token and head of 128, for 4 x 128 multiply-adds a query head: on mma.sync, whose products are far from the limit
 // here (a group of 4 heads fills half of the 8 columns), so that the time is loads and the way from codes to bfloat16.
-//   * A block takes a key/value head and a run of a sequence's pages; its four warps take 16 keys of every page each, with their
+//   * A block takes a key/value head and a run of a sequence's pages; its two warps take 32 keys of every page each, with their
 //     own copies (cp.async into a ring of their own), maxima, sums and outputs, and meet at the run's end in shared memory.  Nothing in
 //     between waits for another warp.
 //   * The 16-row operand of both products is the cache's, the 8 columns are (token, query head) pairs:
@@ -11,17 +11,21 @@
 //   * Which number of a row sits where in an mma's inner dimension is free as long as both operands agree.  A lane therefore takes
 //     32 neighbouring numbers of a key (one 16-byte load, one group, one step), and of a value its 16 numbers of 4 keys; codes come out
 //     of a 32-bit word two at a time, in the places where their shifts leave them.
-//   * A code c becomes the bfloat16 128 + c by one and-or (its 7 bits behind the point hold c), 128 + z is taken off and s
-//     multiplied: both exact.
+//   * A code c becomes the bfloat16 128 + c by one and-or (its 7 bits behind the point hold c) and c s by one fused multiply-add.  The
+//     zero points are taken off as sums: of the scores by one more mma, whose inner dimension holds z s of a lane's group and the sum of the
+//     query's numbers there (in three bfloat16 parts), of the outputs by a row of z s in the mma that adds up the weights.
 //   * The scores' columns are the next product's inner dimension: P^T's operand is two 8 x 8 transpositions (movmatrix).
-//   * A run's softmax is relative to a reference that is raised, and O rescaled, only where a score passes it by 2^8: most tiles vote once
-//     and exchange no maxima.
+//   * A run's softmax is relative to a reference that is raised, and O rescaled, only where a score passes it by 2^8: most pages vote once
+//     and exchange no maxima.  The weights' sum is one more mma with rows of ones, over
+//     the weights as they are rounded for the product.
 // Runs are cut by the sequence's own length (kv4_runs), never by what else is in the batch; a second kernel joins them.
 //
 // The plain kernel: any head size that is a multiple of 32, queries in 32 bits or bfloat16.  A block takes a (token, query head),
 // its four warps every fourth key; a lane holds the numbers lane, lane + 32, ... of the query, of the sums and of a key, so a
 // group of 32 is a step of the loop over them.  Each warp keeps a running maximum, sum and output; they meet in shared memory.
 #include "kv4.cuh"
+
+#include <math.h>
 
 #define KP_WARPS 4
 
@@ -111,9 +115,9 @@ extern "C" int qwb_kv4_attn_plain(const void* q, const unsigned char* pool, cons
 }
 
 // ----------------------------------------------------------------------------- few new tokens: mma.sync
-#define KD_WARPS 4
-#define KD_KEYS 16              // keys of a warp's tile: the mma's 16 rows
-#define KD_STAGES 4             // tiles of a warp's ring
+#define KD_WARPS 2
+#define KD_KEYS 32              // keys of a page that a warp takes: two tiles of the mma's 16 rows
+#define KD_STAGES 3             // pages of a warp's ring
 #define KD_RUNS 16              // a sequence's pages are cut into about so many runs ...
 #define KD_RUN_PAGES 8          // ... of at most this many pages
 #define KD_RAISE 8.f            // a run's reference is raised where a score passes it by 2^8
@@ -154,16 +158,21 @@ __device__ __forceinline__ float kd_exp2(float x) {
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
-// Two codes, in the lowest four bits of each half of `codes`, as the bfloat16 numbers (c - z) s; zero: 128 + z twice, step: s twice.
-__device__ __forceinline__ uint32_t kd_numbers(uint32_t codes, uint32_t zero, uint32_t step) {
-    uint32_t e = (codes & 0x000f000fu) | 0x43004300u;
-    __nv_bfloat162 v = __hmul2(__hsub2(*reinterpret_cast<__nv_bfloat162*>(&e), *reinterpret_cast<__nv_bfloat162*>(&zero)),
-                               *reinterpret_cast<__nv_bfloat162*>(&step));
+// Two codes c, in the lowest four bits of each half of `codes`, as the bfloat16 numbers c s: 128 + c by one and-or, then a fused
+// multiply-add that takes 128 s off, exact throughout.  step: s twice; off: -128 s twice.
+__device__ __forceinline__ uint32_t kd_scaled(uint32_t codes, uint32_t step, uint32_t off) {
+    uint32_t e;
+    asm("lop3.b32 %0, %1, %2, %3, 0xea;" : "=r"(e) : "r"(codes), "r"(0x000f000fu), "r"(0x43004300u));        // written as & and |, two instructions
+    __nv_bfloat162 v = __hfma2(*reinterpret_cast<__nv_bfloat162*>(&e), *reinterpret_cast<__nv_bfloat162*>(&step), *reinterpret_cast<__nv_bfloat162*>(&off));
+    return *reinterpret_cast<uint32_t*>(&v);
+}
+__device__ __forceinline__ uint32_t kd_off(uint32_t step) {
+    __nv_bfloat162 v = __hmul2(*reinterpret_cast<__nv_bfloat162*>(&step), __floats2bfloat162_rn(-128.f, -128.f));
     return *reinterpret_cast<uint32_t*>(&v);
 }
 
 template <int HD>
-struct KdTile {                                             // a warp's 16 keys of a page and head
+struct KdTile {                                             // a warp's keys of a page and head
     static constexpr int CODES = KD_KEYS * HD / 2, WORDS = KD_KEYS * HD / 16, HALF = CODES + WORDS, BYTES = 2 * HALF;
 };
 template <int HD, int NT>
@@ -177,10 +186,10 @@ struct KdSmem {
 // NT: tiles of 8 columns of a block.  part: [rows, max_runs, HD] outputs, then [rows, max_runs, 2] maxima (of scores times log2 e) and sums
 // of the runs of sequences that have more than one; a row is (token, query head).
 template <int HD, int NT>
-__global__ void __launch_bounds__(KD_WARPS * 32, NT == 1 ? 4 : 3)
+__global__ void __launch_bounds__(KD_WARPS * 32, NT == 1 ? 8 : 5)
 kv4_attn_rows_kernel(const bf16* __restrict__ q, const unsigned char* __restrict__ pool, const int* __restrict__ page_table,
                      const int* __restrict__ cu_seqlens, const int* __restrict__ pos0, bf16* __restrict__ out, float* __restrict__ part_o,
-                     float* __restrict__ part_ml, int T, int B, int pool_pages, int Hq, int Hkv, int table_width, float scale_log2, int window,
+                     float* __restrict__ part_ml, int T, int B, int pool_pages, int Hq, int Hkv, int table_width, float scale_log2, uint32_t flip, int window,
                      int tiles, int max_runs) {
     pdl_wait();
     pdl_launch_dependents();
@@ -208,7 +217,7 @@ kv4_attn_rows_kernel(const bf16* __restrict__ q, const unsigned char* __restrict
 
     // this block's columns: their last and first key; the queries, in the order in which a lane holds the keys' numbers
     int last_key[NT][2], first_key[NT][2];
-    uint32_t qf[NT][HD / 16][2];
+    uint32_t qf[NT][HD / 16][2], qz[NT][2];                 // qz: minus the sum of a lane's numbers of the query, in three parts
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
 #pragma unroll
@@ -220,24 +229,35 @@ kv4_attn_rows_kernel(const bf16* __restrict__ q, const unsigned char* __restrict
         const int col = col0 + n * 8 + r;
         const bool live = col < cols;
         const bf16* src = q + ((size_t)(t0 + (live ? col / G : 0)) * Hq + kvh * G + (live ? col % G : 0)) * HD + c * (HD / 4);
+        float sum = 0.f;
 #pragma unroll
         for (int w = 0; w < HD / 32; ++w) {
             uint4 v = make_uint4(0, 0, 0, 0);
-            if (live) v = *reinterpret_cast<const uint4*>(src + 8 * w);
+            if (live) {
+                v = *reinterpret_cast<const uint4*>(src + 8 * w);
+                v = make_uint4(v.x ^ flip, v.y ^ flip, v.z ^ flip, v.w ^ flip);         // the scale's sign
+            }
             qf[n][2 * w][0] = __byte_perm(v.x, v.z, 0x5410);            // numbers 0 and 4, 1 and 5, 2 and 6, 3 and 7 of 8
             qf[n][2 * w][1] = __byte_perm(v.x, v.z, 0x7632);
             qf[n][2 * w + 1][0] = __byte_perm(v.y, v.w, 0x5410);
             qf[n][2 * w + 1][1] = __byte_perm(v.y, v.w, 0x7632);
+            const uint32_t x[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+            for (int i = 0; i < 4; ++i) sum += __uint_as_float(x[i] << 16) + __uint_as_float(x[i] & 0xffff0000u);
         }
+        const float hi = __bfloat162float(__float2bfloat16_rn(sum)), mid = __bfloat162float(__float2bfloat16_rn(sum - hi));
+        qz[n][0] = kd_pack(-hi, -mid);
+        qz[n][1] = kd_pack(hi + mid - sum, 0.f);
     }
     const int see_all_from = window > 0 ? p0 + min(col0 + 8 * NT, cols) / G - window + 1 : 0;    // keys below may be hidden from a column,
     const int see_all_to = p0 + col0 / G;                                                       // keys above as well
 
     unsigned char* ring = smem + (size_t)warp * KD_STAGES * Tile::BYTES;
+    int slot_in = 0, slot_out = 0;
     auto ask = [&](int i) {                                 // the warp's 16 keys of the run's i-th page
         const int page = __shfl_sync(0xffffffffu, my_page, i & 31);
         if (i < n_pages && page >= 0) {
-            unsigned char* dst = ring + (i % KD_STAGES) * Tile::BYTES;
+            unsigned char* dst = ring + slot_in * Tile::BYTES;
             const unsigned char* src = pool + ((size_t)page * Hkv + kvh) * kv4_page_bytes(HD) + warp * Tile::CODES;
             constexpr int WORDS_AT = kv4_code_bytes(HD);
 #pragma unroll
@@ -252,15 +272,20 @@ kv4_attn_rows_kernel(const bf16* __restrict__ q, const unsigned char* __restrict
             }
         }
         asm volatile("cp.async.commit_group;" ::: "memory");
+        slot_in = slot_in == KD_STAGES - 1 ? 0 : slot_in + 1;
     };
 
-    float o[NT][HD / 16][4], m[NT][2], l[NT][2];
+    // outputs; the weights' sums (0, 1: from rows of ones) and what the zero points add to a lane's outputs (2, 3); the reference of the raw scores, what passes it by 2^8, and -reference in the
+    // exponent's units (0 while there is no reference: a weight of a hidden key is then 2^-infinity)
+    float o[NT][HD / 16][4], l[NT][4], m[NT][2], over[NT][2], shift[NT][2];
+    const float raise = KD_RAISE / scale_log2;
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
 #pragma unroll
         for (int i = 0; i < HD / 16; ++i) o[n][i][0] = o[n][i][1] = o[n][i][2] = o[n][i][3] = 0.f;
-        m[n][0] = m[n][1] = -INFINITY;
-        l[n][0] = l[n][1] = 0.f;
+        l[n][0] = l[n][1] = l[n][2] = l[n][3] = 0.f;
+        m[n][0] = m[n][1] = over[n][0] = over[n][1] = -INFINITY;
+        shift[n][0] = shift[n][1] = 0.f;
     }
 #pragma unroll
     for (int i = 0; i < KD_STAGES - 1; ++i) ask(i);
@@ -268,12 +293,14 @@ kv4_attn_rows_kernel(const bf16* __restrict__ q, const unsigned char* __restrict
     // never two lie in the same banks
     const int key_r = (r & 1) ? 4 + ((r >> 1) ^ 1) : r >> 1;
     const int vk0 = c, vk1 = 4 + (c ^ 1);                   // a lane's four keys of a value tile: rows 2c, 2c + 1 and the ones 8 behind
+    constexpr int TILES = KD_KEYS / 16, GROUPS = HD / KV4_GROUP;
 
     for (int i = 0; i < n_pages; ++i) {
         ask(i + KD_STAGES - 1);
         asm volatile("cp.async.wait_group %0;" ::"n"(KD_STAGES - 1) : "memory");
         __syncwarp();
-        const unsigned char* kt = ring + (i % KD_STAGES) * Tile::BYTES;
+        const unsigned char* kt = ring + slot_out * Tile::BYTES;
+        slot_out = slot_out == KD_STAGES - 1 ? 0 : slot_out + 1;
         const unsigned char* vt = kt + Tile::HALF;
         const uint16_t* kw = reinterpret_cast<const uint16_t*>(kt + Tile::CODES);
         const uint16_t* vw = reinterpret_cast<const uint16_t*>(vt + Tile::CODES);
@@ -281,13 +308,14 @@ kv4_attn_rows_kernel(const bf16* __restrict__ q, const unsigned char* __restrict
         const bool there = __shfl_sync(0xffffffffu, my_page, i) >= 0;
         if (there && base < len) {
             // S^T = K Q^T
-            float s[NT][4];
+            float s[TILES][NT][4];
 #pragma unroll
-            for (int n = 0; n < NT; ++n) s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.f;
-            constexpr int LW = HD / 32;                     // 32-bit words of codes of a lane's numbers of a key
-            uint32_t ka[LW], kb[LW], za, sa, zb, sb;
-            {
-                const unsigned char* pa = kt + key_r * (HD / 2) + c * (HD / 8);
+            for (int t = 0; t < TILES; ++t) {
+#pragma unroll
+                for (int n = 0; n < NT; ++n) s[t][n][0] = s[t][n][1] = s[t][n][2] = s[t][n][3] = 0.f;
+                constexpr int LW = HD / 32;                 // 32-bit words of codes of a lane's numbers of a key
+                uint32_t ka[LW], kb[LW];
+                const unsigned char* pa = kt + (16 * t + key_r) * (HD / 2) + c * (HD / 8);
                 const unsigned char* pb = pa + 8 * (HD / 2);
                 if constexpr (LW == 4) {
                     const uint4 va = *reinterpret_cast<const uint4*>(pa), vb = *reinterpret_cast<const uint4*>(pb);
@@ -298,116 +326,131 @@ kv4_attn_rows_kernel(const bf16* __restrict__ q, const unsigned char* __restrict
                     ka[0] = va.x; ka[1] = va.y;
                     kb[0] = vb.x; kb[1] = vb.y;
                 }
-                const int g = c * (HD / 4) / KV4_GROUP;
-                const uint32_t wa = kw[key_r * (HD / KV4_GROUP) + g] * 0x10001u, wb = kw[(key_r + 8) * (HD / KV4_GROUP) + g] * 0x10001u;
-                za = (wa & 0x000f000fu) | 0x43004300u;
-                sa = wa & 0xfff0fff0u;
-                zb = (wb & 0x000f000fu) | 0x43004300u;
-                sb = wb & 0xfff0fff0u;
-            }
+                const uint16_t* words = kw + (16 * t + key_r) * GROUPS + c * (HD / 4) / KV4_GROUP;
+                const uint32_t wa = words[0] * 0x10001u, wb = words[8 * GROUPS] * 0x10001u;
+                const uint32_t sa = wa & 0xfff0fff0u, sb = wb & 0xfff0fff0u, fa = kd_off(sa), fb = kd_off(sb);
+                const uint32_t za = kd_scaled(wa, sa, fa), zb = kd_scaled(wb, sb, fb);
 #pragma unroll
-            for (int k = 0; k < HD / 16; ++k) {
-                const int sh = 8 * (k & 1);
-                const uint32_t a0 = kd_numbers(ka[k / 2] >> sh, za, sa), a1 = kd_numbers(kb[k / 2] >> sh, zb, sb);
-                const uint32_t a2 = kd_numbers(ka[k / 2] >> (sh + 4), za, sa), a3 = kd_numbers(kb[k / 2] >> (sh + 4), zb, sb);
+                for (int n = 0; n < NT; ++n) kd_mma(s[t][n], za, zb, za, zb, qz[n][0], qz[n][1]);
 #pragma unroll
-                for (int n = 0; n < NT; ++n) kd_mma(s[n], a0, a1, a2, a3, qf[n][k][0], qf[n][k][1]);
+                for (int k = 0; k < HD / 16; ++k) {
+                    const int sh = 8 * (k & 1);
+                    const uint32_t a0 = kd_scaled(ka[k / 2] >> sh, sa, fa), a1 = kd_scaled(kb[k / 2] >> sh, sb, fb);
+                    const uint32_t a2 = kd_scaled(ka[k / 2] >> (sh + 4), sa, fa), a3 = kd_scaled(kb[k / 2] >> (sh + 4), sb, fb);
+#pragma unroll
+                    for (int n = 0; n < NT; ++n) kd_mma(s[t][n], a0, a1, a2, a3, qf[n][k][0], qf[n][k][1]);
+                }
             }
             const bool part_hidden = base + KD_KEYS - 1 > see_all_to || base < see_all_from;        // the same for the warp
-            uint32_t w0 = vw[vk0 * (HD / KV4_GROUP) + r * (HD / 8) / KV4_GROUP], w1 = vw[vk1 * (HD / KV4_GROUP) + r * (HD / 8) / KV4_GROUP];
-            uint32_t w2 = vw[(vk0 + 8) * (HD / KV4_GROUP) + r * (HD / 8) / KV4_GROUP], w3 = vw[(vk1 + 8) * (HD / KV4_GROUP) + r * (HD / 8) / KV4_GROUP];
+            if (part_hidden) {
+                // a hidden key counts for nothing whatever it holds: its weight is 0, and a value that is not finite is taken as 0 below and
+                // gives those that see it a score of NaN instead
+#pragma unroll
+                for (int t = 0; t < TILES; ++t)
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        const int row = 16 * t + key_r + 8 * h, key = base + row;
+                        bool bad = false;
+#pragma unroll
+                        for (int g = 0; g < GROUPS; ++g) bad |= kv4_is_nan(vw[row * GROUPS + g]);
+#pragma unroll
+                        for (int n = 0; n < NT; ++n)
+#pragma unroll
+                            for (int e = 0; e < 2; ++e) {
+                                if (bad) s[t][n][2 * h + e] = __uint_as_float(0x7fffffffu);
+                                if (key > last_key[n][e] || key < first_key[n][e]) s[t][n][2 * h + e] = -INFINITY;
+                            }
+                    }
+            }
+            bool raised = false;
 #pragma unroll
             for (int n = 0; n < NT; ++n)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) s[n][e] *= scale_log2;
-            if (part_hidden) {
-                // a hidden key counts for nothing whatever it holds: its weight is 0, and a value that is not finite is taken as 0 here and
-                // gives those that see it a score of NaN instead
-                bool bad[2] = {false, false};
+                for (int e = 0; e < 2; ++e) {
+                    float top = fmaxf(s[0][n][e], s[0][n][e + 2]);
 #pragma unroll
-                for (int g = 0; g < HD / KV4_GROUP; ++g) {
-                    bad[0] |= kv4_is_nan(vw[key_r * (HD / KV4_GROUP) + g]);
-                    bad[1] |= kv4_is_nan(vw[(key_r + 8) * (HD / KV4_GROUP) + g]);
+                    for (int t = 1; t < TILES; ++t) top = fmaxf(top, fmaxf(s[t][n][e], s[t][n][e + 2]));
+                    raised |= top > over[n][e];
                 }
-#pragma unroll
-                for (int n = 0; n < NT; ++n)
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        const int key = base + key_r + (e >> 1) * 8;
-                        if (bad[e >> 1]) s[n][e] = __uint_as_float(0x7fffffffu);
-                        if (key > last_key[n][e & 1] || key < first_key[n][e & 1]) s[n][e] = -INFINITY;
-                    }
-                if (base + vk0 >= len || kv4_is_nan(w0)) w0 = 0;
-                if (base + vk1 >= len || kv4_is_nan(w1)) w1 = 0;
-                if (base + vk0 + 8 >= len || kv4_is_nan(w2)) w2 = 0;
-                if (base + vk1 + 8 >= len || kv4_is_nan(w3)) w3 = 0;
-            }
-            // P = 2^(S - reference)
-            bool over = false;
-#pragma unroll
-            for (int n = 0; n < NT; ++n) over |= fmaxf(s[n][0], s[n][2]) > m[n][0] + KD_RAISE || fmaxf(s[n][1], s[n][3]) > m[n][1] + KD_RAISE;
-            if (__any_sync(0xffffffffu, over)) {
+            if (__any_sync(0xffffffffu, raised)) {
 #pragma unroll
                 for (int n = 0; n < NT; ++n) {
                     float f[2];
 #pragma unroll
                     for (int e = 0; e < 2; ++e) {
-                        float top = fmaxf(s[n][e], s[n][e + 2]);
+                        float top = fmaxf(s[0][n][e], s[0][n][e + 2]);
+#pragma unroll
+                        for (int t = 1; t < TILES; ++t) top = fmaxf(top, fmaxf(s[t][n][e], s[t][n][e + 2]));
                         top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 4));
                         top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
                         top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
                         const float up = fmaxf(m[n][e], top);
-                        f[e] = up == m[n][e] ? 1.f : exp2f(m[n][e] - up);
+                        f[e] = up == m[n][e] ? 1.f : m[n][e] == -INFINITY ? 0.f : kd_exp2((m[n][e] - up) * scale_log2);
                         m[n][e] = up;
-                        l[n][e] *= f[e];
+                        over[n][e] = up + raise;
+                        shift[n][e] = up == -INFINITY ? 0.f : -up * scale_log2;
                     }
 #pragma unroll
-                    for (int k = 0; k < HD / 16; ++k) {
-                        o[n][k][0] *= f[0];
-                        o[n][k][1] *= f[1];
-                        o[n][k][2] *= f[0];
-                        o[n][k][3] *= f[1];
+                    for (int k = 0; k <= HD / 16; ++k) {
+                        float* x = k < HD / 16 ? o[n][k] : l[n];
+                        x[0] *= f[0];
+                        x[1] *= f[1];
+                        x[2] *= f[0];
+                        x[3] *= f[1];
                     }
                 }
             }
-            uint32_t pb[NT][2];
 #pragma unroll
-            for (int n = 0; n < NT; ++n) {
-                const float r0 = m[n][0] == -INFINITY ? 0.f : m[n][0], r1 = m[n][1] == -INFINITY ? 0.f : m[n][1];
-                const uint32_t lo = kd_pack(kd_exp2(s[n][0] - r0), kd_exp2(s[n][1] - r1)), hi = kd_pack(kd_exp2(s[n][2] - r0), kd_exp2(s[n][3] - r1));
-                // the sum of the weights as they are rounded for the product
-                l[n][0] += __uint_as_float(lo << 16) + __uint_as_float(hi << 16);
-                l[n][1] += __uint_as_float(lo & 0xffff0000u) + __uint_as_float(hi & 0xffff0000u);
-                pb[n][0] = kd_transpose(lo);
-                pb[n][1] = kd_transpose(hi);
-            }
-            // O^T += V^T P^T
-            const uint32_t w01 = __byte_perm(w0, w1, 0x5410), w23 = __byte_perm(w2, w3, 0x5410);
-            const uint32_t z01 = (w01 & 0x000f000fu) | 0x43004300u, s01 = w01 & 0xfff0fff0u;
-            const uint32_t z23 = (w23 & 0x000f000fu) | 0x43004300u, s23 = w23 & 0xfff0fff0u;
-            constexpr int VW = HD / 64;                     // words of codes of a lane's numbers of a value
-            uint32_t v0[VW], v1[VW], v2[VW], v3[VW];
-            const unsigned char* pv = vt + r * (HD / 16);
-            if constexpr (VW == 2) {
-                const uint2 x0 = *reinterpret_cast<const uint2*>(pv + vk0 * (HD / 2)), x1 = *reinterpret_cast<const uint2*>(pv + vk1 * (HD / 2));
-                const uint2 x2 = *reinterpret_cast<const uint2*>(pv + (vk0 + 8) * (HD / 2)), x3 = *reinterpret_cast<const uint2*>(pv + (vk1 + 8) * (HD / 2));
-                v0[0] = x0.x; v0[1] = x0.y; v1[0] = x1.x; v1[1] = x1.y; v2[0] = x2.x; v2[1] = x2.y; v3[0] = x3.x; v3[1] = x3.y;
-            } else {
-                v0[0] = *reinterpret_cast<const uint32_t*>(pv + vk0 * (HD / 2));
-                v1[0] = *reinterpret_cast<const uint32_t*>(pv + vk1 * (HD / 2));
-                v2[0] = *reinterpret_cast<const uint32_t*>(pv + (vk0 + 8) * (HD / 2));
-                v3[0] = *reinterpret_cast<const uint32_t*>(pv + (vk1 + 8) * (HD / 2));
-            }
+            for (int t = 0; t < TILES; ++t) {
+                // P = 2^(S - reference)
+                uint32_t pb[NT][2];
 #pragma unroll
-            for (int w = 0; w < VW; ++w) {
-                const uint32_t lo01 = __byte_perm(v0[w], v1[w], 0x5410), hi01 = __byte_perm(v0[w], v1[w], 0x7632);
-                const uint32_t lo23 = __byte_perm(v2[w], v3[w], 0x5410), hi23 = __byte_perm(v2[w], v3[w], 0x7632);
+                for (int n = 0; n < NT; ++n) {
+                    float p[4];
 #pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const uint32_t a0 = kd_numbers(lo01 >> (4 * j), z01, s01), a1 = kd_numbers(hi01 >> (4 * j), z01, s01);
-                    const uint32_t a2 = kd_numbers(lo23 >> (4 * j), z23, s23), a3 = kd_numbers(hi23 >> (4 * j), z23, s23);
+                    for (int e = 0; e < 4; ++e) p[e] = kd_exp2(fmaf(s[t][n][e], scale_log2, shift[n][e & 1]));
+                    pb[n][0] = kd_transpose(kd_pack(p[0], p[1]));
+                    pb[n][1] = kd_transpose(kd_pack(p[2], p[3]));
+                }
+                // O^T += V^T P^T
+                const uint16_t* words = vw + r * (HD / 8) / KV4_GROUP;
+                const int row0 = 16 * t + vk0, row1 = 16 * t + vk1;
+                uint32_t w0 = words[row0 * GROUPS], w1 = words[row1 * GROUPS], w2 = words[(row0 + 8) * GROUPS], w3 = words[(row1 + 8) * GROUPS];
+                if (part_hidden) {
+                    if (base + row0 >= len || kv4_is_nan(w0)) w0 = 0;
+                    if (base + row1 >= len || kv4_is_nan(w1)) w1 = 0;
+                    if (base + row0 + 8 >= len || kv4_is_nan(w2)) w2 = 0;
+                    if (base + row1 + 8 >= len || kv4_is_nan(w3)) w3 = 0;
+                }
+                const uint32_t w01 = __byte_perm(w0, w1, 0x5410), w23 = __byte_perm(w2, w3, 0x5410);
+                const uint32_t s01 = w01 & 0xfff0fff0u, s23 = w23 & 0xfff0fff0u, f01 = kd_off(s01), f23 = kd_off(s23);
+                const uint32_t z01 = kd_scaled(w01, s01, f01), z23 = kd_scaled(w23, s23, f23);
 #pragma unroll
-                    for (int n = 0; n < NT; ++n) kd_mma(o[n][4 * w + j], a0, a1, a2, a3, pb[n][0], pb[n][1]);
+                for (int n = 0; n < NT; ++n) kd_mma(l[n], 0x3f803f80u, z01, 0x3f803f80u, z23, pb[n][0], pb[n][1]);
+                constexpr int VW = HD / 64;                 // words of codes of a lane's numbers of a value
+                uint32_t v0[VW], v1[VW], v2[VW], v3[VW];
+                const unsigned char* pv = vt + r * (HD / 16);
+                if constexpr (VW == 2) {
+                    const uint2 x0 = *reinterpret_cast<const uint2*>(pv + row0 * (HD / 2)), x1 = *reinterpret_cast<const uint2*>(pv + row1 * (HD / 2));
+                    const uint2 x2 = *reinterpret_cast<const uint2*>(pv + (row0 + 8) * (HD / 2)), x3 = *reinterpret_cast<const uint2*>(pv + (row1 + 8) * (HD / 2));
+                    v0[0] = x0.x; v0[1] = x0.y; v1[0] = x1.x; v1[1] = x1.y; v2[0] = x2.x; v2[1] = x2.y; v3[0] = x3.x; v3[1] = x3.y;
+                } else {
+                    v0[0] = *reinterpret_cast<const uint32_t*>(pv + row0 * (HD / 2));
+                    v1[0] = *reinterpret_cast<const uint32_t*>(pv + row1 * (HD / 2));
+                    v2[0] = *reinterpret_cast<const uint32_t*>(pv + (row0 + 8) * (HD / 2));
+                    v3[0] = *reinterpret_cast<const uint32_t*>(pv + (row1 + 8) * (HD / 2));
+                }
+#pragma unroll
+                for (int w = 0; w < VW; ++w) {
+                    const uint32_t lo01 = __byte_perm(v0[w], v1[w], 0x5410), hi01 = __byte_perm(v0[w], v1[w], 0x7632);
+                    const uint32_t lo23 = __byte_perm(v2[w], v3[w], 0x5410), hi23 = __byte_perm(v2[w], v3[w], 0x7632);
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        const uint32_t a0 = kd_scaled(lo01 >> (4 * j), s01, f01), a1 = kd_scaled(hi01 >> (4 * j), s01, f01);
+                        const uint32_t a2 = kd_scaled(lo23 >> (4 * j), s23, f23), a3 = kd_scaled(hi23 >> (4 * j), s23, f23);
+#pragma unroll
+                        for (int n = 0; n < NT; ++n) kd_mma(o[n][4 * w + j], a0, a1, a2, a3, pb[n][0], pb[n][1]);
+                    }
                 }
             }
         }
@@ -423,20 +466,16 @@ kv4_attn_rows_kernel(const bf16* __restrict__ q, const unsigned char* __restrict
     for (int n = 0; n < NT; ++n) {
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-            float sum = l[n][e];
-            sum += __shfl_xor_sync(0xffffffffu, sum, 4);
-            sum += __shfl_xor_sync(0xffffffffu, sum, 8);
-            sum += __shfl_xor_sync(0xffffffffu, sum, 16);
             const int col = n * 8 + 2 * c + e;
             float* dst = join_o + (warp * 8 * NT + col) * Smem::COL + r;
 #pragma unroll
             for (int k = 0; k < HD / 16; ++k) {
-                dst[16 * k] = o[n][k][e];
-                dst[16 * k + 8] = o[n][k][e + 2];
+                dst[16 * k] = o[n][k][e] - l[n][e + 2];
+                dst[16 * k + 8] = o[n][k][e + 2] - l[n][e + 2];
             }
             if (r == 0) {
-                join_ml[(warp * 8 * NT + col) * 2] = m[n][e];
-                join_ml[(warp * 8 * NT + col) * 2 + 1] = sum;
+                join_ml[(warp * 8 * NT + col) * 2] = m[n][e] == -INFINITY ? -INFINITY : m[n][e] * scale_log2;
+                join_ml[(warp * 8 * NT + col) * 2 + 1] = l[n][e];
             }
         }
     }
@@ -532,7 +571,7 @@ static int kv4_launch_rows(const bf16* q, const unsigned char* pool, const int* 
     if (rows > 2147483647ll) return qwb_fail(QWB_ERR_ARG, "kv4_attention: %lld rows of queries", rows);
     float* part_ml = scratch ? scratch + (size_t)rows * max_runs * HD : nullptr;
     qwb_launch(kernel, dim3((unsigned)(tiles * max_runs), Hkv, B), KD_WARPS * 32, Smem::BYTES, stream, q, pool, page_table, cu, pos0, out, scratch, part_ml, T, B,
-               pool_pages, Hq, Hkv, table_width, scale * 1.4426950408889634f, window, (int)tiles, max_runs);
+               pool_pages, Hq, Hkv, table_width, fabsf(scale) * 1.4426950408889634f, scale < 0.f ? 0x80008000u : 0u, window, (int)tiles, max_runs);
     if (max_runs > 1)
         qwb_launch(kv4_attn_join_kernel<HD>, dim3((unsigned)((rows + 3) / 4)), 128, 0, stream, scratch, part_ml, cu, pos0, tok_seq, out, (int)rows, B, Hq, table_width,
                    window, max_runs);

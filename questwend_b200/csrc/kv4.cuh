@@ -7,7 +7,8 @@
 // whatever type and order, reads the same numbers.  (A step with the 8 bits of a bfloat16 would be off by 0.2 % instead of
 // 2 % on average; the codes' own rounding is 14 times larger than either, and z would have needed bytes of its own.)
 // A group of zeros, or whose step would lie under 2^-126, has step 0 and stands for zeros.  A group that holds a number that
-// is not finite stands for NaN: what sees the token is NaN and nothing is lost silently.
+// is not finite, or whose step would be 2^120 or more (so that 128 s is a number), stands for NaN: what sees the token is NaN and nothing
+// is lost silently.
 //
 // A page of 64 tokens and one head: 64 rows of key codes (hd / 2 bytes, the lower half of a byte first), 64 rows of the
 // keys' words (hd / 32 of 16 bits: the bits of s as a bfloat16, whose lowest 4 are zero, with z in them), then the values' codes

@@ -17,7 +17,7 @@ __device__ __forceinline__ uint32_t kv4_word(double lo, double hi, bool finite, 
     const long long up = __double_as_longlong(t) + (1ll << 48);                         // to 4 significant bits: 3 of the 52 behind the point stay
     const double step = __longlong_as_double(up & ~((1ll << 49) - 1));
     s = z = 0.f;
-    if (!finite || !(step < 3.0e38)) return 0x7fc0u;
+    if (!finite || !(step < 1.329227995784916e36)) return 0x7fc0u;
     if (step < 1.1754943508222875e-38) return 0u;
     s = (float)step;
     z = (float)fmin(rint(-lo / step), 15.0);

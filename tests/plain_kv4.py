@@ -16,7 +16,7 @@ def quantise(x):
     with np.errstate(over="ignore"):
         mantissa, exponent = np.frexp((hi - lo) / 15)
         s = np.ldexp(np.floor(mantissa * 16 + 0.5) / 16, exponent)
-    finite &= s < 3e38
+    finite &= s < 2.0 ** 120
     s = np.where(finite & (s >= 2.0 ** -126), s, 0.0)
     d = np.where(s > 0, s, 1.0)
     z = np.where(s > 0, np.minimum(np.rint(-lo / d), 15), 0)

@@ -118,7 +118,7 @@ def test_store_of_groups_at_the_border():
     x[1, hd:] = np.tile(np.arange(32) / 2, 8)
     x[2, hd:] = -np.tile(np.arange(32) / 2, 8)
     x[3, hd:], x[4, hd:], x[5, hd:], x[6, hd:] = 2.5, -1.0, 1e-42, 0.0
-    x[7, hd:] = np.tile([3e38, -3e38] + [1.0] * 30, 8)
+    x[7, hd:] = np.tile([9e36, -9e36] + [1.0] * 30 + [3e37] + [1.0] * 31, 4)
     x[8, hd], x[9, 2 * hd + 5], x[10, hd + 40] = np.nan, np.inf, -np.inf
     x[11, hd:] = np.tile(np.nextafter(np.float32(np.arange(32) / 2 - 3.5), np.float32(100)), 8)
     slots = np.arange(12, dtype=np.int32)

@@ -41,15 +41,15 @@ def test_a_number_is_within_half_a_step_and_exact_in_bfloat16():
 
 
 def test_what_is_not_finite_and_what_is_tiny():
-    x = np.ones((4, 64))
+    x = np.ones((5, 64))
     x[0, 3], x[1, 40], x[2] = np.nan, np.inf, 1e-45
-    x[3, 0], x[3, 1] = 3e38, -3e38
+    x[3, 0], x[3, 1], x[4, 0] = 9e36, -9e36, 3e37             # a step of 1.2e36; of 2e36, 2^120 is 1.33e36
     y = pk.stands_for(*pk.quantise(x))
     one = 15 * 0.065625                                         # a fifteenth to 4 significant bits is 0.0625 1.05
     assert np.isnan(y[0, :32]).all() and np.isclose(y[0, 32:], one, rtol=1e-12).all()
     assert np.isnan(y[1, 32:]).all() and np.isclose(y[1, :32], one, rtol=1e-12).all()
     assert (y[2] == 0).all()
-    assert np.isfinite(y[3]).all() and abs(y[3, 0] / 3e38 - 1) < 0.07
+    assert np.isfinite(y[3]).all() and abs(y[3, 0] / 9e36 - 1) < 0.1 and np.isnan(y[4, :32]).all()
 
 
 @pytest.mark.parametrize("call", [
