@@ -189,7 +189,7 @@ template <int HD, int NT>
 __global__ void __launch_bounds__(KD_WARPS * 32, NT == 1 ? 8 : 5)
 kv4_attn_rows_kernel(const bf16* __restrict__ q, const unsigned char* __restrict__ pool, const int* __restrict__ page_table,
                      const int* __restrict__ cu_seqlens, const int* __restrict__ pos0, bf16* __restrict__ out, float* __restrict__ part_o,
-                     float* __restrict__ part_ml, int T, int B, int pool_pages, int Hq, int Hkv, int table_width, float scale_log2, uint32_t flip, int window,
+                     float* __restrict__ part_ml, int T, int B, int pool_pages, int G, int Hkv, int table_width, float scale_log2, uint32_t flip, int window,
                      int tiles, int max_runs) {
     pdl_wait();
     pdl_launch_dependents();
@@ -197,8 +197,10 @@ kv4_attn_rows_kernel(const bf16* __restrict__ q, const unsigned char* __restrict
     using Smem = KdSmem<HD, NT>;
     extern __shared__ __align__(128) unsigned char smem[];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, r = lane >> 2, c = lane & 3;
-    const int tile = blockIdx.x % tiles, run = blockIdx.x / tiles, kvh = blockIdx.y, b = blockIdx.z;
-    const int G = Hq / Hkv;
+    const int run = tiles == 1 ? blockIdx.x : blockIdx.x / tiles, tile = blockIdx.x - run * tiles, kvh = blockIdx.y, b = blockIdx.z;
+    const int Hq = Hkv * G;
+    const float one_in_g = 1.f / (float)G;
+    auto by_g = [&](int x) { return (int)(((float)x + 0.5f) * one_in_g); };             // x / G: exact for x below 2^20 (the launcher's bound)
     if (blockIdx.x == 0 && kvh == 0 && b == 0) {            // tokens behind the last sequence's: zeros
         for (long long i = (long long)max(cu_seqlens[B], 0) * Hq * HD + threadIdx.x; i < (long long)T * Hq * HD; i += KD_WARPS * 32) out[i] = from_f32<bf16>(0.f);
     }
@@ -223,12 +225,12 @@ kv4_attn_rows_kernel(const bf16* __restrict__ q, const unsigned char* __restrict
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
             const int col = min(col0 + n * 8 + 2 * c + e, cols - 1);
-            last_key[n][e] = p0 + col / G;
-            first_key[n][e] = window > 0 ? p0 + col / G - window + 1 : 0;
+            last_key[n][e] = p0 + by_g(col);
+            first_key[n][e] = window > 0 ? last_key[n][e] - window + 1 : 0;
         }
-        const int col = col0 + n * 8 + r;
+        const int col = col0 + n * 8 + r, tok = by_g(col);
         const bool live = col < cols;
-        const bf16* src = q + ((size_t)(t0 + (live ? col / G : 0)) * Hq + kvh * G + (live ? col % G : 0)) * HD + c * (HD / 4);
+        const bf16* src = q + ((size_t)(t0 + tok) * Hq + kvh * G + col - tok * G) * HD + c * (HD / 4);
         float sum = 0.f;
 #pragma unroll
         for (int w = 0; w < HD / 32; ++w) {
@@ -249,8 +251,8 @@ kv4_attn_rows_kernel(const bf16* __restrict__ q, const unsigned char* __restrict
         qz[n][0] = kd_pack(-hi, -mid);
         qz[n][1] = kd_pack(hi + mid - sum, 0.f);
     }
-    const int see_all_from = window > 0 ? p0 + min(col0 + 8 * NT, cols) / G - window + 1 : 0;    // keys below may be hidden from a column,
-    const int see_all_to = p0 + col0 / G;                                                       // keys above as well
+    const int see_all_from = window > 0 ? p0 + by_g(min(col0 + 8 * NT, cols) - 1) - window + 1 : 0;    // keys below may be hidden from a column,
+    const int see_all_to = p0 + by_g(col0);                                                       // keys above as well
 
     unsigned char* ring = smem + (size_t)warp * KD_STAGES * Tile::BYTES;
     int slot_in = 0, slot_out = 0;
@@ -480,32 +482,40 @@ kv4_attn_rows_kernel(const bf16* __restrict__ q, const unsigned char* __restrict
         }
     }
     __syncthreads();
-    for (int x = threadIdx.x; x < 8 * NT * HD; x += KD_WARPS * 32) {
-        const int col = x / HD, at = x % HD;
+    // a warp every second column, a lane four neighbouring places of it (with heads of 64 two)
+    constexpr int E = HD / 32;
+    for (int col = warp; col < 8 * NT; col += KD_WARPS) {
         if (col0 + col >= cols) break;
-        float top = -INFINITY, total = 0.f, y = 0.f;
-#pragma unroll
-        for (int w = 0; w < KD_WARPS; ++w) top = fmaxf(top, join_ml[(w * 8 * NT + col) * 2]);
+        float mw[KD_WARPS], lw[KD_WARPS], y[E] = {}, top = -INFINITY, total = 0.f;
 #pragma unroll
         for (int w = 0; w < KD_WARPS; ++w) {
-            const float mw = join_ml[(w * 8 * NT + col) * 2], lw = join_ml[(w * 8 * NT + col) * 2 + 1];
-            if (lw != 0.f) {
-                const float f = mw == top ? 1.f : exp2f(mw - top);
-                total += f * lw;
-                y += f * join_o[(w * 8 * NT + col) * Smem::COL + at];
+            mw[w] = join_ml[(w * 8 * NT + col) * 2];
+            lw[w] = join_ml[(w * 8 * NT + col) * 2 + 1];
+            top = fmaxf(top, mw[w]);
+        }
+#pragma unroll
+        for (int w = 0; w < KD_WARPS; ++w) {
+            const float f = lw[w] == 0.f ? 0.f : mw[w] == top ? 1.f : kd_exp2(mw[w] - top);
+            const float* src = join_o + (w * 8 * NT + col) * Smem::COL + lane * E;
+            total += f * lw[w];
+            if (lw[w] != 0.f) {
+#pragma unroll
+                for (int e = 0; e < E; ++e) y[e] += f * src[e];
             }
         }
-        const int t = t0 + (col0 + col) / G, h = kvh * G + (col0 + col) % G;
-        const size_t row = (size_t)t * Hq + h;
+        const int tok = by_g(col0 + col);
+        const size_t row = (size_t)(t0 + tok) * Hq + kvh * G + col0 + col - tok * G;
         if (runs <= 1) {
-            const int mma = at / 16, half = (at >> 3) & 1, d = (at & 7) * (HD / 8) + 8 * (mma >> 2) + 4 * half + (mma & 3);
-            out[row * HD + d] = from_f32<bf16>(total == 0.f ? 0.f : y / total);
-        } else {
-            part_o[(row * max_runs + run) * HD + at] = y;
-            if (at == 0) {
-                part_ml[(row * max_runs + run) * 2] = top;
-                part_ml[(row * max_runs + run) * 2 + 1] = total;
+#pragma unroll
+            for (int e = 0; e < E; ++e) {
+                const int at = lane * E + e, mma = at / 16, half = (at >> 3) & 1, d = (at & 7) * (HD / 8) + 8 * (mma >> 2) + 4 * half + (mma & 3);
+                out[row * HD + d] = from_f32<bf16>(total == 0.f ? 0.f : y[e] / total);
             }
+        } else {
+            float* dst = part_o + (row * max_runs + run) * HD + lane * E;
+            if constexpr (E == 4) *reinterpret_cast<float4*>(dst) = make_float4(y[0], y[1], y[2], y[3]);
+            else *reinterpret_cast<float2*>(dst) = make_float2(y[0], y[1]);
+            if (lane == 0) *reinterpret_cast<float2*>(part_ml + (row * max_runs + run) * 2) = make_float2(top, total);
         }
     }
 }
@@ -531,18 +541,21 @@ kv4_attn_join_kernel(const float* __restrict__ part_o, const float* __restrict__
     top = warp_max(top);
     constexpr int E = HD / 32;
     float y[E] = {}, total = 0.f;
+#pragma unroll 4
     for (int i = 0; i < runs; ++i) {
-        const float lw = ml[2 * i + 1];
-        if (lw == 0.f) continue;
-        const float mw = ml[2 * i], f = mw == top ? 1.f : exp2f(mw - top);
-        total += f * lw;
-        const float* src = part_o + ((size_t)row * max_runs + i) * HD;
+        const float2 x = *reinterpret_cast<const float2*>(ml + 2 * i);
+        const float f = x.y == 0.f ? 0.f : x.x == top ? 1.f : kd_exp2(x.x - top);
+        float v[E];
+        const float* src = part_o + ((size_t)row * max_runs + i) * HD + lane * E;
+        if constexpr (E == 4) *reinterpret_cast<float4*>(v) = *reinterpret_cast<const float4*>(src);
+        else *reinterpret_cast<float2*>(v) = *reinterpret_cast<const float2*>(src);
+        total += f * x.y;
 #pragma unroll
-        for (int e = 0; e < E; ++e) y[e] += f * src[e * 32 + lane];
+        for (int e = 0; e < E; ++e) y[e] = x.y == 0.f ? y[e] : fmaf(f, v[e], y[e]);
     }
 #pragma unroll
     for (int e = 0; e < E; ++e) {
-        const int at = e * 32 + lane, mma = at / 16, half = (at >> 3) & 1, d = (at & 7) * (HD / 8) + 8 * (mma >> 2) + 4 * half + (mma & 3);
+        const int at = lane * E + e, mma = at / 16, half = (at >> 3) & 1, d = (at & 7) * (HD / 8) + 8 * (mma >> 2) + 4 * half + (mma & 3);
         out[(size_t)row * HD + d] = from_f32<bf16>(total == 0.f ? 0.f : y[e] / total);
     }
 }
@@ -565,13 +578,13 @@ static int kv4_launch_rows(const bf16* q, const unsigned char* pool, const int* 
     auto kernel = kv4_attn_rows_kernel<HD, NT>;
     static_assert(Smem::BYTES <= 48 * 1024, "more needs an attribute of the kernel");
     const long long tiles = ((long long)max_new * (Hq / Hkv) + 8 * NT - 1) / (8 * NT);
-    if (tiles * max_runs > 2147483647ll || Hkv > 65535 || B > 65535)
+    if (tiles * max_runs > 2147483647ll || tiles * 8 * NT >= 1 << 20 || Hkv > 65535 || B > 65535)
         return qwb_fail(QWB_ERR_ARG, "kv4_attention: %d sequences of up to %d new tokens, %d heads: too many blocks", B, max_new, Hkv);
     const long long rows = (long long)T * Hq;
     if (rows > 2147483647ll) return qwb_fail(QWB_ERR_ARG, "kv4_attention: %lld rows of queries", rows);
     float* part_ml = scratch ? scratch + (size_t)rows * max_runs * HD : nullptr;
     qwb_launch(kernel, dim3((unsigned)(tiles * max_runs), Hkv, B), KD_WARPS * 32, Smem::BYTES, stream, q, pool, page_table, cu, pos0, out, scratch, part_ml, T, B,
-               pool_pages, Hq, Hkv, table_width, fabsf(scale) * 1.4426950408889634f, scale < 0.f ? 0x80008000u : 0u, window, (int)tiles, max_runs);
+               pool_pages, Hq / Hkv, Hkv, table_width, fabsf(scale) * 1.4426950408889634f, scale < 0.f ? 0x80008000u : 0u, window, (int)tiles, max_runs);
     if (max_runs > 1)
         qwb_launch(kv4_attn_join_kernel<HD>, dim3((unsigned)((rows + 3) / 4)), 128, 0, stream, scratch, part_ml, cu, pos0, tok_seq, out, (int)rows, B, Hq, table_width,
                    window, max_runs);
