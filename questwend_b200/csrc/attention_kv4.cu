@@ -204,10 +204,10 @@ kv4_attn_rows_kernel(const bf16* __restrict__ q, const unsigned char* __restrict
     if (blockIdx.x == 0 && kvh == 0 && b == 0) {            // tokens behind the last sequence's: zeros
         for (long long i = (long long)max(cu_seqlens[B], 0) * Hq * HD + threadIdx.x; i < (long long)T * Hq * HD; i += KD_WARPS * 32) out[i] = from_f32<bf16>(0.f);
     }
-    const int t0 = cu_seqlens[b], n_new = min(cu_seqlens[b + 1], T) - t0;
-    const int col0 = tile * 8 * NT, cols = n_new * G;
+    const int t0 = cu_seqlens[b], t1 = cu_seqlens[b + 1], p0 = pos0[b];
+    const int n_new = min(t1, T) - t0, col0 = tile * 8 * NT, cols = n_new * G;
     if (t0 < 0 || n_new <= 0 || col0 >= cols) return;
-    const int p0 = pos0[b], len = p0 + n_new;
+    const int len = p0 + n_new;
     const Kv4Runs cut = kv4_runs(p0, len, window, table_width);
     const int runs = min(cut.runs, max_runs);               // a sequence beyond max_len: cut off there, never written beyond the scratch
     if (run >= runs && run > 0) return;
@@ -216,6 +216,31 @@ kv4_attn_rows_kernel(const bf16* __restrict__ q, const unsigned char* __restrict
     int my_page = -1;                                       // lane i: the run's i-th page
     if (lane < n_pages) my_page = table[lane];
     if (my_page >= pool_pages) my_page = -1;
+
+    unsigned char* ring = smem + (size_t)warp * KD_STAGES * Tile::BYTES;
+    int slot_in = 0, slot_out = 0;
+    auto ask = [&](int i) {                                 // the warp's 16 keys of the run's i-th page
+        const int page = __shfl_sync(0xffffffffu, my_page, i & 31);
+        if (i < n_pages && page >= 0) {
+            unsigned char* dst = ring + slot_in * Tile::BYTES;
+            const unsigned char* src = pool + ((size_t)page * Hkv + kvh) * kv4_page_bytes(HD) + warp * Tile::CODES;
+            constexpr int WORDS_AT = kv4_code_bytes(HD);
+#pragma unroll
+            for (int o = 0; o < Tile::CODES; o += 512) {
+                kd_copy16(dst + o + lane * 16, src + o + lane * 16);
+                kd_copy16(dst + Tile::HALF + o + lane * 16, src + kv4_half_bytes(HD) + o + lane * 16);
+            }
+            constexpr int PIECES = Tile::WORDS / 16;
+            if (lane < 2 * PIECES) {
+                const int half = lane / PIECES, at = (lane % PIECES) * 16;
+                kd_copy16(dst + half * Tile::HALF + Tile::CODES + at, src + half * kv4_half_bytes(HD) + WORDS_AT - warp * Tile::CODES + warp * Tile::WORDS + at);
+            }
+        }
+        asm volatile("cp.async.commit_group;" ::: "memory");
+        slot_in = slot_in == KD_STAGES - 1 ? 0 : slot_in + 1;
+    };
+#pragma unroll
+    for (int i = 0; i < KD_STAGES - 1; ++i) ask(i);
 
     // this block's columns: their last and first key; the queries, in the order in which a lane holds the keys' numbers
     int last_key[NT][2], first_key[NT][2];
@@ -254,29 +279,6 @@ kv4_attn_rows_kernel(const bf16* __restrict__ q, const unsigned char* __restrict
     const int see_all_from = window > 0 ? p0 + by_g(min(col0 + 8 * NT, cols) - 1) - window + 1 : 0;    // keys below may be hidden from a column,
     const int see_all_to = p0 + by_g(col0);                                                       // keys above as well
 
-    unsigned char* ring = smem + (size_t)warp * KD_STAGES * Tile::BYTES;
-    int slot_in = 0, slot_out = 0;
-    auto ask = [&](int i) {                                 // the warp's 16 keys of the run's i-th page
-        const int page = __shfl_sync(0xffffffffu, my_page, i & 31);
-        if (i < n_pages && page >= 0) {
-            unsigned char* dst = ring + slot_in * Tile::BYTES;
-            const unsigned char* src = pool + ((size_t)page * Hkv + kvh) * kv4_page_bytes(HD) + warp * Tile::CODES;
-            constexpr int WORDS_AT = kv4_code_bytes(HD);
-#pragma unroll
-            for (int o = 0; o < Tile::CODES; o += 512) {
-                kd_copy16(dst + o + lane * 16, src + o + lane * 16);
-                kd_copy16(dst + Tile::HALF + o + lane * 16, src + kv4_half_bytes(HD) + o + lane * 16);
-            }
-            constexpr int PIECES = Tile::WORDS / 16;
-            if (lane < 2 * PIECES) {
-                const int half = lane / PIECES, at = (lane % PIECES) * 16;
-                kd_copy16(dst + half * Tile::HALF + Tile::CODES + at, src + half * kv4_half_bytes(HD) + WORDS_AT - warp * Tile::CODES + warp * Tile::WORDS + at);
-            }
-        }
-        asm volatile("cp.async.commit_group;" ::: "memory");
-        slot_in = slot_in == KD_STAGES - 1 ? 0 : slot_in + 1;
-    };
-
     // outputs; the weights' sums (0, 1: from rows of ones) and what the zero points add to a lane's outputs (2, 3); the reference of the raw scores, what passes it by 2^8, and -reference in the
     // exponent's units (0 while there is no reference: a weight of a hidden key is then 2^-infinity)
     float o[NT][HD / 16][4], l[NT][4], m[NT][2], over[NT][2], shift[NT][2];
@@ -289,8 +291,6 @@ kv4_attn_rows_kernel(const bf16* __restrict__ q, const unsigned char* __restrict
         m[n][0] = m[n][1] = over[n][0] = over[n][1] = -INFINITY;
         shift[n][0] = shift[n][1] = 0.f;
     }
-#pragma unroll
-    for (int i = 0; i < KD_STAGES - 1; ++i) ask(i);
     // row r of a tile is key `key_r` of the 16, row r + 8 the key 8 behind it: of the keys that one load takes from shared memory then
     // never two lie in the same banks
     const int key_r = (r & 1) ? 4 + ((r >> 1) ^ 1) : r >> 1;
@@ -520,43 +520,58 @@ kv4_attn_rows_kernel(const bf16* __restrict__ q, const unsigned char* __restrict
     }
 }
 
-// Joins the runs of a row (a warp each).
+// Joins the runs of a row: a block a row, a warp every fourth run, all loads on their way together.  What says how many runs there are was
+// there before the attention's blocks began, so it is read while the last of them still run (the kernel starts under their tail).
+#define KJ_WARPS 4
 template <int HD>
-__global__ void __launch_bounds__(128)
-kv4_attn_join_kernel(const float* __restrict__ part_o, const float* __restrict__ part_ml, const int* __restrict__ cu_seqlens,
-                     const int* __restrict__ pos0, const int* __restrict__ tok_seq, bf16* __restrict__ out, int rows, int B, int Hq, int table_width,
-                     int window, int max_runs) {
+__global__ void __launch_bounds__(KJ_WARPS * 32)
+kv4_attn_join_kernel(const float* part_o, const float* part_ml, const int* cu_seqlens, const int* pos0, const int* tok_seq, bf16* __restrict__ out, int T, int B,
+                     int Hq, int table_width, int window, int max_runs) {
+    __shared__ float join_o[KJ_WARPS][HD], join_ml[KJ_WARPS][2];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, t = blockIdx.x / Hq;
+    const size_t row = blockIdx.x;
+    const int b = __ldcg(tok_seq + t);
+    int runs = 0;
+    if (b >= 0 && b < B) {
+        const int t0 = __ldcg(cu_seqlens + b), t1 = __ldcg(cu_seqlens + b + 1), p0 = __ldcg(pos0 + b);
+        runs = min(kv4_runs(p0, p0 + min(t1, T) - t0, window, table_width).runs, max_runs);
+    }
     pdl_wait();
     pdl_launch_dependents();
-    const int lane = threadIdx.x & 31, row = blockIdx.x * 4 + (threadIdx.x >> 5);
-    if (row >= rows) return;
-    const int b = tok_seq[row / Hq];
-    if (b < 0 || b >= B) return;
-    const int p0 = pos0[b], len = p0 + min(cu_seqlens[b + 1], rows / Hq) - cu_seqlens[b];
-    const int runs = min(kv4_runs(p0, len, window, table_width).runs, max_runs);
     if (runs <= 1) return;
-    const float* ml = part_ml + (size_t)row * max_runs * 2;
-    float top = -INFINITY;
-    for (int i = lane; i < runs; i += 32) top = fmaxf(top, ml[2 * i]);
-    top = warp_max(top);
     constexpr int E = HD / 32;
-    float y[E] = {}, total = 0.f;
+    float top = -INFINITY, total = 0.f, y[E] = {};
 #pragma unroll 4
-    for (int i = 0; i < runs; ++i) {
-        const float2 x = *reinterpret_cast<const float2*>(ml + 2 * i);
-        const float f = x.y == 0.f ? 0.f : x.x == top ? 1.f : kd_exp2(x.x - top);
+    for (int i = warp; i < runs; i += KJ_WARPS) {
+        const float2 x = __ldcg(reinterpret_cast<const float2*>(part_ml + (row * max_runs + i) * 2));
         float v[E];
-        const float* src = part_o + ((size_t)row * max_runs + i) * HD + lane * E;
-        if constexpr (E == 4) *reinterpret_cast<float4*>(v) = *reinterpret_cast<const float4*>(src);
-        else *reinterpret_cast<float2*>(v) = *reinterpret_cast<const float2*>(src);
-        total += f * x.y;
+        const float* src = part_o + (row * max_runs + i) * HD + lane * E;
+        if constexpr (E == 4) *reinterpret_cast<float4*>(v) = __ldcg(reinterpret_cast<const float4*>(src));
+        else *reinterpret_cast<float2*>(v) = __ldcg(reinterpret_cast<const float2*>(src));
+        if (x.y == 0.f) continue;                           // a run that a row sees nothing of
+        const float up = fmaxf(top, x.x), keep = top == up ? 1.f : kd_exp2(top - up), f = x.x == up ? 1.f : kd_exp2(x.x - up);
+        total = total * keep + f * x.y;
 #pragma unroll
-        for (int e = 0; e < E; ++e) y[e] = x.y == 0.f ? y[e] : fmaf(f, v[e], y[e]);
+        for (int e = 0; e < E; ++e) y[e] = y[e] * keep + f * v[e];
+        top = up;
     }
 #pragma unroll
-    for (int e = 0; e < E; ++e) {
-        const int at = lane * E + e, mma = at / 16, half = (at >> 3) & 1, d = (at & 7) * (HD / 8) + 8 * (mma >> 2) + 4 * half + (mma & 3);
-        out[(size_t)row * HD + d] = from_f32<bf16>(total == 0.f ? 0.f : y[e] / total);
+    for (int e = 0; e < E; ++e) join_o[warp][lane * E + e] = y[e];
+    if (lane == 0) { join_ml[warp][0] = top; join_ml[warp][1] = total; }
+    __syncthreads();
+    for (int at = threadIdx.x; at < HD; at += KJ_WARPS * 32) {
+        float all = -INFINITY, sum = 0.f, o = 0.f;
+#pragma unroll
+        for (int w = 0; w < KJ_WARPS; ++w) all = fmaxf(all, join_ml[w][0]);
+#pragma unroll
+        for (int w = 0; w < KJ_WARPS; ++w) {
+            if (join_ml[w][1] == 0.f) continue;
+            const float f = join_ml[w][0] == all ? 1.f : kd_exp2(join_ml[w][0] - all);
+            sum += f * join_ml[w][1];
+            o += f * join_o[w][at];
+        }
+        const int mma = at / 16, half = (at >> 3) & 1, d = (at & 7) * (HD / 8) + 8 * (mma >> 2) + 4 * half + (mma & 3);
+        out[row * HD + d] = from_f32<bf16>(sum == 0.f ? 0.f : o / sum);
     }
 }
 
@@ -586,8 +601,8 @@ static int kv4_launch_rows(const bf16* q, const unsigned char* pool, const int* 
     qwb_launch(kernel, dim3((unsigned)(tiles * max_runs), Hkv, B), KD_WARPS * 32, Smem::BYTES, stream, q, pool, page_table, cu, pos0, out, scratch, part_ml, T, B,
                pool_pages, Hq / Hkv, Hkv, table_width, fabsf(scale) * 1.4426950408889634f, scale < 0.f ? 0x80008000u : 0u, window, (int)tiles, max_runs);
     if (max_runs > 1)
-        qwb_launch(kv4_attn_join_kernel<HD>, dim3((unsigned)((rows + 3) / 4)), 128, 0, stream, scratch, part_ml, cu, pos0, tok_seq, out, (int)rows, B, Hq, table_width,
-                   window, max_runs);
+        qwb_launch_early(kv4_attn_join_kernel<HD>, dim3((unsigned)rows), KJ_WARPS * 32, 0, stream, scratch, part_ml, cu, pos0, tok_seq, out, T, B, Hq,
+                        table_width, window, max_runs);
     return qwb_check_launch("kv4_attention");
 }
 

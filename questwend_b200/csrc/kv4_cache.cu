@@ -106,6 +106,178 @@ kv4_store_kernel(const float* __restrict__ qkv, const float* __restrict__ q_weig
     }
 }
 
+// The same for heads of 64 and 128 turned over all their numbers (or not at all), the common case.  HD / 8 lanes take a head: lane L of them
+// holds the numbers 4L..4L+3 and HD/2 + 4L..: a number and its rotation partner lie in one lane, and each of its two fours in the group of
+// 8 neighbouring lanes, so that norm and group cost three or four exchanges.  What bounds it is memory: 4 bytes read and (queries) 2 or (keys
+// and values) 9/16 written a number.  So only what decides goes through 64 bits: of keys the sum of squares, its root (32 bits and two
+// of Newton's steps) and the rotation; codes are found in 32 bits and checked against the border.
+__device__ __forceinline__ float kv4_nearest(float x, float s, float inv) {                // rint(x / s): a guess, and x - (guess +- 1/2) s, which is exact
+    float c = rintf(x * inv);
+    const float r = fmaf(-c, s, x), half = 0.5f * s;
+    const bool odd = (int)c & 1;
+    if (r > half || (r == half && odd)) c += 1.f;
+    else if (r < -half || (r == -half && odd)) c -= 1.f;
+    return c;
+}
+__device__ __forceinline__ float kv4_nearest(double x, float s, float inv) {
+    float c = rintf((float)x * inv);
+    const double r = fma(-(double)c, (double)s, x), half = 0.5 * (double)s;
+    const bool odd = (int)c & 1;
+    if (r > half || (r == half && odd)) c += 1.f;
+    else if (r < -half || (r == -half && odd)) c -= 1.f;
+    return c;
+}
+// Four numbers of a lane, and the group of 8 lanes' 32: codes (the first in the lowest bits), and the group's word.
+template <typename T>
+__device__ __forceinline__ uint32_t kv4_four(const T (&x)[4], unsigned mask, uint32_t& word) {
+    T lo = x[0], hi = x[0];
+    bool finite = true;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        finite &= fabs((double)x[i]) <= 3.4028234663852886e38;
+        lo = x[i] < lo ? x[i] : lo;
+        hi = x[i] > hi ? x[i] : hi;
+    }
+    lo = lo < T(0) ? lo : T(0);
+    hi = hi > T(0) ? hi : T(0);
+#pragma unroll
+    for (int o = 1; o < 8; o <<= 1) {
+        const T a = __shfl_xor_sync(mask, lo, o), b = __shfl_xor_sync(mask, hi, o);
+        lo = a < lo ? a : lo;
+        hi = b > hi ? b : hi;
+        finite &= (bool)__shfl_xor_sync(mask, (int)finite, o);
+    }
+    const double d = (double)hi - (double)lo;
+    double t = d * (1.0 / 15.0);                                                        // d / 15, its last bit corrected
+    t = fma(fma(-15.0, t, d), 1.0 / 15.0, t);
+    const double step = __longlong_as_double((__double_as_longlong(t) + (1ll << 48)) & ~((1ll << 49) - 1));
+    if (!finite || !(step < 1.329227995784916e36)) { word = 0x7fc0u; return 0u; }
+    if (step < 1.1754943508222875e-38) { word = 0u; return 0u; }
+    const float s = (float)step, inv = 1.f / s, z = fminf(kv4_nearest((T)-lo, s, inv), 15.f);
+    uint32_t codes = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) codes |= (uint32_t)(int)fminf(fmaxf(kv4_nearest(x[i], s, inv) + z, 0.f), 15.f) << (4 * i);
+    word = (__float_as_uint(s) >> 16) | (uint32_t)(int)z;
+    return codes;
+}
+
+template <typename TQ> __device__ __forceinline__ void kv4_put4(TQ* p, float a, float b, float c, float d);
+template <> __device__ __forceinline__ void kv4_put4<float>(float* p, float a, float b, float c, float d) { *reinterpret_cast<float4*>(p) = make_float4(a, b, c, d); }
+template <> __device__ __forceinline__ void kv4_put4<bf16>(bf16* p, float a, float b, float c, float d) {
+    __nv_bfloat162 v[2] = {__floats2bfloat162_rn(a, b), __floats2bfloat162_rn(c, d)};
+    *reinterpret_cast<uint2*>(p) = *reinterpret_cast<uint2*>(v);
+}
+
+#define KF_BLOCKS 1184              // as many are wanted of a call
+template <typename TQ, int HD>
+__global__ void __launch_bounds__(KS_WARPS * 32)
+kv4_store_fast_kernel(const float* __restrict__ qkv, const float* __restrict__ q_weight, const float* __restrict__ k_weight,
+                      const float* __restrict__ cos_t, const float* __restrict__ sin_t, const int* __restrict__ slot_map,
+                      TQ* __restrict__ q_out, unsigned char* __restrict__ pool, long long n_rows, int Hq, int Hkv, float eps, int store_kv) {
+    pdl_wait();
+    pdl_launch_dependents();
+    constexpr int LANES = HD / 8, HEADS = 32 / LANES;               // heads of a warp
+    const int t = blockIdx.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31, L = lane % LANES, of = lane / LANES;
+    const unsigned mask = HD == 128 ? 0xffffu << (16 * of) : 0xffu << (8 * of);
+    const int n_all = Hq + 2 * Hkv, n_heads = store_kv ? n_all : Hq;
+    const float4* row = reinterpret_cast<const float4*>(qkv + (size_t)t * n_all * HD);
+    float c[4] = {1.f, 1.f, 1.f, 1.f}, sn[4] = {};
+    if (cos_t) {
+        *reinterpret_cast<float4*>(c) = reinterpret_cast<const float4*>(cos_t + (size_t)t * (HD / 2))[L];
+        *reinterpret_cast<float4*>(sn) = reinterpret_cast<const float4*>(sin_t + (size_t)t * (HD / 2))[L];
+    }
+    const long long slot = slot_map[t];
+    const bool has_place = slot >= 0 && slot < n_rows;
+    for (int head = (blockIdx.y * KS_WARPS + warp) * HEADS + of; head < n_heads; head += gridDim.y * KS_WARPS * HEADS) {
+        float a[4], b[4];
+        *reinterpret_cast<float4*>(a) = row[(size_t)head * (HD / 4) + L];
+        *reinterpret_cast<float4*>(b) = row[(size_t)head * (HD / 4) + HD / 8 + L];
+        if (head < Hq) {
+            if (q_weight) {
+                float ss = 0.f, w[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) ss = fmaf(a[i], a[i], fmaf(b[i], b[i], ss));
+#pragma unroll
+                for (int o = 1; o < LANES; o <<= 1) ss += __shfl_xor_sync(mask, ss, o);
+                const float scale = 1.f / sqrtf(ss / (float)HD + eps);
+                *reinterpret_cast<float4*>(w) = reinterpret_cast<const float4*>(q_weight)[L];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) a[i] *= scale * w[i];
+                *reinterpret_cast<float4*>(w) = reinterpret_cast<const float4*>(q_weight)[HD / 8 + L];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) b[i] *= scale * w[i];
+            }
+            float x[4], y[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                x[i] = a[i] * c[i] - b[i] * sn[i];
+                y[i] = a[i] * sn[i] + b[i] * c[i];
+            }
+            TQ* dst = q_out + ((size_t)t * Hq + head) * HD + 4 * L;
+            kv4_put4<TQ>(dst, x[0], x[1], x[2], x[3]);
+            kv4_put4<TQ>(dst + HD / 2, y[0], y[1], y[2], y[3]);
+            continue;
+        }
+        if (!has_place) continue;
+        const bool is_k = head < Hq + Hkv;
+        const int kvh = head - Hq - (is_k ? 0 : Hkv), at = (int)(slot % KV4_PAGE);
+        unsigned char* base = pool + ((size_t)(slot / KV4_PAGE) * Hkv + kvh) * kv4_page_bytes(HD) + (is_k ? 0 : kv4_half_bytes(HD));
+        uint32_t lo, hi, lo_word, hi_word;
+        if (is_k && (k_weight || cos_t)) {
+            double x[4], y[4], scale = 1.0;
+            if (k_weight) {
+                double ss = 0.0;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) ss = fma((double)a[i], (double)a[i], fma((double)b[i], (double)b[i], ss));
+#pragma unroll
+                for (int o = 1; o < LANES; o <<= 1) ss += __shfl_xor_sync(mask, ss, o);
+                const double v = ss / HD + (double)eps;
+                if (v > 1e-30 && v < 1e30) {
+                    scale = (double)rsqrtf((float)v);
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) scale = scale * fma(-0.5 * v * scale, scale, 1.5);
+                } else {
+                    scale = 1.0 / sqrt(v);
+                }
+            }
+            float w[4] = {1.f, 1.f, 1.f, 1.f}, u[4] = {1.f, 1.f, 1.f, 1.f};
+            if (k_weight) {
+                *reinterpret_cast<float4*>(w) = reinterpret_cast<const float4*>(k_weight)[L];
+                *reinterpret_cast<float4*>(u) = reinterpret_cast<const float4*>(k_weight)[HD / 8 + L];
+            }
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const double p = (double)a[i] * scale * (double)w[i], r = (double)b[i] * scale * (double)u[i];
+                x[i] = p * (double)c[i] - r * (double)sn[i];
+                y[i] = p * (double)sn[i] + r * (double)c[i];
+            }
+            lo = kv4_four<double>(x, mask, lo_word);
+            hi = kv4_four<double>(y, mask, hi_word);
+        } else {
+            lo = kv4_four<float>(a, mask, lo_word);
+            hi = kv4_four<float>(b, mask, hi_word);
+        }
+        uint16_t* codes = reinterpret_cast<uint16_t*>(base + (size_t)at * (HD / 2));
+        codes[L] = (uint16_t)lo;
+        codes[HD / 8 + L] = (uint16_t)hi;
+        if ((L & 7) == 0) {
+            uint16_t* words = reinterpret_cast<uint16_t*>(base + kv4_code_bytes(HD)) + at * (HD / KV4_GROUP);
+            words[L / 8] = (uint16_t)lo_word;
+            words[HD / 64 + L / 8] = (uint16_t)hi_word;
+        }
+    }
+}
+
+template <typename TQ, int HD>
+static void kv4_launch_store(const float* qkv, const float* q_weight, const float* k_weight, const float* cos_t, const float* sin_t, const int* slot_map,
+                             void* q_out, unsigned char* pool, long long n_rows, int T, int Hq, int Hkv, float eps, int store_kv, cudaStream_t stream) {
+    const int per_block = KS_WARPS * (256 / HD), heads = store_kv ? Hq + 2 * Hkv : Hq, most = (heads + per_block - 1) / per_block;
+    int share = (KF_BLOCKS + T - 1) / T;                            // few tokens: several blocks share a token's heads
+    if (share > most) share = most;
+    qwb_launch(kv4_store_fast_kernel<TQ, HD>, dim3(T, share), KS_WARPS * 32, 0, stream, qkv, q_weight, k_weight, cos_t, sin_t, slot_map, (TQ*)q_out, pool, n_rows,
+               Hq, Hkv, eps, store_kv);
+}
+
 extern "C" int qwb_kv4_store(const float* qkv, const float* q_weight, const float* k_weight, const float* cos_t, const float* sin_t,
                              const int* slot_map, void* q_out, int q_dtype, unsigned char* pool, int n_pages, int T, int Hq,
                              int Hkv, int hd, int rot, float eps, int store_kv, cudaStream_t stream) {
@@ -114,6 +286,16 @@ extern "C" int qwb_kv4_store(const float* qkv, const float* q_weight, const floa
         return qwb_fail(QWB_ERR_ARG, "kv4_store: bad sizes Hq=%d Hkv=%d hd=%d rot=%d pages=%d", Hq, Hkv, hd, rot, n_pages);
     dim3 grid(T, (Hq + 2 * Hkv + KS_WARPS - 1) / KS_WARPS);
     if (grid.y > 65535) return qwb_fail(QWB_ERR_ARG, "kv4_store: too many heads (%d)", Hq + 2 * Hkv);
+    const bool fast = (hd == 64 || hd == 128) && (rot == 0 || rot == hd) && (uintptr_t)qkv % 16 == 0 && (uintptr_t)q_out % 16 == 0 &&
+                      (uintptr_t)cos_t % 16 == 0 && (uintptr_t)sin_t % 16 == 0 && (uintptr_t)q_weight % 16 == 0 && (uintptr_t)k_weight % 16 == 0 &&
+                      (uintptr_t)pool % 2 == 0;
+    if (fast && (q_dtype == QWB_DT_F32 || q_dtype == QWB_DT_BF16)) {
+        auto launch = q_dtype == QWB_DT_F32 ? (hd == 128 ? kv4_launch_store<float, 128> : kv4_launch_store<float, 64>)
+                                            : (hd == 128 ? kv4_launch_store<bf16, 128> : kv4_launch_store<bf16, 64>);
+        launch(qkv, q_weight, k_weight, rot ? cos_t : nullptr, rot ? sin_t : nullptr, slot_map, q_out, pool, (long long)n_pages * KV4_PAGE, T, Hq, Hkv, eps,
+               store_kv, stream);
+        return qwb_check_launch("kv4_store");
+    }
     if (q_dtype == QWB_DT_F32)
         qwb_launch(kv4_store_kernel<float>, grid, KS_WARPS * 32, 0, stream, qkv, q_weight, k_weight, cos_t, sin_t, slot_map, (float*)q_out, pool,
                    (long long)n_pages * KV4_PAGE, Hq, Hkv, hd, rot, eps, store_kv);
@@ -129,21 +311,27 @@ extern "C" int qwb_kv4_store(const float* qkv, const float* q_weight, const floa
 // sequence's last token are zeros.  A block takes a (page, head), a thread 8 numbers at a time (one 32-bit word of codes).
 // `marked`: a token one of whose values is not finite has values of zero and keys of NaN here, so that a kernel that multiplies
 // what a query does not see by 0 gives NaN to the queries that see it only.
-// Blocks of the first head also write the table that names these pages: [B, width], page_start[b] + j; and with `rows_out` the blocks
-// set rows of `row_bytes` (a multiple of 16) behind row `rows_used` of `rows` there to zero (what no sequence of a padded step writes).
-template <typename T>
+// The blocks also write the table that names these pages: [B, width], page_start[b] + j or 0; and with `rows_out` they set rows of
+// `row_bytes` (a multiple of 16) behind row `rows_used` of `rows` there to zero (what no sequence of a padded step writes).
+// HD: the head size, 0 for any.
+template <typename T, int HD>
 __global__ void __launch_bounds__(256)
 kv4_read_kernel(const unsigned char* __restrict__ pool, const int* __restrict__ pages, const int* __restrict__ page_start,
-                const int* __restrict__ seq_len, T* __restrict__ k_out, T* __restrict__ v_out, int* __restrict__ table, int P, int B,
-                int width, int pool_pages, int Hkv, int hd, int marked, uint4* __restrict__ rows_out, const int* __restrict__ rows_used,
+                const int* __restrict__ seq_len, T* __restrict__ k_out, T* __restrict__ v_out, int* __restrict__ table, int B,
+                int width, int pool_pages, int Hkv, int any_hd, int marked, uint4* __restrict__ rows_out, const int* __restrict__ rows_used,
                 int rows, int row_bytes) {
     pdl_wait();
     pdl_launch_dependents();
+    const int hd = HD ? HD : any_hd;
     const int entry = blockIdx.x, head = blockIdx.y;
+    const long long me = ((long long)head * gridDim.x + entry) * blockDim.x + threadIdx.x, all = (long long)gridDim.x * gridDim.y * blockDim.x;
+    for (long long i = me; i < (long long)B * width; i += all) {
+        const int b = (int)(i / width), j = (int)(i - (long long)b * width), at = page_start[b] + j;
+        table[i] = at >= 0 && at < page_start[b + 1] && at < (int)gridDim.x ? at : 0;
+    }
     if (rows_out) {
-        const long long end = (long long)rows * (row_bytes / 16), step = (long long)gridDim.x * gridDim.y * blockDim.x;
-        for (long long i = (long long)max(*rows_used, 0) * (row_bytes / 16) + ((long long)head * gridDim.x + entry) * blockDim.x + threadIdx.x; i < end; i += step)
-            rows_out[i] = make_uint4(0, 0, 0, 0);
+        const long long end = (long long)rows * (row_bytes / 16);
+        for (long long i = (long long)max(*rows_used, 0) * (row_bytes / 16) + me; i < end; i += all) rows_out[i] = make_uint4(0, 0, 0, 0);
     }
     // the sequence that holds this entry: the last one that begins at or before it
     int lo = 0, hi = B;
@@ -152,7 +340,6 @@ kv4_read_kernel(const unsigned char* __restrict__ pool, const int* __restrict__ 
         if (page_start[mid] <= entry) lo = mid; else hi = mid;
     }
     const int j = entry - page_start[lo];
-    if (head == 0 && threadIdx.x == 0 && j >= 0 && j < width && entry < page_start[lo + 1]) table[(size_t)lo * width + j] = entry;
     const long long page = pages[entry];
     int live = entry < page_start[lo + 1] ? min(max(seq_len[lo] - j * KV4_PAGE, 0), KV4_PAGE) : 0;
     if (j < 0 || page < 0 || page >= pool_pages) live = 0;
@@ -160,7 +347,8 @@ kv4_read_kernel(const unsigned char* __restrict__ pool, const int* __restrict__ 
     const unsigned char* base = pool + ((size_t)(live ? page : 0) * Hkv + head) * kv4_page_bytes(hd);
     const size_t out0 = ((size_t)entry * Hkv + head) * KV4_PAGE * hd;
     const uint16_t* v_words = reinterpret_cast<const uint16_t*>(base + kv4_half_bytes(hd) + kv4_code_bytes(hd));
-    for (int i = threadIdx.x; i < 2 * KV4_PAGE * words; i += blockDim.x) {
+#pragma unroll 4
+    for (int i = threadIdx.x; i < 2 * KV4_PAGE * words; i += 256) {
         const bool is_v = i >= KV4_PAGE * words;
         const int at = is_v ? i - KV4_PAGE * words : i, row = at / words, w = at - row * words;
         const unsigned char* part = base + (is_v ? kv4_half_bytes(hd) : 0);
@@ -204,13 +392,13 @@ extern "C" int qwb_kv4_read(const unsigned char* pool, const int* pages, const i
         return qwb_fail(QWB_ERR_ARG, "kv4_read: pool and outputs must start at a multiple of 16 bytes");
     if (rows_out && ((uintptr_t)rows_out % 16 || row_bytes % 16 || !rows_used))
         return qwb_fail(QWB_ERR_ARG, "kv4_read: rows of %d bytes", row_bytes);
-    if (dtype == QWB_DT_F32)
-        qwb_launch(kv4_read_kernel<float>, dim3(P, Hkv), 256, 0, stream, pool, pages, page_start, seq_len, (float*)k_out, (float*)v_out, table, P, B,
-                   width, pool_pages, Hkv, hd, marked, (uint4*)rows_out, rows_used, rows, row_bytes);
-    else if (dtype == QWB_DT_BF16)
-        qwb_launch(kv4_read_kernel<bf16>, dim3(P, Hkv), 256, 0, stream, pool, pages, page_start, seq_len, (bf16*)k_out, (bf16*)v_out, table, P, B,
-                   width, pool_pages, Hkv, hd, marked, (uint4*)rows_out, rows_used, rows, row_bytes);
-    else
-        return qwb_fail(QWB_ERR_ARG, "kv4_read: unknown dtype %d", dtype);
+    if (dtype != QWB_DT_F32 && dtype != QWB_DT_BF16) return qwb_fail(QWB_ERR_ARG, "kv4_read: unknown dtype %d", dtype);
+#define KV4_READ(T, HD) qwb_launch(kv4_read_kernel<T, HD>, dim3(P, Hkv), 256, 0, stream, pool, pages, page_start, seq_len, (T*)k_out, (T*)v_out, table, B, width, \
+                                   pool_pages, Hkv, hd, marked, (uint4*)rows_out, rows_used, rows, row_bytes)
+    if (dtype == QWB_DT_F32) KV4_READ(float, 0);
+    else if (hd == 128) KV4_READ(bf16, 128);
+    else if (hd == 64) KV4_READ(bf16, 64);
+    else KV4_READ(bf16, 0);
+#undef KV4_READ
     return qwb_check_launch("kv4_read");
 }

@@ -2211,7 +2211,7 @@ def kv4_read(pool: torch.Tensor, pages: torch.Tensor, page_start: torch.Tensor, 
     width = -(-max_len // PAGE_SIZE)
     k = _empty((P, Hkv, PAGE_SIZE, head_dim), dtype=dtype, device=pool.device)
     v = _empty((P, Hkv, PAGE_SIZE, head_dim), dtype=dtype, device=pool.device)
-    table = torch.zeros((B, width), dtype=torch.int32, device=pool.device)
+    table = _empty((B, width), dtype=torch.int32, device=pool.device) if P else torch.zeros((B, width), dtype=torch.int32, device=pool.device)
     _call("kv4_cache", "qwb_kv4_read", _ptr(pool), _ptr(pages), _ptr(page_start), _ptr(seq_len), _ptr(k), _ptr(v), _i(_dt(dtype)), _ptr(table),
           _i(P), _i(B), _i(width), _i(pool.shape[0]), _i(Hkv), _i(head_dim), _i(1 if marked else 0), _ptr(rows), _ptr(used),
           _i(0 if rows is None else rows.shape[0]), _i(0 if rows is None else rows.shape[1] * rows.element_size()), _stream())
