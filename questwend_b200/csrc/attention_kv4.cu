@@ -158,19 +158,6 @@ __device__ __forceinline__ float kd_exp2(float x) {
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
-// Two codes c, in the lowest four bits of each half of `codes`, as the bfloat16 numbers c s: 128 + c by one and-or, then a fused
-// multiply-add that takes 128 s off, exact throughout.  step: s twice; off: -128 s twice.
-__device__ __forceinline__ uint32_t kd_scaled(uint32_t codes, uint32_t step, uint32_t off) {
-    uint32_t e;
-    asm("lop3.b32 %0, %1, %2, %3, 0xea;" : "=r"(e) : "r"(codes), "r"(0x000f000fu), "r"(0x43004300u));        // written as & and |, two instructions
-    __nv_bfloat162 v = __hfma2(*reinterpret_cast<__nv_bfloat162*>(&e), *reinterpret_cast<__nv_bfloat162*>(&step), *reinterpret_cast<__nv_bfloat162*>(&off));
-    return *reinterpret_cast<uint32_t*>(&v);
-}
-__device__ __forceinline__ uint32_t kd_off(uint32_t step) {
-    __nv_bfloat162 v = __hmul2(*reinterpret_cast<__nv_bfloat162*>(&step), __floats2bfloat162_rn(-128.f, -128.f));
-    return *reinterpret_cast<uint32_t*>(&v);
-}
-
 template <int HD>
 struct KdTile {                                             // a warp's keys of a page and head
     static constexpr int CODES = KD_KEYS * HD / 2, WORDS = KD_KEYS * HD / 16, HALF = CODES + WORDS, BYTES = 2 * HALF;
@@ -330,15 +317,15 @@ kv4_attn_rows_kernel(const bf16* __restrict__ q, const unsigned char* __restrict
                 }
                 const uint16_t* words = kw + (16 * t + key_r) * GROUPS + c * (HD / 4) / KV4_GROUP;
                 const uint32_t wa = words[0] * 0x10001u, wb = words[8 * GROUPS] * 0x10001u;
-                const uint32_t sa = wa & 0xfff0fff0u, sb = wb & 0xfff0fff0u, fa = kd_off(sa), fb = kd_off(sb);
-                const uint32_t za = kd_scaled(wa, sa, fa), zb = kd_scaled(wb, sb, fb);
+                const uint32_t sa = wa & 0xfff0fff0u, sb = wb & 0xfff0fff0u, fa = kv4_off(sa), fb = kv4_off(sb);
+                const uint32_t za = kv4_scaled(wa, sa, fa), zb = kv4_scaled(wb, sb, fb);
 #pragma unroll
                 for (int n = 0; n < NT; ++n) kd_mma(s[t][n], za, zb, za, zb, qz[n][0], qz[n][1]);
 #pragma unroll
                 for (int k = 0; k < HD / 16; ++k) {
                     const int sh = 8 * (k & 1);
-                    const uint32_t a0 = kd_scaled(ka[k / 2] >> sh, sa, fa), a1 = kd_scaled(kb[k / 2] >> sh, sb, fb);
-                    const uint32_t a2 = kd_scaled(ka[k / 2] >> (sh + 4), sa, fa), a3 = kd_scaled(kb[k / 2] >> (sh + 4), sb, fb);
+                    const uint32_t a0 = kv4_scaled(ka[k / 2] >> sh, sa, fa), a1 = kv4_scaled(kb[k / 2] >> sh, sb, fb);
+                    const uint32_t a2 = kv4_scaled(ka[k / 2] >> (sh + 4), sa, fa), a3 = kv4_scaled(kb[k / 2] >> (sh + 4), sb, fb);
 #pragma unroll
                     for (int n = 0; n < NT; ++n) kd_mma(s[t][n], a0, a1, a2, a3, qf[n][k][0], qf[n][k][1]);
                 }
@@ -425,8 +412,8 @@ kv4_attn_rows_kernel(const bf16* __restrict__ q, const unsigned char* __restrict
                     if (base + row1 + 8 >= len || kv4_is_nan(w3)) w3 = 0;
                 }
                 const uint32_t w01 = __byte_perm(w0, w1, 0x5410), w23 = __byte_perm(w2, w3, 0x5410);
-                const uint32_t s01 = w01 & 0xfff0fff0u, s23 = w23 & 0xfff0fff0u, f01 = kd_off(s01), f23 = kd_off(s23);
-                const uint32_t z01 = kd_scaled(w01, s01, f01), z23 = kd_scaled(w23, s23, f23);
+                const uint32_t s01 = w01 & 0xfff0fff0u, s23 = w23 & 0xfff0fff0u, f01 = kv4_off(s01), f23 = kv4_off(s23);
+                const uint32_t z01 = kv4_scaled(w01, s01, f01), z23 = kv4_scaled(w23, s23, f23);
 #pragma unroll
                 for (int n = 0; n < NT; ++n) kd_mma(l[n], 0x3f803f80u, z01, 0x3f803f80u, z23, pb[n][0], pb[n][1]);
                 constexpr int VW = HD / 64;                 // words of codes of a lane's numbers of a value
@@ -448,8 +435,8 @@ kv4_attn_rows_kernel(const bf16* __restrict__ q, const unsigned char* __restrict
                     const uint32_t lo23 = __byte_perm(v2[w], v3[w], 0x5410), hi23 = __byte_perm(v2[w], v3[w], 0x7632);
 #pragma unroll
                     for (int j = 0; j < 4; ++j) {
-                        const uint32_t a0 = kd_scaled(lo01 >> (4 * j), s01, f01), a1 = kd_scaled(hi01 >> (4 * j), s01, f01);
-                        const uint32_t a2 = kd_scaled(lo23 >> (4 * j), s23, f23), a3 = kd_scaled(hi23 >> (4 * j), s23, f23);
+                        const uint32_t a0 = kv4_scaled(lo01 >> (4 * j), s01, f01), a1 = kv4_scaled(hi01 >> (4 * j), s01, f01);
+                        const uint32_t a2 = kv4_scaled(lo23 >> (4 * j), s23, f23), a3 = kv4_scaled(hi23 >> (4 * j), s23, f23);
 #pragma unroll
                         for (int n = 0; n < NT; ++n) kd_mma(o[n][4 * w + j], a0, a1, a2, a3, pb[n][0], pb[n][1]);
                     }

@@ -28,3 +28,16 @@ __host__ __device__ constexpr int kv4_page_bytes(int hd) { return 2 * kv4_half_b
 __device__ __forceinline__ float kv4_step(uint32_t word) { return __uint_as_float((word & 0xfff0u) << 16); }
 __device__ __forceinline__ float kv4_zero(uint32_t word) { return (float)(word & 15u); }
 __device__ __forceinline__ bool kv4_is_nan(uint32_t word) { return (word & 0x7f80u) == 0x7f80u; }
+
+// Two codes c, in the lowest four bits of each half of `codes`, as the bfloat16 numbers c s: 128 + c by one and-or, then a fused
+// multiply-add that takes 128 s off, exact throughout.  step: s twice; off: -128 s twice.
+__device__ __forceinline__ uint32_t kv4_scaled(uint32_t codes, uint32_t step, uint32_t off) {
+    uint32_t e;
+    asm("lop3.b32 %0, %1, %2, %3, 0xea;" : "=r"(e) : "r"(codes), "r"(0x000f000fu), "r"(0x43004300u));        // written as & and |, two instructions
+    __nv_bfloat162 v = __hfma2(*reinterpret_cast<__nv_bfloat162*>(&e), *reinterpret_cast<__nv_bfloat162*>(&step), *reinterpret_cast<__nv_bfloat162*>(&off));
+    return *reinterpret_cast<uint32_t*>(&v);
+}
+__device__ __forceinline__ uint32_t kv4_off(uint32_t step) {
+    __nv_bfloat162 v = __hmul2(*reinterpret_cast<__nv_bfloat162*>(&step), __floats2bfloat162_rn(-128.f, -128.f));
+    return *reinterpret_cast<uint32_t*>(&v);
+}

@@ -109,56 +109,97 @@ kv4_store_kernel(const float* __restrict__ qkv, const float* __restrict__ q_weig
 // The same for heads of 64 and 128 turned over all their numbers (or not at all), the common case.  HD / 8 lanes take a head: lane L of them
 // holds the numbers 4L..4L+3 and HD/2 + 4L..: a number and its rotation partner lie in one lane, and each of its two fours in the group of
 // 8 neighbouring lanes, so that norm and group cost three or four exchanges.  What bounds it is memory: 4 bytes read and (queries) 2 or (keys
-// and values) 9/16 written a number.  So only what decides goes through 64 bits: of keys the sum of squares, its root (32 bits and two
-// of Newton's steps) and the rotation; codes are found in 32 bits and checked against the border.
-__device__ __forceinline__ float kv4_nearest(float x, float s, float inv) {                // rint(x / s): a guess, and x - (guess +- 1/2) s, which is exact
-    float c = rintf(x * inv);
-    const float r = fmaf(-c, s, x), half = 0.5f * s;
-    const bool odd = (int)c & 1;
-    if (r > half || (r == half && odd)) c += 1.f;
-    else if (r < -half || (r == -half && odd)) c -= 1.f;
-    return c;
-}
-__device__ __forceinline__ float kv4_nearest(double x, float s, float inv) {
-    float c = rintf((float)x * inv);
-    const double r = fma(-(double)c, (double)s, x), half = 0.5 * (double)s;
-    const bool odd = (int)c & 1;
-    if (r > half || (r == half && odd)) c += 1.f;
-    else if (r < -half || (r == -half && odd)) c -= 1.f;
-    return c;
-}
-// Four numbers of a lane, and the group of 8 lanes' 32: codes (the first in the lowest bits), and the group's word.
-template <typename T>
-__device__ __forceinline__ uint32_t kv4_four(const T (&x)[4], unsigned mask, uint32_t& word) {
-    T lo = x[0], hi = x[0];
-    bool finite = true;
+// and values) 9/16 written a number.  So the choices are made in 32 bits where these leave no doubt: a number whose quotient by the step lies
+// nearer to the border of two codes than its error can be, or a step nearer to the border of two roundings (about one head in 700), sends
+// its head through 64 bits.  With 64 bits for every key a step of 4,096 tokens of 32 + 2 x 8 heads took 45 us, with a warp a head before that 130.
+//
+// Errors of a key in 32 bits, u = 2^-24: the sum of squares 8 + 4 additions, the mean and eps 1, halved by the root; the inverse root
+// 4 (2 units of 2^-23): 11 u; times the weight and the number 2 u; the rotation 2 u of |p| + |r|: 15 u (|p| + |r|) < 2^-20 (|p| + |r|).
+struct Kv4Choice { uint32_t codes, word; bool sure; };
+
+// Four numbers of a lane in a group of 8 lanes' 32, each off by at most e: codes (the first in the lowest bits) and the group's word.
+__device__ __forceinline__ Kv4Choice kv4_four(const float (&x)[4], const float (&e)[4], unsigned mask) {
+    float lo = 0.f, hi = 0.f, off = 0.f;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-        finite &= fabs((double)x[i]) <= 3.4028234663852886e38;
-        lo = x[i] < lo ? x[i] : lo;
-        hi = x[i] > hi ? x[i] : hi;
+        lo = fminf(lo, x[i]);
+        hi = fmaxf(hi, fabsf(x[i]) <= 3.4028234663852886e38f ? x[i] : INFINITY);
+        off = fmaxf(off, e[i]);
     }
-    lo = lo < T(0) ? lo : T(0);
-    hi = hi > T(0) ? hi : T(0);
 #pragma unroll
     for (int o = 1; o < 8; o <<= 1) {
-        const T a = __shfl_xor_sync(mask, lo, o), b = __shfl_xor_sync(mask, hi, o);
-        lo = a < lo ? a : lo;
-        hi = b > hi ? b : hi;
-        finite &= (bool)__shfl_xor_sync(mask, (int)finite, o);
+        lo = fminf(lo, __shfl_xor_sync(mask, lo, o));
+        hi = fmaxf(hi, __shfl_xor_sync(mask, hi, o));
+        off = fmaxf(off, __shfl_xor_sync(mask, off, o));
     }
-    const double d = (double)hi - (double)lo;
-    double t = d * (1.0 / 15.0);                                                        // d / 15, its last bit corrected
-    t = fma(fma(-15.0, t, d), 1.0 / 15.0, t);
-    const double step = __longlong_as_double((__double_as_longlong(t) + (1ll << 48)) & ~((1ll << 49) - 1));
-    if (!finite || !(step < 1.329227995784916e36)) { word = 0x7fc0u; return 0u; }
-    if (step < 1.1754943508222875e-38) { word = 0u; return 0u; }
-    const float s = (float)step, inv = 1.f / s, z = fminf(kv4_nearest((T)-lo, s, inv), 15.f);
-    uint32_t codes = 0;
+    Kv4Choice y;
+    y.codes = y.word = 0;
+    const float t = (hi - lo) * (1.f / 15.f);
+    if (t == 0.f && off == 0.f) { y.sure = true; return y; }
+    // t is off by 2 off / 15 and by less than 3 of its last places: is it that near to the border of two steps?  (Very small, very large and no
+    // numbers: decided in 64 bits.)
+    const int bits = __float_as_int(t), border = abs((bits & 0xfffff) - 0x80000);
+    y.sure = t > 1e-36f && t < 1e36f && (float)(border - 3) * (t * 5.9604644775390625e-8f) > 0.14f * off;
+    const float s = __int_as_float((bits + 0x80000) & ~0xfffff);
+    float inv;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inv) : "f"(s));
+    const float near = 0.499996f * s, z0 = rintf(-lo * inv);
+    y.sure &= fabsf(fmaf(-z0, s, -lo)) + off < near;
+    const float z = fminf(z0, 15.f);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) codes |= (uint32_t)(int)fminf(fmaxf(kv4_nearest(x[i], s, inv) + z, 0.f), 15.f) << (4 * i);
-    word = (__float_as_uint(s) >> 16) | (uint32_t)(int)z;
-    return codes;
+    for (int i = 0; i < 4; ++i) {
+        const float c = rintf(x[i] * inv);
+        y.sure &= fabsf(fmaf(-c, s, x[i])) + e[i] < near;
+        y.codes |= (uint32_t)(int)fminf(fmaxf(c + z, 0.f), 15.f) << (4 * i);
+    }
+    y.word = (__float_as_uint(s) >> 16) | (uint32_t)(int)z;
+    return y;
+}
+// The same in 64 bits, for both fours of a lane and from the projection's numbers on (weight and cosines null: as they are).
+template <int HD>
+__device__ __noinline__ uint4 kv4_head_exactly(const float* src, const float* weight, const float* cos_t, const float* sin_t, int L, float eps, unsigned mask) {
+    double x[8], scale = 1.0;
+    if (weight) {
+        double ss = 0.0;
+        for (int i = 0; i < 4; ++i) ss += (double)src[4 * L + i] * src[4 * L + i] + (double)src[HD / 2 + 4 * L + i] * src[HD / 2 + 4 * L + i];
+        for (int o = 1; o < HD / 8; o <<= 1) ss += __shfl_xor_sync(mask, ss, o);
+        scale = 1.0 / sqrt(ss / HD + (double)eps);
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        double a = src[4 * L + i], b = src[HD / 2 + 4 * L + i];
+        if (weight) {
+            a *= scale * weight[4 * L + i];
+            b *= scale * weight[HD / 2 + 4 * L + i];
+        }
+        const double c = cos_t ? (double)cos_t[4 * L + i] : 1.0, sn = cos_t ? (double)sin_t[4 * L + i] : 0.0;
+        x[i] = cos_t ? a * c - b * sn : a;
+        x[4 + i] = cos_t ? a * sn + b * c : b;
+    }
+    uint32_t out[4];
+#pragma unroll
+    for (int g = 0; g < 2; ++g) {
+        double lo = 0.0, hi = 0.0;
+        int finite = 1;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            finite &= fabs(x[4 * g + i]) <= 3.4028234663852886e38;
+            lo = fmin(lo, x[4 * g + i]);
+            hi = fmax(hi, x[4 * g + i]);
+        }
+        for (int o = 1; o < 8; o <<= 1) {
+            lo = fmin(lo, __shfl_xor_sync(mask, lo, o));
+            hi = fmax(hi, __shfl_xor_sync(mask, hi, o));
+            finite &= __shfl_xor_sync(mask, finite, o);
+        }
+        float s, z;
+        out[2 * g + 1] = kv4_word(lo, hi, finite, s, z);
+        out[2 * g] = 0;
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            if (s > 0.f) out[2 * g] |= (uint32_t)kv4_code(x[4 * g + i], s, z) << (4 * i);
+    }
+    return make_uint4(out[0], out[1], out[2], out[3]);
 }
 
 template <typename TQ> __device__ __forceinline__ void kv4_put4(TQ* p, float a, float b, float c, float d);
@@ -170,7 +211,7 @@ template <> __device__ __forceinline__ void kv4_put4<bf16>(bf16* p, float a, flo
 
 #define KF_BLOCKS 1184              // as many are wanted of a call
 template <typename TQ, int HD>
-__global__ void __launch_bounds__(KS_WARPS * 32)
+__global__ void __launch_bounds__(KS_WARPS * 32, 9)
 kv4_store_fast_kernel(const float* __restrict__ qkv, const float* __restrict__ q_weight, const float* __restrict__ k_weight,
                       const float* __restrict__ cos_t, const float* __restrict__ sin_t, const int* __restrict__ slot_map,
                       TQ* __restrict__ q_out, unsigned char* __restrict__ pool, long long n_rows, int Hq, int Hkv, float eps, int store_kv) {
@@ -188,10 +229,21 @@ kv4_store_fast_kernel(const float* __restrict__ qkv, const float* __restrict__ q
     }
     const long long slot = slot_map[t];
     const bool has_place = slot >= 0 && slot < n_rows;
-    for (int head = (blockIdx.y * KS_WARPS + warp) * HEADS + of; head < n_heads; head += gridDim.y * KS_WARPS * HEADS) {
+    const int step = gridDim.y * KS_WARPS * HEADS;
+    int head = (blockIdx.y * KS_WARPS + warp) * HEADS + of;
+    float4 next_a = make_float4(0.f, 0.f, 0.f, 0.f), next_b = next_a;
+    if (head < n_heads) {
+        next_a = row[(size_t)head * (HD / 4) + L];
+        next_b = row[(size_t)head * (HD / 4) + HD / 8 + L];
+    }
+    for (; head < n_heads; head += step) {
         float a[4], b[4];
-        *reinterpret_cast<float4*>(a) = row[(size_t)head * (HD / 4) + L];
-        *reinterpret_cast<float4*>(b) = row[(size_t)head * (HD / 4) + HD / 8 + L];
+        *reinterpret_cast<float4*>(a) = next_a;
+        *reinterpret_cast<float4*>(b) = next_b;
+        if (head + step < n_heads) {                                // the next head's numbers are on their way meanwhile
+            next_a = row[(size_t)(head + step) * (HD / 4) + L];
+            next_b = row[(size_t)(head + step) * (HD / 4) + HD / 8 + L];
+        }
         if (head < Hq) {
             if (q_weight) {
                 float ss = 0.f, w[4];
@@ -199,7 +251,7 @@ kv4_store_fast_kernel(const float* __restrict__ qkv, const float* __restrict__ q
                 for (int i = 0; i < 4; ++i) ss = fmaf(a[i], a[i], fmaf(b[i], b[i], ss));
 #pragma unroll
                 for (int o = 1; o < LANES; o <<= 1) ss += __shfl_xor_sync(mask, ss, o);
-                const float scale = 1.f / sqrtf(ss / (float)HD + eps);
+                const float scale = rsqrtf(ss * (1.f / HD) + eps);
                 *reinterpret_cast<float4*>(w) = reinterpret_cast<const float4*>(q_weight)[L];
 #pragma unroll
                 for (int i = 0; i < 4; ++i) a[i] *= scale * w[i];
@@ -222,48 +274,51 @@ kv4_store_fast_kernel(const float* __restrict__ qkv, const float* __restrict__ q
         const bool is_k = head < Hq + Hkv;
         const int kvh = head - Hq - (is_k ? 0 : Hkv), at = (int)(slot % KV4_PAGE);
         unsigned char* base = pool + ((size_t)(slot / KV4_PAGE) * Hkv + kvh) * kv4_page_bytes(HD) + (is_k ? 0 : kv4_half_bytes(HD));
-        uint32_t lo, hi, lo_word, hi_word;
-        if (is_k && (k_weight || cos_t)) {
-            double x[4], y[4], scale = 1.0;
+        const bool turned = is_k && (k_weight || cos_t);
+        float w[4] = {1.f, 1.f, 1.f, 1.f}, u[4] = {1.f, 1.f, 1.f, 1.f}, x[4], y[4], e[4] = {}, f[4] = {};
+        if (turned) {
+            float scale = 1.f;
             if (k_weight) {
-                double ss = 0.0;
+                float ss = 0.f;
 #pragma unroll
-                for (int i = 0; i < 4; ++i) ss = fma((double)a[i], (double)a[i], fma((double)b[i], (double)b[i], ss));
+                for (int i = 0; i < 4; ++i) ss = fmaf(a[i], a[i], fmaf(b[i], b[i], ss));
 #pragma unroll
                 for (int o = 1; o < LANES; o <<= 1) ss += __shfl_xor_sync(mask, ss, o);
-                const double v = ss / HD + (double)eps;
-                if (v > 1e-30 && v < 1e30) {
-                    scale = (double)rsqrtf((float)v);
-#pragma unroll
-                    for (int i = 0; i < 2; ++i) scale = scale * fma(-0.5 * v * scale, scale, 1.5);
-                } else {
-                    scale = 1.0 / sqrt(v);
-                }
-            }
-            float w[4] = {1.f, 1.f, 1.f, 1.f}, u[4] = {1.f, 1.f, 1.f, 1.f};
-            if (k_weight) {
+                scale = rsqrtf(ss * (1.f / HD) + eps);
                 *reinterpret_cast<float4*>(w) = reinterpret_cast<const float4*>(k_weight)[L];
                 *reinterpret_cast<float4*>(u) = reinterpret_cast<const float4*>(k_weight)[HD / 8 + L];
             }
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                const double p = (double)a[i] * scale * (double)w[i], r = (double)b[i] * scale * (double)u[i];
-                x[i] = p * (double)c[i] - r * (double)sn[i];
-                y[i] = p * (double)sn[i] + r * (double)c[i];
+                const float p = a[i] * (scale * w[i]), r = b[i] * (scale * u[i]);
+                x[i] = fmaf(p, c[i], -r * sn[i]);
+                y[i] = fmaf(p, sn[i], r * c[i]);
+                e[i] = f[i] = (fabsf(p) + fabsf(r)) * 9.5367431640625e-7f;
             }
-            lo = kv4_four<double>(x, mask, lo_word);
-            hi = kv4_four<double>(y, mask, hi_word);
         } else {
-            lo = kv4_four<float>(a, mask, lo_word);
-            hi = kv4_four<float>(b, mask, hi_word);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                x[i] = a[i];
+                y[i] = b[i];
+            }
+        }
+        Kv4Choice lo = kv4_four(x, e, mask), hi = kv4_four(y, f, mask);
+        if (__any_sync(mask, !lo.sure || !hi.sure)) {
+            const uint4 g = kv4_head_exactly<HD>(reinterpret_cast<const float*>(row) + (size_t)head * HD, turned ? k_weight : nullptr,
+                                                 turned && cos_t ? cos_t + (size_t)t * (HD / 2) : nullptr, turned && cos_t ? sin_t + (size_t)t * (HD / 2) : nullptr,
+                                                 L, eps, mask);
+            lo.codes = g.x;
+            lo.word = g.y;
+            hi.codes = g.z;
+            hi.word = g.w;
         }
         uint16_t* codes = reinterpret_cast<uint16_t*>(base + (size_t)at * (HD / 2));
-        codes[L] = (uint16_t)lo;
-        codes[HD / 8 + L] = (uint16_t)hi;
+        codes[L] = (uint16_t)lo.codes;
+        codes[HD / 8 + L] = (uint16_t)hi.codes;
         if ((L & 7) == 0) {
             uint16_t* words = reinterpret_cast<uint16_t*>(base + kv4_code_bytes(HD)) + at * (HD / KV4_GROUP);
-            words[L / 8] = (uint16_t)lo_word;
-            words[HD / 64 + L / 8] = (uint16_t)hi_word;
+            words[L / 8] = (uint16_t)lo.word;
+            words[HD / 64 + L / 8] = (uint16_t)hi.word;
         }
     }
 }
@@ -347,7 +402,7 @@ kv4_read_kernel(const unsigned char* __restrict__ pool, const int* __restrict__ 
     const unsigned char* base = pool + ((size_t)(live ? page : 0) * Hkv + head) * kv4_page_bytes(hd);
     const size_t out0 = ((size_t)entry * Hkv + head) * KV4_PAGE * hd;
     const uint16_t* v_words = reinterpret_cast<const uint16_t*>(base + kv4_half_bytes(hd) + kv4_code_bytes(hd));
-#pragma unroll 4
+#pragma unroll 8
     for (int i = threadIdx.x; i < 2 * KV4_PAGE * words; i += 256) {
         const bool is_v = i >= KV4_PAGE * words;
         const int at = is_v ? i - KV4_PAGE * words : i, row = at / words, w = at - row * words;
@@ -360,8 +415,24 @@ kv4_read_kernel(const unsigned char* __restrict__ pool, const int* __restrict__ 
             const float z = kv4_zero(word);
             if (marked) {
                 bool bad = false;
-                for (int g = 0; g < groups; ++g) bad |= kv4_is_nan(v_words[row * groups + g]);
-                if (bad) s = is_v ? 0.f : __uint_as_float(0x7fffffffu);
+#pragma unroll
+                for (int g = 0; g < (HD ? HD / KV4_GROUP : 1); ++g) bad |= kv4_is_nan(v_words[row * groups + g]);
+                if constexpr (HD == 0)
+                    for (int g = 1; g < groups; ++g) bad |= kv4_is_nan(v_words[row * groups + g]);
+                if (bad) s = is_v ? 0.f : __uint_as_float(0x7fc00000u);
+            }
+            if constexpr (sizeof(T) == 2) {                 // two codes at a time, all of it exact: c s - z s
+                const uint32_t step = (__float_as_uint(s) >> 16) * 0x10001u, less = kv4_off(step), zs = kv4_scaled(word * 0x10001u, step, less);
+                uint32_t p[4];
+#pragma unroll
+                for (int n = 0; n < 4; ++n) {
+                    const uint32_t v = kv4_scaled(codes >> (4 * n), step, less);
+                    __nv_bfloat162 d = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&v), *reinterpret_cast<const __nv_bfloat162*>(&zs));
+                    p[n] = *reinterpret_cast<uint32_t*>(&d);
+                }
+                *reinterpret_cast<uint4*>((is_v ? v_out : k_out) + out0 + (size_t)at * 8) =
+                    make_uint4(__byte_perm(p[0], p[1], 0x5410), __byte_perm(p[2], p[3], 0x5410), __byte_perm(p[0], p[1], 0x7632), __byte_perm(p[2], p[3], 0x7632));
+                continue;
             }
 #pragma unroll
             for (int n = 0; n < 8; ++n) y[n] = ((float)((codes >> (4 * n)) & 15u) - z) * s;
