@@ -18,7 +18,9 @@
 //   * A run's softmax is relative to a reference that is raised, and O rescaled, only where a score passes it by 2^8: most pages vote once
 //     and exchange no maxima.  The weights' sum is one more mma with rows of ones, over
 //     the weights as they are rounded for the product.
-// Runs are cut by the sequence's own length (kv4_runs), never by what else is in the batch; a second kernel joins them.
+// Runs are cut by the sequence's own length (kv4_runs), never by what else is in the batch.  Up to 16 of them are the blocks of a cluster, which
+// read each other's results from shared memory; more leave them in scratch memory for a second kernel.  Both join them in the same order,
+// so that which way it went cannot be told from the result (qwb_kv4_plan says which, with times).
 //
 // The plain kernel: any head size that is a multiple of 32, queries in 32 bits or bfloat16.  A block takes a (token, query head),
 // its four warps every fourth key; a lane holds the numbers lane, lane + 32, ... of the query, of the sums and of a key, so a
@@ -162,17 +164,41 @@ template <int HD>
 struct KdTile {                                             // a warp's keys of a page and head
     static constexpr int CODES = KD_KEYS * HD / 2, WORDS = KD_KEYS * HD / 16, HALF = CODES + WORDS, BYTES = 2 * HALF;
 };
+#define KD_CLUSTER 16           // blocks of the largest cluster
 template <int HD, int NT>
 struct KdSmem {
     static constexpr int RING = KD_WARPS * KD_STAGES * KdTile<HD>::BYTES;
     static constexpr int COL = HD + 4;                      // floats of a column of outputs: two columns are 8 banks apart
     static constexpr int JOIN = KD_WARPS * 8 * NT * (COL + 2) * 4;
-    static constexpr int BYTES = RING > JOIN ? RING : JOIN;
+    static constexpr int DONE = 8 * NT * (COL + 2) * 4;     // the block's own outputs, maxima and sums, behind its warps'
+    static constexpr int BYTES = RING > JOIN + DONE ? RING : JOIN + DONE;
 };
 
-// NT: tiles of 8 columns of a block.  part: [rows, max_runs, HD] outputs, then [rows, max_runs, 2] maxima (of scores times log2 e) and sums
+// The join of a row's runs: relative to the largest maximum, in four sums of every fourth run, which are then added.
+__device__ __forceinline__ float kd_share(float m, float l, float top) { return l == 0.f ? 0.f : m == top ? 1.f : kd_exp2(m - top); }
+__device__ __forceinline__ float kd_four(const float (&x)[4]) { return (x[0] + x[1]) + (x[2] + x[3]); }
+__device__ __forceinline__ float2 kd_remote2(uint32_t at) {
+    float2 v;
+    asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(at) : "memory");
+    return v;
+}
+__device__ __forceinline__ float kd_remote(uint32_t at) {
+    float v;
+    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(at) : "memory");
+    return v;
+}
+__device__ __forceinline__ uint32_t kd_of_block(uint32_t mine, int rank) {                     // an address of this block's shared memory, in the cluster's `rank`th
+    uint32_t at;
+    asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(mine), "r"(rank));
+    return at;
+}
+__device__ __forceinline__ void kd_cluster_sync() {
+    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+
+// NT: tiles of 8 columns of a block.  CLUSTER: the runs of a tile are the blocks of a cluster.  part: [rows, max_runs, HD] outputs, then [rows, max_runs, 2] maxima (of scores times log2 e) and sums
 // of the runs of sequences that have more than one; a row is (token, query head).
-template <int HD, int NT>
+template <int HD, int NT, bool CLUSTER>
 __global__ void __launch_bounds__(KD_WARPS * 32, NT == 1 ? 8 : 5)
 kv4_attn_rows_kernel(const bf16* __restrict__ q, const unsigned char* __restrict__ pool, const int* __restrict__ page_table,
                      const int* __restrict__ cu_seqlens, const int* __restrict__ pos0, bf16* __restrict__ out, float* __restrict__ part_o,
@@ -184,7 +210,15 @@ kv4_attn_rows_kernel(const bf16* __restrict__ q, const unsigned char* __restrict
     using Smem = KdSmem<HD, NT>;
     extern __shared__ __align__(128) unsigned char smem[];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, r = lane >> 2, c = lane & 3;
-    const int run = tiles == 1 ? blockIdx.x : blockIdx.x / tiles, tile = blockIdx.x - run * tiles, kvh = blockIdx.y, b = blockIdx.z;
+    int run, tile;
+    if (CLUSTER) {
+        tile = blockIdx.x / max_runs;                       // max_runs: the cluster's blocks
+        run = blockIdx.x - tile * max_runs;
+    } else {
+        run = tiles == 1 ? blockIdx.x : blockIdx.x / tiles;
+        tile = blockIdx.x - run * tiles;
+    }
+    const int kvh = blockIdx.y, b = blockIdx.z;
     const int Hq = Hkv * G;
     const float one_in_g = 1.f / (float)G;
     auto by_g = [&](int x) { return (int)(((float)x + 0.5f) * one_in_g); };             // x / G: exact for x below 2^20 (the launcher's bound)
@@ -197,8 +231,8 @@ kv4_attn_rows_kernel(const bf16* __restrict__ q, const unsigned char* __restrict
     const int len = p0 + n_new;
     const Kv4Runs cut = kv4_runs(p0, len, window, table_width);
     const int runs = min(cut.runs, max_runs);               // a sequence beyond max_len: cut off there, never written beyond the scratch
-    if (run >= runs && run > 0) return;
-    const int first_page = cut.first + run * cut.per_run, n_pages = min(cut.per_run, cut.count - run * cut.per_run);
+    if (!CLUSTER && run >= runs && run > 0) return;         // (a block of a cluster stays for its barriers, without pages)
+    const int first_page = cut.first + run * cut.per_run, n_pages = max(min(cut.per_run, cut.count - run * cut.per_run), 0);
     const int* table = page_table + (size_t)b * table_width + first_page;
     int my_page = -1;                                       // lane i: the run's i-th page
     if (lane < n_pages) my_page = table[lane];
@@ -471,6 +505,8 @@ kv4_attn_rows_kernel(const bf16* __restrict__ q, const unsigned char* __restrict
     __syncthreads();
     // a warp every second column, a lane four neighbouring places of it (with heads of 64 two)
     constexpr int E = HD / 32;
+    float* done_o = join_ml + KD_WARPS * 8 * NT * 2;
+    float* done_ml = done_o + 8 * NT * Smem::COL;
     for (int col = warp; col < 8 * NT; col += KD_WARPS) {
         if (col0 + col >= cols) break;
         float mw[KD_WARPS], lw[KD_WARPS], y[E] = {}, top = -INFINITY, total = 0.f;
@@ -482,7 +518,7 @@ kv4_attn_rows_kernel(const bf16* __restrict__ q, const unsigned char* __restrict
         }
 #pragma unroll
         for (int w = 0; w < KD_WARPS; ++w) {
-            const float f = lw[w] == 0.f ? 0.f : mw[w] == top ? 1.f : kd_exp2(mw[w] - top);
+            const float f = kd_share(mw[w], lw[w], top);
             const float* src = join_o + (w * 8 * NT + col) * Smem::COL + lane * E;
             total += f * lw[w];
             if (lw[w] != 0.f) {
@@ -492,29 +528,57 @@ kv4_attn_rows_kernel(const bf16* __restrict__ q, const unsigned char* __restrict
         }
         const int tok = by_g(col0 + col);
         const size_t row = (size_t)(t0 + tok) * Hq + kvh * G + col0 + col - tok * G;
-        if (runs <= 1) {
+        if (CLUSTER ? max_runs == 1 : runs <= 1) {
 #pragma unroll
             for (int e = 0; e < E; ++e) {
                 const int at = lane * E + e, mma = at / 16, half = (at >> 3) & 1, d = (at & 7) * (HD / 8) + 8 * (mma >> 2) + 4 * half + (mma & 3);
                 out[row * HD + d] = from_f32<bf16>(total == 0.f ? 0.f : y[e] / total);
             }
         } else {
-            float* dst = part_o + (row * max_runs + run) * HD + lane * E;
+            float* dst = CLUSTER ? done_o + col * Smem::COL + lane * E : part_o + (row * max_runs + run) * HD + lane * E;
             if constexpr (E == 4) *reinterpret_cast<float4*>(dst) = make_float4(y[0], y[1], y[2], y[3]);
             else *reinterpret_cast<float2*>(dst) = make_float2(y[0], y[1]);
-            if (lane == 0) *reinterpret_cast<float2*>(part_ml + (row * max_runs + run) * 2) = make_float2(top, total);
+            if (lane == 0) *reinterpret_cast<float2*>(CLUSTER ? done_ml + 2 * col : part_ml + (row * max_runs + run) * 2) = make_float2(top, total);
         }
+    }
+    if (CLUSTER && max_runs > 1) {
+        kd_cluster_sync();
+        // 32 places of a column at a time, all warps of the cluster side by side
+        const uint32_t o_at = (uint32_t)__cvta_generic_to_shared(done_o), ml_at = (uint32_t)__cvta_generic_to_shared(done_ml);
+        const int n_runs = max(runs, 1), live = min(8 * NT, cols - col0);
+        for (int piece = run * KD_WARPS + warp; piece < live * E; piece += max_runs * KD_WARPS) {
+            const int col = piece / E, at = (piece % E) * 32 + lane;
+            float2 ml = make_float2(-INFINITY, 0.f);
+            if (lane < n_runs) ml = kd_remote2(kd_of_block(ml_at + 8 * col, lane));
+            float v[KD_CLUSTER];
+#pragma unroll
+            for (int i = 0; i < KD_CLUSTER; ++i) v[i] = i < n_runs ? kd_remote(kd_of_block(o_at + 4 * (col * Smem::COL + at), i)) : 0.f;
+            const float f = kd_share(ml.x, ml.y, warp_max(ml.x)), fl = f * ml.y;
+            float sum[4] = {}, y[4] = {};
+#pragma unroll
+            for (int i = 0; i < KD_CLUSTER; ++i) {
+                const float fi = __shfl_sync(0xffffffffu, f, i), l_i = __shfl_sync(0xffffffffu, ml.y, i);
+                if (l_i != 0.f) {
+                    sum[i & 3] += __shfl_sync(0xffffffffu, fl, i);
+                    y[i & 3] = fmaf(fi, v[i], y[i & 3]);
+                }
+            }
+            const float total = kd_four(sum);
+            const int tok = by_g(col0 + col), mma = at / 16, half = (at >> 3) & 1, d = (at & 7) * (HD / 8) + 8 * (mma >> 2) + 4 * half + (mma & 3);
+            out[((size_t)(t0 + tok) * Hq + kvh * G + col0 + col - tok * G) * HD + d] = from_f32<bf16>(total == 0.f ? 0.f : kd_four(y) / total);
+        }
+        kd_cluster_sync();                                  // nobody leaves while its shared memory is read
     }
 }
 
 // Joins the runs of a row: a block a row, a warp every fourth run, all loads on their way together.  What says how many runs there are was
 // there before the attention's blocks began, so it is read while the last of them still run (the kernel starts under their tail).
-#define KJ_WARPS 4
+#define KJ_WARPS 4              // the four sums
 template <int HD>
 __global__ void __launch_bounds__(KJ_WARPS * 32)
 kv4_attn_join_kernel(const float* part_o, const float* part_ml, const int* cu_seqlens, const int* pos0, const int* tok_seq, bf16* __restrict__ out, int T, int B,
                      int Hq, int table_width, int window, int max_runs) {
-    __shared__ float join_o[KJ_WARPS][HD], join_ml[KJ_WARPS][2];
+    __shared__ float join_o[KJ_WARPS][HD], join_l[KJ_WARPS];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, t = blockIdx.x / Hq;
     const size_t row = blockIdx.x;
     const int b = __ldcg(tok_seq + t);
@@ -527,49 +591,63 @@ kv4_attn_join_kernel(const float* part_o, const float* part_ml, const int* cu_se
     pdl_launch_dependents();
     if (runs <= 1) return;
     constexpr int E = HD / 32;
-    float top = -INFINITY, total = 0.f, y[E] = {};
+    const float* mls = part_ml + row * max_runs * 2;
+    float top = -INFINITY;
+    for (int i = lane; i < runs; i += 32) top = fmaxf(top, __ldcg(mls + 2 * i));
+    top = warp_max(top);
+    float sum = 0.f, y[E] = {};
 #pragma unroll 4
-    for (int i = warp; i < runs; i += KJ_WARPS) {
-        const float2 x = __ldcg(reinterpret_cast<const float2*>(part_ml + (row * max_runs + i) * 2));
+    for (int i = warp; i < runs; i += KJ_WARPS) {           // this warp's of the four sums
+        const float2 x = __ldcg(reinterpret_cast<const float2*>(mls + 2 * i));
         float v[E];
         const float* src = part_o + (row * max_runs + i) * HD + lane * E;
         if constexpr (E == 4) *reinterpret_cast<float4*>(v) = __ldcg(reinterpret_cast<const float4*>(src));
         else *reinterpret_cast<float2*>(v) = __ldcg(reinterpret_cast<const float2*>(src));
-        if (x.y == 0.f) continue;                           // a run that a row sees nothing of
-        const float up = fmaxf(top, x.x), keep = top == up ? 1.f : kd_exp2(top - up), f = x.x == up ? 1.f : kd_exp2(x.x - up);
-        total = total * keep + f * x.y;
+        const float f = kd_share(x.x, x.y, top), fl = f * x.y;
+        if (x.y != 0.f) {                                   // (0: a run that the row sees nothing of)
+            sum += fl;
 #pragma unroll
-        for (int e = 0; e < E; ++e) y[e] = y[e] * keep + f * v[e];
-        top = up;
+            for (int e = 0; e < E; ++e) y[e] = fmaf(f, v[e], y[e]);
+        }
     }
 #pragma unroll
     for (int e = 0; e < E; ++e) join_o[warp][lane * E + e] = y[e];
-    if (lane == 0) { join_ml[warp][0] = top; join_ml[warp][1] = total; }
+    if (lane == 0) join_l[warp] = sum;
     __syncthreads();
     for (int at = threadIdx.x; at < HD; at += KJ_WARPS * 32) {
-        float all = -INFINITY, sum = 0.f, o = 0.f;
-#pragma unroll
-        for (int w = 0; w < KJ_WARPS; ++w) all = fmaxf(all, join_ml[w][0]);
-#pragma unroll
-        for (int w = 0; w < KJ_WARPS; ++w) {
-            if (join_ml[w][1] == 0.f) continue;
-            const float f = join_ml[w][0] == all ? 1.f : kd_exp2(join_ml[w][0] - all);
-            sum += f * join_ml[w][1];
-            o += f * join_o[w][at];
-        }
+        const float l[4] = {join_l[0], join_l[1], join_l[2], join_l[3]}, o[4] = {join_o[0][at], join_o[1][at], join_o[2][at], join_o[3][at]};
+        const float total = kd_four(l);
         const int mma = at / 16, half = (at >> 3) & 1, d = (at & 7) * (HD / 8) + 8 * (mma >> 2) + 4 * half + (mma & 3);
-        out[row * HD + d] = from_f32<bf16>(sum == 0.f ? 0.f : o / sum);
+        out[row * HD + d] = from_f32<bf16>(total == 0.f ? 0.f : kd_four(o) / total);
     }
 }
 
 // The most runs of a sequence of up to max_len tokens of which it brings up to max_new.
-extern "C" int qwb_kv4_max_runs(int max_len, int max_new, int window, int table_width) {
-    long long pages = ((long long)max_len + KV4_PAGE - 1) / KV4_PAGE;
+static long long kv4_max_runs(long long max_len, int max_new, int window, int table_width) {
+    long long pages = (max_len + KV4_PAGE - 1) / KV4_PAGE;
     if (window > 0 && ((long long)window + max_new) / KV4_PAGE + 2 < pages) pages = ((long long)window + max_new) / KV4_PAGE + 2;
     if (pages > table_width) pages = table_width;
-    if (pages <= KD_RUNS) return pages < 1 ? 1 : (int)pages;
+    if (pages <= KD_RUNS) return pages < 1 ? 1 : pages;
     const long long even = (pages + KD_RUN_PAGES - 1) / KD_RUN_PAGES;
-    return (int)(even > KD_RUNS ? even : KD_RUNS);
+    return even > KD_RUNS ? even : KD_RUNS;
+}
+static int kv4_columns(int max_new, int G) { return (long long)max_new * G > 8 ? 16 : 8; }      // of a block
+static int kv4_cluster_size(long long runs) {
+    int size = 1;
+    while (size < runs) size *= 2;
+    return size;
+}
+
+// How a call's runs are joined: the most runs of a sequence, times 2, plus 1 if by scratch memory and a second kernel.  Up to 16 runs go
+// as clusters while these are all on the chip at once (7 blocks an SM, 4 with 16 columns): a second launch and a kernel's start less, 8.0
+// and 7.0 us for one sequence of 2,048 tokens, 15.0 and 13.6 for 16,384; 8 sequences of 4,096, 1,024 blocks, are even (16.1).  Beyond that a
+// cluster waits for 16 free places: 64 sequences of 1,000 take 66.8 us against 36.6, 4 of 8,192 with 6 new tokens 45.7 against 30.9.
+extern "C" int qwb_kv4_plan(int max_len, int max_new, int window, int table_width, int B, int Hq, int Hkv) {
+    const long long runs = kv4_max_runs(max_len, max_new, window, table_width);
+    const int columns = kv4_columns(max_new, Hq / Hkv);
+    const long long tiles = ((long long)max_new * (Hq / Hkv) + columns - 1) / columns;
+    const bool clusters = runs <= KD_CLUSTER && tiles * kv4_cluster_size(runs) * Hkv * B <= 148 * (columns == 8 ? 7 : 4);
+    return (int)(2 * runs + (runs > 1 && !clusters ? 1 : 0));
 }
 
 template <int HD, int NT>
@@ -577,32 +655,60 @@ static int kv4_launch_rows(const bf16* q, const unsigned char* pool, const int* 
                            float* scratch, int T, int B, int pool_pages, int max_new, int Hq, int Hkv, int table_width, float scale, int window, int max_runs,
                            cudaStream_t stream) {
     using Smem = KdSmem<HD, NT>;
-    auto kernel = kv4_attn_rows_kernel<HD, NT>;
     static_assert(Smem::BYTES <= 48 * 1024, "more needs an attribute of the kernel");
-    const long long tiles = ((long long)max_new * (Hq / Hkv) + 8 * NT - 1) / (8 * NT);
+    const long long tiles = ((long long)max_new * (Hq / Hkv) + 8 * NT - 1) / (8 * NT), rows = (long long)T * Hq;
     if (tiles * max_runs > 2147483647ll || tiles * 8 * NT >= 1 << 20 || Hkv > 65535 || B > 65535)
         return qwb_fail(QWB_ERR_ARG, "kv4_attention: %d sequences of up to %d new tokens, %d heads: too many blocks", B, max_new, Hkv);
-    const long long rows = (long long)T * Hq;
     if (rows > 2147483647ll) return qwb_fail(QWB_ERR_ARG, "kv4_attention: %lld rows of queries", rows);
-    float* part_ml = scratch ? scratch + (size_t)rows * max_runs * HD : nullptr;
-    qwb_launch(kernel, dim3((unsigned)(tiles * max_runs), Hkv, B), KD_WARPS * 32, Smem::BYTES, stream, q, pool, page_table, cu, pos0, out, scratch, part_ml, T, B,
-               pool_pages, Hq / Hkv, Hkv, table_width, fabsf(scale) * 1.4426950408889634f, scale < 0.f ? 0x80008000u : 0u, window, (int)tiles, max_runs);
-    if (max_runs > 1)
-        qwb_launch_early(kv4_attn_join_kernel<HD>, dim3((unsigned)rows), KJ_WARPS * 32, 0, stream, scratch, part_ml, cu, pos0, tok_seq, out, T, B, Hq,
-                        table_width, window, max_runs);
+    const float log2_scale = fabsf(scale) * 1.4426950408889634f;
+    const uint32_t flip = scale < 0.f ? 0x80008000u : 0u;
+    if (!scratch) {
+        auto kernel = kv4_attn_rows_kernel<HD, NT, true>;
+        const int size = kv4_cluster_size(max_runs);
+        if (size > 8) {                                     // more than 8 blocks have to be allowed, once a device
+            static bool allowed[64];
+            int device = 0;
+            cudaError_t e = cudaGetDevice(&device);
+            if (e == cudaSuccess && (device < 0 || device >= 64 || !allowed[device])) {
+                e = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+                if (e == cudaSuccess && device >= 0 && device < 64) allowed[device] = true;
+            }
+            if (e != cudaSuccess) return qwb_fail(QWB_ERR_CUDA, "kv4_attention: %s", cudaGetErrorString(e));
+        }
+        cudaLaunchConfig_t cfg = {};
+        cfg.gridDim = dim3((unsigned)(tiles * size), Hkv, B);
+        cfg.blockDim = dim3(KD_WARPS * 32);
+        cfg.dynamicSmemBytes = Smem::BYTES;
+        cfg.stream = stream;
+        cudaLaunchAttribute attr[1];
+        attr[0].id = cudaLaunchAttributeClusterDimension;
+        attr[0].val.clusterDim.x = size;
+        attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+        cfg.attrs = attr;
+        cfg.numAttrs = 1;
+        const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, q, pool, page_table, cu, pos0, out, (float*)nullptr, (float*)nullptr, T, B, pool_pages, Hq / Hkv, Hkv,
+                                                 table_width, log2_scale, flip, window, (int)tiles, size);
+        if (e != cudaSuccess) return qwb_fail(QWB_ERR_CUDA, "kv4_attention: %s", cudaGetErrorString(e));
+        return qwb_check_launch("kv4_attention");
+    }
+    float* part_ml = scratch + (size_t)rows * max_runs * HD;
+    qwb_launch(kv4_attn_rows_kernel<HD, NT, false>, dim3((unsigned)(tiles * max_runs), Hkv, B), KD_WARPS * 32, Smem::BYTES, stream, q, pool, page_table, cu, pos0, out,
+               scratch, part_ml, T, B, pool_pages, Hq / Hkv, Hkv, table_width, log2_scale, flip, window, (int)tiles, max_runs);
+    qwb_launch_early(kv4_attn_join_kernel<HD>, dim3((unsigned)rows), KJ_WARPS * 32, 0, stream, scratch, part_ml, cu, pos0, tok_seq, out, T, B, Hq, table_width, window,
+                     max_runs);
     return qwb_check_launch("kv4_attention");
 }
 
-// scratch: T * Hq * max_runs * (hd + 2) floats where max_runs (qwb_kv4_max_runs) is above 1
+// max_runs, and whether there is scratch memory, T * Hq * max_runs * (hd + 2) floats: as qwb_kv4_plan says, or with scratch memory anyway
 extern "C" int qwb_kv4_attn_rows(const void* q, const unsigned char* pool, const int* page_table, const int* cu, const int* pos0, const int* tok_seq,
                                  void* out, float* scratch, int T, int B, int pool_pages, int max_new, int Hq, int Hkv, int hd, int table_width, float scale,
                                  int window, int max_runs, cudaStream_t stream) {
     if (T <= 0) return 0;
     if (Hkv <= 0 || Hq <= 0 || Hq % Hkv || (hd != 64 && hd != 128) || table_width <= 0 || window < 0 || max_new <= 0 || max_runs <= 0 || B <= 0)
         return qwb_fail(QWB_ERR_ARG, "kv4_attention: heads of 64 or 128 only: Hq=%d Hkv=%d hd=%d width=%d window=%d", Hq, Hkv, hd, table_width, window);
-    if (max_runs > 1 && !scratch) return qwb_fail(QWB_ERR_ARG, "kv4_attention: no scratch for %d runs", max_runs);
+    if (max_runs > KD_CLUSTER && !scratch) return qwb_fail(QWB_ERR_ARG, "kv4_attention: no scratch for %d runs", max_runs);
     if ((uintptr_t)q % 16 || (uintptr_t)pool % 16) return qwb_fail(QWB_ERR_ARG, "kv4_attention: q and the pool must start at a multiple of 16 bytes");
-    const bool two = (long long)max_new * (Hq / Hkv) > 8;
+    const bool two = kv4_columns(max_new, Hq / Hkv) == 16;
 #define KV4_ROWS(HD, NT) kv4_launch_rows<HD, NT>((const bf16*)q, pool, page_table, cu, pos0, tok_seq, (bf16*)out, scratch, T, B, pool_pages, max_new, Hq, Hkv, \
                                                  table_width, scale, window, max_runs, stream)
     if (hd == 128) return two ? KV4_ROWS(128, 2) : KV4_ROWS(128, 1);

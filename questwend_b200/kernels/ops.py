@@ -2258,11 +2258,12 @@ def kv4_attention(q: torch.Tensor, pool: torch.Tensor, tables: StepTables, max_n
                           f"{'' if reads else ' (or has no list of pages)'}")
     out = _empty((T, Hq * hd), dtype=q.dtype, device=q.device)
     if impl == "rows":
-        max_runs = _lookup("attention_kv4", "qwb_kv4_max_runs")[1](max_len, max_new, window, table.shape[1])
-        scratch = _empty((T * Hq * max_runs * (hd + 2),), dtype=torch.float32, device=q.device) if max_runs > 1 else None
+        plan = _lookup("attention_kv4", "qwb_kv4_plan")[1](max_len, max_new, window, table.shape[1], B, Hq, Hkv)
+        max_runs = plan >> 1
+        scratch = _empty((T * Hq * max_runs * (hd + 2),), dtype=torch.float32, device=q.device) if plan & 1 else None
         _call("attention_kv4", "qwb_kv4_attn_rows", _ptr(q), _ptr(pool), _ptr(table), _ptr(cu), _ptr(pos0), _ptr(tok_seq), _ptr(out), _ptr(scratch), _i(T),
               _i(B), _i(pool.shape[0]), _i(max_new), _i(Hq), _i(Hkv), _i(hd), _i(table.shape[1]), _f(scale), _i(window), _i(max_runs), _stream(),
-              kernels=2 if max_runs > 1 else 1)
+              kernels=1 if scratch is None else 2)
         return out
     if impl == "read":
         k, v, compact = kv4_read(pool, tables.pages, tables.page_start, tables.seq_len, max_len, hd, q.dtype, marked=True, rest=(out, cu[B:]))
@@ -2312,8 +2313,10 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top: int = 0, out
                 raise KernelError(f"token_logprobs: {name} of {tuple(t.shape)} for {R} rows and {top} alternatives")
     _here("token_logprobs", logits, tokens, *out)
     if R:
-        segments = _lookup("logprobs", "qwb_logprobs_segments")[1](V)
-        scratch = _empty((R * segments * (259 if top else 3),), dtype=torch.float32, device=dev)
+        size = _lookup("logprobs", "qwb_logprobs_scratch")[1]
+        size.restype = ctypes.c_longlong
+        floats = size(R, V, top)
+        scratch = _empty((floats,), dtype=torch.float32, device=dev) if floats else None
         _call("logprobs", "qwb_logprobs", _ptr(logits), _ptr(tokens), _ptr(out.logprob), _ptr(out.entropy), _ptr(out.top_ids), _ptr(out.top_logprobs),
-              _ptr(scratch), _i(R), _i(V), _i(top), _stream(), kernels=2)
+              _ptr(scratch), _i(R), _i(V), _i(top), _stream(), kernels=2 if floats else 1)
     return out

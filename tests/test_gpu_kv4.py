@@ -305,16 +305,21 @@ def test_a_token_that_is_not_finite_reaches_those_that_see_it_only(dtype, n_new)
             assert got[-2:, 2:, :32].isnan().all(), f
 
 
-def test_attention_does_not_depend_on_the_batch():
-    lens = [300, 1000, 70]
-    pool, order, start, seqs, rng = _cache(8, lens, 2, 128)
-    q = torch.from_numpy(rng.standard_normal((3, 8, 128))).to(BF).to(DEV)
-    pos0 = [n - 1 for n in lens]
-    whole = ops.kv4_attention(q, pool, _tables(order, start, pos0, [1] * 3), 1, max(lens), 0.09)
-    for b in range(3):
-        alone = ops.kv4_attention(q[b:b + 1].contiguous(), pool, _tables(order[start[b]:start[b + 1]], [0, start[b + 1] - start[b]], [pos0[b]], [1]),
-                                  1, lens[b], 0.09)
-        assert torch.equal(whole[b:b + 1], alone)
+@pytest.mark.parametrize("Hq,Hkv,hd,n_new,window", [(8, 2, 128, 1, 0), (8, 2, 64, 1, 0), (8, 2, 128, 3, 0), (4, 4, 128, 1, 500), (32, 2, 64, 1, 0)])
+def test_attention_does_not_depend_on_the_batch(Hq, Hkv, hd, n_new, window):
+    """Bit for bit: alone or with others, and whether the runs of a sequence are joined by a cluster's blocks or, where a longer sequence
+    could be in the batch, by a second kernel."""
+    lens = [300, 1000, 70, 2100]
+    pool, order, start, seqs, rng = _cache(8, lens, Hkv, hd)
+    new, B = [n_new] * len(lens), len(lens)
+    q = torch.from_numpy(rng.standard_normal((B * n_new, Hq, hd))).to(BF).to(DEV)
+    pos0 = [n - n_new for n in lens]
+    run = lambda q, t, most: ops.kv4_attention(q, pool, t, n_new, most, 0.09, window=window, impl="rows")
+    whole = run(q, _tables(order, start, pos0, new), max(lens))
+    assert torch.equal(whole, run(q, _tables(order, start, pos0, new, width=150), 150 * 64))
+    for b in range(B):
+        alone = run(q[b * n_new:(b + 1) * n_new].contiguous(), _tables(order[start[b]:start[b + 1]], [0, start[b + 1] - start[b]], [pos0[b]], [n_new]), lens[b])
+        assert torch.equal(whole[b * n_new:(b + 1) * n_new], alone)
 
 
 @pytest.mark.parametrize("impl", ["plain", "rows"])

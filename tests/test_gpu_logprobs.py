@@ -45,7 +45,7 @@ def test_rows(R, V, top):
     check(x, rng.integers(0, V, R).tolist(), min(top, V))
 
 
-@pytest.mark.parametrize("R,V", [(300, 5000), (70, 20000)])
+@pytest.mark.parametrize("R,V", [(300, 5000), (700, 20000), (3, 270000), (2, 262144)])
 def test_many_rows(R, V):
     rng = np.random.default_rng(R)
     check((rng.standard_normal((R, V)) * 3).astype(np.float32), rng.integers(0, V, R).tolist(), 7)
@@ -106,6 +106,8 @@ def test_a_row_does_not_depend_on_the_others():
     x = (torch.randn(40, 30000, generator=g) * 3).to(DEV)
     t = torch.arange(40, dtype=torch.int32, device=DEV)
     whole = ops.token_logprobs(x, t, top=9)
+    two = ops.token_logprobs(x.repeat(8, 1), t.repeat(8), top=9)            # many rows: no clusters
+    assert all(torch.equal(a, b[:40]) for a, b in zip(whole, two))
     for i in (0, 17, 39):
         one = ops.token_logprobs(x[i:i + 1].contiguous(), t[i:i + 1].contiguous(), top=9)
         assert all(torch.equal(a[i:i + 1], b) for a, b in zip(whole, one))
