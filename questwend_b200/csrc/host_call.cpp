@@ -1,4 +1,4 @@
-// The way from Python to the kernels' launchers: a Python module of five functions.  A step of few tokens is a handful of launches of a few
+// The way from Python to the kernels' launchers: a Python module of six functions.  A step of few tokens is a handful of launches of a few
 // microseconds each, and through ctypes making a launcher's arguments (an object each), checking its tensors and asking for its outputs took
 // longer than the launches: one token through Mamba-2's convolution and recurrence 27 us of the host for 6 us of the GPU.
 //
@@ -6,6 +6,8 @@
 //                                         ctypes objects where another type is wanted (double, unsigned, 64-bit)
 //     fits(tensor, dtype, dimensions)     whether it is a contiguous CUDA tensor of this type (None: any) and number of dimensions (None: any)
 //     empty(shape, dtype=, device=)       torch.empty for these arguments
+//     pieces(like, dtype, shape, ...)     a tuple of uninitialised tensors of these types and shapes on like's device, in one piece of memory, each at a
+//                                         multiple of 256 bytes (six of them 3 us, one after the other 7)
 //     same(x)                             x
 //     fill(array, numbers)                a list's whole numbers into a contiguous array of as many 32-bit ones; False where the list holds anything
 //                                         else, or a number that does not fit: the array then holds any part of them
@@ -162,6 +164,55 @@ PyObject* empty(PyObject*, PyObject* const* args, Py_ssize_t n, PyObject* names)
     END_HANDLE_TH_ERRORS
 }
 
+#define QWB_MAX_PIECES 8
+
+PyObject* pieces(PyObject*, PyObject* const* args, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    const Py_ssize_t count = (n - 1) / 2;
+    if (n < 3 || n % 2 == 0 || count > QWB_MAX_PIECES || !THPVariable_Check(args[0])) return PyErr_Format(PyExc_TypeError, "pieces: a tensor, then types and shapes");
+    int64_t sizes[QWB_MAX_PIECES][4], offset[QWB_MAX_PIECES], bytes = 0;
+    int dims[QWB_MAX_PIECES];
+    at::ScalarType type[QWB_MAX_PIECES];
+    for (Py_ssize_t i = 0; i < count; ++i) {
+        PyObject *dtype = args[1 + 2 * i], *shape = args[2 + 2 * i];
+        if (!THPDtype_Check(dtype) || !PyTuple_CheckExact(shape) || PyTuple_GET_SIZE(shape) > 4) return PyErr_Format(PyExc_TypeError, "pieces: a type and a tuple of up to 4 sizes");
+        type[i] = reinterpret_cast<THPDtype*>(dtype)->scalar_type;
+        dims[i] = (int)PyTuple_GET_SIZE(shape);
+        int64_t numel = 1;
+        for (int d = 0; d < dims[i]; ++d) {
+            sizes[i][d] = PyLong_AsLongLong(PyTuple_GET_ITEM(shape, d));
+            if (PyErr_Occurred()) return nullptr;
+            if (sizes[i][d] < 0 || (sizes[i][d] && numel > ((int64_t)1 << 50) / sizes[i][d])) return PyErr_Format(PyExc_ValueError, "pieces: a size of %lld", (long long)sizes[i][d]);
+            numel *= sizes[i][d];
+        }
+        offset[i] = bytes;
+        bytes += (numel * (int64_t)c10::elementSize(type[i]) + 255) / 256 * 256;
+    }
+    at::Tensor t[QWB_MAX_PIECES];
+    {
+        const auto options = at::TensorOptions().dtype(at::kByte).device(THPVariable_Unpack(args[0]).device());
+        WithoutGil gil;
+        const at::Tensor whole = at::empty({bytes}, options);
+        for (Py_ssize_t i = 0; i < count; ++i) {
+            t[i] = at::detail::make_tensor<c10::TensorImpl>(c10::Storage(whole.storage()), whole.key_set(), c10::scalarTypeToTypeMeta(type[i]));
+            c10::TensorImpl* impl = t[i].unsafeGetTensorImpl();
+            impl->set_storage_offset(offset[i] / (int64_t)c10::elementSize(type[i]));
+            impl->set_sizes_contiguous(at::IntArrayRef(sizes[i], (size_t)dims[i]));
+        }
+    }
+    PyObject* out = PyTuple_New(count);
+    for (Py_ssize_t i = 0; out && i < count; ++i) {
+        PyObject* o = THPVariable_Wrap(std::move(t[i]));
+        if (!o) {
+            Py_DECREF(out);
+            return nullptr;
+        }
+        PyTuple_SET_ITEM(out, i, o);
+    }
+    return out;
+    END_HANDLE_TH_ERRORS
+}
+
 PyObject* same(PyObject*, PyObject* x) {
     Py_INCREF(x);
     return x;
@@ -188,6 +239,7 @@ PyObject* fill(PyObject*, PyObject* const* args, Py_ssize_t n) {
 PyMethodDef methods[] = {{"call", (PyCFunction)(void*)call, METH_FASTCALL, nullptr},
                          {"fits", (PyCFunction)(void*)fits, METH_FASTCALL, nullptr},
                          {"empty", (PyCFunction)(void*)empty, METH_FASTCALL | METH_KEYWORDS, nullptr},
+                         {"pieces", (PyCFunction)(void*)pieces, METH_FASTCALL, nullptr},
                          {"same", same, METH_O, nullptr},
                          {"fill", (PyCFunction)(void*)fill, METH_FASTCALL, nullptr},
                          {nullptr, nullptr, 0, nullptr}};

@@ -53,14 +53,18 @@ def _ptr_object(t: torch.Tensor | None) -> ctypes.c_void_p:
     return ctypes.c_void_p(0 if t is None else t.data_ptr())
 
 
+def _plain_pieces(like: torch.Tensor, *spec) -> tuple:
+    return tuple(torch.empty(shape, dtype=dtype, device=like.device) for dtype, shape in zip(spec[::2], spec[1::2]))
+
+
 def _bind_host(module) -> None:
     """Let the launchers' arguments go through this module, or through ctypes (None)."""
-    global _HOST, _ptr, _i, _f, _address, _empty
+    global _HOST, _ptr, _i, _f, _address, _empty, _pieces
     if module is not None:
         _HOST = module                  # first: arguments for it are made only where it is
-        _ptr, _i, _f, _address, _empty = module.same, operator.index, float, module.same, module.empty
+        _ptr, _i, _f, _address, _empty, _pieces = module.same, operator.index, float, module.same, module.empty, module.pieces
     else:
-        _ptr, _i, _f, _address, _empty = _ptr_object, ctypes.c_int, ctypes.c_float, ctypes.c_void_p, torch.empty
+        _ptr, _i, _f, _address, _empty, _pieces = _ptr_object, ctypes.c_int, ctypes.c_float, ctypes.c_void_p, torch.empty, _plain_pieces
         _HOST = None
 
 
@@ -2124,11 +2128,12 @@ def step_tables(pages: torch.Tensor, page_start: torch.Tensor, pos0: torch.Tenso
                           f"starts do not belong together")
     if T < 0 or W < 0 or T >= 2 ** 31 or W >= 2 ** 31:
         raise KernelError(f"step_tables: {T} tokens, a table of {W} columns")
-    dev = pos0.device
-    table = _empty((B, W), dtype=torch.int32, device=dev)
-    cu = seq_len = tok_seq = tok_pos = slot = None
-    if tokens:      # one piece of memory: a tensor made anew takes the host longer than a view
-        cu, seq_len, tok_seq, tok_pos, slot = _empty((2 * B + 1 + 3 * T,), dtype=torch.int32, device=dev).split((B + 1, B, T, T, T))
+    whole = torch.int32
+    if tokens:
+        table, cu, seq_len, tok_seq, tok_pos, slot = _pieces(pos0, whole, (B, W), whole, (B + 1,), whole, (B,), whole, (T,), whole, (T,), whole, (T,))
+    else:
+        (table,) = _pieces(pos0, whole, (B, W))
+        cu = seq_len = tok_seq = tok_pos = slot = None
     _call("step_tables", "qwb_step_tables", _ptr(pages), _ptr(page_start), _ptr(pos0), _ptr(n_new), _ptr(cu), _ptr(seq_len), _ptr(tok_seq),
           _ptr(tok_pos), _ptr(slot), _ptr(table), _i(pages.numel()), _i(B), _i(T), _i(W), _i(PAGE_SIZE), _i(1 if tokens else 0), _stream())
     return StepTables(cu, seq_len, tok_seq, tok_pos, table, slot, pos0, pages, page_start)
@@ -2209,9 +2214,10 @@ def kv4_read(pool: torch.Tensor, pages: torch.Tensor, page_start: torch.Tensor, 
         _need(used, "rest", torch.int32)
         _here("kv4_read", rows, used)
     width = -(-max_len // PAGE_SIZE)
-    k = _empty((P, Hkv, PAGE_SIZE, head_dim), dtype=dtype, device=pool.device)
-    v = _empty((P, Hkv, PAGE_SIZE, head_dim), dtype=dtype, device=pool.device)
-    table = _empty((B, width), dtype=torch.int32, device=pool.device) if P else torch.zeros((B, width), dtype=torch.int32, device=pool.device)
+    shape = (P, Hkv, PAGE_SIZE, head_dim)
+    k, v, table = _pieces(pool, dtype, shape, dtype, shape, torch.int32, (B, width))
+    if not P:
+        table.zero_()
     _call("kv4_cache", "qwb_kv4_read", _ptr(pool), _ptr(pages), _ptr(page_start), _ptr(seq_len), _ptr(k), _ptr(v), _i(_dt(dtype)), _ptr(table),
           _i(P), _i(B), _i(width), _i(pool.shape[0]), _i(Hkv), _i(head_dim), _i(1 if marked else 0), _ptr(rows), _ptr(used),
           _i(0 if rows is None else rows.shape[0]), _i(0 if rows is None else rows.shape[1] * rows.element_size()), _stream())
@@ -2303,8 +2309,7 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top: int = 0, out
         raise KernelError(f"token_logprobs: 0 to {LOGPROBS_MAX_TOP} alternatives of a vocabulary of at least as many: {top} of {V}")
     dev = logits.device
     if out is None:
-        out = TokenLogprobs(_empty((R,), dtype=torch.float32, device=dev), _empty((R,), dtype=torch.float32, device=dev),
-                            _empty((R, top), dtype=torch.int32, device=dev), _empty((R, top), dtype=torch.float32, device=dev))
+        out = TokenLogprobs(*_pieces(logits, torch.float32, (R,), torch.float32, (R,), torch.int32, (R, top), torch.float32, (R, top)))
     else:
         for name, t, dtype, shape in (("logprob", out.logprob, torch.float32, (R,)), ("entropy", out.entropy, torch.float32, (R,)),
                                       ("top_ids", out.top_ids, torch.int32, (R, top)), ("top_logprobs", out.top_logprobs, torch.float32, (R, top))):

@@ -4,7 +4,7 @@ import pytest
 import torch
 
 import plain_kv4 as pk
-from questwend_b200.kernels import ops
+from questwend_b200.kernels import build, ops
 from questwend_b200.kernels.limits import kv4_refusal
 from questwend_b200.kernels.ops import KernelError
 
@@ -67,3 +67,28 @@ def test_plain_tables():
     assert cu == [0, 6, 6, 8] and length == [66, 0, 7] and seq == [0] * 6 + [2, 2, -1]
     assert pos == [60, 61, 62, 63, 64, 65, 5, 6, -1] and table == [[7, 3], [0, 0], [9, 0]]
     assert slot == [7 * 64 + 60, 7 * 64 + 61, 7 * 64 + 62, 7 * 64 + 63, 3 * 64, 3 * 64 + 1, 9 * 64 + 5, 9 * 64 + 6, -1]
+
+
+@pytest.mark.parametrize("way", ["native", "plain"])
+def test_pieces(way):
+    make = ops._plain_pieces
+    if way == "native":
+        module = build.host_calls()
+        if module is None:
+            pytest.skip("no native module")
+        make = module.pieces
+    like = torch.zeros(3)
+    a, b, c, d = make(like, torch.int32, (2, 5), torch.float32, (7,), torch.bfloat16, (0, 3), torch.uint8, (1, 2, 3, 4))
+    assert [tuple(t.shape) for t in (a, b, c, d)] == [(2, 5), (7,), (0, 3), (1, 2, 3, 4)]
+    assert [t.dtype for t in (a, b, c, d)] == [torch.int32, torch.float32, torch.bfloat16, torch.uint8]
+    assert all(t.is_contiguous() and t.device == like.device and not t.requires_grad for t in (a, b, c, d))
+    for i, t in enumerate((a, b, d)):
+        t.fill_(i + 1)
+    assert (a == 1).all() and (b == 2).all() and (d == 3).all() and all(t.data_ptr() % 64 == a.data_ptr() % 64 for t in (b, d) if way == "native")
+    keep = b.clone()
+    del a, d
+    assert torch.equal(b, keep) and torch.equal(b.view(torch.int32).view(torch.float32), keep)
+    if way == "native":
+        for args in [(like,), (like, torch.int32), (1, torch.int32, (2,)), (like, 3, (2,)), (like, torch.int32, [2]), (like, torch.int32, (-1,))]:
+            with pytest.raises((TypeError, ValueError)):
+                make(*args)
