@@ -25,6 +25,7 @@
 // The plain kernel: any head size that is a multiple of 32, queries in 32 bits or bfloat16.  A block takes a (token, query head),
 // its four warps every fourth key; a lane holds the numbers lane, lane + 32, ... of the query, of the sums and of a key, so a
 // group of 32 is a step of the loop over them.  Each warp keeps a running maximum, sum and output; they meet in shared memory.
+#include "attention_pieces.h"
 #include "kv4.cuh"
 
 #include <math.h>
@@ -119,7 +120,7 @@ extern "C" int qwb_kv4_attn_plain(const void* q, const unsigned char* pool, cons
 // ----------------------------------------------------------------------------- few new tokens: mma.sync
 #define KD_WARPS 2
 #define KD_KEYS 32              // keys of a page that a warp takes: two tiles of the mma's 16 rows
-#define KD_STAGES 3             // pages of a warp's ring
+#define KD_STAGES 2             // pages of a warp's ring: 8 x 4,096 tokens 15.0 us, with three 16.0
 #define KD_RUNS 16              // a sequence's pages are cut into about so many runs ...
 #define KD_RUN_PAGES 8          // ... of at most this many pages
 #define KD_RAISE 8.f            // a run's reference is raised where a score passes it by 2^8
@@ -638,16 +639,35 @@ static int kv4_cluster_size(long long runs) {
     return size;
 }
 
-// How a call's runs are joined: the most runs of a sequence, times 2, plus 1 if by scratch memory and a second kernel.  Up to 16 runs go
-// as clusters while these are all on the chip at once (7 blocks an SM, 4 with 16 columns): a second launch and a kernel's start less, 8.0
-// and 7.0 us for one sequence of 2,048 tokens, 15.0 and 13.6 for 16,384; 8 sequences of 4,096, 1,024 blocks, are even (16.1).  Beyond that a
-// cluster waits for 16 free places: 64 sequences of 1,000 take 66.8 us against 36.6, 4 of 8,192 with 6 new tokens 45.7 against 30.9.
-extern "C" int qwb_kv4_plan(int max_len, int max_new, int window, int table_width, int B, int Hq, int Hkv) {
+// Whether a step that brings more than a few tokens is faster with its pages read as bfloat16 once and the tcgen05 prompt kernel.  That kernel
+// reaches six times the rate, but the pages go through memory twice more; as rows every run of every 16 columns is a block, with a start and an
+// end that cost as much as 3.5 pages.  Both in microseconds, from measurements (32 query and 8 key heads of 128, as rows / read, with 8, 32 and 128
+// new tokens a sequence): one sequence of 1,000 tokens 12 / 20, 15 / 21, 38 / 21; of 8,192 19 / 36, 41 / 37, 121 / 49; of 60,000 68 / 151, 205 / 152, 768 / 225;
+// 8 of 8,192 66 / 116, 218 / 185, 742 / 267.
+// tokens, listed: the step's tokens and its sequences' pages (which say more of unequal sequences than the most of each).
+static bool kv4_read_is_faster(int max_len, int max_new, int window, int table_width, int B, int Hq, int Hkv, int hd, int tokens, int listed) {
+    const int G = Hq / Hkv;
+    if (G > 64 || listed <= 0 || (long long)max_new * G <= 16) return false;
+    if (max_new > max_len) max_new = max_len;
+    long long mean_len = (long long)listed * KV4_PAGE / B;
+    if (mean_len > max_len) mean_len = max_len;
+    const Kv4Runs cut = kv4_runs(mean_len > max_new ? (int)(mean_len - max_new) : 0, (int)mean_len, window, table_width);
+    const double columns = (double)tokens * G / 16.0 + 0.5 * B;
+    const double rows = 5.0 + columns * Hkv * cut.runs * (cut.per_run + 3.5) / (hd == 128 ? 340.0 : 580.0);
+    return 8.0 + at_pieces(tokens, B, max_new, max_len, Hq, Hkv, hd, window).us + (double)listed * Hkv * (hd == 128 ? 0.0095 : 0.005) < rows;
+}
+
+// How a call goes: the most runs of a sequence, times 4, plus 2 if they are joined by scratch memory and a second kernel, plus 1 if reading
+// the pages first is faster.  Up to 16 runs go as clusters, up to 64 of these and while they are all on the chip at once (7 blocks an SM, 4 with
+// 16 columns): a second launch and a kernel's start less, 8.0 and 7.0 us for one sequence of 2,048 tokens, 15.0 and 13.6 for 16,384; 8 sequences
+// of 4,096, 1,024 blocks, are even.  Beyond that a cluster waits for 16 free places, and many small ones start slowly: 64 sequences of 1,000 take 66.8
+// us against 36.6, 4 of 8,192 with 6 new tokens 45.7 against 30.9, one prompt of 128, 256 clusters of 2, 26 against 16.
+extern "C" int qwb_kv4_plan(int max_len, int max_new, int window, int table_width, int B, int Hq, int Hkv, int hd, int tokens, int listed) {
     const long long runs = kv4_max_runs(max_len, max_new, window, table_width);
     const int columns = kv4_columns(max_new, Hq / Hkv);
     const long long tiles = ((long long)max_new * (Hq / Hkv) + columns - 1) / columns;
-    const bool clusters = runs <= KD_CLUSTER && tiles * kv4_cluster_size(runs) * Hkv * B <= 148 * (columns == 8 ? 7 : 4);
-    return (int)(2 * runs + (runs > 1 && !clusters ? 1 : 0));
+    const bool clusters = runs <= KD_CLUSTER && tiles * Hkv * B <= 64 && tiles * kv4_cluster_size(runs) * Hkv * B <= 148 * (columns == 8 ? 7 : 4);
+    return (int)(4 * runs) + (runs > 1 && !clusters ? 2 : 0) + (kv4_read_is_faster(max_len, max_new, window, table_width, B, Hq, Hkv, hd, tokens, listed) ? 1 : 0);
 }
 
 template <int HD, int NT>
@@ -708,10 +728,10 @@ extern "C" int qwb_kv4_attn_rows(const void* q, const unsigned char* pool, const
         return qwb_fail(QWB_ERR_ARG, "kv4_attention: heads of 64 or 128 only: Hq=%d Hkv=%d hd=%d width=%d window=%d", Hq, Hkv, hd, table_width, window);
     if (max_runs > KD_CLUSTER && !scratch) return qwb_fail(QWB_ERR_ARG, "kv4_attention: no scratch for %d runs", max_runs);
     if ((uintptr_t)q % 16 || (uintptr_t)pool % 16) return qwb_fail(QWB_ERR_ARG, "kv4_attention: q and the pool must start at a multiple of 16 bytes");
-    const bool two = kv4_columns(max_new, Hq / Hkv) == 16;
+    const int columns = kv4_columns(max_new, Hq / Hkv);
 #define KV4_ROWS(HD, NT) kv4_launch_rows<HD, NT>((const bf16*)q, pool, page_table, cu, pos0, tok_seq, (bf16*)out, scratch, T, B, pool_pages, max_new, Hq, Hkv, \
                                                  table_width, scale, window, max_runs, stream)
-    if (hd == 128) return two ? KV4_ROWS(128, 2) : KV4_ROWS(128, 1);
-    return two ? KV4_ROWS(64, 2) : KV4_ROWS(64, 1);
+    if (hd == 128) return columns == 16 ? KV4_ROWS(128, 2) : KV4_ROWS(128, 1);
+    return columns == 16 ? KV4_ROWS(64, 2) : KV4_ROWS(64, 1);
 #undef KV4_ROWS
 }

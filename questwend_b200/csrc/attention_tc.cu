@@ -23,6 +23,7 @@
 // keys and values once).
 #include "common.cuh"
 
+#include "attention_pieces.h"
 #include "attention_tc.cuh"
 
 #define AT_THREADS 192
@@ -40,13 +41,18 @@ struct AtSmem {
 };
 
 // HD, VD: key and value sizes filled up to 64 or 128; vd: the value size itself.
-template <int HD, int VD, bool SHAPED>      // SHAPED: the softmax also takes a distance bias per head and a sink (else the kernel is as it was)
+// SHAPED: the softmax also takes a distance bias per head and a sink (else the kernel is as it was).
+// PIECES: a block takes `piece_tiles` tiles of its rows' keys and leaves its sums, maximum (of scores times log2 e) and denominator to
+// attn_tc_join_kernel, in part_o [T * Hq, pieces, VD] and part_ml [T * Hq, pieces, 2] (with few rows and long contexts a block a row's tile
+// would walk over all keys by itself while most SMs stand idle).
+template <int HD, int VD, bool SHAPED, bool PIECES = false>
 __global__ void __launch_bounds__(AT_THREADS)
 attn_tc_prefill_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
                        const __grid_constant__ CUtensorMap map_v, const int* __restrict__ page_table,
                        const int* __restrict__ cu_seqlens, const int* __restrict__ pos0, bf16* __restrict__ out, int Hq, int Hkv,
                        int vd, int table_width, float scale, int window, int chunk, int G, int* error,
-                       const float* __restrict__ slopes, const float* __restrict__ sinks) {
+                       const float* __restrict__ slopes, const float* __restrict__ sinks, int pieces, int piece_tiles, float* __restrict__ part_o,
+                       float* __restrict__ part_ml) {
     using Smem = AtSmem<HD, VD>;
     constexpr uint32_t K_BYTES = Smem::K_BYTES, V_BYTES = Smem::V_BYTES;
     constexpr uint32_t TMEM_COLS = 256;                                     // S: 2 x 64 columns, O: VD columns
@@ -73,7 +79,7 @@ attn_tc_prefill_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(o_full + 1);
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int b = blockIdx.z, kvh = blockIdx.x;
+    const int b = PIECES ? blockIdx.z / pieces : blockIdx.z, piece = PIECES ? blockIdx.z - b * pieces : 0, kvh = blockIdx.x;
     const int tok_per_block = AT_ROWS / G;
     const int t0 = cu_seqlens[b], n_new = cu_seqlens[b + 1] - t0;
     // The last tokens see the most keys: their blocks go first, so that the long blocks do not form the tail of the launch.
@@ -87,7 +93,9 @@ attn_tc_prefill_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
     const int k_last = p0 + last_tok;
     // with `chunk` > 0 a query sees only the keys of its own block of `chunk` positions, counted from position 0
     const int k_first = chunk > 0 ? ((p0 + q0) / chunk) * chunk : (window > 0 ? max(0, p0 + q0 - window + 1) : 0);
-    const int tile_first = k_first / AT_KEYS, tile_last = k_last / AT_KEYS;
+    const int tile_first = k_first / AT_KEYS + (PIECES ? piece * piece_tiles : 0);
+    const int tile_last = PIECES ? min(k_last / AT_KEYS, tile_first + piece_tiles - 1) : k_last / AT_KEYS;
+    if (PIECES && tile_first > tile_last) return;
     const int n_tiles = tile_last - tile_first + 1;
     const int* pages = page_table + (size_t)b * table_width;
 
@@ -306,6 +314,20 @@ attn_tc_prefill_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
         if (ok) {
             // a sink: one more term of the denominator, exp(sink), relative to the row's reference
             if (SHAPED && sinks && row_ok) l += at_exp2(sinks[head] * 1.4426950408889634f - (m_ref == -INFINITY ? 0.f : m_ref * sl2));
+            if constexpr (PIECES) {
+                const size_t at = ((size_t)(t0 + tok) * Hq + head) * pieces + piece;
+                float* part = part_o + at * VD;
+#pragma unroll 1
+                for (int c = 0; c < VD; c += 32) {
+                    uint32_t ov[32];
+                    at_ld32(tmem_o + lane_off + c, ov);
+                    if (row_ok) {
+#pragma unroll
+                        for (int i = 0; i < 32; i += 4) *reinterpret_cast<uint4*>(part + c + i) = make_uint4(ov[i], ov[i + 1], ov[i + 2], ov[i + 3]);
+                    }
+                }
+                if (row_ok) *reinterpret_cast<float2*>(part_ml + 2 * at) = make_float2(m_ref == -INFINITY ? -INFINITY : m_ref * sl2, l);
+            } else {
             const float inv = l > 0.f ? 1.f / l : 0.f;
             bf16* dst = out + ((size_t)(t0 + tok) * Hq + head) * vd;
 #pragma unroll 1
@@ -325,6 +347,7 @@ attn_tc_prefill_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
                     }
                 }
             }
+            }
         }
     }
     at_fence_before();
@@ -335,11 +358,56 @@ attn_tc_prefill_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
     }
 }
 
+// Joins the pieces of a row, a warp each: relative to the largest maximum, in their order.
+template <int VD>
+__global__ void __launch_bounds__(256)
+attn_tc_join_kernel(const float* __restrict__ part_o, const float* __restrict__ part_ml, const int* __restrict__ tok_seq, const int* __restrict__ cu_seqlens,
+                    const int* __restrict__ pos0, bf16* __restrict__ out, int rows, int B, int Hq, int tok_per_block, int window, int pieces, int piece_tiles) {
+    pdl_wait();
+    pdl_launch_dependents();
+    const int lane = threadIdx.x & 31;
+    const long long row = (long long)blockIdx.x * 8 + (threadIdx.x >> 5);
+    if (row >= rows) return;
+    const int t = (int)(row / Hq), b = tok_seq[t];
+    if (b < 0 || b >= B) return;
+    // the tiles that the row's block went over, as it found them
+    const int t0 = cu_seqlens[b], n_new = cu_seqlens[b + 1] - t0, q0 = (t - t0) / tok_per_block * tok_per_block, p0 = pos0[b];
+    const int first = (window > 0 ? max(0, p0 + q0 - window + 1) : 0) / AT_KEYS, last = (p0 + min(n_new, q0 + tok_per_block) - 1) / AT_KEYS;
+    const int count = min((last - first) / piece_tiles + 1, pieces);
+    const float* ml = part_ml + row * pieces * 2;
+    float top = -INFINITY;
+    for (int i = lane; i < count; i += 32) top = fmaxf(top, ml[2 * i]);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+    constexpr int E = VD / 32;
+    float y[E] = {}, total = 0.f;
+#pragma unroll 4
+    for (int i = 0; i < count; ++i) {
+        const float2 x = *reinterpret_cast<const float2*>(ml + 2 * i);
+        float v[E];
+        const float* src = part_o + (row * pieces + i) * VD + lane * E;
+        if constexpr (E == 4) *reinterpret_cast<float4*>(v) = *reinterpret_cast<const float4*>(src);
+        else *reinterpret_cast<float2*>(v) = *reinterpret_cast<const float2*>(src);
+        if (x.y == 0.f) continue;                            // a piece that the row sees nothing of
+        const float f = x.x == top ? 1.f : at_exp2(x.x - top);
+        total += f * x.y;
+#pragma unroll
+        for (int e = 0; e < E; ++e) y[e] = fmaf(f, v[e], y[e]);
+    }
+    const float inv = total == 0.f ? 0.f : 1.f / total;
+    __nv_bfloat162 p[E / 2];
+#pragma unroll
+    for (int e = 0; e < E / 2; ++e) p[e] = __floats2bfloat162_rn(y[2 * e] * inv, y[2 * e + 1] * inv);
+    if constexpr (E == 4) *reinterpret_cast<uint2*>(out + row * VD + lane * E) = *reinterpret_cast<uint2*>(p);
+    else *reinterpret_cast<__nv_bfloat162*>(out + row * VD + lane * E) = p[0];
+}
+
 // ------------------------------------------------------------------------------------------- host side
 template <int HD, int VD>
 static int launch_attn_tc(const void* q, const void* k_pool, const void* v_pool, const int* page_table, const int* cu_seqlens,
                           const int* pos0, void* out, int B, int T, int max_new, int n_pages, int Hq, int Hkv, int hd, int vd, int table_width,
-                          float scale, int window, int chunk, int* error, const float* slopes, const float* sinks, cudaStream_t stream) {
+                          float scale, int window, int chunk, int* error, const float* slopes, const float* sinks, cudaStream_t stream,
+                          int pieces = 1, int piece_tiles = 0, float* scratch = nullptr, const int* tok_seq = nullptr) {
     AtEncodeFn enc = at_encode();
     if (!enc) return qwb_fail(QWB_ERR_CUDA, "attn_tc_prefill: cuTensorMapEncodeTiled is not available from this driver");
     const int G = Hq / Hkv;
@@ -369,15 +437,24 @@ static int launch_attn_tc(const void* q, const void* k_pool, const void* v_pool,
     }
     const size_t smem = AtSmem<HD, VD>::BYTES;
     const int tok_per_block = AT_ROWS / G;
-    dim3 grid(Hkv, (max_new + tok_per_block - 1) / tok_per_block, B);
+    dim3 grid(Hkv, (max_new + tok_per_block - 1) / tok_per_block, B * pieces);
+    float* part_ml = scratch ? scratch + (size_t)T * Hq * pieces * VD : nullptr;
     auto go = [&](auto kernel) -> int {
         cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
         if (e != cudaSuccess) return qwb_fail(QWB_ERR_CUDA, "attn_tc_prefill: %s", cudaGetErrorString(e));
         e = qwb_launch(kernel, grid, AT_THREADS, smem, stream, map_q, map_k, map_v, page_table, cu_seqlens, pos0,
-                       (bf16*)out, Hq, Hkv, vd, table_width, scale, window, chunk, G, error, slopes, sinks);
+                       (bf16*)out, Hq, Hkv, vd, table_width, scale, window, chunk, G, error, slopes, sinks, pieces, piece_tiles, scratch, part_ml);
         if (e != cudaSuccess) return qwb_fail(QWB_ERR_CUDA, "attn_tc_prefill: launch failed: %s", cudaGetErrorString(e));
         return qwb_check_launch("attn_tc_prefill");
     };
+    if (pieces > 1) {
+        if constexpr (HD == VD) {
+            if (int rc = go(attn_tc_prefill_kernel<HD, VD, false, true>)) return rc;
+            qwb_launch(attn_tc_join_kernel<VD>, dim3((unsigned)(((long long)T * Hq + 7) / 8)), 256, 0, stream, scratch, part_ml, tok_seq, cu_seqlens, pos0, (bf16*)out,
+                       T * Hq, B, Hq, tok_per_block, window, pieces, piece_tiles);
+            return qwb_check_launch("attn_tc_prefill_pieces");
+        }
+    }
     if (slopes || sinks) {
         if constexpr (HD == VD) return go(attn_tc_prefill_kernel<HD, VD, true>);
         else return qwb_fail(QWB_ERR_ARG, "attn_tc_prefill: a distance bias or a sink goes with keys and values of about one size, not %d and %d", hd, vd);
@@ -418,4 +495,31 @@ extern "C" int qwb_attn_tc_prefill(const void* q, const void* k_pool, const void
     if (vd <= 64) QWB_AT_LAUNCH(128, 64);
     QWB_AT_LAUNCH(128, 128);
 #undef QWB_AT_LAUNCH
+}
+
+// The pieces that a step's keys are best cut into, and the tiles of 64 keys of each: 2^32 tiles + pieces.  32 query and 8 key heads of 128, over pages
+// read from a cache in 4 bits, that included: 64 new tokens of a sequence of 60,000 999 us whole, 171 in 17 pieces; of 8,192 143 and 42.
+extern "C" long long qwb_attn_tc_pieces(int T, int B, int max_new, int max_len, int Hq, int Hkv, int hd, int window) {
+    const AtPieces p = at_pieces(T, B, max_new, max_len, Hq, Hkv, hd, window);
+    return ((long long)p.tiles << 32) + p.pieces;
+}
+
+// qwb_attn_tc_prefill without chunks, biases and sinks, heads of 64 or 128, the keys cut into `pieces` of `piece_tiles` tiles of 64.  tok_seq [T]: each
+// token's sequence, or -1; scratch: T * Hq * pieces * (hd + 2) floats.
+extern "C" int qwb_attn_tc_prefill_pieces(const void* q, const void* k_pool, const void* v_pool, const int* page_table, const int* cu_seqlens,
+                                          const int* pos0, const int* tok_seq, void* out, float* scratch, int B, int T, int max_new, int n_pages, int Hq, int Hkv,
+                                          int hd, int table_width, float scale, int window, int pieces, int piece_tiles, int* error, cudaStream_t stream) {
+    if (B <= 0 || max_new <= 0 || T <= 0) return 0;
+    if ((hd != 64 && hd != 128) || Hq <= 0 || Hkv <= 0 || Hq % Hkv || Hq / Hkv > AT_ROWS / 2 || window < 0 || pieces < 2 || piece_tiles < 1 || !scratch || !error ||
+        !tok_seq)
+        return qwb_fail(QWB_ERR_ARG, "attn_tc_prefill_pieces: %d heads of 64 or 128 (not %d) over %d, %d pieces of %d tiles", Hq, hd, Hkv, pieces, piece_tiles);
+    const int G = Hq / Hkv;
+    if ((long long)B * pieces > 65535 || (max_new + AT_ROWS / G - 1) / (AT_ROWS / G) > 65535 || (long long)T * Hq > 2147483647ll)
+        return qwb_fail(QWB_ERR_ARG, "attn_tc_prefill_pieces: batch %d in %d pieces or %d new tokens of a sequence are more than the grid takes", B, pieces, max_new);
+    if ((uintptr_t)q % 16 || (uintptr_t)k_pool % 16 || (uintptr_t)v_pool % 16 || (uintptr_t)out % 16 || (uintptr_t)scratch % 16)
+        return qwb_fail(QWB_ERR_ARG, "attn_tc_prefill_pieces: operands must be 16-byte aligned");
+    return hd == 64 ? launch_attn_tc<64, 64>(q, k_pool, v_pool, page_table, cu_seqlens, pos0, out, B, T, max_new, n_pages, Hq, Hkv, hd, hd, table_width, scale, window, 0,
+                                             error, nullptr, nullptr, stream, pieces, piece_tiles, scratch, tok_seq)
+                    : launch_attn_tc<128, 128>(q, k_pool, v_pool, page_table, cu_seqlens, pos0, out, B, T, max_new, n_pages, Hq, Hkv, hd, hd, table_width, scale, window, 0,
+                                               error, nullptr, nullptr, stream, pieces, piece_tiles, scratch, tok_seq);
 }

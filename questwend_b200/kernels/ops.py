@@ -2224,9 +2224,6 @@ def kv4_read(pool: torch.Tensor, pages: torch.Tensor, page_start: torch.Tensor, 
     return k, v, table
 
 
-KV4_ROWS_MAX_COLUMNS = 64       # new tokens of a sequence times query heads of a group up to which a prompt's pieces go as rows
-
-
 def kv4_attention(q: torch.Tensor, pool: torch.Tensor, tables: StepTables, max_new: int, max_len: int, scale: float, window: int = 0,
                   impl: str = "auto") -> torch.Tensor:
     """Causal attention of a step's tokens over the cache in 4 bits (their own rows written before).  ``q`` [T, Hq, hd] float32
@@ -2257,22 +2254,34 @@ def kv4_attention(q: torch.Tensor, pool: torch.Tensor, tables: StepTables, max_n
     group = Hq // Hkv
     fits = q.dtype == torch.bfloat16 and hd in (64, 128)
     reads = fits and group <= 64 and tables.pages is not None and tables.page_start is not None
+    plan = 0
+    if fits and impl != "plain":
+        plan = _lookup("attention_kv4", "qwb_kv4_plan")[1](max_len, max_new, window, table.shape[1], B, Hq, Hkv, hd, T,
+                                                                tables.pages.numel() if reads else 0)
     if impl == "auto":
-        impl = "plain" if not fits else "read" if reads and max_new * group > KV4_ROWS_MAX_COLUMNS else "rows"
+        impl = "plain" if not fits else "read" if reads and plan & 1 else "rows"
     if (impl == "rows" and not fits) or (impl == "read" and not reads):
         raise KernelError(f"kv4_attention: form '{impl}' does not take {q.dtype} queries of {hd}, groups of {group}"
                           f"{'' if reads else ' (or has no list of pages)'}")
     out = _empty((T, Hq * hd), dtype=q.dtype, device=q.device)
     if impl == "rows":
-        plan = _lookup("attention_kv4", "qwb_kv4_plan")[1](max_len, max_new, window, table.shape[1], B, Hq, Hkv)
-        max_runs = plan >> 1
-        scratch = _empty((T * Hq * max_runs * (hd + 2),), dtype=torch.float32, device=q.device) if plan & 1 else None
+        max_runs = plan >> 2
+        scratch = _empty((T * Hq * max_runs * (hd + 2),), dtype=torch.float32, device=q.device) if plan & 2 else None
         _call("attention_kv4", "qwb_kv4_attn_rows", _ptr(q), _ptr(pool), _ptr(table), _ptr(cu), _ptr(pos0), _ptr(tok_seq), _ptr(out), _ptr(scratch), _i(T),
               _i(B), _i(pool.shape[0]), _i(max_new), _i(Hq), _i(Hkv), _i(hd), _i(table.shape[1]), _f(scale), _i(window), _i(max_runs), _stream(),
               kernels=1 if scratch is None else 2)
         return out
     if impl == "read":
         k, v, compact = kv4_read(pool, tables.pages, tables.page_start, tables.seq_len, max_len, hd, q.dtype, marked=True, rest=(out, cu[B:]))
+        cut = _lookup("attention_tc", "qwb_attn_tc_pieces")[1]
+        cut.restype = ctypes.c_longlong
+        tiles, pieces = divmod(cut(T, B, max_new, max_len, Hq, Hkv, hd, window), 2 ** 32)
+        if pieces > 1:
+            scratch = _empty((T * Hq * pieces * (hd + 2),), dtype=torch.float32, device=q.device)
+            _call("attention_tc", "qwb_attn_tc_prefill_pieces", _ptr(q), _ptr(k), _ptr(v), _ptr(compact), _ptr(cu), _ptr(pos0), _ptr(tok_seq), _ptr(out),
+                  _ptr(scratch), _i(B), _i(T), _i(max_new), _i(k.shape[0]), _i(Hq), _i(Hkv), _i(hd), _i(compact.shape[1]), _f(scale), _i(window), _i(pieces),
+                  _i(tiles), _ptr(gemm_tc_error_word(q.device)), _stream(), kernels=2)
+            return out
         _call("attention_tc", "qwb_attn_tc_prefill", _ptr(q), _ptr(k), _ptr(v), _ptr(compact), _ptr(cu), _ptr(pos0), _ptr(out), _i(B), _i(T), _i(max_new),
               _i(k.shape[0]), _i(Hq), _i(Hkv), _i(hd), _i(hd), _i(PAGE_SIZE), _i(compact.shape[1]), _f(scale), _i(window), _i(0), _ptr(None), _ptr(None),
               _ptr(gemm_tc_error_word(q.device)), _stream())

@@ -258,6 +258,21 @@ def test_a_longer_prompt(dtype, hd):
         _check(pool, _tables(order, start, pos0, n_new), seqs, q, pos0, n_new, max(lens), hd ** -0.5, window)
 
 
+@pytest.mark.parametrize("Hq,Hkv,hd", [(8, 2, 128), (6, 2, 64)])
+@pytest.mark.parametrize("window", [0, 1500])
+def test_few_tokens_behind_long_contexts(Hq, Hkv, hd, window):
+    """The prompt kernel cuts the keys of such a step into pieces, joined by a kernel of its own."""
+    lens, n_new = [5000, 700, 2950], [20, 33, 1]
+    pool, order, start, seqs, rng = _cache(Hq, lens, Hkv, hd)
+    pos0 = [a - b for a, b in zip(lens, n_new)]
+    q = torch.from_numpy(rng.standard_normal((sum(n_new) + 3, Hq, hd))).to(BF).to(DEV)
+    t = _tables(order, start, pos0, n_new, behind=3)
+    _check(pool, t, seqs, q, pos0, n_new, max(lens), hd ** -0.5, window)
+    before = ops.LAUNCHES[0]
+    ops.kv4_attention(q, pool, t, max(n_new), max(lens), 0.1, window=window, impl="read")
+    assert ops.LAUNCHES[0] - before == 3                   # pages, pieces, join
+
+
 @pytest.mark.parametrize("dtype", [F32, BF])
 def test_large_scores(dtype):
     """Scores of hundreds: one key carries all the weight; and a maximum that grows along the sequence."""
