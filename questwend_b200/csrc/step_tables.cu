@@ -7,7 +7,7 @@
 #include "common.cuh"
 
 #define ST_THREADS 256
-#define ST_MAX_SEQS 8192        // counts that a block's shared memory holds
+#define ST_MAX_SEQS 58000       // counts that a block's shared memory holds
 #define ST_PER_THREAD 4         // tokens, and table entries, of a thread
 
 __global__ void __launch_bounds__(ST_THREADS)
@@ -90,7 +90,12 @@ extern "C" int qwb_step_tables(const int* pages, const int* page_start, const in
     const long long table_blocks = ((long long)B * width + per_block - 1) / per_block;
     if (token_blocks + table_blocks > 2147483647ll) return qwb_fail(QWB_ERR_ARG, "step_tables: a table of %d x %d is too large", B, width);
     if (token_blocks + table_blocks == 0) return 0;
-    qwb_launch(step_tables_kernel, dim3((unsigned)(token_blocks + table_blocks)), ST_THREADS, (B + 1) * sizeof(int), stream, pages, page_start, pos0, n_new,
+    const size_t smem = (B + 1) * sizeof(int);
+    if (smem > 48 * 1024) {
+        const cudaError_t e = cudaFuncSetAttribute(step_tables_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+        if (e != cudaSuccess) return qwb_fail(QWB_ERR_CUDA, "step_tables: %s", cudaGetErrorString(e));
+    }
+    qwb_launch(step_tables_kernel, dim3((unsigned)(token_blocks + table_blocks)), ST_THREADS, smem, stream, pages, page_start, pos0, n_new,
                cu, seq_len, tok_seq, tok_pos, slot_map, table, P, B, T, width, page_size, token_blocks);
     return qwb_check_launch("step_tables");
 }

@@ -12,6 +12,7 @@ returns the last position's logits only (core/runtime.h:52-54).
 """
 from __future__ import annotations
 
+import contextlib
 from dataclasses import dataclass, field
 
 import numpy as np
@@ -66,6 +67,8 @@ def build_step_context(cache: CacheManager, entries: list, vocab_size: int, devi
     if len(set(slots)) != len(slots):
         raise EngineError(f"a slot appears twice in one step: {slots}")
     B = len(entries)
+    if B > ops.STEP_TABLES_MAX_SEQS:
+        raise EngineError(f"a step takes up to {ops.STEP_TABLES_MAX_SEQS} sequences, not {B}")
     n_new = []
     for e in entries:
         if len(e.tokens) == 0:
@@ -74,13 +77,8 @@ def build_step_context(cache: CacheManager, entries: list, vocab_size: int, devi
     T = sum(n_new)
     pos0 = [cache.length(s) for s in slots]
 
-    # what only the host knows, as one int32 array: the tokens, each sequence's length, count and slot, the places wanted
-    n_want = sum(len(e.want) for e in entries)
-    offs = np.cumsum([0, T, B, B, B, n_want]).tolist()
-    buf = np.empty(offs[-1], dtype=np.int32)
-    ids, p0, counts, slot_a, want = (buf[offs[i]:offs[i + 1]] for i in range(5))
+    ids, want = np.empty(T, dtype=np.int32), []
     t = 0
-    w = 0
     for b, e in enumerate(entries):
         n = n_new[b]
         if not fill_int32(ids[t:t + n], e.tokens):
@@ -91,41 +89,42 @@ def build_step_context(cache: CacheManager, entries: list, vocab_size: int, devi
         for i in e.want:
             if not 0 <= i < n:
                 raise EngineError(f"slot {e.slot}: wanted place {i} is outside this step's {n} tokens")
-            want[w] = t + i
-            w += 1
+            want.append(t + i)
         t += n
     if T and (ids.min() < 0 or ids.max() >= vocab_size):
         bad = int(ids[(ids < 0) | (ids >= vocab_size)][0])
         raise EngineError(f"token id {bad} is outside the vocabulary of {vocab_size}")
-    p0[:] = pos0
-    counts[:] = n_new
-    slot_a[:] = slots
     slen = [p + n for p, n in zip(pos0, n_new)]
     cache.reserve(dict(zip(slots, slen)))     # after every check: a refused step holds nothing
-    # behind it each cache group's pages, one sequence after the other, and where each one's begin: one copy to the device,
-    # which makes everything else (``ops.step_tables``: a launch a group)
-    group_pages, ends = [], [offs[-1]]
-    for gid in range(max(1, cache.n_groups())):
-        lists = cache.page_lists(gid, slots) if cache.n_groups() else [[] for _ in slots]
-        start = np.zeros(B + 1, dtype=np.int32)
-        np.cumsum([len(p) for p in lists], out=start[1:])
-        flat = np.empty(int(start[B]), dtype=np.int32)
-        for b, p in enumerate(lists):
-            if not fill_int32(flat[start[b]:start[b + 1]], p):
-                flat[start[b]:start[b + 1]] = p
-        group_pages += [start, flat]
-        ends += [ends[-1] + B + 1, ends[-1] + B + 1 + len(flat)]
-    dev = torch.from_numpy(np.concatenate([buf, *group_pages])).to(device)
-    parts = [dev[offs[i]:offs[i + 1]] for i in range(5)]
+    # What only the host knows goes to the device in one copy: the tokens, each sequence's length, count and slot, the places wanted,
+    # and for each cache group where each sequence's pages begin and the pages, one sequence after the other.  Everything else is made
+    # of it there (``ops.step_tables``: a launch a group).
+    groups = cache.n_groups()
+    rest, sizes = [*pos0, *n_new, *slots, *want], [T, B, B, B, len(want)]
+    for gid in range(max(1, groups)):
+        lists = cache.page_lists(gid, slots) if groups else [()] * B
+        starts = [0]
+        for pages in lists:
+            starts.append(starts[-1] + len(pages))
+        rest += starts
+        for pages in lists:
+            rest += pages
+        sizes += [B + 1, starts[-1]]
+    buf = np.empty(T + len(rest), dtype=np.int32)
+    buf[:T] = ids
+    if not fill_int32(buf[T:], rest):
+        buf[T:] = rest
+    dev = torch.from_numpy(buf).to(device)
+    parts = dev.split(sizes)
+    width = cache.table_width if groups else 0
     tables, first = {}, None
-    for gid in range(max(1, cache.n_groups())):
-        start, flat = dev[ends[2 * gid]:ends[2 * gid + 1]], dev[ends[2 * gid + 1]:ends[2 * gid + 2]]
-        of_tokens = first is None or cache.group_spec(gid).bits == 4
-        with torch.cuda.device(dev.device):
-            made = ops.step_tables(flat, start, parts[1], parts[2], T, cache.table_width if cache.n_groups() else 0, tokens=of_tokens)
-        first = first or made
-        if cache.n_groups():
-            tables[gid] = made
+    with contextlib.nullcontext() if dev.get_device() == torch.cuda.current_device() else torch.cuda.device(dev.device):
+        for gid in range(max(1, groups)):
+            of_tokens = first is None or cache.group_spec(gid).bits == 4
+            made = ops.step_tables(parts[6 + 2 * gid], parts[5 + 2 * gid], parts[1], parts[2], T, width, tokens=of_tokens)
+            first = first or made
+            if groups:
+                tables[gid] = made
     ctx = StepContext(n_tokens=T, n_seqs=B, token_ids=parts[0], tok_seq=first.tok_seq, tok_pos=first.tok_pos,
                       cu_seqlens=first.cu_seqlens, pos0=parts[1], seq_len=first.seq_len, slots=parts[3],
                       max_new=max(n_new), min_new=min(n_new), max_len=max(slen), single_token=all(n == 1 for n in n_new),

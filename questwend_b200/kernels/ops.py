@@ -2108,7 +2108,7 @@ class StepTables(NamedTuple):
     page_start: torch.Tensor | None = None      # [B + 1] ... where each sequence's begin
 
 
-STEP_TABLES_MAX_SEQS = 8192     # csrc/step_tables.cu: ST_MAX_SEQS
+STEP_TABLES_MAX_SEQS = 58000    # csrc/step_tables.cu: ST_MAX_SEQS
 
 
 def step_tables(pages: torch.Tensor, page_start: torch.Tensor, pos0: torch.Tensor, n_new: torch.Tensor, n_tokens: int, table_width: int,

@@ -23,7 +23,7 @@ def f64(t):
 
 # ----------------------------------------------------------------------------- tables
 @pytest.mark.parametrize("pos0,n_new,behind", [([0], [1], 0), ([63, 64, 0], [1, 1, 1], 0), ([5, 0, 200, 64], [70, 0, 3, 1], 11), ([100], [3000], 0),
-                                               ([7] * 300, [1, 0, 2] * 100, 5), ([0, 0], [0, 0], 4)])
+                                               ([7] * 300, [1, 0, 2] * 100, 5), ([70] * 14000, [1] * 14000, 3), ([0, 0], [0, 0], 4)])
 @pytest.mark.parametrize("extra", [0, 2])
 def test_step_tables(pos0, n_new, behind, extra):
     rng = np.random.default_rng(len(pos0) + behind)
@@ -51,7 +51,7 @@ def test_step_tables_with_too_few_pages_and_starts_beyond_them():
 def test_step_tables_refusals():
     a = ints([0, 1])
     for args in [(a, a, a, a, 1, 1), (a, ints([0, 1, 2]), a, ints([1]), 1, 1), (a, ints([0, 1, 2]), a, a, -1, 1), (a, ints([0, 1, 2]), a, a, 1, -1),
-                 (a, ints([0]), ints([]), ints([]), 1, 1), (a, ints([0] * 8194), ints([0] * 8193), ints([0] * 8193), 1, 1)]:
+                 (a, ints([0]), ints([]), ints([]), 1, 1), (a, ints([0] * 58002), ints([0] * 58001), ints([0] * 58001), 1, 1)]:
         with pytest.raises(KernelError, match="step_tables"):
             ops.step_tables(*args)
     with pytest.raises(KernelError, match="int32"):
