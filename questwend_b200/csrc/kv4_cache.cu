@@ -114,7 +114,8 @@ kv4_store_kernel(const float* __restrict__ qkv, const float* __restrict__ q_weig
 // its head through 64 bits.  With 64 bits for every key a step of 4,096 tokens of 32 + 2 x 8 heads took 45 us, with a warp a head before that 130.
 //
 // Errors of a key in 32 bits, u = 2^-24: the sum of squares 8 + 4 additions, the mean and eps 1, halved by the root; the inverse root
-// 4 (2 units of 2^-23): 11 u; times the weight and the number 2 u; the rotation 2 u of |p| + |r|: 15 u (|p| + |r|) < 2^-20 (|p| + |r|).
+// 4 (2 units of 2^-23): 11 u; times the weight and the number 2 u; the rotation's products and sum 2 u: of p c - r s it is 15 u (|p c| + |r s|)
+// < 2^-20 (|p c| + |r s|).
 struct Kv4Choice { uint32_t codes, word; bool sure; };
 
 // Four numbers of a lane in a group of 8 lanes' 32, each off by at most e: codes (the first in the lowest bits) and the group's word.
@@ -276,6 +277,7 @@ kv4_store_fast_kernel(const float* __restrict__ qkv, const float* __restrict__ q
         unsigned char* base = pool + ((size_t)(slot / KV4_PAGE) * Hkv + kvh) * kv4_page_bytes(HD) + (is_k ? 0 : kv4_half_bytes(HD));
         const bool turned = is_k && (k_weight || cos_t);
         float w[4] = {1.f, 1.f, 1.f, 1.f}, u[4] = {1.f, 1.f, 1.f, 1.f}, x[4], y[4], e[4] = {}, f[4] = {};
+        bool in_range = true;
         if (turned) {
             float scale = 1.f;
             if (k_weight) {
@@ -284,16 +286,20 @@ kv4_store_fast_kernel(const float* __restrict__ qkv, const float* __restrict__ q
                 for (int i = 0; i < 4; ++i) ss = fmaf(a[i], a[i], fmaf(b[i], b[i], ss));
 #pragma unroll
                 for (int o = 1; o < LANES; o <<= 1) ss += __shfl_xor_sync(mask, ss, o);
-                scale = rsqrtf(ss * (1.f / HD) + eps);
+                const float mean = ss * (1.f / HD) + eps;
+                in_range = mean > 1e-30f && mean < 1e30f;           // else squares were lost or are too large: decided in 64 bits
+                scale = rsqrtf(mean);
                 *reinterpret_cast<float4*>(w) = reinterpret_cast<const float4*>(k_weight)[L];
                 *reinterpret_cast<float4*>(u) = reinterpret_cast<const float4*>(k_weight)[HD / 8 + L];
             }
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 const float p = a[i] * (scale * w[i]), r = b[i] * (scale * u[i]);
-                x[i] = fmaf(p, c[i], -r * sn[i]);
-                y[i] = fmaf(p, sn[i], r * c[i]);
-                e[i] = f[i] = (fabsf(p) + fabsf(r)) * 9.5367431640625e-7f;
+                const float pc = p * c[i], rs = r * sn[i], ps = p * sn[i], rc = r * c[i];
+                x[i] = pc - rs;
+                y[i] = ps + rc;
+                e[i] = (fabsf(pc) + fabsf(rs)) * 9.5367431640625e-7f;
+                f[i] = (fabsf(ps) + fabsf(rc)) * 9.5367431640625e-7f;
             }
         } else {
 #pragma unroll
@@ -303,7 +309,7 @@ kv4_store_fast_kernel(const float* __restrict__ qkv, const float* __restrict__ q
             }
         }
         Kv4Choice lo = kv4_four(x, e, mask), hi = kv4_four(y, f, mask);
-        if (__any_sync(mask, !lo.sure || !hi.sure)) {
+        if (__any_sync(mask, !(in_range && lo.sure && hi.sure))) {
             const uint4 g = kv4_head_exactly<HD>(reinterpret_cast<const float*>(row) + (size_t)head * HD, turned ? k_weight : nullptr,
                                                  turned && cos_t ? cos_t + (size_t)t * (HD / 2) : nullptr, turned && cos_t ? sin_t + (size_t)t * (HD / 2) : nullptr,
                                                  L, eps, mask);

@@ -110,6 +110,25 @@ def test_store(T, Hq, Hkv, hd, rot, norm, dtype):
     assert torch.equal(on_gpu, before) and torch.equal(q, q2)
 
 
+@pytest.mark.parametrize("size", [1e25, 1e-25, 1e-40])
+@pytest.mark.parametrize("eps,factor", [(1e-6, 1.0), (1e-38, 1.7), (0.0, 0.3)])
+@pytest.mark.parametrize("hd", [64, 128])
+def test_store_of_large_and_small_numbers(size, eps, factor, hd):
+    """Squares that 32 bits do not hold, an eps that counts or does not, a rotation that scales."""
+    T, Hkv = 20, 2
+    x, cos, sin, slots, pool, rng = _write_case(3, T, 1, Hkv, hd, hd, 2)
+    x = (x * size).astype(np.float32)
+    cos, sin = (cos * factor).astype(np.float32), (sin * factor).astype(np.float32)
+    kw = (1 + 0.3 * rng.standard_normal(hd)).astype(np.float32)
+    dev = lambda a: torch.from_numpy(a).to(DEV)
+    on_gpu = dev(pool)
+    ops.kv4_store(dev(x), None, dev(kw), dev(cos), dev(sin), dev(slots), on_gpu, 1, Hkv, hd, hd, eps, BF)
+    h = x.astype(np.float64).reshape(T, -1, hd)
+    k = pk.norm_rope(h[:, 1:1 + Hkv], kw.astype(np.float64), cos.astype(np.float64), sin.astype(np.float64), float(np.float32(eps)))
+    for got, ref in zip(pk.unpack(on_gpu.cpu().numpy(), hd), _expected_pool(pool, k, h[:, 1 + Hkv:], slots, hd)):
+        assert (got == ref).all()
+
+
 def test_store_of_groups_at_the_border():
     """Numbers halfway between two codes, zeros, equal numbers, tiny and huge ones, and some that are not finite."""
     hd = 128

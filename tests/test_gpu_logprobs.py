@@ -113,6 +113,17 @@ def test_a_row_does_not_depend_on_the_others():
         assert all(torch.equal(a[i:i + 1], b) for a, b in zip(whole, one))
 
 
+@pytest.mark.parametrize("R", [2, 300])
+def test_logits_that_do_not_begin_at_16_bytes(R):
+    x = (torch.randn(R * 9000 + 1, generator=torch.Generator().manual_seed(4)) * 3).to(DEV)
+    t = torch.zeros(R, dtype=torch.int32, device=DEV)
+    odd = x[1:].view(R, 9000)
+    got, want = ops.token_logprobs(odd, t, top=5), ops.token_logprobs(odd.clone(), t, top=5)
+    assert torch.equal(got.top_ids, want.top_ids)
+    for a, b in ((got.logprob, want.logprob), (got.entropy, want.entropy), (got.top_logprobs, want.top_logprobs)):
+        assert (a - b).abs().max() <= 1e-5                  # another order of the sums
+
+
 def test_out_and_a_replayed_graph():
     g = torch.Generator().manual_seed(2)
     x = (torch.randn(5, 20000, generator=g) * 3).to(DEV)
