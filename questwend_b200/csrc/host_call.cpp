@@ -1,4 +1,4 @@
-// The way from Python to the kernels' launchers: a Python module of six functions.  A step of few tokens is a handful of launches of a few
+// The way from Python to the kernels' launchers: a Python module of seven functions.  A step of few tokens is a handful of launches of a few
 // microseconds each, and through ctypes making a launcher's arguments (an object each), checking its tensors and asking for its outputs took
 // longer than the launches: one token through Mamba-2's convolution and recurrence 27 us of the host for 6 us of the GPU.
 //
@@ -8,6 +8,7 @@
 //     empty(shape, dtype=, device=)       torch.empty for these arguments
 //     pieces(like, dtype, shape, ...)     a tuple of uninitialised tensors of these types and shapes on like's device, in one piece of memory, each at a
 //                                         multiple of 256 bytes (six of them 3 us, one after the other 7)
+//     here(device, *tensors)              whether all tensors (or None) lie on CUDA device number `device`
 //     same(x)                             x
 //     fill(array, numbers)                a list's whole numbers into a contiguous array of as many 32-bit ones; False where the list holds anything
 //                                         else, or a number that does not fit: the array then holds any part of them
@@ -213,6 +214,22 @@ PyObject* pieces(PyObject*, PyObject* const* args, Py_ssize_t n) {
     END_HANDLE_TH_ERRORS
 }
 
+PyObject* here(PyObject*, PyObject* const* args, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    if (n < 1) return PyErr_Format(PyExc_TypeError, "here: no device");
+    const long device = PyLong_AsLong(args[0]);
+    if (PyErr_Occurred()) return nullptr;
+    bool ok = true;
+    for (Py_ssize_t i = 1; ok && i < n; ++i) {
+        if (args[i] == Py_None) continue;
+        if (!THPVariable_Check(args[i])) Py_RETURN_FALSE;
+        const at::Tensor& t = THPVariable_Unpack(args[i]);
+        ok = t.is_cuda() && t.get_device() == device;
+    }
+    return PyBool_FromLong(ok);
+    END_HANDLE_TH_ERRORS
+}
+
 PyObject* same(PyObject*, PyObject* x) {
     Py_INCREF(x);
     return x;
@@ -240,6 +257,7 @@ PyMethodDef methods[] = {{"call", (PyCFunction)(void*)call, METH_FASTCALL, nullp
                          {"fits", (PyCFunction)(void*)fits, METH_FASTCALL, nullptr},
                          {"empty", (PyCFunction)(void*)empty, METH_FASTCALL | METH_KEYWORDS, nullptr},
                          {"pieces", (PyCFunction)(void*)pieces, METH_FASTCALL, nullptr},
+                         {"here", (PyCFunction)(void*)here, METH_FASTCALL, nullptr},
                          {"same", same, METH_O, nullptr},
                          {"fill", (PyCFunction)(void*)fill, METH_FASTCALL, nullptr},
                          {nullptr, nullptr, 0, nullptr}};

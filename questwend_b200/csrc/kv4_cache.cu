@@ -111,21 +111,23 @@ kv4_store_kernel(const float* __restrict__ qkv, const float* __restrict__ q_weig
 // 8 neighbouring lanes, so that norm and group cost three or four exchanges.  What bounds it is memory: 4 bytes read and (queries) 2 or (keys
 // and values) 9/16 written a number.  So the choices are made in 32 bits where these leave no doubt: a number whose quotient by the step lies
 // nearer to the border of two codes than its error can be, or a step nearer to the border of two roundings (about one head in 700), sends
-// its head through 64 bits.  With 64 bits for every key a step of 4,096 tokens of 32 + 2 x 8 heads took 45 us, with a warp a head before that 130.
+// its head through 64 bits.  A step of 4,096 tokens of 32 + 2 x 8 heads: a warp a head 130 us, with 64 bits for
+// every key 45, so 34 (4.2 TB/s; what is left is arithmetic and the chain of a head's exchanges, at 8 blocks an SM).
 //
 // Errors of a key in 32 bits, u = 2^-24: the sum of squares 8 + 4 additions, the mean and eps 1, halved by the root; the inverse root
 // 4 (2 units of 2^-23): 11 u; times the weight and the number 2 u; the rotation's products and sum 2 u: of p c - r s it is 15 u (|p c| + |r s|)
 // < 2^-20 (|p c| + |r s|).
 struct Kv4Choice { uint32_t codes, word; bool sure; };
 
-// Four numbers of a lane in a group of 8 lanes' 32, each off by at most e: codes (the first in the lowest bits) and the group's word.
-__device__ __forceinline__ Kv4Choice kv4_four(const float (&x)[4], const float (&e)[4], unsigned mask) {
-    float lo = 0.f, hi = 0.f, off = 0.f;
+// Four numbers of a lane in a group of 8 lanes' 32, each off by at most `off` of its lane: codes (the first in the lowest bits) and the
+// group's word.  A number plus 3 x 2^22 is rounded to a whole one by the addition, and whole ones add up to the packed codes as floats: roundings
+// and conversions as such have a fraction of the rate.
+__device__ __forceinline__ Kv4Choice kv4_four(const float (&x)[4], float off, unsigned mask) {
+    float lo = 0.f, hi = 0.f;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
         lo = fminf(lo, x[i]);
         hi = fmaxf(hi, fabsf(x[i]) <= 3.4028234663852886e38f ? x[i] : INFINITY);
-        off = fmaxf(off, e[i]);
     }
 #pragma unroll
     for (int o = 1; o < 8; o <<= 1) {
@@ -140,20 +142,20 @@ __device__ __forceinline__ Kv4Choice kv4_four(const float (&x)[4], const float (
     // t is off by 2 off / 15 and by less than 3 of its last places: is it that near to the border of two steps?  (Very small, very large and no
     // numbers: decided in 64 bits.)
     const int bits = __float_as_int(t), border = abs((bits & 0xfffff) - 0x80000);
-    y.sure = t > 1e-36f && t < 1e36f && (float)(border - 3) * (t * 5.9604644775390625e-8f) > 0.14f * off;
-    const float s = __int_as_float((bits + 0x80000) & ~0xfffff);
+    const float s = __int_as_float((bits + 0x80000) & ~0xfffff), whole = 12582912.f;
     float inv;
     asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inv) : "f"(s));
-    const float near = 0.499996f * s, z0 = rintf(-lo * inv);
-    y.sure &= fabsf(fmaf(-z0, s, -lo)) + off < near;
-    const float z = fminf(z0, 15.f);
+    const float z0 = fmaf(-lo, inv, whole) - whole, z = fminf(z0, 15.f);
+    float far = fabsf(fmaf(-z0, s, -lo)), packed = 0.f;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-        const float c = rintf(x[i] * inv);
-        y.sure &= fabsf(fmaf(-c, s, x[i])) + e[i] < near;
-        y.codes |= (uint32_t)(int)fminf(fmaxf(c + z, 0.f), 15.f) << (4 * i);
+        const float c = fmaf(x[i], inv, whole) - whole;
+        far = fmaxf(far, fabsf(fmaf(-c, s, x[i])));
+        packed = fmaf(fminf(fmaxf(c + z, 0.f), 15.f), (float)(1 << (4 * i)), packed);
     }
-    y.word = (__float_as_uint(s) >> 16) | (uint32_t)(int)z;
+    y.sure = t > 1e-36f && t < 1e36f && (float)(border - 3) * (t * 5.9604644775390625e-8f) > 0.14f * off && far + off < 0.499996f * s;
+    y.codes = __float_as_uint(packed + 8388608.f) & 0xffffu;
+    y.word = (__float_as_uint(s) >> 16) | (__float_as_uint(z + 8388608.f) & 15u);
     return y;
 }
 // The same in 64 bits, for both fours of a lane and from the projection's numbers on (weight and cosines null: as they are).
@@ -212,7 +214,7 @@ template <> __device__ __forceinline__ void kv4_put4<bf16>(bf16* p, float a, flo
 
 #define KF_BLOCKS 1184              // as many are wanted of a call
 template <typename TQ, int HD>
-__global__ void __launch_bounds__(KS_WARPS * 32, 9)
+__global__ void __launch_bounds__(KS_WARPS * 32, 8)
 kv4_store_fast_kernel(const float* __restrict__ qkv, const float* __restrict__ q_weight, const float* __restrict__ k_weight,
                       const float* __restrict__ cos_t, const float* __restrict__ sin_t, const int* __restrict__ slot_map,
                       TQ* __restrict__ q_out, unsigned char* __restrict__ pool, long long n_rows, int Hq, int Hkv, float eps, int store_kv) {
@@ -276,7 +278,7 @@ kv4_store_fast_kernel(const float* __restrict__ qkv, const float* __restrict__ q
         const int kvh = head - Hq - (is_k ? 0 : Hkv), at = (int)(slot % KV4_PAGE);
         unsigned char* base = pool + ((size_t)(slot / KV4_PAGE) * Hkv + kvh) * kv4_page_bytes(HD) + (is_k ? 0 : kv4_half_bytes(HD));
         const bool turned = is_k && (k_weight || cos_t);
-        float w[4] = {1.f, 1.f, 1.f, 1.f}, u[4] = {1.f, 1.f, 1.f, 1.f}, x[4], y[4], e[4] = {}, f[4] = {};
+        float w[4] = {1.f, 1.f, 1.f, 1.f}, u[4] = {1.f, 1.f, 1.f, 1.f}, x[4], y[4], e = 0.f, f = 0.f;
         bool in_range = true;
         if (turned) {
             float scale = 1.f;
@@ -298,8 +300,8 @@ kv4_store_fast_kernel(const float* __restrict__ qkv, const float* __restrict__ q
                 const float pc = p * c[i], rs = r * sn[i], ps = p * sn[i], rc = r * c[i];
                 x[i] = pc - rs;
                 y[i] = ps + rc;
-                e[i] = (fabsf(pc) + fabsf(rs)) * 9.5367431640625e-7f;
-                f[i] = (fabsf(ps) + fabsf(rc)) * 9.5367431640625e-7f;
+                e = fmaxf(e, (fabsf(pc) + fabsf(rs)) * 9.5367431640625e-7f);
+                f = fmaxf(f, (fabsf(ps) + fabsf(rc)) * 9.5367431640625e-7f);
             }
         } else {
 #pragma unroll
@@ -421,10 +423,7 @@ kv4_read_kernel(const unsigned char* __restrict__ pool, const int* __restrict__ 
             const float z = kv4_zero(word);
             if (marked) {
                 bool bad = false;
-#pragma unroll
-                for (int g = 0; g < (HD ? HD / KV4_GROUP : 1); ++g) bad |= kv4_is_nan(v_words[row * groups + g]);
-                if constexpr (HD == 0)
-                    for (int g = 1; g < groups; ++g) bad |= kv4_is_nan(v_words[row * groups + g]);
+                for (int g = 0; g < groups; ++g) bad |= kv4_is_nan(v_words[row * groups + g]);
                 if (bad) s = is_v ? 0.f : __uint_as_float(0x7fc00000u);
             }
             if constexpr (sizeof(T) == 2) {                 // two codes at a time, all of it exact: c s - z s

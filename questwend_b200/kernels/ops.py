@@ -93,6 +93,8 @@ def _need(t: torch.Tensor, name: str, dtype=None, ndim=None):
 def _here(what: str, *tensors) -> None:
     """Refuse tensors of another device than the current one: the launch would run here on memory that lies there."""
     here = torch.cuda.current_device()
+    if _HOST is not None and _HOST.here(here, *tensors):
+        return
     for t in tensors:
         if t is not None and t.get_device() != here:
             raise KernelError(f"{what}: a tensor on {t.device}, while the current device is cuda:{here} (use torch.cuda.device)")

@@ -92,3 +92,29 @@ def test_pieces(way):
         for args in [(like,), (like, torch.int32), (1, torch.int32, (2,)), (like, 3, (2,)), (like, torch.int32, [2]), (like, torch.int32, (-1,))]:
             with pytest.raises((TypeError, ValueError)):
                 make(*args)
+
+
+def test_here():
+    module = build.host_calls()
+    if module is None:
+        pytest.skip("no native module")
+    t = torch.zeros(2)
+    assert module.here(0) and module.here(0, None, None) and not module.here(0, t) and not module.here(0, None, 3)
+    with pytest.raises(TypeError):
+        module.here()
+    with pytest.raises(TypeError):
+        module.here("0", t)
+
+
+def test_a_tensor_of_another_device_is_refused(monkeypatch):
+    """Not the device that is current: refused, with what to do, whichever way the check goes."""
+    class Elsewhere:
+        device = "cuda:1"
+
+        def get_device(self):
+            return 1
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: 0)
+    for host in (None, ops._HOST):
+        monkeypatch.setattr(ops, "_HOST", host)
+        with pytest.raises(KernelError, match="use torch.cuda.device"):
+            ops._here("kv4_store", None, Elsewhere())
