@@ -642,8 +642,8 @@ static int kv4_cluster_size(long long runs) {
 // Whether a step that brings more than a few tokens is faster with its pages read as bfloat16 once and the tcgen05 prompt kernel.  That kernel
 // reaches six times the rate, but the pages go through memory twice more; as rows every run of every 16 columns is a block, with a start and an
 // end that cost as much as 3.5 pages.  Both in microseconds, from measurements (32 query and 8 key heads of 128, as rows / read, with 8, 32 and 128
-// new tokens a sequence): one sequence of 1,000 tokens 12 / 20, 15 / 21, 38 / 21; of 8,192 19 / 36, 41 / 37, 121 / 49; of 60,000 68 / 151, 205 / 152, 768 / 225;
-// 8 of 8,192 66 / 116, 218 / 185, 742 / 267.
+// new tokens a sequence): one sequence of 1,000 tokens 12 / 19, 15 / 19, 38 / 19; of 8,192 19 / 34, 41 / 35, 121 / 46; of 60,000 68 / 124, 205 / 124, 768 / 197;
+// 8 of 8,192 65 / 95, 218 / 162, 742 / 243; a whole prompt of 128 16 / 10, of 900 262 / 27.
 // tokens, listed: the step's tokens and its sequences' pages (which say more of unequal sequences than the most of each).
 static bool kv4_read_is_faster(int max_len, int max_new, int window, int table_width, int B, int Hq, int Hkv, int hd, int tokens, int listed) {
     const int G = Hq / Hkv;
@@ -654,7 +654,7 @@ static bool kv4_read_is_faster(int max_len, int max_new, int window, int table_w
     const Kv4Runs cut = kv4_runs(mean_len > max_new ? (int)(mean_len - max_new) : 0, (int)mean_len, window, table_width);
     const double columns = (double)tokens * G / 16.0 + 0.5 * B;
     const double rows = 5.0 + columns * Hkv * cut.runs * (cut.per_run + 3.5) / (hd == 128 ? 340.0 : 580.0);
-    return 8.0 + at_pieces(tokens, B, max_new, max_len, Hq, Hkv, hd, window).us + (double)listed * Hkv * (hd == 128 ? 0.0095 : 0.005) < rows;
+    return 4.0 + at_pieces(tokens, B, max_new, max_len, Hq, Hkv, hd, window).us + (double)listed * Hkv * (hd == 128 ? 0.0065 : 0.0045) < rows;
 }
 
 // How a call goes: the most runs of a sequence, times 4, plus 2 if they are joined by scratch memory and a second kernel, plus 1 if reading

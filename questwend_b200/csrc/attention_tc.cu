@@ -498,7 +498,7 @@ extern "C" int qwb_attn_tc_prefill(const void* q, const void* k_pool, const void
 }
 
 // The pieces that a step's keys are best cut into, and the tiles of 64 keys of each: 2^32 tiles + pieces.  32 query and 8 key heads of 128, over pages
-// read from a cache in 4 bits, that included: 64 new tokens of a sequence of 60,000 999 us whole, 171 in 17 pieces; of 8,192 143 and 42.
+// read from a cache in 4 bits, that included: 64 new tokens of a sequence of 60,000 999 us whole, 143 in 17 pieces; of 8,192 143 and 40.
 extern "C" long long qwb_attn_tc_pieces(int T, int B, int max_new, int max_len, int Hq, int Hkv, int hd, int window) {
     const AtPieces p = at_pieces(T, B, max_new, max_len, Hq, Hkv, hd, window);
     return ((long long)p.tiles << 32) + p.pieces;

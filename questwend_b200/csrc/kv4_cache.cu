@@ -376,84 +376,117 @@ extern "C" int qwb_kv4_store(const float* qkv, const float* q_weight, const floa
 // what a query does not see by 0 gives NaN to the queries that see it only.
 // The blocks also write the table that names these pages: [B, width], page_start[b] + j or 0; and with `rows_out` they set rows of
 // `row_bytes` (a multiple of 16) behind row `rows_used` of `rows` there to zero (what no sequence of a padded step writes).
-// HD: the head size, 0 for any.
-template <typename T, int HD>
-__global__ void __launch_bounds__(256)
-kv4_read_kernel(const unsigned char* __restrict__ pool, const int* __restrict__ pages, const int* __restrict__ page_start,
-                const int* __restrict__ seq_len, T* __restrict__ k_out, T* __restrict__ v_out, int* __restrict__ table, int B,
-                int width, int pool_pages, int Hkv, int any_hd, int marked, uint4* __restrict__ rows_out, const int* __restrict__ rows_used,
-                int rows, int row_bytes) {
-    pdl_wait();
-    pdl_launch_dependents();
-    const int hd = HD ? HD : any_hd;
+struct Kv4ReadArgs {
+    const unsigned char* pool;
+    const int *pages, *page_start, *seq_len, *rows_used;
+    int* table;
+    uint4* rows_out;
+    int B, width, pool_pages, Hkv, hd, marked, rows, row_bytes;
+};
+// The table and the rows; then what this block's page holds: its bytes of this head, and how many rows of it live.
+__device__ __forceinline__ const unsigned char* kv4_read_begin(const Kv4ReadArgs& a, int hd, int& live) {
     const int entry = blockIdx.x, head = blockIdx.y;
     const long long me = ((long long)head * gridDim.x + entry) * blockDim.x + threadIdx.x, all = (long long)gridDim.x * gridDim.y * blockDim.x;
-    for (long long i = me; i < (long long)B * width; i += all) {
-        const int b = (int)(i / width), j = (int)(i - (long long)b * width), at = page_start[b] + j;
-        table[i] = at >= 0 && at < page_start[b + 1] && at < (int)gridDim.x ? at : 0;
+    for (long long i = me; i < (long long)a.B * a.width; i += all) {
+        const int b = (int)(i / a.width), j = (int)(i - (long long)b * a.width), at = a.page_start[b] + j;
+        a.table[i] = at >= 0 && at < a.page_start[b + 1] && at < (int)gridDim.x ? at : 0;
     }
-    if (rows_out) {
-        const long long end = (long long)rows * (row_bytes / 16);
-        for (long long i = (long long)max(*rows_used, 0) * (row_bytes / 16) + me; i < end; i += all) rows_out[i] = make_uint4(0, 0, 0, 0);
+    if (a.rows_out) {
+        const long long end = (long long)a.rows * (a.row_bytes / 16);
+        for (long long i = (long long)max(*a.rows_used, 0) * (a.row_bytes / 16) + me; i < end; i += all) a.rows_out[i] = make_uint4(0, 0, 0, 0);
     }
     // the sequence that holds this entry: the last one that begins at or before it
-    int lo = 0, hi = B;
+    int lo = 0, hi = a.B;
     while (hi - lo > 1) {
         const int mid = (lo + hi) >> 1;
-        if (page_start[mid] <= entry) lo = mid; else hi = mid;
+        if (a.page_start[mid] <= entry) lo = mid; else hi = mid;
     }
-    const int j = entry - page_start[lo];
-    const long long page = pages[entry];
-    int live = entry < page_start[lo + 1] ? min(max(seq_len[lo] - j * KV4_PAGE, 0), KV4_PAGE) : 0;
-    if (j < 0 || page < 0 || page >= pool_pages) live = 0;
-    const int words = hd / 8, groups = hd / KV4_GROUP;
-    const unsigned char* base = pool + ((size_t)(live ? page : 0) * Hkv + head) * kv4_page_bytes(hd);
-    const size_t out0 = ((size_t)entry * Hkv + head) * KV4_PAGE * hd;
+    const int j = entry - a.page_start[lo];
+    const long long page = a.pages[entry];
+    live = entry < a.page_start[lo + 1] ? min(max(a.seq_len[lo] - j * KV4_PAGE, 0), KV4_PAGE) : 0;
+    if (j < 0 || page < 0 || page >= a.pool_pages) live = 0;
+    return a.pool + ((size_t)(live ? page : 0) * a.Hkv + head) * kv4_page_bytes(hd);
+}
+
+template <typename T>
+__global__ void __launch_bounds__(256)
+kv4_read_kernel(const Kv4ReadArgs a, T* __restrict__ k_out, T* __restrict__ v_out) {
+    pdl_wait();
+    pdl_launch_dependents();
+    int live;
+    const int hd = a.hd, words = hd / 8, groups = hd / KV4_GROUP;
+    const unsigned char* base = kv4_read_begin(a, hd, live);
+    const size_t out0 = ((size_t)blockIdx.x * a.Hkv + blockIdx.y) * KV4_PAGE * hd;
     const uint16_t* v_words = reinterpret_cast<const uint16_t*>(base + kv4_half_bytes(hd) + kv4_code_bytes(hd));
-#pragma unroll 8
     for (int i = threadIdx.x; i < 2 * KV4_PAGE * words; i += 256) {
         const bool is_v = i >= KV4_PAGE * words;
         const int at = is_v ? i - KV4_PAGE * words : i, row = at / words, w = at - row * words;
         const unsigned char* part = base + (is_v ? kv4_half_bytes(hd) : 0);
-        float y[8];
-        if (row < live) {
-            const uint32_t codes = reinterpret_cast<const uint32_t*>(part)[at];
-            const uint32_t word = reinterpret_cast<const uint16_t*>(part + kv4_code_bytes(hd))[row * groups + w / 4];
-            float s = kv4_step(word);
-            const float z = kv4_zero(word);
-            if (marked) {
-                bool bad = false;
-                for (int g = 0; g < groups; ++g) bad |= kv4_is_nan(v_words[row * groups + g]);
-                if (bad) s = is_v ? 0.f : __uint_as_float(0x7fc00000u);
-            }
-            if constexpr (sizeof(T) == 2) {                 // two codes at a time, all of it exact: c s - z s
-                const uint32_t step = (__float_as_uint(s) >> 16) * 0x10001u, less = kv4_off(step), zs = kv4_scaled(word * 0x10001u, step, less);
-                uint32_t p[4];
-#pragma unroll
-                for (int n = 0; n < 4; ++n) {
-                    const uint32_t v = kv4_scaled(codes >> (4 * n), step, less);
-                    __nv_bfloat162 d = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&v), *reinterpret_cast<const __nv_bfloat162*>(&zs));
-                    p[n] = *reinterpret_cast<uint32_t*>(&d);
-                }
-                *reinterpret_cast<uint4*>((is_v ? v_out : k_out) + out0 + (size_t)at * 8) =
-                    make_uint4(__byte_perm(p[0], p[1], 0x5410), __byte_perm(p[2], p[3], 0x5410), __byte_perm(p[0], p[1], 0x7632), __byte_perm(p[2], p[3], 0x7632));
-                continue;
-            }
-#pragma unroll
-            for (int n = 0; n < 8; ++n) y[n] = ((float)((codes >> (4 * n)) & 15u) - z) * s;
-        } else {
-#pragma unroll
-            for (int n = 0; n < 8; ++n) y[n] = 0.f;
-        }
         T* dst = (is_v ? v_out : k_out) + out0 + (size_t)at * 8;
-        if constexpr (sizeof(T) == 4) {
-            reinterpret_cast<float4*>(dst)[0] = make_float4(y[0], y[1], y[2], y[3]);
-            reinterpret_cast<float4*>(dst)[1] = make_float4(y[4], y[5], y[6], y[7]);
-        } else {
-            __nv_bfloat162 p[4];
+        uint32_t codes = 0, word = 0;
+        float s = 0.f;
+        if (row < live) {
+            codes = reinterpret_cast<const uint32_t*>(part)[at];
+            word = reinterpret_cast<const uint16_t*>(part + kv4_code_bytes(hd))[row * groups + w / 4];
+            s = kv4_step(word);
+            bool bad = false;
+            for (int g = 0; a.marked && g < groups; ++g) bad |= kv4_is_nan(v_words[row * groups + g]);
+            if (bad) s = is_v ? 0.f : __uint_as_float(0x7fffffffu);
+        }
+        const float z = kv4_zero(word);
 #pragma unroll
-            for (int n = 0; n < 4; ++n) p[n] = __floats2bfloat162_rn(y[2 * n], y[2 * n + 1]);
-            *reinterpret_cast<uint4*>(dst) = *reinterpret_cast<uint4*>(p);
+        for (int n = 0; n < 8; ++n) dst[n] = from_f32<T>(((float)((codes >> (4 * n)) & 15u) - z) * s);
+    }
+}
+
+// bfloat16, heads of 64 and 128: a thread takes the same 8 numbers of every 16th (32nd) row, all its loads on their way before the first
+// is used, and two codes at a time, all of it exact: c s - z s.  What bounds it: 32 KB written a page and head of 128 for 9 KB read; 7,500 of them
+// 54 us, 5.8 TB/s (one word and its address at a time 82).
+template <int HD>
+__global__ void __launch_bounds__(256)
+kv4_read_fast_kernel(const Kv4ReadArgs a, bf16* __restrict__ k_out, bf16* __restrict__ v_out) {
+    pdl_wait();
+    pdl_launch_dependents();
+    constexpr int WORDS = HD / 8, ROWS = 256 / WORDS, PASSES = KV4_PAGE / ROWS, HALF = kv4_half_bytes(HD), CODES = kv4_code_bytes(HD);
+    int live;
+    const unsigned char* base = kv4_read_begin(a, HD, live);
+    const int tid = threadIdx.x, w = tid % WORDS, r0 = tid / WORDS, g = w / 4;
+    const unsigned twice = (2 * g) | (2 * g + 1) << 4 | (2 * g) << 8 | (2 * g + 1) << 12;          // selects the group's word twice
+    uint32_t codes[2][PASSES];
+    uint2 words[2][PASSES];
+#pragma unroll
+    for (int p = 0; p < 2; ++p)
+#pragma unroll
+        for (int i = 0; i < PASSES; ++i) {
+            const int row = r0 + i * ROWS;
+            codes[p][i] = 0;
+            words[p][i] = make_uint2(0, 0);
+            if (row < live) {
+                codes[p][i] = reinterpret_cast<const uint32_t*>(base + p * HALF)[i * 256 + tid];
+                if (HD == 128) words[p][i] = reinterpret_cast<const uint2*>(base + p * HALF + CODES)[row];
+                else words[p][i].x = reinterpret_cast<const uint32_t*>(base + p * HALF + CODES)[row];
+            }
+        }
+    const size_t out0 = ((size_t)blockIdx.x * a.Hkv + blockIdx.y) * KV4_PAGE * HD;
+#pragma unroll
+    for (int i = 0; i < PASSES; ++i) {
+        const uint2 v = words[1][i];
+        const bool bad = a.marked && (__vcmpeq2(v.x & 0x7f807f80u, 0x7f807f80u) | __vcmpeq2(v.y & 0x7f807f80u, 0x7f807f80u));
+#pragma unroll
+        for (int p = 0; p < 2; ++p) {
+            const uint32_t word = __byte_perm(words[p][i].x, words[p][i].y, twice);
+            uint32_t step = word & 0xfff0fff0u;
+            if (bad) step = p ? 0u : 0x7fc07fc0u;
+            const uint32_t off = kv4_off(step), zs = kv4_scaled(word, step, off);
+            uint32_t x[4];
+#pragma unroll
+            for (int n = 0; n < 4; ++n) {
+                const uint32_t cs = kv4_scaled(codes[p][i] >> (4 * n), step, off);
+                const __nv_bfloat162 d = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&cs), *reinterpret_cast<const __nv_bfloat162*>(&zs));
+                x[n] = *reinterpret_cast<const uint32_t*>(&d);
+            }
+            *reinterpret_cast<uint4*>((p ? v_out : k_out) + out0 + (size_t)(i * 256 + tid) * 8) =
+                make_uint4(__byte_perm(x[0], x[1], 0x5410), __byte_perm(x[2], x[3], 0x5410), __byte_perm(x[0], x[1], 0x7632), __byte_perm(x[2], x[3], 0x7632));
         }
     }
 }
@@ -468,13 +501,12 @@ extern "C" int qwb_kv4_read(const unsigned char* pool, const int* pages, const i
         return qwb_fail(QWB_ERR_ARG, "kv4_read: pool and outputs must start at a multiple of 16 bytes");
     if (rows_out && ((uintptr_t)rows_out % 16 || row_bytes % 16 || !rows_used))
         return qwb_fail(QWB_ERR_ARG, "kv4_read: rows of %d bytes", row_bytes);
-    if (dtype != QWB_DT_F32 && dtype != QWB_DT_BF16) return qwb_fail(QWB_ERR_ARG, "kv4_read: unknown dtype %d", dtype);
-#define KV4_READ(T, HD) qwb_launch(kv4_read_kernel<T, HD>, dim3(P, Hkv), 256, 0, stream, pool, pages, page_start, seq_len, (T*)k_out, (T*)v_out, table, B, width, \
-                                   pool_pages, Hkv, hd, marked, (uint4*)rows_out, rows_used, rows, row_bytes)
-    if (dtype == QWB_DT_F32) KV4_READ(float, 0);
-    else if (hd == 128) KV4_READ(bf16, 128);
-    else if (hd == 64) KV4_READ(bf16, 64);
-    else KV4_READ(bf16, 0);
-#undef KV4_READ
+    const Kv4ReadArgs args = {pool, pages, page_start, seq_len, rows_used, table, (uint4*)rows_out, B, width, pool_pages, Hkv, hd, marked, rows, row_bytes};
+    const dim3 grid(P, Hkv);
+    if (dtype == QWB_DT_F32) qwb_launch(kv4_read_kernel<float>, grid, 256, 0, stream, args, (float*)k_out, (float*)v_out);
+    else if (dtype != QWB_DT_BF16) return qwb_fail(QWB_ERR_ARG, "kv4_read: unknown dtype %d", dtype);
+    else if (hd == 128) qwb_launch(kv4_read_fast_kernel<128>, grid, 256, 0, stream, args, (bf16*)k_out, (bf16*)v_out);
+    else if (hd == 64) qwb_launch(kv4_read_fast_kernel<64>, grid, 256, 0, stream, args, (bf16*)k_out, (bf16*)v_out);
+    else qwb_launch(kv4_read_kernel<bf16>, grid, 256, 0, stream, args, (bf16*)k_out, (bf16*)v_out);
     return qwb_check_launch("kv4_read");
 }
