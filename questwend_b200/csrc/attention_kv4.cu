@@ -653,7 +653,7 @@ static bool kv4_read_is_faster(int max_len, int max_new, int window, int table_w
     if (mean_len > max_len) mean_len = max_len;
     const Kv4Runs cut = kv4_runs(mean_len > max_new ? (int)(mean_len - max_new) : 0, (int)mean_len, window, table_width);
     const double columns = (double)tokens * G / 16.0 + 0.5 * B;
-    const double rows = 5.0 + columns * Hkv * cut.runs * (cut.per_run + 3.5) / (hd == 128 ? 340.0 : 580.0);
+    const double rows = 5.0 + columns * Hkv * cut.runs * (cut.per_run + 3.5) / (hd == 128 ? 400.0 : 580.0);
     return 4.0 + at_pieces(tokens, B, max_new, max_len, Hq, Hkv, hd, window).us + (double)listed * Hkv * (hd == 128 ? 0.0065 : 0.0045) < rows;
 }
 
