@@ -223,10 +223,12 @@ kv4_attn_rows_kernel(const bf16* __restrict__ q, const unsigned char* __restrict
     const int Hq = Hkv * G;
     const float one_in_g = 1.f / (float)G;
     auto by_g = [&](int x) { return (int)(((float)x + 0.5f) * one_in_g); };             // x / G: exact for x below 2^20 (the launcher's bound)
-    if (blockIdx.x == 0 && kvh == 0 && b == 0) {            // tokens behind the last sequence's: zeros
-        for (long long i = (long long)max(cu_seqlens[B], 0) * Hq * HD + threadIdx.x; i < (long long)T * Hq * HD; i += KD_WARPS * 32) out[i] = from_f32<bf16>(0.f);
+    const int t0 = cu_seqlens[b], t1 = cu_seqlens[b + 1], p0 = pos0[b], used = max(cu_seqlens[B], 0);
+    if (used < T) {                                         // tokens behind the last sequence's: zeros
+        const long long me = (((long long)b * gridDim.y + kvh) * gridDim.x + blockIdx.x) * (KD_WARPS * 32) + threadIdx.x;
+        const long long all = (long long)gridDim.x * gridDim.y * gridDim.z * (KD_WARPS * 32), end = (long long)T * Hq * (HD / 8);
+        for (long long i = (long long)used * Hq * (HD / 8) + me; i < end; i += all) reinterpret_cast<uint4*>(out)[i] = make_uint4(0, 0, 0, 0);
     }
-    const int t0 = cu_seqlens[b], t1 = cu_seqlens[b + 1], p0 = pos0[b];
     const int n_new = min(t1, T) - t0, col0 = tile * 8 * NT, cols = n_new * G;
     if (t0 < 0 || n_new <= 0 || col0 >= cols) return;
     const int len = p0 + n_new;

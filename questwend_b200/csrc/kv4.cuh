@@ -4,8 +4,9 @@
 // lo = min(x, 0) and hi = max(x, 0) over a group its step is s = (hi - lo) / 15, rounded to 4 significant bits, its zero
 // point z = rint(-lo / s) in 0..15, a number's code c = rint(x / s) + z, kept in 0..15, and the number that it stands for
 // (c - z) s.  c - z has 4 bits and s has 4, so that number is exact in bfloat16 and in 32 bits: whoever reads the cache, in
-// whatever type and order, reads the same numbers.  (A step with the 8 bits of a bfloat16 would be off by 0.2 % instead of
-// 2 % on average; the codes' own rounding is 14 times larger than either, and z would have needed bytes of its own.)
+// whatever type and order, reads the same numbers.  (Rounding the step
+// makes it 2 % larger or smaller on average, and the codes' own rounding, half a step at most, with it; the largest numbers may then lie up to
+// 15/16 of a step beyond the last code instead of half a step.)
 // A group of zeros, or whose step would lie under 2^-126, has step 0 and stands for zeros.  A group that holds a number that
 // is not finite, or whose step would be 2^120 or more (so that 128 s is a number), stands for NaN: what sees the token is NaN and nothing
 // is lost silently.

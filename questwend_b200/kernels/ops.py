@@ -2255,7 +2255,7 @@ def kv4_attention(q: torch.Tensor, pool: torch.Tensor, tables: StepTables, max_n
     _here("kv4_attention", q, pool, table, tok_seq, tok_pos, cu, pos0)
     group = Hq // Hkv
     fits = q.dtype == torch.bfloat16 and hd in (64, 128)
-    reads = fits and group <= 64 and tables.pages is not None and tables.page_start is not None
+    reads = fits and group <= 64 and tables.pages is not None and tables.page_start is not None and tables.pages.numel() > 0
     plan = 0
     if fits and impl != "plain":
         plan = _lookup("attention_kv4", "qwb_kv4_plan")[1](max_len, max_new, window, table.shape[1], B, Hq, Hkv, hd, T,
