@@ -20,10 +20,10 @@
 #define LP_PER_THREAD 64
 #define LP_SEG (LP_THREADS * LP_PER_THREAD)
 #define LP_MAX_TOP 64
-#define LP_LINK_ROWS 16         // up to so many rows the joining kernel starts under the tail of the one before it
-#define LP_HELD 8              // maxima of a thread of the joining kernel that it keeps in registers: 131,072 logits' worth
+#define LP_JOIN_THREADS 128      // of a row's end: all of 2,048 rows' ends are on the chip at once
+#define LP_HELD 8               // maxima of a thread of the joining kernel that it keeps in registers: 65,536 logits' worth
 #define LP_CLUSTER 16           // segments of a row that can be a cluster: 262,144 logits
-#define LP_GATHER 1024          // candidates of a row that shared memory holds
+#define LP_GATHER 512           // candidates of a row that shared memory holds
 
 // Larger logits first, of equal ones the lower id (id < 0: nothing).
 __device__ __forceinline__ bool lp_before(float a, int ia, float b, int ib) { return ib < 0 ? ia >= 0 : (ia >= 0 && (a > b || (a == b && ia < ib))); }
@@ -66,13 +66,14 @@ __device__ __forceinline__ void lp_raise(float& S, float& U, float from, float t
 // again and what is at or above the bar gathered in shared memory; each one's rank is how many stand before it.  Where more are there
 // than fit (equal logits, orders that put the largest into few threads) the list is found one by one.
 //   held: the thread's maxima of the first segments; more: those of all segments, for the ones behind (null: there are none)
-template <bool VEC, int HELD>
+template <bool VEC, int HELD, int THREADS>
 __device__ __forceinline__ void lp_finish(const float* x, int token, float m, float S, float U, const float (&held)[HELD], const float* more, float* logprob,
                                           float* entropy, int* top_ids, float* top_lps, int V, int segs, int top) {
-    constexpr int WARPS = LP_THREADS / 32;
+    constexpr int WARPS = THREADS / 32;
     __shared__ float warp_t[WARPS], found_v[LP_GATHER];
     __shared__ int found_i[LP_GATHER], holders[LP_GATHER], picked[LP_GATHER], n_found, n_holders, n_picked;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int shares = segs * (LP_THREADS / THREADS);           // maxima of a thread
     const float lnS = logf(S);
     if (tid == 0) {
         *logprob = (token >= 0 && token < V) ? (x[token] - m) - lnS : __uint_as_float(0x7fffffffu);
@@ -83,7 +84,7 @@ __device__ __forceinline__ void lp_finish(const float* x, int token, float m, fl
     float largest = -INFINITY;
 #pragma unroll
     for (int j = 0; j < HELD; ++j) largest = fmaxf(largest, held[j]);
-    for (int j = HELD; j < segs; ++j) largest = fmaxf(largest, __ldcg(more + j * LP_THREADS + tid));
+    for (int j = HELD; j < shares; ++j) largest = fmaxf(largest, __ldcg(more + j * THREADS + tid));
     int left = lp_key(largest), kth = __reduce_max_sync(0xffffffffu, left);
     for (int k = 1; k < (top + WARPS - 1) / WARPS; ++k) {                               // take the warp's largest out, look again
         const unsigned at = __ballot_sync(0xffffffffu, left == kth);
@@ -105,16 +106,16 @@ __device__ __forceinline__ void lp_finish(const float* x, int token, float m, fl
         };
 #pragma unroll
         for (int j = 0; j < HELD; ++j)
-            if (j < segs && held[j] >= bar) hold(j * LP_THREADS + tid, held[j]);
-        for (int j = HELD; j < segs; ++j) {
-            const float y = __ldcg(more + j * LP_THREADS + tid);
-            if (y >= bar) hold(j * LP_THREADS + tid, y);
+            if (j < shares && held[j] >= bar) hold(j * THREADS + tid, held[j]);
+        for (int j = HELD; j < shares; ++j) {
+            const float y = __ldcg(more + j * THREADS + tid);
+            if (y >= bar) hold(j * THREADS + tid, y);
         }
     }
     __syncthreads();
     // the top-th largest of the maxima found is a higher bar, with about half as many at or above it
     const int n_held = min(n_holders, LP_GATHER);
-    for (int i = tid; i < n_held; i += LP_THREADS) {
+    for (int i = tid; i < n_held; i += THREADS) {
         const float a = found_v[i];
         int above = 0, same = 0;
         for (int j = 0; j < n_held; ++j) {
@@ -125,13 +126,13 @@ __device__ __forceinline__ void lp_finish(const float* x, int token, float m, fl
     }
     __syncthreads();
     if (n_holders <= LP_GATHER) bar = warp_t[0];
-    for (int i = tid; i < n_held; i += LP_THREADS)
+    for (int i = tid; i < n_held; i += THREADS)
         if (found_v[i] >= bar) picked[atomicAdd(&n_picked, 1)] = holders[i];
     __syncthreads();
     // 64 logits of each, all threads side by side
     const int looks = n_picked * LP_PER_THREAD;
 #pragma unroll 4
-    for (int j = tid; j < looks; j += LP_THREADS) {
+    for (int j = tid; j < looks; j += THREADS) {
         const int who = picked[j / LP_PER_THREAD], i = who / LP_THREADS * LP_SEG + lp_index<VEC>(j % LP_PER_THREAD, who % LP_THREADS);
         const float y = i < V ? x[i] : -INFINITY;
         if (y >= bar && i < V) {
@@ -149,14 +150,14 @@ __device__ __forceinline__ void lp_finish(const float* x, int token, float m, fl
         top_lps[rank] = ia < 0 ? __uint_as_float(0x7fffffffu) : (a - m) - lnS;
     };
     if (n <= LP_GATHER && n_holders <= LP_GATHER) {
-        for (int i = tid; i < n; i += LP_THREADS) {
+        for (int i = tid; i < n; i += THREADS) {
             const float a = found_v[i];
             const int ia = found_i[i];
             int rank = 0;
             for (int j = 0; j < n; ++j) rank += lp_before(found_v[j], found_i[j], a, ia);
             if (rank < top) leave(rank, a, ia);
         }
-        for (int i = n + tid; i < top; i += LP_THREADS) leave(i, -INFINITY, -1);
+        for (int i = n + tid; i < top; i += THREADS) leave(i, -INFINITY, -1);
         return;
     }
     // one after the other: everyone's largest that is behind the last one found
@@ -165,7 +166,7 @@ __device__ __forceinline__ void lp_finish(const float* x, int token, float m, fl
     for (int k = 0; k < top; ++k) {
         float bv = -INFINITY;
         int bi = -1;
-        for (int i = tid; i < V; i += LP_THREADS) {
+        for (int i = tid; i < V; i += THREADS) {
             const float y = x[i];
             const bool open = y == y && (last_i < 0 || lp_before(last, last_i, y, i));
             if (open && lp_before(y, i, bv, bi)) { bv = y; bi = i; }
@@ -298,14 +299,17 @@ lp_segments_kernel(const float* __restrict__ logits, float* __restrict__ sums, f
         if (lane < segs) lp_raise(Ss, Us, m, all);
         S = warp_sum(Ss);
         U = warp_sum(Us);
-        lp_finish<VEC, LP_CLUSTER>(logits + row * V, tokens[row], all, S, U, held, nullptr, logprob + row, entropy + row, top_ids + row * top, top_lps + row * top, V,
-                                   segs, top);
+        lp_finish<VEC, LP_CLUSTER, LP_THREADS>(logits + row * V, tokens[row], all, S, U, held, nullptr, logprob + row, entropy + row, top_ids + row * top,
+                                               top_lps + row * top, V, segs, top);
     }
 }
 
-// A block a row: the segments' sums, then the row's end.
+// A block a row: the segments' sums, then the row's end.  Its reads wait for one another, so it wants all rows' blocks on the chip at once
+// and the first of them there before the segments' last: 2,048 rows of 151,936 logits with a top of 5 / 20 / 64 take 204 / 215 / 252 us with
+// blocks of 256 threads and 1,024 candidates, 211 / 228 / 282 with half the threads, 201 / 211 / 247 with half the candidates too (16 blocks
+// an SM), 213 / 232 / - with 64 threads.
 template <bool VEC>
-__global__ void __launch_bounds__(LP_THREADS, 8)
+__global__ void __launch_bounds__(LP_JOIN_THREADS, 2048 / LP_JOIN_THREADS)
 lp_join_kernel(const float* __restrict__ logits, const int* __restrict__ tokens, const float* sums, const float* maxima,
                float* __restrict__ logprob, float* __restrict__ entropy, int* __restrict__ top_ids, float* __restrict__ top_lps, int V, int segs,
                int top) {
@@ -317,7 +321,8 @@ lp_join_kernel(const float* __restrict__ logits, const int* __restrict__ tokens,
     const float* at_most = maxima + row * segs * LP_THREADS;
     float held[LP_HELD];                    // this thread's share of the maxima, the first of them in registers
 #pragma unroll
-    for (int j = 0; j < LP_HELD; ++j) held[j] = top && j < segs ? __ldcg(at_most + j * LP_THREADS + tid) : -INFINITY;
+    for (int j = 0; j < LP_HELD; ++j)
+        held[j] = top && j < segs * (LP_THREADS / LP_JOIN_THREADS) ? __ldcg(at_most + j * LP_JOIN_THREADS + tid) : -INFINITY;
     // every warp has the sums: the same additions in the same order
     float m = LP_LOWEST;
     for (int s = lane; s < segs; s += 32) m = fmaxf(m, __ldcg(mine + s * 3));
@@ -331,8 +336,8 @@ lp_join_kernel(const float* __restrict__ logits, const int* __restrict__ tokens,
     }
     S = warp_sum(S);
     U = warp_sum(U);
-    lp_finish<VEC, LP_HELD>(logits + row * V, tokens[row], m, S, U, held, at_most, logprob + row, entropy + row, top_ids + row * top, top_lps + row * top, V,
-                            segs, top);
+    lp_finish<VEC, LP_HELD, LP_JOIN_THREADS>(logits + row * V, tokens[row], m, S, U, held, at_most, logprob + row, entropy + row, top_ids + row * top,
+                                             top_lps + row * top, V, segs, top);
 }
 
 
@@ -385,7 +390,7 @@ extern "C" int qwb_logprobs(const float* logits, const int* tokens, float* logpr
     float* maxima = top ? scratch + (size_t)rows * segs * 3 : nullptr;
     qwb_launch(vec ? lp_segments_kernel<true, false> : lp_segments_kernel<false, false>, dim3(segs, rows), LP_THREADS, 0, stream, logits, scratch, maxima, tokens,
                logprob, entropy, top_ids, top_lps, V, segs, top);
-    qwb_launch_link(rows, LP_LINK_ROWS, vec ? lp_join_kernel<true> : lp_join_kernel<false>, dim3(rows), LP_THREADS, 0, stream, logits, tokens, scratch, maxima,
+    qwb_launch_link(1, 1, vec ? lp_join_kernel<true> : lp_join_kernel<false>, dim3(rows), LP_JOIN_THREADS, 0, stream, logits, tokens, scratch, maxima,
                     logprob, entropy, top_ids, top_lps, V, segs, top);
     return qwb_check_launch("token_logprobs");
 }
