@@ -201,7 +201,7 @@ __device__ __forceinline__ void kd_cluster_sync() {
 // of the runs of sequences that have more than one; a row is (token, query head).
 // ROOM: blocks an SM that registers leave room for.  With 8 columns 7, as many as shared memory does: 32 x 16,384 tokens 113 us, 116 with 8, 120 with 6.  With
 // 16 columns 5 (168 registers, some of them spilled), and 4 where no more are launched than so fit at once: 4 new tokens of one sequence of 8,192
-// 15.3 us instead of 17.7, of four sequences, 1,000 blocks, 33.4 instead of 30.1.
+// 15.6 us instead of 17.7, of four sequences, 1,000 blocks, 33.4 instead of 30.1.
 template <int HD, int NT, bool CLUSTER, int ROOM>
 __global__ void __launch_bounds__(KD_WARPS * 32, ROOM)
 kv4_attn_rows_kernel(const bf16* __restrict__ q, const unsigned char* __restrict__ pool, const int* __restrict__ page_table,

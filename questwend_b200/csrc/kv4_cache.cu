@@ -110,30 +110,36 @@ kv4_store_kernel(const float* __restrict__ qkv, const float* __restrict__ q_weig
 // holds the numbers 4L..4L+3 and HD/2 + 4L..: a number and its rotation partner lie in one lane, and each of its two fours in the group of
 // 8 neighbouring lanes, so that norm and group cost three or four exchanges.  What bounds it is memory: 4 bytes read and (queries) 2 or (keys
 // and values) 9/16 written a number.  So the choices are made in 32 bits where these leave no doubt: a number whose quotient by the step lies
-// nearer to the border of two codes than its error can be, or a step nearer to the border of two roundings (about one head in 700), sends
+// nearer to the border of two codes than its error can be, or a step nearer to the border of two roundings (about one head in 220), sends
 // its head through 64 bits.  A step of 4,096 tokens of 32 + 2 x 8 heads: a warp a head 130 us, with 64 bits for
-// every key 45, so 34 (4.2 TB/s; what is left is arithmetic and the chain of a head's exchanges, at 8 blocks an SM).
+// every key 45, so 34 with the next head on its way in registers and 29 (4.8 TB/s) with two by cp.async; what is left is latency and 3.5 waves
+// of blocks: 16,384 tokens run at 5.7 TB/s.  (Fewer instructions for codes and errors, 16 % of them, changed nothing before that.)
 //
 // Errors of a key in 32 bits, u = 2^-24: the sum of squares 8 + 4 additions, the mean and eps 1, halved by the root; the inverse root
 // 4 (2 units of 2^-23): 11 u; times the weight and the number 2 u; the rotation's products and sum 2 u: of p c - r s it is 15 u (|p c| + |r s|)
-// < 2^-20 (|p c| + |r s|).
+// < 2^-20 (|p| + |r|) times the largest of |c|, |s| and 1; the largest of that in the 8 lanes is taken for both of their groups.
 struct Kv4Choice { uint32_t codes, word; bool sure; };
 
-// Four numbers of a lane in a group of 8 lanes' 32, each off by at most `off` of its lane: codes (the first in the lowest bits) and the
+__device__ __forceinline__ float kv4_max_nan(float a, float b) {
+    float y;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(a), "f"(b));
+    return y;
+}
+
+// Four numbers of a lane in a group of 8 lanes' 32, each off by at most `off` (the same for the group): codes (the first in the lowest bits) and the
 // group's word.  A number plus 3 x 2^22 is rounded to a whole one by the addition, and whole ones add up to the packed codes as floats: roundings
-// and conversions as such have a fraction of the rate.
+// and conversions as such have a fraction of the rate.  Codes are kept in range as sixteenths, whose lower end is an instruction's own.
 __device__ __forceinline__ Kv4Choice kv4_four(const float (&x)[4], float off, unsigned mask) {
-    float lo = 0.f, hi = 0.f;
+    float lo = 0.f, hi = 0.f;                                       // hi: a NaN stays one, and t below with it
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
         lo = fminf(lo, x[i]);
-        hi = fmaxf(hi, fabsf(x[i]) <= 3.4028234663852886e38f ? x[i] : INFINITY);
+        hi = kv4_max_nan(hi, x[i]);
     }
 #pragma unroll
     for (int o = 1; o < 8; o <<= 1) {
         lo = fminf(lo, __shfl_xor_sync(mask, lo, o));
-        hi = fmaxf(hi, __shfl_xor_sync(mask, hi, o));
-        off = fmaxf(off, __shfl_xor_sync(mask, off, o));
+        hi = kv4_max_nan(hi, __shfl_xor_sync(mask, hi, o));
     }
     Kv4Choice y;
     y.codes = y.word = 0;
@@ -146,12 +152,13 @@ __device__ __forceinline__ Kv4Choice kv4_four(const float (&x)[4], float off, un
     float inv;
     asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inv) : "f"(s));
     const float z0 = fmaf(-lo, inv, whole) - whole, z = fminf(z0, 15.f);
+    const float from = fmaf(z, 0.0625f, -0.0625f * whole);          // (z - whole) / 16, exact
     float far = fabsf(fmaf(-z0, s, -lo)), packed = 0.f;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-        const float c = fmaf(x[i], inv, whole) - whole;
+        const float v = fmaf(x[i], inv, whole), c = v - whole;
         far = fmaxf(far, fabsf(fmaf(-c, s, x[i])));
-        packed = fmaf(fminf(fmaxf(c + z, 0.f), 15.f), (float)(1 << (4 * i)), packed);
+        packed = fmaf(fminf(__saturatef(fmaf(v, 0.0625f, from)), 0.9375f), (float)(16 << (4 * i)), packed);
     }
     y.sure = t > 1e-36f && t < 1e36f && (float)(border - 3) * (t * 5.9604644775390625e-8f) > 0.14f * off && far + off < 0.499996f * s;
     y.codes = __float_as_uint(packed + 8388608.f) & 0xffffu;
@@ -212,6 +219,10 @@ template <> __device__ __forceinline__ void kv4_put4<bf16>(bf16* p, float a, flo
     *reinterpret_cast<uint2*>(p) = *reinterpret_cast<uint2*>(v);
 }
 
+__device__ __forceinline__ void kv4_copy16(void* dst, const void* src) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"((uint32_t)__cvta_generic_to_shared(dst)), "l"(src) : "memory");
+}
+#define KF_STAGES 3                 // heads in a warp's ring, two of them on their way: 4,096 tokens 29 us; one on its way 32, three 30, five 34
 #define KF_BLOCKS 1184              // as many are wanted of a call
 template <typename TQ, int HD>
 __global__ void __launch_bounds__(KS_WARPS * 32, 8)
@@ -225,28 +236,37 @@ kv4_store_fast_kernel(const float* __restrict__ qkv, const float* __restrict__ q
     const unsigned mask = HD == 128 ? 0xffffu << (16 * of) : 0xffu << (8 * of);
     const int n_all = Hq + 2 * Hkv, n_heads = store_kv ? n_all : Hq;
     const float4* row = reinterpret_cast<const float4*>(qkv + (size_t)t * n_all * HD);
-    float c[4] = {1.f, 1.f, 1.f, 1.f}, sn[4] = {};
+    // a lane's numbers of the next heads are on their way into its own places
+    __shared__ float4 ring[KS_WARPS][KF_STAGES][2][32];
+    const int step = gridDim.y * KS_WARPS * HEADS;
+    int head = (blockIdx.y * KS_WARPS + warp) * HEADS + of, slot_in = 0, slot_out = 0;
+    auto ask = [&](int h) {
+        if (h < n_heads) {
+            kv4_copy16(&ring[warp][slot_in][0][lane], row + (size_t)h * (HD / 4) + L);
+            kv4_copy16(&ring[warp][slot_in][1][lane], row + (size_t)h * (HD / 4) + HD / 8 + L);
+        }
+        asm volatile("cp.async.commit_group;" ::: "memory");
+        slot_in = slot_in == KF_STAGES - 1 ? 0 : slot_in + 1;
+    };
+#pragma unroll
+    for (int i = 0; i < KF_STAGES - 1; ++i) ask(head + i * step);
+    float c[4] = {1.f, 1.f, 1.f, 1.f}, sn[4] = {}, turn = 1.f;
     if (cos_t) {
         *reinterpret_cast<float4*>(c) = reinterpret_cast<const float4*>(cos_t + (size_t)t * (HD / 2))[L];
         *reinterpret_cast<float4*>(sn) = reinterpret_cast<const float4*>(sin_t + (size_t)t * (HD / 2))[L];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) turn = fmaxf(turn, fmaxf(fabsf(c[i]), fabsf(sn[i])));
     }
-    const long long slot = slot_map[t];
+    const int slot = slot_map[t], at = slot % KV4_PAGE;
     const bool has_place = slot >= 0 && slot < n_rows;
-    const int step = gridDim.y * KS_WARPS * HEADS;
-    int head = (blockIdx.y * KS_WARPS + warp) * HEADS + of;
-    float4 next_a = make_float4(0.f, 0.f, 0.f, 0.f), next_b = next_a;
-    if (head < n_heads) {
-        next_a = row[(size_t)head * (HD / 4) + L];
-        next_b = row[(size_t)head * (HD / 4) + HD / 8 + L];
-    }
+    unsigned char* page = pool + (has_place ? (size_t)(slot / KV4_PAGE) * Hkv * kv4_page_bytes(HD) : 0);
     for (; head < n_heads; head += step) {
+        ask(head + (KF_STAGES - 1) * step);
+        asm volatile("cp.async.wait_group %0;" ::"n"(KF_STAGES - 1) : "memory");
         float a[4], b[4];
-        *reinterpret_cast<float4*>(a) = next_a;
-        *reinterpret_cast<float4*>(b) = next_b;
-        if (head + step < n_heads) {                                // the next head's numbers are on their way meanwhile
-            next_a = row[(size_t)(head + step) * (HD / 4) + L];
-            next_b = row[(size_t)(head + step) * (HD / 4) + HD / 8 + L];
-        }
+        *reinterpret_cast<float4*>(a) = ring[warp][slot_out][0][lane];
+        *reinterpret_cast<float4*>(b) = ring[warp][slot_out][1][lane];
+        slot_out = slot_out == KF_STAGES - 1 ? 0 : slot_out + 1;
         if (head < Hq) {
             if (q_weight) {
                 float ss = 0.f, w[4];
@@ -275,10 +295,10 @@ kv4_store_fast_kernel(const float* __restrict__ qkv, const float* __restrict__ q
         }
         if (!has_place) continue;
         const bool is_k = head < Hq + Hkv;
-        const int kvh = head - Hq - (is_k ? 0 : Hkv), at = (int)(slot % KV4_PAGE);
-        unsigned char* base = pool + ((size_t)(slot / KV4_PAGE) * Hkv + kvh) * kv4_page_bytes(HD) + (is_k ? 0 : kv4_half_bytes(HD));
+        const int kvh = head - Hq - (is_k ? 0 : Hkv);
+        unsigned char* base = page + (size_t)kvh * kv4_page_bytes(HD) + (is_k ? 0 : kv4_half_bytes(HD));
         const bool turned = is_k && (k_weight || cos_t);
-        float w[4] = {1.f, 1.f, 1.f, 1.f}, u[4] = {1.f, 1.f, 1.f, 1.f}, x[4], y[4], e = 0.f, f = 0.f;
+        float w[4] = {1.f, 1.f, 1.f, 1.f}, u[4] = {1.f, 1.f, 1.f, 1.f}, x[4], y[4], off = 0.f;
         bool in_range = true;
         if (turned) {
             float scale = 1.f;
@@ -297,12 +317,13 @@ kv4_store_fast_kernel(const float* __restrict__ qkv, const float* __restrict__ q
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 const float p = a[i] * (scale * w[i]), r = b[i] * (scale * u[i]);
-                const float pc = p * c[i], rs = r * sn[i], ps = p * sn[i], rc = r * c[i];
-                x[i] = pc - rs;
-                y[i] = ps + rc;
-                e = fmaxf(e, (fabsf(pc) + fabsf(rs)) * 9.5367431640625e-7f);
-                f = fmaxf(f, (fabsf(ps) + fabsf(rc)) * 9.5367431640625e-7f);
+                x[i] = p * c[i] - r * sn[i];
+                y[i] = p * sn[i] + r * c[i];
+                off = fmaxf(off, fabsf(p) + fabsf(r));
             }
+            off *= turn * 9.5367431640625e-7f;
+#pragma unroll
+            for (int o = 1; o < 8; o <<= 1) off = fmaxf(off, __shfl_xor_sync(mask, off, o));
         } else {
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
@@ -310,7 +331,7 @@ kv4_store_fast_kernel(const float* __restrict__ qkv, const float* __restrict__ q
                 y[i] = b[i];
             }
         }
-        Kv4Choice lo = kv4_four(x, e, mask), hi = kv4_four(y, f, mask);
+        Kv4Choice lo = kv4_four(x, off, mask), hi = kv4_four(y, off, mask);
         if (__any_sync(mask, !(in_range && lo.sure && hi.sure))) {
             const uint4 g = kv4_head_exactly<HD>(reinterpret_cast<const float*>(row) + (size_t)head * HD, turned ? k_weight : nullptr,
                                                  turned && cos_t ? cos_t + (size_t)t * (HD / 2) : nullptr, turned && cos_t ? sin_t + (size_t)t * (HD / 2) : nullptr,
