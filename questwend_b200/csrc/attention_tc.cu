@@ -9,9 +9,12 @@
 //     S = Q K^T      tcgen05.mma, Q and K from shared memory (TMA, 128-byte swizzle), S in tensor memory (64 columns, two
 //                    buffers: the tensor core is up to two tiles ahead of the softmax)
 //     P = softmax    four warps, one thread per row: read S, mask, running maximum and sum in 32-bit, write P as
-//                    bfloat16 into shared memory in the layout the tensor core reads
-//     O += P V       tcgen05.mma, P and V from shared memory, O accumulates in tensor memory (VD columns).  V is read as
-//                    it lies in the cache ([key][d], d contiguous): the "MN-major" operand form.
+//                    bfloat16 back into tensor memory, over the scores it came from
+//     O += P V       tcgen05.mma, P from tensor memory, V from shared memory, O accumulates in tensor memory (VD columns).
+//                    V is read as it lies in the cache ([key][d], d contiguous): the "MN-major" operand form.
+// With P in shared memory its way in and out took a quarter of what an SM's shared memory moves a tile (with heads of 128 about 1,000
+// cycles, as long as the tile took): one prompt of 4,096 tokens, 32 heads of 128, 137 us with P in tensor memory instead of 147.  (Registers for
+// two blocks an SM, without spills: 147 instead of 159.)
 // O lives in tensor memory across the tiles.  It carries a reference maximum per row; when a tile raises a row's
 // maximum by more than 2^8 the row's O and sum are rescaled (read, scale, write back), else the old reference stays
 // and the probabilities are simply larger than 1 for a while: the result is the same, most tiles need no rescale.
@@ -36,8 +39,10 @@ struct AtSmem {
     static constexpr size_t Q_BYTES = (size_t)AT_ROWS * HD * 2;            // K_ATOMS blocks of [128 rows][128 bytes]
     static constexpr size_t K_BYTES = (size_t)AT_KEYS * HD * 2;            // K_ATOMS blocks of [64 keys][128 bytes]
     static constexpr size_t V_BYTES = (size_t)AT_KEYS * VD * 2;            // V_ATOMS such blocks
-    static constexpr size_t P_BYTES = (size_t)AT_ROWS * AT_KEYS * 2;       // [128 rows][128 bytes]
-    static constexpr size_t BYTES = Q_BYTES + AT_KV_STAGES * (K_BYTES + V_BYTES) + P_BYTES + 128;   // 128: barriers, tensor-memory slot
+    static constexpr size_t USED = Q_BYTES + AT_KV_STAGES * (K_BYTES + V_BYTES) + 128;              // 128: barriers, tensor-memory slot
+    // Two blocks an SM hold all of its tensor memory: a third one, where it fits otherwise, would wait there for one of them to end, while other
+    // SMs may stand idle (256 blocks with heads of 64 and 8,500 keys each: 242 us, 168 without it).
+    static constexpr size_t BYTES = USED > 80 * 1024 ? USED : 80 * 1024;
 };
 
 // HD, VD: key and value sizes filled up to 64 or 128; vd: the value size itself.
@@ -46,7 +51,7 @@ struct AtSmem {
 // attn_tc_join_kernel, in part_o [T * Hq, pieces, VD] and part_ml [T * Hq, pieces, 2] (with few rows and long contexts a block a row's tile
 // would walk over all keys by itself while most SMs stand idle).
 template <int HD, int VD, bool SHAPED, bool PIECES = false>
-__global__ void __launch_bounds__(AT_THREADS)
+__global__ void __launch_bounds__(AT_THREADS, 2)
 attn_tc_prefill_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
                        const __grid_constant__ CUtensorMap map_v, const int* __restrict__ page_table,
                        const int* __restrict__ cu_seqlens, const int* __restrict__ pos0, bf16* __restrict__ out, int Hq, int Hkv,
@@ -55,7 +60,7 @@ attn_tc_prefill_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
                        float* __restrict__ part_ml) {
     using Smem = AtSmem<HD, VD>;
     constexpr uint32_t K_BYTES = Smem::K_BYTES, V_BYTES = Smem::V_BYTES;
-    constexpr uint32_t TMEM_COLS = 256;                                     // S: 2 x 64 columns, O: VD columns
+    constexpr uint32_t TMEM_COLS = 256;                                     // S and P: 2 x 64 columns, O: VD columns
     // The tiles need 1024-byte alignment (128-byte swizzle).  No padding to reach it: at head size 128 the block's
     // 113 KB then leave room for a second block on the SM, whose products run while this block's softmax does.
     extern __shared__ __align__(1024) unsigned char smem_raw[];
@@ -66,15 +71,13 @@ attn_tc_prefill_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
     unsigned char* q_tile = smem_raw;
     unsigned char* k_tiles = q_tile + Smem::Q_BYTES;
     unsigned char* v_tiles = k_tiles + AT_KV_STAGES * K_BYTES;
-    unsigned char* p_tile = v_tiles + AT_KV_STAGES * V_BYTES;
-    uint64_t* q_full = reinterpret_cast<uint64_t*>(p_tile + Smem::P_BYTES);
+    uint64_t* q_full = reinterpret_cast<uint64_t*>(v_tiles + AT_KV_STAGES * V_BYTES);
     uint64_t* k_full = q_full + 1;                       // K and V have barriers of their own: a K buffer is free as soon
     uint64_t* k_empty = k_full + AT_KV_STAGES;           // as its scores are formed, long before its tile's V buffer is
     uint64_t* v_full = k_empty + AT_KV_STAGES;
     uint64_t* v_empty = v_full + AT_KV_STAGES;
     uint64_t* s_full = v_empty + AT_KV_STAGES;           // [2]: the two S buffers
-    uint64_t* s_empty = s_full + 2;                      // [2]
-    uint64_t* p_full = s_empty + 2;
+    uint64_t* p_full = s_full + 2;
     uint64_t* o_full = p_full + 1;
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(o_full + 1);
 
@@ -105,7 +108,7 @@ attn_tc_prefill_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
             at_bar_init(&k_full[s], 1); at_bar_init(&k_empty[s], 1);
             at_bar_init(&v_full[s], 1); at_bar_init(&v_empty[s], 1);
         }
-        for (int i = 0; i < 2; ++i) { at_bar_init(&s_full[i], 1); at_bar_init(&s_empty[i], 4); }
+        for (int i = 0; i < 2; ++i) at_bar_init(&s_full[i], 1);
         at_bar_init(p_full, 4);
         at_bar_init(o_full, 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -167,7 +170,6 @@ attn_tc_prefill_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
             auto issue_s = [&](int j) -> bool {
                 const int s = j % AT_KV_STAGES;
                 if (!at_wait(&k_full[s], (j / AT_KV_STAGES) & 1)) return false;
-                if (j >= 2 && !at_wait(&s_empty[j & 1], ((j >> 1) - 1) & 1)) return false;
                 at_fence_after();
                 const unsigned char* kt = k_tiles + (size_t)s * K_BYTES;
 #pragma unroll
@@ -190,13 +192,12 @@ attn_tc_prefill_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
                 const unsigned char* vt = v_tiles + (size_t)s * V_BYTES;
 #pragma unroll
                 for (int k = 0; k < AT_KEYS / 16; ++k) {                               // 16 keys per product
-                    const uint64_t da = at_desc_kmajor(p_tile) + 2 * k;
                     const uint64_t db = at_desc_mnmajor(vt + (size_t)k * 16 * 128, AT_KEYS * 128);
-                    at_mma(tmem_o, da, db, idesc_o, (j > 0 || k > 0) ? 1u : 0u);
+                    at_mma_ts(tmem_o, tmem_s + (uint32_t)(j & 1) * 64 + 8 * k, db, idesc_o, (j > 0 || k > 0) ? 1u : 0u);
                 }
                 at_commit(&v_empty[s]);                                                // V of this tile is read
                 at_commit(o_full);
-                if (j + 2 < n_tiles) ok = issue_s(j + 2);
+                if (j + 2 < n_tiles) ok = at_wait(o_full, j & 1) && issue_s(j + 2);    // P of this tile lies where those scores go
             }
             if (!ok) {
                 atomicExch(error, 2);
@@ -217,7 +218,6 @@ attn_tc_prefill_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
         // raw score here, as everything before the exponential
         const float slope_raw = (SHAPED && slopes && row_ok) ? slopes[head] / scale : 0.f;
         float m_ref = -INFINITY, l = 0.f;                                              // reference maximum (raw score) and sum
-        uint4* p_row = reinterpret_cast<uint4*>(p_tile + (size_t)r * 128);
         bool ok = true;
         for (int j = 0; j < n_tiles; ++j) {
             ok = at_wait(&s_full[j & 1], (j >> 1) & 1);
@@ -227,9 +227,6 @@ attn_tc_prefill_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
             uint32_t sv[2][32];
             at_ld32(tmem_s + (uint32_t)(j & 1) * 64 + lane_off, sv[0]);
             at_ld32(tmem_s + (uint32_t)(j & 1) * 64 + lane_off + 32, sv[1]);
-            at_fence_before();                                                          // this S buffer may be filled again
-            __syncwarp();
-            if (lane == 0) at_arrive(&s_empty[j & 1]);
             if (SHAPED && slopes) {                                                     // one fused multiply-add a score
                 const float c0 = -slope_raw * (float)(qp - key0);
 #pragma unroll
@@ -281,6 +278,7 @@ attn_tc_prefill_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
                     __nv_bfloat162 v = __floats2bfloat162_rn(p0v, p1v);
                     pk[h][i / 2] = *reinterpret_cast<uint32_t*>(&v);
                 }
+            at_st32(tmem_s + (uint32_t)(j & 1) * 64 + lane_off, &pk[0][0]);      // where this tile's scores were
             if (j > 0) {                                                               // the product before this one has read P and written O
                 ok = at_wait(o_full, (j - 1) & 1);
                 at_fence_after();
@@ -296,13 +294,7 @@ attn_tc_prefill_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
                     }
                 }
             }
-#pragma unroll
-            for (int h = 0; h < 2; ++h)
-#pragma unroll
-                for (int i = 0; i < 4; ++i)
-                    p_row[(h * 4 + i) ^ (r & 7)] = make_uint4(pk[h][4 * i], pk[h][4 * i + 1], pk[h][4 * i + 2], pk[h][4 * i + 3]);
             at_fence_before();                                                          // O is rescaled (if at all); P is written
-            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             __syncwarp();
             if (lane == 0) at_arrive(p_full);
         }
