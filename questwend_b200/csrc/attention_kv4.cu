@@ -647,8 +647,8 @@ static int kv4_cluster_size(long long runs) {
 // Whether a step that brings more than a few tokens is faster with its pages read as bfloat16 once and the tcgen05 prompt kernel.  That kernel
 // reaches six times the rate, but the pages go through memory twice more; as rows every run of every 16 columns is a block, with a start and an
 // end that cost as much as 3.5 pages.  Both in microseconds, from measurements (32 query and 8 key heads of 128, as rows / read, with 8, 32 and 128
-// new tokens a sequence): one sequence of 1,000 tokens 12 / 19, 15 / 19, 38 / 19; of 8,192 19 / 34, 41 / 35, 121 / 46; of 60,000 68 / 124, 205 / 124, 768 / 197;
-// 8 of 8,192 65 / 95, 218 / 162, 742 / 243; a whole prompt of 128 16 / 10, of 900 262 / 27.
+// new tokens a sequence): one sequence of 1,000 tokens 11 / 19, 15 / 18, 38 / 18; of 8,192 16 / 34, 40 / 32, 121 / 44; of 60,000 68 / 119, 205 / 121, 769 / 186;
+// 8 of 8,192 66 / 91, 219 / 151, 743 / 212; a whole prompt of 128 15 / 9, of 900 262 / 24.
 // tokens, listed: the step's tokens and its sequences' pages (which say more of unequal sequences than the most of each).
 static bool kv4_read_is_faster(int max_len, int max_new, int window, int table_width, int B, int Hq, int Hkv, int hd, int tokens, int listed) {
     const int G = Hq / Hkv;
