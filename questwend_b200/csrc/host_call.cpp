@@ -1,4 +1,4 @@
-// The way from Python to the kernels' launchers: a Python module of seven functions.  A step of few tokens is a handful of launches of a few
+// The way from Python to the kernels' launchers: a Python module of eight functions.  A step of few tokens is a handful of launches of a few
 // microseconds each, and through ctypes making a launcher's arguments (an object each), checking its tensors and asking for its outputs took
 // longer than the launches: one token through Mamba-2's convolution and recurrence 27 us of the host for 6 us of the GPU.
 //
@@ -9,6 +9,8 @@
 //     pieces(like, dtype, shape, ...)     a tuple of uninitialised tensors of these types and shapes on like's device, in one piece of memory, each at a
 //                                         multiple of 256 bytes (six of them 3 us, one after the other 7)
 //     here(device, *tensors)              whether all tensors (or None) lie on CUDA device number `device`
+//     ready(tensor, dtype, dimensions, ...)           the number of the CUDA device on which all tensors (or None) lie, each as `fits` says; -1: not
+//                                         so (seven of them 0.4 us, a call of `fits` each and one of `here` 2)
 //     same(x)                             x
 //     fill(array, numbers)                a list's whole numbers into a contiguous array of as many 32-bit ones; False where the list holds anything
 //                                         else, or a number that does not fit: the array then holds any part of them
@@ -122,15 +124,38 @@ PyObject* call(PyObject*, PyObject* const* args, Py_ssize_t n) {
     END_HANDLE_TH_ERRORS
 }
 
+bool tensor_fits(PyObject* tensor, PyObject* dtype, PyObject* dims) {
+    const at::Tensor& t = THPVariable_Unpack(tensor);
+    bool ok = t.is_cuda() && t.is_contiguous();
+    if (ok && dtype != Py_None) ok = THPDtype_Check(dtype) && t.scalar_type() == reinterpret_cast<THPDtype*>(dtype)->scalar_type;
+    if (ok && dims != Py_None) ok = t.dim() == PyLong_AsLong(dims);
+    return ok;
+}
+
 PyObject* fits(PyObject*, PyObject* const* args, Py_ssize_t n) {
     HANDLE_TH_ERRORS
     if (n != 3 || !THPVariable_Check(args[0])) Py_RETURN_FALSE;
-    const at::Tensor& t = THPVariable_Unpack(args[0]);
-    bool ok = t.is_cuda() && t.is_contiguous();
-    if (ok && args[1] != Py_None) ok = THPDtype_Check(args[1]) && t.scalar_type() == reinterpret_cast<THPDtype*>(args[1])->scalar_type;
-    if (ok && args[2] != Py_None) ok = t.dim() == PyLong_AsLong(args[2]);
+    const bool ok = tensor_fits(args[0], args[1], args[2]);
     if (PyErr_Occurred()) return nullptr;
     return PyBool_FromLong(ok);
+    END_HANDLE_TH_ERRORS
+}
+
+PyObject* ready(PyObject*, PyObject* const* args, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    if (n % 3) return PyErr_Format(PyExc_TypeError, "ready: a tensor, a type and a number of dimensions each");
+    long device = -1;
+    bool ok = true;
+    for (Py_ssize_t i = 0; ok && i < n; i += 3) {
+        if (args[i] == Py_None) continue;
+        ok = THPVariable_Check(args[i]) && tensor_fits(args[i], args[i + 1], args[i + 2]);
+        if (!ok) break;
+        const long its = THPVariable_Unpack(args[i]).get_device();
+        ok = device < 0 || its == device;
+        device = its;
+    }
+    if (PyErr_Occurred()) return nullptr;
+    return PyLong_FromLong(ok ? device : -1);
     END_HANDLE_TH_ERRORS
 }
 
@@ -258,6 +283,7 @@ PyMethodDef methods[] = {{"call", (PyCFunction)(void*)call, METH_FASTCALL, nullp
                          {"empty", (PyCFunction)(void*)empty, METH_FASTCALL | METH_KEYWORDS, nullptr},
                          {"pieces", (PyCFunction)(void*)pieces, METH_FASTCALL, nullptr},
                          {"here", (PyCFunction)(void*)here, METH_FASTCALL, nullptr},
+                         {"ready", (PyCFunction)(void*)ready, METH_FASTCALL, nullptr},
                          {"same", same, METH_O, nullptr},
                          {"fill", (PyCFunction)(void*)fill, METH_FASTCALL, nullptr},
                          {nullptr, nullptr, 0, nullptr}};

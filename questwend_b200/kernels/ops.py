@@ -100,6 +100,15 @@ def _here(what: str, *tensors) -> None:
             raise KernelError(f"{what}: a tensor on {t.device}, while the current device is cuda:{here} (use torch.cuda.device)")
 
 
+def _ready(*checks) -> bool:
+    """Whether the tensors (or None) of ``checks``, each with its type and number of dimensions (None: any), are what ``_need`` and ``_here``
+    would have them be, all asked at once; False too where that cannot be asked natively."""
+    if _HOST is None:
+        return False
+    device = _HOST.ready(*checks)
+    return device >= 0 and device == torch.cuda.current_device()
+
+
 def _column_gate(what: str, gate: torch.Tensor | None, col0: int, T: int, H: int):
     """The arguments (pointer, row stride) of a gate: columns ``col0 ..`` of the float32 matrix ``gate`` [T, ld], one a head."""
     if gate is None:
@@ -145,6 +154,31 @@ def _call(module: str, fn: str, *args, kernels: int = 1):
     LAUNCHES[0] += kernels
     if rc != 0:
         raise KernelError(_FUNCTIONS[name][0].qwb_last_error().decode("utf-8", "replace") or f"{fn} failed with code {rc}")
+
+
+def _plain_argument(x):
+    if x is None or isinstance(x, torch.Tensor):
+        return _ptr_object(x)
+    return ctypes.c_int(x) if isinstance(x, int) else ctypes.c_float(x) if isinstance(x, float) else x
+
+
+def _run(module: str, fn: str, *args, kernels: int = 1):
+    """``_call`` with the arguments as they are: tensors (None: a null pointer), whole numbers, floats, and the stream last, as ``_stream()``."""
+    if _HOST is None:
+        stream = args[-1]
+        args = [_plain_argument(x) for x in args[:-1]] + [stream]
+    _call(module, fn, *args, kernels=kernels)
+
+
+def _ask(module: str, fn: str, *args) -> int:
+    """What a function of whole numbers says, a whole number of 32 bits; nothing is launched."""
+    if _HOST is None:
+        return _lookup(module, fn)[1](*args)
+    address = _ADDRESSES.get((module, fn))
+    if address is None:
+        _lookup(module, fn)
+        address = _ADDRESSES[module, fn]
+    return _HOST.call(address, *args)
 
 
 # ----------------------------------------------------------------------------- elementwise
@@ -2121,23 +2155,24 @@ def step_tables(pages: torch.Tensor, page_start: torch.Tensor, pos0: torch.Tenso
     table (0: none is made), pages beyond it are left out.  A token for which its sequence has no page has slot -1.  ``tokens`` False:
     the page table alone (another group of the same step); the tensors of the tokens are then None.  Reads nothing on the host, so it
     can be captured into a graph; page ids are below 2^25, so that rows are whole numbers of 32 bits."""
-    for name, t in (("pages", pages), ("page_start", page_start), ("pos0", pos0), ("n_new", n_new)):
-        _need(t, name, torch.int32, 1)
-    _here("step_tables", pages, page_start, pos0, n_new)
+    whole = torch.int32
+    if not _ready(pages, whole, 1, page_start, whole, 1, pos0, whole, 1, n_new, whole, 1):
+        for name, t in (("pages", pages), ("page_start", page_start), ("pos0", pos0), ("n_new", n_new)):
+            _need(t, name, whole, 1)
+        _here("step_tables", pages, page_start, pos0, n_new)
     B, T, W = pos0.numel(), int(n_tokens), int(table_width)
     if B < 1 or B > STEP_TABLES_MAX_SEQS or n_new.numel() != B or page_start.numel() != B + 1:
         raise KernelError(f"step_tables: {B} lengths (1 to {STEP_TABLES_MAX_SEQS}), {n_new.numel()} counts and {page_start.numel()} page "
                           f"starts do not belong together")
     if T < 0 or W < 0 or T >= 2 ** 31 or W >= 2 ** 31:
         raise KernelError(f"step_tables: {T} tokens, a table of {W} columns")
-    whole = torch.int32
     if tokens:
         table, cu, seq_len, tok_seq, tok_pos, slot = _pieces(pos0, whole, (B, W), whole, (B + 1,), whole, (B,), whole, (T,), whole, (T,), whole, (T,))
     else:
         (table,) = _pieces(pos0, whole, (B, W))
         cu = seq_len = tok_seq = tok_pos = slot = None
-    _call("step_tables", "qwb_step_tables", _ptr(pages), _ptr(page_start), _ptr(pos0), _ptr(n_new), _ptr(cu), _ptr(seq_len), _ptr(tok_seq),
-          _ptr(tok_pos), _ptr(slot), _ptr(table), _i(pages.numel()), _i(B), _i(T), _i(W), _i(PAGE_SIZE), _i(1 if tokens else 0), _stream())
+    _run("step_tables", "qwb_step_tables", pages, page_start, pos0, n_new, cu, seq_len, tok_seq, tok_pos, slot, table, pages.numel(), B, T, W,
+         PAGE_SIZE, 1 if tokens else 0, _stream())
     return StepTables(cu, seq_len, tok_seq, tok_pos, table, slot, pos0, pages, page_start)
 
 
@@ -2150,12 +2185,19 @@ def kv4_page_bytes(head_dim: int) -> int:
     return 2 * PAGE_SIZE * (head_dim // 2 + 2 * (head_dim // KV4_GROUP))
 
 
-def _kv4_pool(what: str, pool: torch.Tensor, head_dim: int) -> None:
-    _need(pool, "pool", torch.uint8, 3)
-    if pool.shape[2] != kv4_page_bytes(head_dim):
+_KV4_PAGE_BYTES: dict = {}      # head size -> kv4_page_bytes
+
+
+def _kv4_pool(what: str, pool: torch.Tensor, head_dim: int) -> tuple[int, int]:
+    """The pool's pages and heads; refused if it is no pool for heads of this size."""
+    pages, heads, page_bytes = pool.shape
+    if head_dim not in _KV4_PAGE_BYTES:
+        _KV4_PAGE_BYTES[head_dim] = kv4_page_bytes(head_dim)
+    if page_bytes != _KV4_PAGE_BYTES[head_dim]:
         raise KernelError(f"{what}: a pool of {tuple(pool.shape)} does not hold heads of {head_dim} ({kv4_page_bytes(head_dim)} bytes a page)")
     if pool.data_ptr() % 16:
         raise KernelError(f"{what}: the pool must start at a multiple of 16 bytes")
+    return pages, heads
 
 
 def kv4_store(qkv: torch.Tensor, q_weight, k_weight, cos, sin, slot_map: torch.Tensor, pool: torch.Tensor, n_heads: int, n_kv_heads: int,
@@ -2167,32 +2209,34 @@ def kv4_store(qkv: torch.Tensor, q_weight, k_weight, cos, sin, slot_map: torch.T
     32 neighbouring numbers of a key or value share a step s of 4 significant bits and a zero point z; each is held as a code c of
     0..15 and stands for (c - z) s, the nearest of the 16 such numbers.  Keys are normed, turned and rounded to codes in 64 bits.  A group
     with a number that is not finite stands for NaN."""
-    _need(qkv, "qkv", torch.float32, 2)
-    _kv4_pool("kv4_store", pool, head_dim)
-    _need(slot_map, "slot_map", torch.int32, 1)
-    T = qkv.shape[0]
-    if qkv.shape[1] != (n_heads + 2 * n_kv_heads) * head_dim or slot_map.numel() != T or pool.shape[1] != n_kv_heads:
+    single = torch.float32
+    if not rotary_dim:
+        cos = sin = None
+    elif cos is None or sin is None:
+        raise KernelError(f"kv4_store: no cosines and sines for a rotary size of {rotary_dim}")
+    if not _ready(qkv, single, 2, pool, torch.uint8, 3, slot_map, torch.int32, 1, q_weight, single, 1, k_weight, single, 1, cos, single, 2, sin, single, 2):
+        _need(qkv, "qkv", single, 2)
+        _need(pool, "pool", torch.uint8, 3)
+        _need(slot_map, "slot_map", torch.int32, 1)
+        for name, t, dims in (("q_weight", q_weight, 1), ("k_weight", k_weight, 1), ("cos", cos, 2), ("sin", sin, 2)):
+            if t is not None:
+                _need(t, name, single, dims)
+        _here("kv4_store", qkv, q_weight, k_weight, cos, sin, slot_map, pool)
+    n_pages, heads = _kv4_pool("kv4_store", pool, head_dim)
+    T, columns = qkv.shape
+    if columns != (n_heads + 2 * n_kv_heads) * head_dim or slot_map.numel() != T or heads != n_kv_heads:
         raise KernelError(f"kv4_store: qkv {tuple(qkv.shape)} and {slot_map.numel()} slots for {n_heads} + 2 x {n_kv_heads} heads of {head_dim} and a "
-                          f"pool of {pool.shape[1]} heads")
+                          f"pool of {heads} heads")
     for name, t in (("q_weight", q_weight), ("k_weight", k_weight)):
-        if t is not None:
-            _need(t, name, torch.float32, 1)
-            if t.numel() != head_dim:
-                raise KernelError(f"kv4_store: {name} has {t.numel()} entries for heads of {head_dim}")
+        if t is not None and t.numel() != head_dim:
+            raise KernelError(f"kv4_store: {name} has {t.numel()} entries for heads of {head_dim}")
     if rotary_dim < 0 or rotary_dim > head_dim or rotary_dim % 2:
         raise KernelError(f"kv4_store: rotary size {rotary_dim} for heads of {head_dim}")
-    if rotary_dim:
-        _need(cos, "cos", torch.float32, 2)
-        _need(sin, "sin", torch.float32, 2)
-        if tuple(cos.shape) != (T, rotary_dim // 2) or sin.shape != cos.shape:
-            raise KernelError(f"kv4_store: cos/sin {tuple(cos.shape)} do not fit {T} tokens and rotary size {rotary_dim}")
-    else:
-        cos = sin = None
-    _here("kv4_store", qkv, q_weight, k_weight, cos, sin, slot_map, pool)
+    if rotary_dim and (cos.shape != (T, rotary_dim // 2) or sin.shape != cos.shape):
+        raise KernelError(f"kv4_store: cos/sin {tuple(cos.shape)} do not fit {T} tokens and rotary size {rotary_dim}")
     q_out = _empty((T, n_heads, head_dim), dtype=q_dtype, device=qkv.device)
-    _call("kv4_cache", "qwb_kv4_store", _ptr(qkv), _ptr(q_weight), _ptr(k_weight), _ptr(cos), _ptr(sin), _ptr(slot_map), _ptr(q_out), _i(_dt(q_dtype)),
-          _ptr(pool), _i(pool.shape[0]), _i(T), _i(n_heads), _i(n_kv_heads), _i(head_dim), _i(rotary_dim), _f(eps),
-          _i(1 if store_kv else 0), _stream())
+    _run("kv4_cache", "qwb_kv4_store", qkv, q_weight, k_weight, cos, sin, slot_map, q_out, _dt(q_dtype), pool, n_pages, T, n_heads, n_kv_heads, head_dim,
+         rotary_dim, float(eps), 1 if store_kv else 0, _stream())
     return q_out
 
 
@@ -2203,13 +2247,15 @@ def kv4_read(pool: torch.Tensor, pages: torch.Tensor, page_start: torch.Tensor, 
     them (0 where a sequence has no page).  Both types hold the numbers exactly.  ``marked``: a token with a value that is not finite has
     values of 0 and keys of NaN instead (what a kernel needs that multiplies unseen values by 0).  ``rest`` (rows [n, bytes a multiple of
     16], one int32 on the device): the rows from that number on are set to zero."""
-    _kv4_pool("kv4_read", pool, head_dim)
-    for name, t in (("pages", pages), ("page_start", page_start), ("seq_len", seq_len)):
-        _need(t, name, torch.int32, 1)
-    P, B, Hkv = pages.numel(), seq_len.numel(), pool.shape[1]
+    if not _ready(pool, torch.uint8, 3, pages, torch.int32, 1, page_start, torch.int32, 1, seq_len, torch.int32, 1):
+        _need(pool, "pool", torch.uint8, 3)
+        for name, t in (("pages", pages), ("page_start", page_start), ("seq_len", seq_len)):
+            _need(t, name, torch.int32, 1)
+        _here("kv4_read", pool, pages, page_start, seq_len)
+    n_pages, Hkv = _kv4_pool("kv4_read", pool, head_dim)
+    P, B = pages.numel(), seq_len.numel()
     if B < 1 or page_start.numel() != B + 1 or max_len < 1:
         raise KernelError(f"kv4_read: {page_start.numel()} page starts for {B} sequences of up to {max_len} tokens")
-    _here("kv4_read", pool, pages, page_start, seq_len)
     rows, used = rest if rest is not None else (None, None)
     if rest is not None:
         _need(rows, "rest", ndim=2)
@@ -2220,9 +2266,8 @@ def kv4_read(pool: torch.Tensor, pages: torch.Tensor, page_start: torch.Tensor, 
     k, v, table = _pieces(pool, dtype, shape, dtype, shape, torch.int32, (B, width))
     if not P:
         table.zero_()
-    _call("kv4_cache", "qwb_kv4_read", _ptr(pool), _ptr(pages), _ptr(page_start), _ptr(seq_len), _ptr(k), _ptr(v), _i(_dt(dtype)), _ptr(table),
-          _i(P), _i(B), _i(width), _i(pool.shape[0]), _i(Hkv), _i(head_dim), _i(1 if marked else 0), _ptr(rows), _ptr(used),
-          _i(0 if rows is None else rows.shape[0]), _i(0 if rows is None else rows.shape[1] * rows.element_size()), _stream())
+    _run("kv4_cache", "qwb_kv4_read", pool, pages, page_start, seq_len, k, v, _dt(dtype), table, P, B, width, n_pages, Hkv, head_dim, 1 if marked else 0, rows,
+         used, 0 if rows is None else rows.shape[0], 0 if rows is None else rows.shape[1] * rows.element_size(), _stream())
     return k, v, table
 
 
@@ -2235,43 +2280,45 @@ def kv4_attention(q: torch.Tensor, pool: torch.Tensor, tables: StepTables, max_n
     ``impl``: "rows" (bfloat16, heads of 64 or 128: codes to tensor-core fragments, a sequence's keys cut into runs; for few new tokens), "read"
     (the same sizes, groups of up to 64 heads, ``tables.pages`` given: the step's pages as bfloat16 once, then the tcgen05 prompt kernel), "plain"
     (every size and type), or "auto": the fastest that takes the case."""
-    _need(q, "q", ndim=3)
-    T, Hq, hd = q.shape
-    _kv4_pool("kv4_attention", pool, hd)
     table, tok_seq, tok_pos, cu, pos0 = tables.page_table, tables.tok_seq, tables.tok_pos, tables.cu_seqlens, tables.pos0
-    _need(table, "page_table", torch.int32, 2)
-    for name, t in (("tok_seq", tok_seq), ("tok_pos", tok_pos), ("cu_seqlens", cu), ("pos0", pos0)):
-        _need(t, name, torch.int32, 1)
-    B, Hkv = pos0.numel(), pool.shape[1]
-    if tok_seq.numel() != T or tok_pos.numel() != T or cu.numel() != B + 1 or table.shape[0] < B or Hq % Hkv:
+    whole = torch.int32
+    if not _ready(q, None, 3, pool, torch.uint8, 3, table, whole, 2, tok_seq, whole, 1, tok_pos, whole, 1, cu, whole, 1, pos0, whole, 1):
+        _need(q, "q", ndim=3)
+        _need(pool, "pool", torch.uint8, 3)
+        _need(table, "page_table", whole, 2)
+        for name, t in (("tok_seq", tok_seq), ("tok_pos", tok_pos), ("cu_seqlens", cu), ("pos0", pos0)):
+            _need(t, name, whole, 1)
+        _here("kv4_attention", q, pool, table, tok_seq, tok_pos, cu, pos0)
+    T, Hq, hd = q.shape
+    n_pages, Hkv = _kv4_pool("kv4_attention", pool, hd)
+    B, (table_rows, width) = pos0.numel(), table.shape
+    if tok_seq.numel() != T or tok_pos.numel() != T or cu.numel() != B + 1 or table_rows < B or Hq % Hkv:
         raise KernelError(f"kv4_attention: tables of {tok_seq.numel()} tokens, {cu.numel() - 1} and {B} sequences for queries {tuple(q.shape)} over "
                           f"{Hkv} heads")
-    if max_new < 1 or max_len < 1 or table.shape[1] < 1 or window < 0:
+    if max_new < 1 or max_len < 1 or width < 1 or window < 0:
         raise KernelError(f"kv4_attention: up to {max_new} new tokens of sequences of up to {max_len}, window {window}, a page table of "
-                          f"{table.shape[1]} columns")
-    max_len = min(max_len, table.shape[1] * PAGE_SIZE)
+                          f"{width} columns")
+    max_len = min(max_len, width * PAGE_SIZE)
     if impl not in ("auto", "plain", "rows", "read"):
         raise KernelError(f"kv4_attention: unknown form '{impl}'")
-    _here("kv4_attention", q, pool, table, tok_seq, tok_pos, cu, pos0)
-    group = Hq // Hkv
-    fits = q.dtype == torch.bfloat16 and hd in (64, 128)
-    reads = fits and group <= 64 and tables.pages is not None and tables.page_start is not None and tables.pages.numel() > 0
+    group, dtype = Hq // Hkv, q.dtype
+    fits = dtype == torch.bfloat16 and hd in (64, 128)
+    listed = tables.pages.numel() if fits and group <= 64 and tables.pages is not None and tables.page_start is not None else 0
+    reads = listed > 0
     plan = 0
     if fits and impl != "plain":
-        plan = _lookup("attention_kv4", "qwb_kv4_plan")[1](max_len, max_new, window, table.shape[1], B, Hq, Hkv, hd, T,
-                                                                tables.pages.numel() if reads else 0)
+        plan = _ask("attention_kv4", "qwb_kv4_plan", max_len, max_new, window, width, B, Hq, Hkv, hd, T, listed)
     if impl == "auto":
         impl = "plain" if not fits else "read" if reads and plan & 1 else "rows"
     if (impl == "rows" and not fits) or (impl == "read" and not reads):
         raise KernelError(f"kv4_attention: form '{impl}' does not take {q.dtype} queries of {hd}, groups of {group}"
                           f"{'' if reads else ' (or has no list of pages)'}")
-    out = _empty((T, Hq * hd), dtype=q.dtype, device=q.device)
+    out = _empty((T, Hq * hd), dtype=dtype, device=q.device)
     if impl == "rows":
         max_runs = plan >> 2
         scratch = _empty((T * Hq * max_runs * (hd + 2),), dtype=torch.float32, device=q.device) if plan & 2 else None
-        _call("attention_kv4", "qwb_kv4_attn_rows", _ptr(q), _ptr(pool), _ptr(table), _ptr(cu), _ptr(pos0), _ptr(tok_seq), _ptr(out), _ptr(scratch), _i(T),
-              _i(B), _i(pool.shape[0]), _i(max_new), _i(Hq), _i(Hkv), _i(hd), _i(table.shape[1]), _f(scale), _i(window), _i(max_runs), _stream(),
-              kernels=1 if scratch is None else 2)
+        _run("attention_kv4", "qwb_kv4_attn_rows", q, pool, table, cu, pos0, tok_seq, out, scratch, T, B, n_pages, max_new, Hq, Hkv, hd, width, float(scale), window,
+             max_runs, _stream(), kernels=1 if scratch is None else 2)
         return out
     if impl == "read":
         k, v, compact = kv4_read(pool, tables.pages, tables.page_start, tables.seq_len, max_len, hd, q.dtype, marked=True, rest=(out, cu[B:]))
@@ -2288,8 +2335,7 @@ def kv4_attention(q: torch.Tensor, pool: torch.Tensor, tables: StepTables, max_n
               _i(k.shape[0]), _i(Hq), _i(Hkv), _i(hd), _i(hd), _i(PAGE_SIZE), _i(compact.shape[1]), _f(scale), _i(window), _i(0), _ptr(None), _ptr(None),
               _ptr(gemm_tc_error_word(q.device)), _stream())
         return out
-    _call("attention_kv4", "qwb_kv4_attn_plain", _ptr(q), _ptr(pool), _ptr(table), _ptr(tok_seq), _ptr(tok_pos), _ptr(out), _i(_dt(q.dtype)), _i(T),
-          _i(B), _i(pool.shape[0]), _i(Hq), _i(Hkv), _i(hd), _i(table.shape[1]), _f(scale), _i(window), _stream())
+    _run("attention_kv4", "qwb_kv4_attn_plain", q, pool, table, tok_seq, tok_pos, out, _dt(dtype), T, B, n_pages, Hq, Hkv, hd, width, float(scale), window, _stream())
     return out
 
 
@@ -2311,14 +2357,15 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top: int = 0, out
     A row with a NaN, with +infinity or with nothing but -infinity has no distribution: its numbers are NaN (a NaN logit is not among the
     alternatives; where fewer than ``top`` remain the id is -1).  A token outside 0..V-1 has log probability NaN.  ``out``: tensors of
     an earlier call of the same sizes to write into."""
-    _need(logits, "logits", torch.float32, 2)
-    _need(tokens, "tokens", torch.int32, 1)
+    if not _ready(logits, torch.float32, 2, tokens, torch.int32, 1):
+        _need(logits, "logits", torch.float32, 2)
+        _need(tokens, "tokens", torch.int32, 1)
+        _here("token_logprobs", logits, tokens)
     R, V = logits.shape
     if tokens.numel() != R or R > LOGPROBS_MAX_ROWS:
         raise KernelError(f"token_logprobs: {tokens.numel()} tokens for {R} rows (at most {LOGPROBS_MAX_ROWS})")
     if not 0 <= top <= min(V, LOGPROBS_MAX_TOP) or V < 1:
         raise KernelError(f"token_logprobs: 0 to {LOGPROBS_MAX_TOP} alternatives of a vocabulary of at least as many: {top} of {V}")
-    dev = logits.device
     if out is None:
         out = TokenLogprobs(*_pieces(logits, torch.float32, (R,), torch.float32, (R,), torch.int32, (R, top), torch.float32, (R, top)))
     else:
@@ -2327,12 +2374,9 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top: int = 0, out
             _need(t, name, dtype, len(shape))
             if tuple(t.shape) != shape:
                 raise KernelError(f"token_logprobs: {name} of {tuple(t.shape)} for {R} rows and {top} alternatives")
-    _here("token_logprobs", logits, tokens, *out)
+        _here("token_logprobs", *out)
     if R:
-        size = _lookup("logprobs", "qwb_logprobs_scratch")[1]
-        size.restype = ctypes.c_longlong
-        floats = size(R, V, top)
-        scratch = _empty((floats,), dtype=torch.float32, device=dev) if floats else None
-        _call("logprobs", "qwb_logprobs", _ptr(logits), _ptr(tokens), _ptr(out.logprob), _ptr(out.entropy), _ptr(out.top_ids), _ptr(out.top_logprobs),
-              _ptr(scratch), _i(R), _i(V), _i(top), _stream(), kernels=2 if floats else 1)
+        floats = _ask("logprobs", "qwb_logprobs_scratch", R, V, top)
+        scratch = _empty((R * floats,), dtype=torch.float32, device=logits.device) if floats else None
+        _run("logprobs", "qwb_logprobs", logits, tokens, *out, scratch, R, V, top, _stream(), kernels=2 if floats else 1)
     return out
