@@ -105,6 +105,12 @@ PyObject* call(PyObject*, PyObject* const* args, Py_ssize_t n) {
             is_real = true;
         } else if (THPVariable_Check(o)) {
             v = (uint64_t)THPVariable_Unpack(o).mutable_data_ptr();
+        } else if (PyIndex_Check(o)) {                              // another library's whole number
+            PyObject* number = PyNumber_Index(o);
+            if (!number) return nullptr;
+            v = PyLong_AsUnsignedLongLongMask(number);
+            Py_DECREF(number);
+            if (v == (uint64_t)-1 && PyErr_Occurred()) return nullptr;
         } else if (!from_ctypes(o, v, d, is_real)) {
             return nullptr;
         }

@@ -159,7 +159,7 @@ def _call(module: str, fn: str, *args, kernels: int = 1):
 def _plain_argument(x):
     if x is None or isinstance(x, torch.Tensor):
         return _ptr_object(x)
-    return ctypes.c_int(x) if isinstance(x, int) else ctypes.c_float(x) if isinstance(x, float) else x
+    return ctypes.c_float(x) if isinstance(x, float) else ctypes.c_int(operator.index(x))
 
 
 def _run(module: str, fn: str, *args, kernels: int = 1):
@@ -173,7 +173,7 @@ def _run(module: str, fn: str, *args, kernels: int = 1):
 def _ask(module: str, fn: str, *args) -> int:
     """What a function of whole numbers says, a whole number of 32 bits; nothing is launched."""
     if _HOST is None:
-        return _lookup(module, fn)[1](*args)
+        return _lookup(module, fn)[1](*map(operator.index, args))
     address = _ADDRESSES.get((module, fn))
     if address is None:
         _lookup(module, fn)
@@ -2324,7 +2324,7 @@ def kv4_attention(q: torch.Tensor, pool: torch.Tensor, tables: StepTables, max_n
         k, v, compact = kv4_read(pool, tables.pages, tables.page_start, tables.seq_len, max_len, hd, q.dtype, marked=True, rest=(out, cu[B:]))
         cut = _lookup("attention_tc", "qwb_attn_tc_pieces")[1]
         cut.restype = ctypes.c_longlong
-        tiles, pieces = divmod(cut(T, B, max_new, max_len, Hq, Hkv, hd, window), 2 ** 32)
+        tiles, pieces = divmod(cut(T, B, operator.index(max_new), operator.index(max_len), Hq, Hkv, hd, operator.index(window)), 2 ** 32)
         if pieces > 1:
             scratch = _empty((T * Hq * pieces * (hd + 2),), dtype=torch.float32, device=q.device)
             _call("attention_tc", "qwb_attn_tc_prefill_pieces", _ptr(q), _ptr(k), _ptr(v), _ptr(compact), _ptr(cu), _ptr(pos0), _ptr(tok_seq), _ptr(out),

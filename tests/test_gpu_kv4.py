@@ -434,3 +434,31 @@ def test_store_and_read_refusals():
         ops.kv4_read(pool, s, s, s, 64, 64, F32)
     with pytest.raises(KernelError, match="does not hold"):
         ops.kv4_read(pool, s, ints([0, 1]), s, 64, 128, F32)
+
+
+def test_calls_through_ctypes_and_with_other_whole_numbers_give_the_same_bits(monkeypatch):
+    rng = np.random.default_rng(3)
+    B, Hq, Hkv, hd = 3, 8, 2, 64
+    pos0, n_new, start = ints([100, 0, 63]), ints([2, 1, 3]), ints([0, 2, 3, 5])
+    qkv = torch.from_numpy(rng.standard_normal((6, (Hq + 2 * Hkv) * hd)).astype(np.float32)).to(DEV)
+    weight, angle = torch.rand(hd, device=DEV) + 0.5, torch.rand(6, hd // 2, device=DEV)
+    logits = torch.from_numpy(rng.standard_normal((5, 3000)).astype(np.float32)).to(DEV)
+
+    def step(whole):
+        t = ops.step_tables(ints([4, 1, 0, 2, 3]), start, pos0, n_new, whole(6), whole(2))
+        pool = torch.zeros(5, Hkv, ops.kv4_page_bytes(hd), dtype=torch.uint8, device=DEV)
+        q = ops.kv4_store(qkv, weight, weight, angle.cos(), angle.sin(), t.slot_map, pool, whole(Hq), whole(Hkv), whole(hd), whole(hd), np.float32(1e-6), BF)
+        k, v, table = ops.kv4_read(pool, t.pages, t.page_start, t.seq_len, whole(102), whole(hd), F32)
+        outs = [ops.kv4_attention(x, pool, t, whole(3), whole(102), np.float32(0.1), whole(0), impl=impl)
+                for x, impl in ((q, "rows"), (q, "read"), (q, "auto"), (q, "plain"), (q.float(), "auto"))]
+        return [x for x in t if x is not None] + [q, pool, k, v, table] + outs + list(ops.token_logprobs(logits, ints([0, 1, 2, 3, 4]), top=5))
+
+    first, host = step(int), ops._HOST
+    monkeypatch.setattr(ops, "_host_wanted", False)
+    ops._bind_host(None)
+    try:
+        plain = step(int)
+    finally:
+        ops._bind_host(host)
+    for other in (plain, step(np.int64)):
+        assert len(first) == len(other) and all(torch.equal(a, b) for a, b in zip(first, other))

@@ -1,4 +1,6 @@
 """The 4-bit cache's format and the plain implementations that the GPU tests compare with (CPU)."""
+import ctypes
+
 import numpy as np
 import pytest
 import torch
@@ -104,6 +106,32 @@ def test_here():
         module.here()
     with pytest.raises(TypeError):
         module.here("0", t)
+
+
+def test_ready():
+    module = build.host_calls()
+    if module is None:
+        pytest.skip("no native module")
+    t = torch.zeros(2)
+    assert module.ready() == -1 and module.ready(None, None, None) == -1 and module.ready(t, torch.float32, 1) == -1 and module.ready(3, None, None) == -1
+    for args in [(t,), (t, torch.float32), (0, t, torch.float32, 1)]:
+        with pytest.raises(TypeError):
+            module.ready(*args)
+
+
+def test_arguments_as_they_are(monkeypatch):
+    """What goes natively as it is goes through ctypes as objects: the types that the launchers take."""
+    t = torch.zeros(3)
+    monkeypatch.setattr(ops, "_HOST", None)
+    seen = []
+    monkeypatch.setattr(ops, "_call", lambda module, fn, *args, kernels=1: seen.append((module, fn, kernels, args)))
+    ops._run("m", "f", t, None, 7, np.int64(-3), True, 0.5, "the stream", kernels=2)
+    (module, fn, kernels, args), = seen
+    assert (module, fn, kernels) == ("m", "f", 2) and args[-1] == "the stream"
+    assert [type(a) for a in args[:-1]] == [ctypes.c_void_p] * 2 + [ctypes.c_int] * 3 + [ctypes.c_float]
+    assert [a.value for a in args[:-1]] == [t.data_ptr(), None, 7, -3, 1, 0.5]
+    with pytest.raises(TypeError):
+        ops._run("m", "f", "no number", None)
 
 
 def test_a_tensor_of_another_device_is_refused(monkeypatch):
