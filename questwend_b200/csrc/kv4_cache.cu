@@ -113,7 +113,7 @@ kv4_store_kernel(const float* __restrict__ qkv, const float* __restrict__ q_weig
 // nearer to the border of two codes than its error can be, or a step nearer to the border of two roundings (about one head in 220), sends
 // its head through 64 bits.  A step of 4,096 tokens of 32 + 2 x 8 heads: a warp a head 130 us, with 64 bits for
 // every key 45, so 34 with the next head on its way in registers and 29 (4.8 TB/s) with two by cp.async; what is left is latency and 3.5 waves
-// of blocks: 16,384 tokens run at 5.7 TB/s.  (Fewer instructions for codes and errors, 16 % of them, changed nothing before that.)
+// of blocks: 16,384 tokens run at 5.7 TB/s.
 //
 // Errors of a key in 32 bits, u = 2^-24: the sum of squares 8 + 4 additions, the mean and eps 1, halved by the root; the inverse root
 // 4 (2 units of 2^-23): 11 u; times the weight and the number 2 u; the rotation's products and sum 2 u: of p c - r s it is 15 u (|p c| + |r s|)
