@@ -524,10 +524,11 @@ extern "C" int qwb_kv4_read(const unsigned char* pool, const int* pages, const i
         return qwb_fail(QWB_ERR_ARG, "kv4_read: rows of %d bytes", row_bytes);
     const Kv4ReadArgs args = {pool, pages, page_start, seq_len, rows_used, table, (uint4*)rows_out, B, width, pool_pages, Hkv, hd, marked, rows, row_bytes};
     const dim3 grid(P, Hkv);
-    if (dtype == QWB_DT_F32) qwb_launch(kv4_read_kernel<float>, grid, 256, 0, stream, args, (float*)k_out, (float*)v_out);
+    // early: its blocks wait at their beginning, its launch does not; one token's write and read 4.7 -> 4.1 us
+    if (dtype == QWB_DT_F32) qwb_launch_early(kv4_read_kernel<float>, grid, 256, 0, stream, args, (float*)k_out, (float*)v_out);
     else if (dtype != QWB_DT_BF16) return qwb_fail(QWB_ERR_ARG, "kv4_read: unknown dtype %d", dtype);
-    else if (hd == 128) qwb_launch(kv4_read_fast_kernel<128>, grid, 256, 0, stream, args, (bf16*)k_out, (bf16*)v_out);
-    else if (hd == 64) qwb_launch(kv4_read_fast_kernel<64>, grid, 256, 0, stream, args, (bf16*)k_out, (bf16*)v_out);
-    else qwb_launch(kv4_read_kernel<bf16>, grid, 256, 0, stream, args, (bf16*)k_out, (bf16*)v_out);
+    else if (hd == 128) qwb_launch_early(kv4_read_fast_kernel<128>, grid, 256, 0, stream, args, (bf16*)k_out, (bf16*)v_out);
+    else if (hd == 64) qwb_launch_early(kv4_read_fast_kernel<64>, grid, 256, 0, stream, args, (bf16*)k_out, (bf16*)v_out);
+    else qwb_launch_early(kv4_read_kernel<bf16>, grid, 256, 0, stream, args, (bf16*)k_out, (bf16*)v_out);
     return qwb_check_launch("kv4_read");
 }

@@ -2325,15 +2325,9 @@ def kv4_attention(q: torch.Tensor, pool: torch.Tensor, tables: StepTables, max_n
         cut = _lookup("attention_tc", "qwb_attn_tc_pieces")[1]
         cut.restype = ctypes.c_longlong
         tiles, pieces = divmod(cut(T, B, operator.index(max_new), operator.index(max_len), Hq, Hkv, hd, operator.index(window)), 2 ** 32)
-        if pieces > 1:
-            scratch = _empty((T * Hq * pieces * (hd + 2),), dtype=torch.float32, device=q.device)
-            _call("attention_tc", "qwb_attn_tc_prefill_pieces", _ptr(q), _ptr(k), _ptr(v), _ptr(compact), _ptr(cu), _ptr(pos0), _ptr(tok_seq), _ptr(out),
-                  _ptr(scratch), _i(B), _i(T), _i(max_new), _i(k.shape[0]), _i(Hq), _i(Hkv), _i(hd), _i(compact.shape[1]), _f(scale), _i(window), _i(pieces),
-                  _i(tiles), _ptr(gemm_tc_error_word(q.device)), _stream(), kernels=2)
-            return out
-        _call("attention_tc", "qwb_attn_tc_prefill", _ptr(q), _ptr(k), _ptr(v), _ptr(compact), _ptr(cu), _ptr(pos0), _ptr(out), _i(B), _i(T), _i(max_new),
-              _i(k.shape[0]), _i(Hq), _i(Hkv), _i(hd), _i(hd), _i(PAGE_SIZE), _i(compact.shape[1]), _f(scale), _i(window), _i(0), _ptr(None), _ptr(None),
-              _ptr(gemm_tc_error_word(q.device)), _stream())
+        scratch = _empty((T * Hq * pieces * (hd + 2),), dtype=torch.float32, device=q.device) if pieces > 1 else None
+        _run("attention_tc", "qwb_attn_tc_prefill_pieces", q, k, v, compact, cu, pos0, tok_seq, out, scratch, B, T, max_new, k.shape[0], Hq, Hkv, hd,
+             compact.shape[1], float(scale), window, pieces, tiles, gemm_tc_error_word(q.device), _stream(), kernels=1 if scratch is None else 2)
         return out
     _run("attention_kv4", "qwb_kv4_attn_plain", q, pool, table, tok_seq, tok_pos, out, _dt(dtype), T, B, n_pages, Hq, Hkv, hd, width, float(scale), window, _stream())
     return out
