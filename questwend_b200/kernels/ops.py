@@ -34,12 +34,13 @@ def _dt(t: torch.dtype) -> int:
 
 
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+_device_number = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)      # a quarter of current_device()'s time, once CUDA is up
 
 
 def _stream():
     """The current stream of the current device (also inside a graph capture, which runs on a stream of its own)."""
     if _raw_stream is not None:                      # the handle itself: a tenth of the cost of making a Stream object
-        return _address(_raw_stream(torch.cuda.current_device()))
+        return _address(_raw_stream(_device_number() if torch.cuda.is_initialized() else torch.cuda.current_device()))
     return _address(torch.cuda.current_stream().cuda_stream)
 
 
@@ -106,7 +107,7 @@ def _ready(*checks) -> bool:
     if _HOST is None:
         return False
     device = _HOST.ready(*checks)
-    return device >= 0 and device == torch.cuda.current_device()
+    return device >= 0 and device == _device_number()
 
 
 def _column_gate(what: str, gate: torch.Tensor | None, col0: int, T: int, H: int):
@@ -141,6 +142,10 @@ def _lookup(module: str, fn: str):
     return entry
 
 
+def _refusal(name: tuple[str, str], rc: int) -> KernelError:
+    return KernelError(_FUNCTIONS[name][0].qwb_last_error().decode("utf-8", "replace") or f"{name[1]} failed with code {rc}")
+
+
 def _call(module: str, fn: str, *args, kernels: int = 1):
     name = module, fn
     if _HOST is None:
@@ -153,7 +158,7 @@ def _call(module: str, fn: str, *args, kernels: int = 1):
         rc = _HOST.call(address, *args)
     LAUNCHES[0] += kernels
     if rc != 0:
-        raise KernelError(_FUNCTIONS[name][0].qwb_last_error().decode("utf-8", "replace") or f"{fn} failed with code {rc}")
+        raise _refusal(name, rc)
 
 
 def _plain_argument(x):
@@ -166,8 +171,16 @@ def _run(module: str, fn: str, *args, kernels: int = 1):
     """``_call`` with the arguments as they are: tensors (None: a null pointer), whole numbers, floats, and the stream last, as ``_stream()``."""
     if _HOST is None:
         stream = args[-1]
-        args = [_plain_argument(x) for x in args[:-1]] + [stream]
-    _call(module, fn, *args, kernels=kernels)
+        return _call(module, fn, *[_plain_argument(x) for x in args[:-1]], stream, kernels=kernels)
+    name = module, fn
+    address = _ADDRESSES.get(name)
+    if address is None:
+        _lookup(module, fn)
+        address = _ADDRESSES[name]
+    rc = _HOST.call(address, *args)
+    LAUNCHES[0] += kernels
+    if rc != 0:
+        raise _refusal(name, rc)
 
 
 def _ask(module: str, fn: str, *args) -> int:
