@@ -10,7 +10,7 @@
 //                                         multiple of 256 bytes (six of them 3 us, one after the other 7)
 //     here(device, *tensors)              whether all tensors (or None) lie on CUDA device number `device`
 //     ready(tensor, dtype, dimensions, ...)           the number of the CUDA device on which all tensors (or None) lie, each as `fits` says; -1: not
-//                                         so (seven of them 0.4 us, a call of `fits` each and one of `here` 2)
+//                                         so (seven of them 0.4 us, a call of `fits` each and one of `here` 1.1)
 //     same(x)                             x
 //     fill(array, numbers)                a list's whole numbers into a contiguous array of as many 32-bit ones; False where the list holds anything
 //                                         else, or a number that does not fit: the array then holds any part of them
