@@ -53,7 +53,7 @@ struct AtSmem {
 template <int HD, int VD, bool SHAPED, bool PIECES = false>
 __global__ void __launch_bounds__(AT_THREADS, 2)
 attn_tc_prefill_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
-                       const __grid_constant__ CUtensorMap map_v, const int* __restrict__ page_table,
+                       const __grid_constant__ CUtensorMap map_v, const int* page_table,
                        const int* __restrict__ cu_seqlens, const int* __restrict__ pos0, bf16* __restrict__ out, int Hq, int Hkv,
                        int vd, int table_width, float scale, int window, int chunk, int G, int* error,
                        const float* __restrict__ slopes, const float* __restrict__ sinks, int pieces, int piece_tiles, float* __restrict__ part_o,
@@ -140,7 +140,8 @@ attn_tc_prefill_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
                 uint64_t* empty = is_k ? &k_empty[s] : &v_empty[s];
                 uint64_t* full = is_k ? &k_full[s] : &v_full[s];
                 if (j >= AT_KV_STAGES && !at_wait(empty, ((j / AT_KV_STAGES) - 1) & 1)) return false;
-                const int row0 = (pages[tile_first + j] * Hkv + kvh) * AT_KEYS;        // the (page, head) block's first row
+                // the (page, head) block's first row; the table may have been written by the kernel that this one was launched under
+                const int row0 = (__ldcg(pages + tile_first + j) * Hkv + kvh) * AT_KEYS;
                 const uint32_t bytes = is_k ? K_BYTES : V_BYTES;
                 unsigned char* dst = (is_k ? k_tiles : v_tiles) + (size_t)s * bytes;
                 at_expect_tx(full, bytes);
@@ -497,7 +498,8 @@ extern "C" long long qwb_attn_tc_pieces(int T, int B, int max_new, int max_len, 
 }
 
 // qwb_attn_tc_prefill without chunks, biases and sinks, heads of 64 or 128, behind the kernel that writes its pages and their table (kv4_cache.cu), under
-// whose tail it is launched: what it reads before that kernel has ended (cu_seqlens, pos0) has to be older than it.  A prompt of 128 tokens 9.0 -> 7.8 us with
+// whose tail it is launched: what it reads before that kernel has ended, or through the read-only path (cu_seqlens, pos0), has to be older than it; pages
+// and their table are what that kernel writes, and are read behind the wait and at L2.  A prompt of 128 tokens 9.0 -> 7.8 us with
 // it, three of 900 behind 5,000 95 -> 90.  The keys are cut into `pieces` of `piece_tiles` tiles of 64; with more than one tok_seq [T] says each token's
 // sequence, or -1, and scratch holds T * Hq * pieces * (hd + 2) floats.
 extern "C" int qwb_attn_tc_prefill_pieces(const void* q, const void* k_pool, const void* v_pool, const int* page_table, const int* cu_seqlens,

@@ -1,0 +1,30 @@
+"""What a kernel that starts under the tail of the one before it may do (read from the sources: a race does not show itself in every run)."""
+import os
+import re
+
+CSRC = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "questwend_b200", "csrc")
+
+
+def kernel(file, name):
+    """(parameters, body) of a kernel."""
+    with open(os.path.join(CSRC, file)) as f:
+        text = f.read()
+    at = re.search(r"__global__[^;{]*?\b" + name + r"\(", text).end()
+    end, depth = at, 1
+    while depth:
+        depth += {"(": 1, ")": -1}.get(text[end], 0)
+        end += 1
+    parameters, begin, depth = text[at:end - 1], text.index("{", end), 0
+    for i in range(begin, len(text)):
+        depth += {"{": 1, "}": -1}.get(text[i], 0)
+        if depth == 0:
+            return parameters, text[begin + 1:i]
+
+
+def test_the_prompt_kernel_reads_the_table_that_the_kernel_before_it_writes_at_l2():
+    """``kv4_read`` writes the page table while the prompt kernel's blocks are already there: not through the read-only path."""
+    parameters, body = kernel("attention_tc.cu", "attn_tc_prefill_kernel")
+    declared, = [p for p in parameters.split(",") if p.split()[-1] == "page_table"]
+    assert "__restrict__" not in declared
+    reads = re.findall(r"(\w*\(?)pages(?: \+|\[)", body)
+    assert reads and all(r == "__ldcg(" for r in reads)
