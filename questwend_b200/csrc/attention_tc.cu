@@ -64,8 +64,10 @@ attn_tc_prefill_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
     // The tiles need 1024-byte alignment (128-byte swizzle).  No padding to reach it: at head size 128 the block's
     // 113 KB then leave room for a second block on the SM, whose products run while this block's softmax does.
     extern __shared__ __align__(1024) unsigned char smem_raw[];
+    // Whoever returns early waits first: a grid that ended before the one it was launched under would let the next kernel begin beside that one.
     if (at_smem(smem_raw) & 1023u) {                      // never seen; refuse rather than compute with a wrong layout
         if (threadIdx.x == 0) atomicExch(error, 7);
+        pdl_wait();
         return;
     }
     unsigned char* q_tile = smem_raw;
@@ -89,7 +91,10 @@ attn_tc_prefill_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
     // Blocks start in the order of blockIdx.x, then y: the key/value head is x, so that the longest blocks of every head
     // start before any short one.
     const int q0 = (int)(gridDim.y - 1 - blockIdx.y) * tok_per_block;
-    if (q0 >= n_new) return;
+    if (q0 >= n_new) {
+        pdl_wait();
+        return;
+    }
     const int p0 = pos0[b];
     const int len = p0 + n_new;
     const int last_tok = min(n_new, q0 + tok_per_block) - 1;
@@ -98,7 +103,10 @@ attn_tc_prefill_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
     const int k_first = chunk > 0 ? ((p0 + q0) / chunk) * chunk : (window > 0 ? max(0, p0 + q0 - window + 1) : 0);
     const int tile_first = k_first / AT_KEYS + (PIECES ? piece * piece_tiles : 0);
     const int tile_last = PIECES ? min(k_last / AT_KEYS, tile_first + piece_tiles - 1) : k_last / AT_KEYS;
-    if (PIECES && tile_first > tile_last) return;
+    if (PIECES && tile_first > tile_last) {
+        pdl_wait();
+        return;
+    }
     const int n_tiles = tile_last - tile_first + 1;
     const int* pages = page_table + (size_t)b * table_width;
 

@@ -28,3 +28,11 @@ def test_the_prompt_kernel_reads_the_table_that_the_kernel_before_it_writes_at_l
     assert "__restrict__" not in declared
     reads = re.findall(r"(\w*\(?)pages(?: \+|\[)", body)
     assert reads and all(r == "__ldcg(" for r in reads)
+
+
+def test_a_block_of_the_prompt_kernel_that_has_nothing_to_do_waits_all_the_same():
+    """In a step that brings nothing all blocks are such: the grid must not end before the kernel that it was launched under."""
+    _, body = kernel("attention_tc.cu", "attn_tc_prefill_kernel")
+    before = body[:body.index("pdl_launch_dependents()")]
+    returns = [m.start() for m in re.finditer(r"\breturn;", before)]
+    assert len(returns) >= 3 and all("pdl_wait();" in before[before.rindex("{", 0, at):at] for at in returns)

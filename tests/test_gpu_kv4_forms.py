@@ -29,3 +29,17 @@ def test_calls_one_behind_the_other_read_their_own_pages(hd, lens, n_new):
         assert (want[-1].float() - ops.kv4_attention(*step, impl="rows").float()).abs().max() < 0.1
     got = [ops.kv4_attention(*steps[i % 2], impl="read") for i in range(40)]
     assert all(torch.equal(out, want[i % 2]) for i, out in enumerate(got))
+
+
+@pytest.mark.parametrize("hd", [64, 128])
+def test_a_step_that_brings_nothing(hd):
+    """Padding alone, as pages read back as well: zeros, and what comes behind the call finds them and its own memory."""
+    pool, order, start, _, _ = _cache(22, [300, 70], 2, hd)
+    t = _tables(order, start, [300, 70], [0, 0], behind=40)
+    q = torch.ones(40, 8, hd, dtype=BF, device=DEV)
+    for impl in forms(q):
+        for _ in range(20):
+            out = ops.kv4_attention(q, pool, t, 40, 300, 0.1, impl=impl)
+            behind = out + 1
+            again = torch.full_like(out, 3.0)
+            assert (out == 0).all() and (behind == 1).all() and (again == 3).all()
