@@ -102,9 +102,17 @@ attn_tc_prefill_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
     // with `chunk` > 0 a query sees only the keys of its own block of `chunk` positions, counted from position 0
     const int k_first = chunk > 0 ? ((p0 + q0) / chunk) * chunk : (window > 0 ? max(0, p0 + q0 - window + 1) : 0);
     const int tile_first = k_first / AT_KEYS + (PIECES ? piece * piece_tiles : 0);
-    const int tile_last = PIECES ? min(k_last / AT_KEYS, tile_first + piece_tiles - 1) : k_last / AT_KEYS;
-    if (PIECES && tile_first > tile_last) {
+    // a sequence longer than its row of the table: keys that this does not name are not seen
+    const int tile_end = min(k_last / AT_KEYS, table_width - 1), tile_last = PIECES ? min(tile_end, tile_first + piece_tiles - 1) : tile_end;
+    if (tile_first > tile_last) {
         pdl_wait();
+        if (!PIECES) {                                      // the rows see nothing: zeros
+            const int run = G * vd / 8;                     // of a token, 16 bytes each
+            for (int i = threadIdx.x; i < (last_tok - q0 + 1) * run; i += AT_THREADS) {
+                const int tok = i / run;
+                *reinterpret_cast<uint4*>(out + ((size_t)(t0 + q0 + tok) * Hq + kvh * G) * vd + 8 * (i - tok * run)) = make_uint4(0, 0, 0, 0);
+            }
+        }
         return;
     }
     const int n_tiles = tile_last - tile_first + 1;
@@ -363,7 +371,8 @@ attn_tc_prefill_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
 template <int VD>
 __global__ void __launch_bounds__(256)
 attn_tc_join_kernel(const float* __restrict__ part_o, const float* __restrict__ part_ml, const int* __restrict__ tok_seq, const int* __restrict__ cu_seqlens,
-                    const int* __restrict__ pos0, bf16* __restrict__ out, int rows, int B, int Hq, int tok_per_block, int window, int pieces, int piece_tiles) {
+                    const int* __restrict__ pos0, bf16* __restrict__ out, int rows, int B, int Hq, int tok_per_block, int window, int table_width, int pieces,
+                    int piece_tiles) {
     pdl_wait();
     pdl_launch_dependents();
     const int lane = threadIdx.x & 31;
@@ -373,8 +382,8 @@ attn_tc_join_kernel(const float* __restrict__ part_o, const float* __restrict__ 
     if (b < 0 || b >= B) return;
     // the tiles that the row's block went over, as it found them
     const int t0 = cu_seqlens[b], n_new = cu_seqlens[b + 1] - t0, q0 = (t - t0) / tok_per_block * tok_per_block, p0 = pos0[b];
-    const int first = (window > 0 ? max(0, p0 + q0 - window + 1) : 0) / AT_KEYS, last = (p0 + min(n_new, q0 + tok_per_block) - 1) / AT_KEYS;
-    const int count = min((last - first) / piece_tiles + 1, pieces);
+    const int first = (window > 0 ? max(0, p0 + q0 - window + 1) : 0) / AT_KEYS, last = min((p0 + min(n_new, q0 + tok_per_block) - 1) / AT_KEYS, table_width - 1);
+    const int count = last < first ? 0 : min((last - first) / piece_tiles + 1, pieces);
     const float* ml = part_ml + row * pieces * 2;
     float top = -INFINITY;
     for (int i = lane; i < count; i += 32) top = fmaxf(top, ml[2 * i]);
@@ -452,7 +461,7 @@ static int launch_attn_tc(const void* q, const void* k_pool, const void* v_pool,
         if constexpr (HD == VD) {
             if (int rc = go(attn_tc_prefill_kernel<HD, VD, false, true>)) return rc;
             qwb_launch(attn_tc_join_kernel<VD>, dim3((unsigned)(((long long)T * Hq + 7) / 8)), 256, 0, stream, scratch, part_ml, tok_seq, cu_seqlens, pos0, (bf16*)out,
-                       T * Hq, B, Hq, tok_per_block, window, pieces, piece_tiles);
+                       T * Hq, B, Hq, tok_per_block, window, table_width, pieces, piece_tiles);
             return qwb_check_launch("attn_tc_prefill_pieces");
         }
     }

@@ -2288,7 +2288,8 @@ def kv4_attention(q: torch.Tensor, pool: torch.Tensor, tables: StepTables, max_n
                   impl: str = "auto") -> torch.Tensor:
     """Causal attention of a step's tokens over the cache in 4 bits (their own rows written before).  ``q`` [T, Hq, hd] float32
     or bfloat16; ``max_new`` and ``max_len`` bound what a sequence brings and holds; with ``window`` > 0 a query sees the last ``window``
-    keys, its own among them.  Returns [T, Hq * hd] in q's type, zeros for a token of no sequence.
+    keys, its own among them.  A key behind what the page table's columns name is not seen (of a sequence that holds more than ``max_len``, whether
+    keys behind that are is left open).  Returns [T, Hq * hd] in q's type, zeros for a token of no sequence.
 
     ``impl``: "rows" (bfloat16, heads of 64 or 128: codes to tensor-core fragments, a sequence's keys cut into runs; for few new tokens), "read"
     (the same sizes, groups of up to 64 heads, ``tables.pages`` given: the step's pages as bfloat16 once, then the tcgen05 prompt kernel), "plain"

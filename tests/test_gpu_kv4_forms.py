@@ -43,3 +43,34 @@ def test_a_step_that_brings_nothing(hd):
             behind = out + 1
             again = torch.full_like(out, 3.0)
             assert (out == 0).all() and (behind == 1).all() and (again == 3).all()
+
+
+@pytest.mark.parametrize("hd,group", [(128, 4), (64, 3)])
+@pytest.mark.parametrize("window", [0, 50, 700])
+@pytest.mark.parametrize("n_new", [1, 90])
+def test_a_sequence_longer_than_its_row_of_the_page_table(hd, group, window, n_new):
+    """Keys that the table does not name are not seen; rows that then see nothing are zeros.  The same in every form."""
+    lens, pos0, width = [900, 130], [900 - n_new, 129], 3
+    pool, order, start, seqs, rng = _cache(23, lens, 2, hd)
+    q = torch.from_numpy(rng.standard_normal((n_new + 1, 2 * group, hd))).to(BF).to(DEV)
+    t = _tables(order, start, pos0, [n_new, 1], width=width)
+    _check(pool, t, [[x[:64 * width] for x in s] for s in seqs], q, pos0, [n_new, 1], 900, hd ** -0.5, window)
+    for most in (192, 130, 64, 1):                        # a bound that does not hold: as many pages as it says are read, and no more
+        got = f64(ops.kv4_attention(q, pool, t, n_new, most, hd ** -0.5, window=window, impl="read")).reshape(n_new + 1, 2 * group, hd)
+        pages = -(-most // 64)
+        for b, (at, n) in enumerate(((0, n_new), (n_new, 1))):
+            out, mass, big = pk.attention(f64(q[at:at + n]), *(x[:64 * pages] for x in seqs[b]), [pos0[b] + i for i in range(n)], hd ** -0.5, window)
+            assert (np.abs(got[at:at + n] - out) <= tolerance(BF, hd, mass, big, out, 192)).all(), (most, b)
+
+
+def test_a_sequence_longer_than_the_table_in_pieces():
+    """Few tokens behind a long context, whose keys the prompt kernel cuts into pieces: the join knows of the table's end too."""
+    hd, L, n_new = 128, 6000, 12
+    pool, order, start, seqs, rng = _cache(24, [L], 1, hd)
+    q = torch.from_numpy(rng.standard_normal((n_new, 4, hd))).to(BF).to(DEV)
+    for width, window in ((40, 0), (40, 4000), (40, 100), (93, 0)):
+        t = _tables(order, start, [L - n_new], [n_new], width=width)
+        before = ops.LAUNCHES[0]
+        ops.kv4_attention(q, pool, t, n_new, L, hd ** -0.5, window=window, impl="read")
+        assert ops.LAUNCHES[0] - before == (2 if window == 100 else 3)
+        _check(pool, t, [[x[:64 * width] for x in seqs[0]]], q, [L - n_new], [n_new], L, hd ** -0.5, window)
