@@ -2319,6 +2319,8 @@ def kv4_attention(q: torch.Tensor, pool: torch.Tensor, tables: StepTables, max_n
     fits = dtype == torch.bfloat16 and hd in (64, 128)
     listed = tables.pages.numel() if fits and group <= 64 and tables.pages is not None and tables.page_start is not None else 0
     reads = listed > 0
+    if reads and (tables.seq_len is None or tables.seq_len.numel() != B or tables.page_start.numel() != B + 1):
+        raise KernelError(f"kv4_attention: a list of pages goes with lengths and page starts of all {B} sequences")
     plan = 0
     if fits and impl != "plain":
         plan = _ask("attention_kv4", "qwb_kv4_plan", max_len, max_new, window, width, B, Hq, Hkv, hd, T, listed)

@@ -74,3 +74,15 @@ def test_a_sequence_longer_than_the_table_in_pieces():
         ops.kv4_attention(q, pool, t, n_new, L, hd ** -0.5, window=window, impl="read")
         assert ops.LAUNCHES[0] - before == (2 if window == 100 else 3)
         _check(pool, t, [[x[:64 * width] for x in seqs[0]]], q, [L - n_new], [n_new], L, hd ** -0.5, window)
+
+
+@pytest.mark.parametrize("impl", ["read", "auto"])
+def test_lengths_of_fewer_sequences_are_refused(impl):
+    """The table of the pages that are read back has a row for each length: with fewer than sequences the others' rows would lie behind it."""
+    pool, order, start, _, _ = _cache(25, [200, 100], 2, 64)
+    t = _tables(order, start, [0, 0], [200, 100])
+    q = torch.zeros(300, 4, 64, dtype=BF, device=DEV)
+    for more in ({"seq_len": ints([200]), "page_start": ints(start[:2])}, {"seq_len": ints([200])}, {"seq_len": None},
+                 {"seq_len": ints([200, 100, 0]), "page_start": ints(start + start[-1:])}):
+        with pytest.raises(KernelError, match="2 sequences"):
+            ops.kv4_attention(q, pool, t._replace(**more), 200, 200, 0.1, impl=impl)
