@@ -54,7 +54,7 @@ template <int HD, int VD, bool SHAPED, bool PIECES = false>
 __global__ void __launch_bounds__(AT_THREADS, 2)
 attn_tc_prefill_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
                        const __grid_constant__ CUtensorMap map_v, const int* page_table,
-                       const int* __restrict__ cu_seqlens, const int* __restrict__ pos0, bf16* __restrict__ out, int Hq, int Hkv,
+                       const int* __restrict__ cu_seqlens, const int* __restrict__ pos0, bf16* __restrict__ out, int T, int Hq, int Hkv,
                        int vd, int table_width, float scale, int window, int chunk, int G, int* error,
                        const float* __restrict__ slopes, const float* __restrict__ sinks, int pieces, int piece_tiles, float* __restrict__ part_o,
                        float* __restrict__ part_ml) {
@@ -86,7 +86,7 @@ attn_tc_prefill_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int b = PIECES ? blockIdx.z / pieces : blockIdx.z, piece = PIECES ? blockIdx.z - b * pieces : 0, kvh = blockIdx.x;
     const int tok_per_block = AT_ROWS / G;
-    const int t0 = cu_seqlens[b], n_new = cu_seqlens[b + 1] - t0;
+    const int t0 = cu_seqlens[b], n_new = min(cu_seqlens[b + 1], T) - t0;             // counts beyond the step's T tokens: nothing is written there
     // The last tokens see the most keys: their blocks go first, so that the long blocks do not form the tail of the launch.
     // Blocks start in the order of blockIdx.x, then y: the key/value head is x, so that the longest blocks of every head
     // start before any short one.
@@ -381,7 +381,7 @@ attn_tc_join_kernel(const float* __restrict__ part_o, const float* __restrict__ 
     const int t = (int)(row / Hq), b = tok_seq[t];
     if (b < 0 || b >= B) return;
     // the tiles that the row's block went over, as it found them
-    const int t0 = cu_seqlens[b], n_new = cu_seqlens[b + 1] - t0, q0 = (t - t0) / tok_per_block * tok_per_block, p0 = pos0[b];
+    const int t0 = cu_seqlens[b], n_new = min(cu_seqlens[b + 1], rows / Hq) - t0, q0 = (t - t0) / tok_per_block * tok_per_block, p0 = pos0[b];
     const int first = (window > 0 ? max(0, p0 + q0 - window + 1) : 0) / AT_KEYS, last = min((p0 + min(n_new, q0 + tok_per_block) - 1) / AT_KEYS, table_width - 1);
     const int count = last < first ? 0 : min((last - first) / piece_tiles + 1, pieces);
     const float* ml = part_ml + row * pieces * 2;
@@ -453,7 +453,7 @@ static int launch_attn_tc(const void* q, const void* k_pool, const void* v_pool,
         cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
         if (e != cudaSuccess) return qwb_fail(QWB_ERR_CUDA, "attn_tc_prefill: %s", cudaGetErrorString(e));
         e = qwb_launch_attr(early ? qwb_pdl_mode() >= 1 : qwb_pdl_mode() == 2, kernel, grid, AT_THREADS, smem, stream, map_q, map_k, map_v, page_table, cu_seqlens, pos0,
-                       (bf16*)out, Hq, Hkv, vd, table_width, scale, window, chunk, G, error, slopes, sinks, pieces, piece_tiles, scratch, part_ml);
+                       (bf16*)out, T, Hq, Hkv, vd, table_width, scale, window, chunk, G, error, slopes, sinks, pieces, piece_tiles, scratch, part_ml);
         if (e != cudaSuccess) return qwb_fail(QWB_ERR_CUDA, "attn_tc_prefill: launch failed: %s", cudaGetErrorString(e));
         return qwb_check_launch("attn_tc_prefill");
     };

@@ -86,3 +86,22 @@ def test_lengths_of_fewer_sequences_are_refused(impl):
                  {"seq_len": ints([200, 100, 0]), "page_start": ints(start + start[-1:])}):
         with pytest.raises(KernelError, match="2 sequences"):
             ops.kv4_attention(q, pool, t._replace(**more), 200, 200, 0.1, impl=impl)
+
+
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("lens", [[200, 120], [4000, 60]])
+def test_counts_beyond_the_tokens_that_there_are(hd, lens):
+    """A step that was made for fewer tokens than its sequences bring: the tokens that there are get what they would, nothing is written behind them."""
+    T, new, pos0 = 70, [40, 60], [lens[0] - 40, lens[1] - 60]
+    pool, order, start, seqs, rng = _cache(26, lens, 2, hd)
+    q = torch.from_numpy(rng.standard_normal((100, 4, hd))).to(BF).to(DEV)
+    whole = _tables(order, start, pos0, new)
+    t = ops.step_tables(ints(order), ints(start), ints(pos0), ints(new), T, whole.page_table.shape[1])
+    assert t.cu_seqlens.tolist() == [0, 40, 100]
+    for impl in forms(q):
+        got = ops.kv4_attention(q[:T].contiguous(), pool, t, 60, max(lens), hd ** -0.5, impl=impl)
+        at = 0
+        for b, n in enumerate((40, 30)):
+            out, mass, big = pk.attention(f64(q[at:at + n]), *seqs[b], [pos0[b] + i for i in range(n)], hd ** -0.5)
+            assert (np.abs(f64(got[at:at + n]).reshape(out.shape) - out) <= tolerance(BF, hd, mass, big, out, max(lens))).all(), (impl, b)
+            at += n
