@@ -24,6 +24,8 @@
 // Keys of the last page beyond the sequence's length are masked in S; their V rows are multiplied by P = 0, so the
 // cache must hold finite numbers there (the cache is zeroed when it is made, and later holds only values that were
 // keys and values once).
+#include <type_traits>
+
 #include "common.cuh"
 
 #include "attention_pieces.h"
@@ -50,7 +52,8 @@ struct AtSmem {
 // PIECES: a block takes `piece_tiles` tiles of its rows' keys and leaves its sums, maximum (of scores times log2 e) and denominator to
 // attn_tc_join_kernel, in part_o [T * Hq, pieces, VD] and part_ml [T * Hq, pieces, 2] (with few rows and long contexts a block a row's tile
 // would walk over all keys by itself while most SMs stand idle).
-template <int HD, int VD, bool SHAPED, bool PIECES = false>
+// GAPS: the table may hold pages that are not there (below 0); their keys are not seen.
+template <int HD, int VD, bool SHAPED, bool GAPS = false, bool PIECES = false>
 __global__ void __launch_bounds__(AT_THREADS, 2)
 attn_tc_prefill_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
                        const __grid_constant__ CUtensorMap map_v, const int* page_table,
@@ -157,7 +160,7 @@ attn_tc_prefill_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
                 uint64_t* full = is_k ? &k_full[s] : &v_full[s];
                 if (j >= AT_KV_STAGES && !at_wait(empty, ((j / AT_KV_STAGES) - 1) & 1)) return false;
                 // the (page, head) block's first row; the table may have been written by the kernel that this one was launched under
-                const int row0 = (__ldcg(pages + tile_first + j) * Hkv + kvh) * AT_KEYS;
+                const int page = __ldcg(pages + tile_first + j), row0 = ((GAPS ? max(page, 0) : page) * Hkv + kvh) * AT_KEYS;
                 const uint32_t bytes = is_k ? K_BYTES : V_BYTES;
                 unsigned char* dst = (is_k ? k_tiles : v_tiles) + (size_t)s * bytes;
                 at_expect_tx(full, bytes);
@@ -236,6 +239,15 @@ attn_tc_prefill_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
         const float slope_raw = (SHAPED && slopes && row_ok) ? slopes[head] / scale : 0.f;
         float m_ref = -INFINITY, l = 0.f;                                              // reference maximum (raw score) and sum
         bool ok = true;
+        // A page that is not there is the exception: the loop that looks for it is one of its own (as one more test in the loop of the others three
+        // chunks of 900 behind 5,000 took 93 to 97 us, 92 so and without).
+        bool gaps = false;
+        if (GAPS) {
+            for (int j = lane; j < n_tiles; j += 32) gaps |= __ldcg(pages + tile_first + j) < 0;
+            gaps = __any_sync(0xffffffffu, gaps);
+        }
+        auto walk = [&](auto some_gone) {
+        constexpr bool with_gaps = decltype(some_gone)::value;
         for (int j = 0; j < n_tiles; ++j) {
             ok = at_wait(&s_full[j & 1], (j >> 1) & 1);
             at_fence_after();
@@ -254,7 +266,8 @@ attn_tc_prefill_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
             }
             // a tile that lies wholly inside what this row may see needs no mask
             const int own = chunk > 0 && qp >= 0 ? (qp / chunk) * chunk : 0;                    // the first key of the row's own chunk
-            const bool all_visible = key0 + AT_KEYS - 1 <= qp && key0 + AT_KEYS - 1 < len && (window <= 0 || key0 > qp - window) && key0 >= own;
+            const bool there = !with_gaps || __ldcg(pages + tile_first + j) >= 0;
+            const bool all_visible = key0 + AT_KEYS - 1 <= qp && key0 + AT_KEYS - 1 < len && (window <= 0 || key0 > qp - window) && key0 >= own && there;
             float mx = -INFINITY;
             if (all_visible) {
 #pragma unroll
@@ -265,7 +278,7 @@ attn_tc_prefill_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
                 // this row sees the tile's keys [first, end): one subtraction and one unsigned comparison per key
                 const int end = min(min(qp, len - 1) - key0 + 1, AT_KEYS);
                 const int first = max(window > 0 ? max(qp - window + 1 - key0, 0) : 0, own - key0);
-                const unsigned span = end > first ? (unsigned)(end - first) : 0u;
+                const unsigned span = end > first && there ? (unsigned)(end - first) : 0u;
 #pragma unroll
                 for (int h = 0; h < 2; ++h)
 #pragma unroll
@@ -315,6 +328,9 @@ attn_tc_prefill_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
             __syncwarp();
             if (lane == 0) at_arrive(p_full);
         }
+        };
+        if (GAPS && gaps) walk(std::true_type());
+        else walk(std::false_type());
         if (ok) {
             ok = at_wait(o_full, (n_tiles - 1) & 1);
             at_fence_after();
@@ -459,11 +475,14 @@ static int launch_attn_tc(const void* q, const void* k_pool, const void* v_pool,
     };
     if (pieces > 1) {
         if constexpr (HD == VD) {
-            if (int rc = go(attn_tc_prefill_kernel<HD, VD, false, true>)) return rc;
+            if (int rc = go(attn_tc_prefill_kernel<HD, VD, false, true, true>)) return rc;
             qwb_launch(attn_tc_join_kernel<VD>, dim3((unsigned)(((long long)T * Hq + 7) / 8)), 256, 0, stream, scratch, part_ml, tok_seq, cu_seqlens, pos0, (bf16*)out,
                        T * Hq, B, Hq, tok_per_block, window, table_width, pieces, piece_tiles);
             return qwb_check_launch("attn_tc_prefill_pieces");
         }
+    }
+    if (early) {
+        if constexpr (HD == VD) return go(attn_tc_prefill_kernel<HD, VD, false, true>);
     }
     if (slopes || sinks) {
         if constexpr (HD == VD) return go(attn_tc_prefill_kernel<HD, VD, true>);
@@ -516,7 +535,7 @@ extern "C" long long qwb_attn_tc_pieces(int T, int B, int max_new, int max_len, 
 
 // qwb_attn_tc_prefill without chunks, biases and sinks, heads of 64 or 128, behind the kernel that writes its pages and their table (kv4_cache.cu), under
 // whose tail it is launched: what it reads before that kernel has ended, or through the read-only path (cu_seqlens, pos0), has to be older than it; pages
-// and their table are what that kernel writes, and are read behind the wait and at L2.  A prompt of 128 tokens 9.0 -> 7.8 us with
+// and their table (a page below 0: its keys are not seen) are what that kernel writes, and are read behind the wait and at L2.  A prompt of 128 tokens 9.0 -> 7.8 us with
 // it, three of 900 behind 5,000 95 -> 90.  The keys are cut into `pieces` of `piece_tiles` tiles of 64; with more than one tok_seq [T] says each token's
 // sequence, or -1, and scratch holds T * Hq * pieces * (hd + 2) floats.
 extern "C" int qwb_attn_tc_prefill_pieces(const void* q, const void* k_pool, const void* v_pool, const int* page_table, const int* cu_seqlens,

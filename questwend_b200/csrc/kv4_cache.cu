@@ -395,7 +395,8 @@ extern "C" int qwb_kv4_store(const float* qkv, const float* q_weight, const floa
 // sequence's last token are zeros.  A block takes a (page, head), a thread 8 numbers at a time (one 32-bit word of codes).
 // `marked`: a token one of whose values is not finite has values of zero and keys of NaN here, so that a kernel that multiplies
 // what a query does not see by 0 gives NaN to the queries that see it only.
-// The blocks also write the table that names these pages: [B, width], page_start[b] + j or 0; and with `rows_out` they set rows of
+// The blocks also write the table that names these pages: [B, width], page_start[b] + j or 0 where a sequence has none (with `marked` -1, there and where
+// the pool does not have the page: the kernel that takes the table then sees nothing of it); and with `rows_out` they set rows of
 // `row_bytes` (a multiple of 16) behind row `rows_used` of `rows` there to zero (what no sequence of a padded step writes).
 struct Kv4ReadArgs {
     const unsigned char* pool;
@@ -410,7 +411,13 @@ __device__ __forceinline__ const unsigned char* kv4_read_begin(const Kv4ReadArgs
     const long long me = ((long long)head * gridDim.x + entry) * blockDim.x + threadIdx.x, all = (long long)gridDim.x * gridDim.y * blockDim.x;
     for (long long i = me; i < (long long)a.B * a.width; i += all) {
         const int b = (int)(i / a.width), j = (int)(i - (long long)b * a.width), at = a.page_start[b] + j;
-        a.table[i] = at >= 0 && at < a.page_start[b + 1] && at < (int)gridDim.x ? at : 0;
+        const bool listed = at >= 0 && at < a.page_start[b + 1] && at < (int)gridDim.x;
+        int entry = listed ? at : 0;
+        if (a.marked) {
+            const int page = listed ? a.pages[at] : -1;
+            if (page < 0 || page >= a.pool_pages) entry = -1;
+        }
+        a.table[i] = entry;
     }
     if (a.rows_out) {
         const long long end = (long long)a.rows * (a.row_bytes / 16);

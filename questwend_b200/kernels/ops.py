@@ -2258,7 +2258,8 @@ def kv4_read(pool: torch.Tensor, pages: torch.Tensor, page_start: torch.Tensor, 
     """What the 4-bit cache holds for a step's sequences, as plain pages: keys and values [P, Hkv, 64, hd] in ``dtype`` of the P
     entries of ``pages`` (``StepTables``), zeros behind a sequence's last token, and the page table [B, pages of ``max_len``] that names
     them (0 where a sequence has no page).  Both types hold the numbers exactly.  ``marked``: a token with a value that is not finite has
-    values of 0 and keys of NaN instead (what a kernel needs that multiplies unseen values by 0).  ``rest`` (rows [n, bytes a multiple of
+    values of 0 and keys of NaN instead (what a kernel needs that multiplies unseen values by 0), and the table has -1 where a sequence has no page or
+    the pool does not have it.  ``rest`` (rows [n, bytes a multiple of
     16], one int32 on the device): the rows from that number on are set to zero."""
     if not _ready(pool, torch.uint8, 3, pages, torch.int32, 1, page_start, torch.int32, 1, seq_len, torch.int32, 1):
         _need(pool, "pool", torch.uint8, 3)
@@ -2288,7 +2289,8 @@ def kv4_attention(q: torch.Tensor, pool: torch.Tensor, tables: StepTables, max_n
                   impl: str = "auto") -> torch.Tensor:
     """Causal attention of a step's tokens over the cache in 4 bits (their own rows written before).  ``q`` [T, Hq, hd] float32
     or bfloat16; ``max_new`` and ``max_len`` bound what a sequence brings and holds; with ``window`` > 0 a query sees the last ``window``
-    keys, its own among them.  A key behind what the page table's columns name is not seen (of a sequence that holds more than ``max_len``, whether
+    keys, its own among them.  A key behind what the page table's columns name, or of a page
+    that the pool does not have, is not seen (of a sequence that holds more than ``max_len``, whether
     keys behind that are is left open).  Returns [T, Hq * hd] in q's type, zeros for a token of no sequence.
 
     ``impl``: "rows" (bfloat16, heads of 64 or 128: codes to tensor-core fragments, a sequence's keys cut into runs; for few new tokens), "read"

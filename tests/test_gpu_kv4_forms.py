@@ -105,3 +105,31 @@ def test_counts_beyond_the_tokens_that_there_are(hd, lens):
             out, mass, big = pk.attention(f64(q[at:at + n]), *seqs[b], [pos0[b] + i for i in range(n)], hd ** -0.5)
             assert (np.abs(f64(got[at:at + n]).reshape(out.shape) - out) <= tolerance(BF, hd, mass, big, out, max(lens))).all(), (impl, b)
             at += n
+
+
+@pytest.mark.parametrize("hd,group", [(128, 4), (64, 2), (32, 2)])
+@pytest.mark.parametrize("lens,n_new,window", [([900, 200], [1, 1], 0), ([900, 200], [80, 40], 0), ([900, 200], [80, 40], 300), ([3000, 130], [20, 1], 0),
+                                               ([300, 64], [300, 10], 0)])
+def test_pages_that_the_pool_does_not_have_are_not_seen(hd, group, lens, n_new, window):
+    """In every form, whatever stands around them; a row that sees no other page is zero."""
+    pool, order, start, seqs, rng = _cache(27, lens, 2, hd)
+    gone = [{2, 3, 7} if lens[0] > 500 else {0, 2}, {0}]
+    for b in range(2):
+        for n, j in enumerate(sorted(gone[b])):
+            order[start[b] + j] = [pool.shape[0], -5, pool.shape[0] + 1000][n]
+    pos0 = [a - b for a, b in zip(lens, n_new)]
+    q = torch.from_numpy(rng.standard_normal((sum(n_new), 2 * group, hd))).to(BF).to(DEV)
+    t, qd = _tables(order, start, pos0, n_new), f64(q)
+    got = {f: f64(ops.kv4_attention(q, pool, t, max(n_new), max(lens), hd ** -0.5, window=window, impl=f)).reshape(qd.shape) for f in forms(q)}
+    at = 0
+    for b, n in enumerate(n_new):
+        for i in range(n):
+            pos = pos0[b] + i
+            seen = [j for j in range(max(0, pos - window + 1) if window else 0, pos + 1) if j // 64 not in gone[b]]
+            out, mass, big = pk.attention(qd[at:at + 1], *(x[seen] for x in seqs[b]), [len(seen) - 1], hd ** -0.5)
+            for f, y in got.items():
+                assert (np.abs(y[at] - out[0]) <= tolerance(BF, hd, mass, big, out, max(lens))[0]).all(), (f, b, i)
+            at += 1
+    k, v, table = ops.kv4_read(pool, t.pages, t.page_start, t.seq_len, max(lens), hd, F32, marked=True)
+    assert [(r < 0).nonzero().flatten().tolist() for r in table] == [sorted(gone[b] | set(range(-(-lens[b] // 64), table.shape[1]))) for b in range(2)]
+    assert all((x[start[b] + j] == 0).all() for x in (k, v) for b in range(2) for j in gone[b])
