@@ -13,7 +13,8 @@
 //     of a 32-bit word two at a time, in the places where their shifts leave them.
 //   * A code c becomes the bfloat16 128 + c by one and-or (its 7 bits behind the point hold c) and c s by one fused multiply-add.  The
 //     zero points are taken off as sums: of the scores by one more mma, whose inner dimension holds z s of a lane's group and the sum of the
-//     query's numbers there (in three bfloat16 parts), of the outputs by a row of z s in the mma that adds up the weights.
+//     query's numbers there (in three bfloat16 parts), of the outputs by a row of z s in the mma that adds up the weights.  (What the two sums have in
+//     common is lost from their difference: an output is off by up to 2^-23 of its group's 15 steps, also where it is much smaller itself.)
 //   * The scores' columns are the next product's inner dimension: P^T's operand is two 8 x 8 transpositions (movmatrix).
 //   * A run's softmax is relative to a reference that is raised, and O rescaled, only where a score passes it by 2^8: most pages vote once
 //     and exchange no maxima.  The weights' sum is one more mma with rows of ones, over
@@ -104,8 +105,8 @@ extern "C" int qwb_kv4_attn_plain(const void* q, const unsigned char* pool, cons
                                   void* out, int dtype, int T, int B, int pool_pages, int Hq, int Hkv, int hd, int table_width,
                                   float scale, int window, cudaStream_t stream) {
     if (T <= 0) return 0;
-    if (Hkv <= 0 || Hq <= 0 || Hq % Hkv || Hq > 65535 || hd <= 0 || hd % KV4_GROUP || hd > KV4_MAX_DIM || table_width <= 0 || window < 0)
-        return qwb_fail(QWB_ERR_ARG, "kv4_attention: bad sizes Hq=%d Hkv=%d hd=%d width=%d window=%d", Hq, Hkv, hd, table_width, window);
+    if (Hkv <= 0 || Hq <= 0 || Hq % Hkv || Hq > 65535 || hd <= 0 || hd % KV4_GROUP || hd > KV4_MAX_DIM || table_width <= 0 || window < 0 || !(scale > 0.f))
+        return qwb_fail(QWB_ERR_ARG, "kv4_attention: bad sizes Hq=%d Hkv=%d hd=%d width=%d window=%d scale=%g", Hq, Hkv, hd, table_width, window, (double)scale);
     if (dtype == QWB_DT_F32)
         qwb_launch(kv4_attn_plain_kernel<float>, dim3(T, Hq), KP_WARPS * 32, 0, stream, (const float*)q, pool, page_table, tok_seq, tok_pos, (float*)out,
                    B, pool_pages, Hq, Hkv, hd, table_width, scale, window);
@@ -206,7 +207,7 @@ template <int HD, int NT, bool CLUSTER, int ROOM>
 __global__ void __launch_bounds__(KD_WARPS * 32, ROOM)
 kv4_attn_rows_kernel(const bf16* __restrict__ q, const unsigned char* __restrict__ pool, const int* __restrict__ page_table,
                      const int* __restrict__ cu_seqlens, const int* __restrict__ pos0, bf16* __restrict__ out, float* __restrict__ part_o,
-                     float* __restrict__ part_ml, int T, int B, int pool_pages, int G, int Hkv, int table_width, float scale_log2, uint32_t flip, int window,
+                     float* __restrict__ part_ml, int T, int B, int pool_pages, int G, int Hkv, int table_width, float scale_log2, int window,
                      int tiles, int max_runs) {
     pdl_wait();
     pdl_launch_dependents();
@@ -287,10 +288,7 @@ kv4_attn_rows_kernel(const bf16* __restrict__ q, const unsigned char* __restrict
 #pragma unroll
         for (int w = 0; w < HD / 32; ++w) {
             uint4 v = make_uint4(0, 0, 0, 0);
-            if (live) {
-                v = *reinterpret_cast<const uint4*>(src + 8 * w);
-                v = make_uint4(v.x ^ flip, v.y ^ flip, v.z ^ flip, v.w ^ flip);         // the scale's sign
-            }
+            if (live) v = *reinterpret_cast<const uint4*>(src + 8 * w);
             qf[n][2 * w][0] = __byte_perm(v.x, v.z, 0x5410);            // numbers 0 and 4, 1 and 5, 2 and 6, 3 and 7 of 8
             qf[n][2 * w][1] = __byte_perm(v.x, v.z, 0x7632);
             qf[n][2 * w + 1][0] = __byte_perm(v.y, v.w, 0x5410);
@@ -685,8 +683,7 @@ static int kv4_launch_rows(const bf16* q, const unsigned char* pool, const int* 
     if (tiles * max_runs > 2147483647ll || tiles * 8 * NT >= 1 << 20 || Hkv > 65535 || B > 65535)
         return qwb_fail(QWB_ERR_ARG, "kv4_attention: %d sequences of up to %d new tokens, %d heads: too many blocks", B, max_new, Hkv);
     if (rows > 2147483647ll) return qwb_fail(QWB_ERR_ARG, "kv4_attention: %lld rows of queries", rows);
-    const float log2_scale = fabsf(scale) * 1.4426950408889634f;
-    const uint32_t flip = scale < 0.f ? 0x80008000u : 0u;
+    const float log2_scale = scale * 1.4426950408889634f;
     if (!scratch) {
         auto kernel = kv4_attn_rows_kernel<HD, NT, true, NT == 1 ? 7 : 4>;
         const int size = kv4_cluster_size(max_runs);
@@ -712,14 +709,14 @@ static int kv4_launch_rows(const bf16* q, const unsigned char* pool, const int* 
         cfg.attrs = attr;
         cfg.numAttrs = 1;
         const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, q, pool, page_table, cu, pos0, out, (float*)nullptr, (float*)nullptr, T, B, pool_pages, Hq / Hkv, Hkv,
-                                                 table_width, log2_scale, flip, window, (int)tiles, size);
+                                                 table_width, log2_scale, window, (int)tiles, size);
         if (e != cudaSuccess) return qwb_fail(QWB_ERR_CUDA, "kv4_attention: %s", cudaGetErrorString(e));
         return qwb_check_launch("kv4_attention");
     }
     float* part_ml = scratch + (size_t)rows * max_runs * HD;
     auto kernel = tiles * max_runs * Hkv * B <= 148 * 4 ? kv4_attn_rows_kernel<HD, NT, false, NT == 1 ? 7 : 4> : kv4_attn_rows_kernel<HD, NT, false, NT == 1 ? 7 : 5>;
     qwb_launch(kernel, dim3((unsigned)(tiles * max_runs), Hkv, B), KD_WARPS * 32, Smem::BYTES, stream, q, pool, page_table, cu, pos0, out,
-               scratch, part_ml, T, B, pool_pages, Hq / Hkv, Hkv, table_width, log2_scale, flip, window, (int)tiles, max_runs);
+               scratch, part_ml, T, B, pool_pages, Hq / Hkv, Hkv, table_width, log2_scale, window, (int)tiles, max_runs);
     qwb_launch_early(kv4_attn_join_kernel<HD>, dim3((unsigned)rows), KJ_WARPS * 32, 0, stream, scratch, part_ml, cu, pos0, tok_seq, out, T, B, Hq, table_width, window,
                      max_runs);
     return qwb_check_launch("kv4_attention");
@@ -730,8 +727,9 @@ extern "C" int qwb_kv4_attn_rows(const void* q, const unsigned char* pool, const
                                  void* out, float* scratch, int T, int B, int pool_pages, int max_new, int Hq, int Hkv, int hd, int table_width, float scale,
                                  int window, int max_runs, cudaStream_t stream) {
     if (T <= 0) return 0;
-    if (Hkv <= 0 || Hq <= 0 || Hq % Hkv || (hd != 64 && hd != 128) || table_width <= 0 || window < 0 || max_new <= 0 || max_runs <= 0 || B <= 0)
-        return qwb_fail(QWB_ERR_ARG, "kv4_attention: heads of 64 or 128 only: Hq=%d Hkv=%d hd=%d width=%d window=%d", Hq, Hkv, hd, table_width, window);
+    if (Hkv <= 0 || Hq <= 0 || Hq % Hkv || (hd != 64 && hd != 128) || table_width <= 0 || window < 0 || max_new <= 0 || max_runs <= 0 || B <= 0 || !(scale > 0.f))
+        return qwb_fail(QWB_ERR_ARG, "kv4_attention: heads of 64 or 128 only, a scale above 0: Hq=%d Hkv=%d hd=%d width=%d window=%d scale=%g", Hq, Hkv, hd, table_width, window,
+                        (double)scale);
     if (max_runs > KD_CLUSTER && !scratch) return qwb_fail(QWB_ERR_ARG, "kv4_attention: no scratch for %d runs", max_runs);
     if ((uintptr_t)q % 16 || (uintptr_t)pool % 16) return qwb_fail(QWB_ERR_ARG, "kv4_attention: q and the pool must start at a multiple of 16 bytes");
     const int columns = kv4_columns(max_new, Hq / Hkv);

@@ -542,9 +542,10 @@ extern "C" int qwb_attn_tc_prefill_pieces(const void* q, const void* k_pool, con
                                           const int* pos0, const int* tok_seq, void* out, float* scratch, int B, int T, int max_new, int n_pages, int Hq, int Hkv,
                                           int hd, int table_width, float scale, int window, int pieces, int piece_tiles, int* error, cudaStream_t stream) {
     if (B <= 0 || max_new <= 0 || T <= 0) return 0;
-    if ((hd != 64 && hd != 128) || Hq <= 0 || Hkv <= 0 || Hq % Hkv || Hq / Hkv > AT_ROWS / 2 || window < 0 || pieces < 1 || !error ||
+    if ((hd != 64 && hd != 128) || Hq <= 0 || Hkv <= 0 || Hq % Hkv || Hq / Hkv > AT_ROWS / 2 || window < 0 || pieces < 1 || !error || !(scale > 0.f) ||
         (pieces > 1 && (piece_tiles < 1 || !scratch || !tok_seq)))
-        return qwb_fail(QWB_ERR_ARG, "attn_tc_prefill_pieces: %d heads of 64 or 128 (not %d) over %d, %d pieces of %d tiles", Hq, hd, Hkv, pieces, piece_tiles);
+        return qwb_fail(QWB_ERR_ARG, "attn_tc_prefill_pieces: %d heads of 64 or 128 (not %d) over %d, %d pieces of %d tiles, a scale above 0 (not %g)", Hq, hd, Hkv,
+                        pieces, piece_tiles, (double)scale);
     const int G = Hq / Hkv;
     if ((long long)B * pieces > 65535 || (max_new + AT_ROWS / G - 1) / (AT_ROWS / G) > 65535 || (long long)T * Hq > 2147483647ll)
         return qwb_fail(QWB_ERR_ARG, "attn_tc_prefill_pieces: batch %d in %d pieces or %d new tokens of a sequence are more than the grid takes", B, pieces, max_new);

@@ -92,10 +92,19 @@ def shaped_attention_refusal(dim: int, vdim: int) -> str | None:
     return None
 
 KV4_GROUP = 32              # csrc/kv4.cuh: numbers of a row of the 4-bit cache that share a step
+KV4_SCALE = 2.0 ** -100, 2.0 ** 100     # of the scores of its attention: finite in 32 bits, and so is its inverse
 
 
 def kv4_refusal(head_dim: int) -> str | None:
     """None if keys and values of this size can be held in 4 bits, else why not."""
     if head_dim <= 0 or head_dim % KV4_GROUP or head_dim > MAX_HEAD_DIM:
         return f"a cache in 4 bits holds heads of a multiple of {KV4_GROUP} numbers up to {MAX_HEAD_DIM}, not {head_dim}"
+    return None
+
+
+def kv4_scale_refusal(scale: float) -> str | None:
+    """None if attention over a cache in 4 bits takes scores times this, else why not: a hidden key's score is minus infinity ahead of the scale,
+    so with one that is not above 0 it would not be the lowest."""
+    if not KV4_SCALE[0] <= scale <= KV4_SCALE[1]:
+        return f"attention over a cache in 4 bits takes a scale above 0 (2^-100 to 2^100), not {scale}"
     return None

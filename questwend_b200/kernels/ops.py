@@ -15,7 +15,7 @@ from typing import NamedTuple
 import torch
 
 from .build import host_calls, host_calls_built, load_module
-from .limits import KV4_GROUP, kv4_refusal
+from .limits import KV4_GROUP, kv4_refusal, kv4_scale_refusal
 
 DT_F32, DT_BF16 = 0, 1
 PAGE_SIZE = 64          # tokens per cache page
@@ -2289,7 +2289,7 @@ def kv4_attention(q: torch.Tensor, pool: torch.Tensor, tables: StepTables, max_n
                   impl: str = "auto") -> torch.Tensor:
     """Causal attention of a step's tokens over the cache in 4 bits (their own rows written before).  ``q`` [T, Hq, hd] float32
     or bfloat16; ``max_new`` and ``max_len`` bound what a sequence brings and holds; with ``window`` > 0 a query sees the last ``window``
-    keys, its own among them.  A key behind what the page table's columns name, or of a page
+    keys, its own among them; ``scale`` is above 0.  A key behind what the page table's columns name, or of a page
     that the pool does not have, is not seen (of a sequence that holds more than ``max_len``, whether
     keys behind that are is left open).  Returns [T, Hq * hd] in q's type, zeros for a token of no sequence.
 
@@ -2314,6 +2314,8 @@ def kv4_attention(q: torch.Tensor, pool: torch.Tensor, tables: StepTables, max_n
     if max_new < 1 or max_len < 1 or width < 1 or window < 0:
         raise KernelError(f"kv4_attention: up to {max_new} new tokens of sequences of up to {max_len}, window {window}, a page table of "
                           f"{width} columns")
+    if kv4_scale_refusal(scale):
+        raise KernelError(f"kv4_attention: {kv4_scale_refusal(scale)}")
     max_len = min(max_len, width * PAGE_SIZE)
     if impl not in ("auto", "plain", "rows", "read"):
         raise KernelError(f"kv4_attention: unknown form '{impl}'")

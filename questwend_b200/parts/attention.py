@@ -9,7 +9,7 @@ import math
 import torch
 
 from ..kernels import ops
-from ..kernels.limits import (conv_taps_refusal, head_dim_refusal, kv4_refusal, maps_attention_refusal, pool_attention_refusal,
+from ..kernels.limits import (conv_taps_refusal, head_dim_refusal, kv4_refusal, kv4_scale_refusal, maps_attention_refusal, pool_attention_refusal,
                               shaped_attention_refusal)
 from ..weights.manifest import MATRIX, NORM_WEIGHT, VECTOR, TensorSpec
 from .base import KVSpec, Mixer, StateSpec, take_weight
@@ -53,8 +53,9 @@ class GroupedQueryAttention(Mixer):
         if refusal:
             raise ValueError(f"grouped-query attention '{self.prefix}': parameter 'head_dim': {refusal}")
         self.cache_bits = getattr(runtime, "cache_bits", 0)
-        if self.cache_bits and kv4_refusal(self.head_dim):
-            raise ValueError(f"grouped-query attention '{self.prefix}': {kv4_refusal(self.head_dim)}")
+        refusal = self.cache_bits and (kv4_refusal(self.head_dim) or kv4_scale_refusal(self.scale))
+        if refusal:
+            raise ValueError(f"grouped-query attention '{self.prefix}': {refusal}")
         if self.rotary_dim > self.head_dim:
             raise ValueError(f"rotary size {self.rotary_dim} exceeds the head size {self.head_dim}")
         self.w_qkv = self.w_o = self.q_norm_w = self.k_norm_w = None

@@ -133,3 +133,38 @@ def test_pages_that_the_pool_does_not_have_are_not_seen(hd, group, lens, n_new, 
     k, v, table = ops.kv4_read(pool, t.pages, t.page_start, t.seq_len, max(lens), hd, F32, marked=True)
     assert [(r < 0).nonzero().flatten().tolist() for r in table] == [sorted(gone[b] | set(range(-(-lens[b] // 64), table.shape[1]))) for b in range(2)]
     assert all((x[start[b] + j] == 0).all() for x in (k, v) for b in range(2) for j in gone[b])
+
+
+@pytest.mark.parametrize("scale", [0.0, -0.125, float("nan"), float("inf"), 1e-40, 1e35])
+def test_a_scale_that_is_not_above_0_is_refused(scale):
+    """By every form: a hidden key's score would not be the lowest one, and the forms would not agree on what comes of it."""
+    pool, order, start, _, _ = _cache(28, [70], 1, 64)
+    t = _tables(order, start, [60], [10])
+    for dtype in (BF, F32):
+        q = torch.ones(10, 2, 64, dtype=dtype, device=DEV)
+        for impl in forms(q):
+            with pytest.raises(KernelError, match="scale above 0"):
+                ops.kv4_attention(q, pool, t, 10, 70, scale, impl=impl)
+
+
+@pytest.mark.parametrize("scale", [2.0 ** -60, 3.0])
+def test_small_and_large_scales(scale):
+    """With a large scale one key has nearly all the weight, and where its number is 0 the result is what the others' tiny weights leave.  As rows a number
+    c s - z s is formed from two sums over the keys, of p c s and of p z s (exact products): each is off by at most 2^-23 a key of
+    itself, and both are at most 15 s times the weights' sum, 1 behind the division.  So 2 x 15 s 2^-23 a key comes on top of ``tolerance``,
+    which counts errors of p (c s - z s) alone."""
+    lens, n_new, hd = [300, 100], [100, 7], 64
+    pool, order, start, seqs, rng = _cache(29, lens, 1, hd)
+    words = pk.unpack(pool.cpu().numpy(), hd)[3].astype(np.uint32)
+    step = float(((words[(words & 0x7F80) != 0x7F80] & 0xFFF0) << 16).view(np.float32).max())
+    pos0 = [a - b for a, b in zip(lens, n_new)]
+    q = torch.from_numpy(rng.standard_normal((sum(n_new), 2, hd))).to(BF).to(DEV)
+    t = _tables(order, start, pos0, n_new)
+    for window in (0, 50):
+        for impl in forms(q):
+            got, at = f64(ops.kv4_attention(q, pool, t, max(n_new), max(lens), scale, window=window, impl=impl)).reshape(-1, 2, hd), 0
+            for b, n in enumerate(n_new):
+                out, mass, big = pk.attention(f64(q[at:at + n]), *seqs[b], [pos0[b] + i for i in range(n)], scale, window)
+                more = 0.0 if impl in ("plain", "read") else 2 * 15 * step * lens[b] * 2.0 ** -23
+                assert (np.abs(got[at:at + n] - out) <= tolerance(BF, hd, mass, big, out, lens[b]) + more).all(), (impl, b, window)
+                at += n

@@ -77,3 +77,13 @@ def test_score_and_generate_refusals():
             score(engine, seqs, **kw)
     with pytest.raises(ValueError, match="logprobs"):
         generate(engine, [[1]], logprobs=65)
+
+
+@pytest.mark.parametrize("scale", [0.0, -1.0, float("inf")])
+def test_a_scale_that_the_attention_does_not_take_is_refused_before_a_weight_is_read(scale):
+    from questwend_b200.parts.attention import GroupedQueryAttention
+    from questwend_b200.parts.base import PartSpec
+    spec = PartSpec("gqa", {"hidden_size": 64, "n_heads": 2, "n_kv_heads": 1, "head_dim": 32, "scale": scale}, "layers.0.self_attn.")
+    with pytest.raises(ValueError, match="scale above 0"):
+        GroupedQueryAttention(spec, Runtime(torch.device("cpu"), torch.bfloat16, 4))
+    GroupedQueryAttention(spec, Runtime(torch.device("cpu"), torch.bfloat16))
