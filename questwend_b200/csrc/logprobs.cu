@@ -168,7 +168,7 @@ __device__ __forceinline__ void lp_finish(const float* x, int token, float m, fl
         int bi = -1;
         for (int i = tid; i < V; i += THREADS) {
             const float y = x[i];
-            const bool open = y == y && (last_i < 0 || lp_before(last, last_i, y, i));
+            const bool open = y == y && (k == 0 || lp_before(last, last_i, y, i));
             if (open && lp_before(y, i, bv, bi)) { bv = y; bi = i; }
         }
         lp_warp_best(bv, bi);
@@ -179,6 +179,10 @@ __device__ __forceinline__ void lp_finish(const float* x, int token, float m, fl
         bi = found_i[0];
         for (int w = 1; w < WARPS; ++w)
             if (lp_before(found_v[w], found_i[w], bv, bi)) { bv = found_v[w]; bi = found_i[w]; }
+        if (bi < 0) {                                               // no logit is left that is a number
+            for (int i = k + tid; i < top; i += THREADS) leave(i, -INFINITY, -1);
+            return;
+        }
         if (tid == 0) leave(k, bv, bi);
         last = bv;
         last_i = bi;
