@@ -660,8 +660,15 @@ static bool kv4_read_is_faster(int max_len, int max_new, int window, int table_w
     return 4.0 + at_pieces(tokens, B, max_new, max_len, Hq, Hkv, hd, window).us + (double)listed * Hkv * (hd == 128 ? 0.0065 : 0.0045) < rows;
 }
 
-// How a call goes: the most runs of a sequence, times 4, plus 2 if they are joined by scratch memory and a second kernel, plus 1 if reading
-// the pages first is faster.  Up to 16 runs go as clusters, up to 64 of these and while they are all on the chip at once (7 blocks an SM, 4 with
+// Whether a step is more than the rows kernel's grid, or its division by the group, takes: one whose longest prompt is of 2^20 / group tokens, for instance.
+static bool kv4_rows_refuse(int T, int B, int max_new, int Hq, int Hkv, long long max_runs) {
+    const int columns = kv4_columns(max_new, Hq / Hkv);
+    const long long tiles = ((long long)max_new * (Hq / Hkv) + columns - 1) / columns;
+    return tiles * columns >= 1 << 20 || tiles * max_runs > 2147483647ll || Hkv > 65535 || B > 65535 || (long long)T * Hq > 2147483647ll;
+}
+
+// How a call goes: the most runs of a sequence, times 8, plus 4 if it cannot go as rows, plus 2 if its runs are joined by scratch memory and a second
+// kernel, plus 1 if reading the pages first is faster.  Up to 16 runs go as clusters, up to 64 of these and while they are all on the chip at once (7 blocks an SM, 4 with
 // 16 columns): a second launch and a kernel's start less, 8.0 and 7.0 us for one sequence of 2,048 tokens, 15.0 and 13.6 for 16,384; 8 sequences
 // of 4,096, 1,024 blocks, are even.  Beyond that a cluster waits for 16 free places, and many small ones start slowly: 64 sequences of 1,000 take 66.8
 // us against 36.6, 4 of 8,192 with 6 new tokens 45.7 against 30.9, one prompt of 128, 256 clusters of 2, 26 against 16.
@@ -670,7 +677,7 @@ extern "C" int qwb_kv4_plan(int max_len, int max_new, int window, int table_widt
     const int columns = kv4_columns(max_new, Hq / Hkv);
     const long long tiles = ((long long)max_new * (Hq / Hkv) + columns - 1) / columns;
     const bool clusters = runs <= KD_CLUSTER && tiles * Hkv * B <= 64 && tiles * kv4_cluster_size(runs) * Hkv * B <= 148 * (columns == 8 ? 7 : 4);
-    return (int)(4 * runs) + (runs > 1 && !clusters ? 2 : 0) + (kv4_read_is_faster(max_len, max_new, window, table_width, B, Hq, Hkv, hd, tokens, listed) ? 1 : 0);
+    return (int)(8 * runs) + (kv4_rows_refuse(tokens, B, max_new, Hq, Hkv, runs) ? 4 : 0) + (runs > 1 && !clusters ? 2 : 0) + (kv4_read_is_faster(max_len, max_new, window, table_width, B, Hq, Hkv, hd, tokens, listed) ? 1 : 0);
 }
 
 template <int HD, int NT>
@@ -680,9 +687,8 @@ static int kv4_launch_rows(const bf16* q, const unsigned char* pool, const int* 
     using Smem = KdSmem<HD, NT>;
     static_assert(Smem::BYTES <= 48 * 1024, "more needs an attribute of the kernel");
     const long long tiles = ((long long)max_new * (Hq / Hkv) + 8 * NT - 1) / (8 * NT), rows = (long long)T * Hq;
-    if (tiles * max_runs > 2147483647ll || tiles * 8 * NT >= 1 << 20 || Hkv > 65535 || B > 65535)
-        return qwb_fail(QWB_ERR_ARG, "kv4_attention: %d sequences of up to %d new tokens, %d heads: too many blocks", B, max_new, Hkv);
-    if (rows > 2147483647ll) return qwb_fail(QWB_ERR_ARG, "kv4_attention: %lld rows of queries", rows);
+    if (kv4_rows_refuse(T, B, max_new, Hq, Hkv, max_runs))
+        return qwb_fail(QWB_ERR_ARG, "kv4_attention: %d sequences of up to %d new tokens, %d heads: too many blocks as rows", B, max_new, Hq);
     const float log2_scale = scale * 1.4426950408889634f;
     if (!scratch) {
         auto kernel = kv4_attn_rows_kernel<HD, NT, true, NT == 1 ? 7 : 4>;

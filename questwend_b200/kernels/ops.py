@@ -2295,7 +2295,7 @@ def kv4_attention(q: torch.Tensor, pool: torch.Tensor, tables: StepTables, max_n
 
     ``impl``: "rows" (bfloat16, heads of 64 or 128: codes to tensor-core fragments, a sequence's keys cut into runs; for few new tokens), "read"
     (the same sizes, groups of up to 64 heads, ``tables.pages`` given: the step's pages as bfloat16 once, then the tcgen05 prompt kernel), "plain"
-    (every size and type), or "auto": the fastest that takes the case."""
+    (every size and type), or "auto": the fastest that takes the case (rows take up to 2^20 / group new tokens of a sequence)."""
     table, tok_seq, tok_pos, cu, pos0 = tables.page_table, tables.tok_seq, tables.tok_pos, tables.cu_seqlens, tables.pos0
     whole = torch.int32
     if not _ready(q, None, 3, pool, torch.uint8, 3, table, whole, 2, tok_seq, whole, 1, tok_pos, whole, 1, cu, whole, 1, pos0, whole, 1):
@@ -2325,17 +2325,21 @@ def kv4_attention(q: torch.Tensor, pool: torch.Tensor, tables: StepTables, max_n
     reads = listed > 0
     if reads and (tables.seq_len is None or tables.seq_len.numel() != B or tables.page_start.numel() != B + 1):
         raise KernelError(f"kv4_attention: a list of pages goes with lengths and page starts of all {B} sequences")
+    if reads and max_new > 65535 * (128 // group):         # more blocks than the prompt kernel's grid takes
+        listed, reads = 0, False
     plan = 0
     if fits and impl != "plain":
         plan = _ask("attention_kv4", "qwb_kv4_plan", max_len, max_new, window, width, B, Hq, Hkv, hd, T, listed)
     if impl == "auto":
-        impl = "plain" if not fits else "read" if reads and plan & 1 else "rows"
+        impl = "plain" if not fits else "read" if reads and plan & 5 else "plain" if plan & 4 else "rows"
     if (impl == "rows" and not fits) or (impl == "read" and not reads):
         raise KernelError(f"kv4_attention: form '{impl}' does not take {q.dtype} queries of {hd}, groups of {group}"
-                          f"{'' if reads else ' (or has no list of pages)'}")
+                          f"{'' if reads else ' (or has no list of pages, or too many tokens of a sequence)'}")
+    if impl == "rows" and plan & 4:
+        raise KernelError(f"kv4_attention: {B} sequences of up to {max_new} new tokens, groups of {group} heads: too many blocks as rows")
     out = _empty((T, Hq * hd), dtype=dtype, device=q.device)
     if impl == "rows":
-        max_runs = plan >> 2
+        max_runs = plan >> 3
         scratch = _empty((T * Hq * max_runs * (hd + 2),), dtype=torch.float32, device=q.device) if plan & 2 else None
         _run("attention_kv4", "qwb_kv4_attn_rows", q, pool, table, cu, pos0, tok_seq, out, scratch, T, B, n_pages, max_new, Hq, Hkv, hd, width, float(scale), window,
              max_runs, _stream(), kernels=1 if scratch is None else 2)

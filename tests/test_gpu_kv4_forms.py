@@ -168,3 +168,41 @@ def test_small_and_large_scales(scale):
                 more = 0.0 if impl in ("plain", "read") else 2 * 15 * step * lens[b] * 2.0 ** -23
                 assert (np.abs(got[at:at + n] - out) <= tolerance(BF, hd, mass, big, out, lens[b]) + more).all(), (impl, b, window)
                 at += n
+
+
+def _sampled(q, got, seqs, pos0, n_new, hd, scale, at_most=12):
+    """Some of the tokens of every sequence, its first and last among them, against the 64-bit implementation."""
+    rng, t = np.random.default_rng(0), 0
+    for b, n in enumerate(n_new):
+        for i in sorted({0, n - 1, *rng.integers(0, n, at_most).tolist()}):
+            out, mass, big = pk.attention(f64(q[t + i:t + i + 1]), *seqs[b], [pos0[b] + i], scale)
+            lim = tolerance(q.dtype, hd, mass, big, out, pos0[b] + n)
+            assert (np.abs(f64(got[t + i]).reshape(out.shape) - out) <= lim).all(), (b, i)
+        t += n
+
+
+@pytest.mark.parametrize("Hq,Hkv,hd,lens,n_new,listed", [(128, 1, 64, [8192], [8192], True), (72, 1, 64, [70, 14600], [1, 14600], True),
+                                                         (128, 1, 128, [8200], [8195], False), (8, 1, 64, [500, 131073, 64], [1, 131073, 1], True)])
+def test_prompts_too_long_for_rows(Hq, Hkv, hd, lens, n_new, listed):
+    """What the rows form refuses goes another way, by itself: groups beyond 64 heads, tables without a list of pages, single tokens beside a long prompt."""
+    pool, order, start, seqs, rng = _cache(30, lens, Hkv, hd)
+    pos0 = [a - b for a, b in zip(lens, n_new)]
+    q = torch.randn(sum(n_new), Hq, hd, generator=torch.Generator().manual_seed(1)).to(BF).to(DEV)
+    t = _tables(order, start, pos0, n_new)
+    if not listed:
+        t = t._replace(pages=None, page_start=None)
+    with pytest.raises(KernelError, match="as rows"):
+        ops.kv4_attention(q, pool, t, max(n_new), max(lens), hd ** -0.5, impl="rows")
+    _sampled(q, ops.kv4_attention(q, pool, t, max(n_new), max(lens), hd ** -0.5), seqs, pos0, n_new, hd, hd ** -0.5)
+
+
+def test_more_tokens_of_a_sequence_than_the_prompt_kernels_grid_takes():
+    """As a bound that says so: read back it is refused, by itself it goes plainly."""
+    pool, order, start, seqs, rng = _cache(31, [100], 1, 64)
+    q = torch.from_numpy(rng.standard_normal((20, 64, 64))).to(BF).to(DEV)
+    t, most = _tables(order, start, [80], [20]), 65535 * 2 + 1
+    for impl, words in (("read", "too many tokens"), ("rows", "as rows")):
+        with pytest.raises(KernelError, match=words):
+            ops.kv4_attention(q, pool, t, most, 100, 0.125, impl=impl)
+    assert torch.equal(ops.kv4_attention(q, pool, t, most, 100, 0.125), ops.kv4_attention(q, pool, t, 20, 100, 0.125, impl="plain"))
+    _sampled(q, ops.kv4_attention(q, pool, t, most - 1, 100, 0.125, impl="read"), seqs, [80], [20], 64, 0.125)
