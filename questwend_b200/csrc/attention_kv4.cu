@@ -646,7 +646,9 @@ static int kv4_cluster_size(long long runs) {
 // reaches six times the rate, but the pages go through memory twice more; as rows every run of every 16 columns is a block, with a start and an
 // end that cost as much as 3.5 pages.  Both in microseconds, from measurements (32 query and 8 key heads of 128, as rows / read, with 8, 32 and 128
 // new tokens a sequence): one sequence of 1,000 tokens 11 / 19, 15 / 18, 38 / 18; of 8,192 16 / 34, 40 / 32, 121 / 44; of 60,000 68 / 119, 205 / 121, 769 / 186;
-// 8 of 8,192 66 / 91, 219 / 151, 743 / 212; a whole prompt of 128 15 / 9, of 900 262 / 24.
+// 8 of 8,192 66 / 91, 219 / 151, 743 / 212; a whole prompt of 128 15 / 9, of 900 262 / 24.  Steps of unequal sequences: a prompt of 4,096 beside 63 single
+// tokens behind 4,095 10,711 / 864, of 512 1,187 / 470, of 2,048 beside 31 behind 16,383 5,070 / 999, of 512 beside 7 behind 4,095 232 / 105, of 128 beside 15
+// 95 / 124.  (The rule is wrong for 300 new tokens beside 31 single ones, all behind 8,000: 608 / 497, goes as rows.)
 // tokens, listed: the step's tokens and its sequences' pages (which say more of unequal sequences than the most of each).
 static bool kv4_read_is_faster(int max_len, int max_new, int window, int table_width, int B, int Hq, int Hkv, int hd, int tokens, int listed) {
     const int G = Hq / Hkv;
@@ -677,7 +679,8 @@ extern "C" int qwb_kv4_plan(int max_len, int max_new, int window, int table_widt
     const int columns = kv4_columns(max_new, Hq / Hkv);
     const long long tiles = ((long long)max_new * (Hq / Hkv) + columns - 1) / columns;
     const bool clusters = runs <= KD_CLUSTER && tiles * Hkv * B <= 64 && tiles * kv4_cluster_size(runs) * Hkv * B <= 148 * (columns == 8 ? 7 : 4);
-    return (int)(8 * runs) + (kv4_rows_refuse(tokens, B, max_new, Hq, Hkv, runs) ? 4 : 0) + (runs > 1 && !clusters ? 2 : 0) + (kv4_read_is_faster(max_len, max_new, window, table_width, B, Hq, Hkv, hd, tokens, listed) ? 1 : 0);
+    const bool refused = kv4_rows_refuse(tokens, B, max_new, Hq, Hkv, runs), read = kv4_read_is_faster(max_len, max_new, window, table_width, B, Hq, Hkv, hd, tokens, listed);
+    return (int)(8 * runs) + (refused ? 4 : 0) + (runs > 1 && !clusters ? 2 : 0) + (read ? 1 : 0);
 }
 
 template <int HD, int NT>
