@@ -675,6 +675,7 @@ static bool kv4_rows_refuse(int T, int B, int max_new, int Hq, int Hkv, long lon
 // of 4,096, 1,024 blocks, are even.  Beyond that a cluster waits for 16 free places, and many small ones start slowly: 64 sequences of 1,000 take 66.8
 // us against 36.6, 4 of 8,192 with 6 new tokens 45.7 against 30.9, one prompt of 128, 256 clusters of 2, 26 against 16.
 extern "C" int qwb_kv4_plan(int max_len, int max_new, int window, int table_width, int B, int Hq, int Hkv, int hd, int tokens, int listed) {
+    if (B <= 0 || Hkv <= 0 || Hq < Hkv) return 8 + 4;                   // nothing that could go as rows
     const long long runs = kv4_max_runs(max_len, max_new, window, table_width);
     const int columns = kv4_columns(max_new, Hq / Hkv);
     const long long tiles = ((long long)max_new * (Hq / Hkv) + columns - 1) / columns;

@@ -2308,7 +2308,7 @@ def kv4_attention(q: torch.Tensor, pool: torch.Tensor, tables: StepTables, max_n
     T, Hq, hd = q.shape
     n_pages, Hkv = _kv4_pool("kv4_attention", pool, hd)
     B, (table_rows, width) = pos0.numel(), table.shape
-    if tok_seq.numel() != T or tok_pos.numel() != T or cu.numel() != B + 1 or table_rows < B or Hq % Hkv:
+    if tok_seq.numel() != T or tok_pos.numel() != T or cu.numel() != B + 1 or table_rows < B or B < 1 or Hkv < 1 or Hq < 1 or Hq % Hkv:
         raise KernelError(f"kv4_attention: tables of {tok_seq.numel()} tokens, {cu.numel() - 1} and {B} sequences for queries {tuple(q.shape)} over "
                           f"{Hkv} heads")
     if max_new < 1 or max_len < 1 or width < 1 or window < 0:

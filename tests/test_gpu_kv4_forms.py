@@ -206,3 +206,13 @@ def test_more_tokens_of_a_sequence_than_the_prompt_kernels_grid_takes():
             ops.kv4_attention(q, pool, t, most, 100, 0.125, impl=impl)
     assert torch.equal(ops.kv4_attention(q, pool, t, most, 100, 0.125), ops.kv4_attention(q, pool, t, 20, 100, 0.125, impl="plain"))
     _sampled(q, ops.kv4_attention(q, pool, t, most - 1, 100, 0.125, impl="read"), seqs, [80], [20], 64, 0.125)
+
+
+def test_steps_without_sequences_or_heads_are_refused():
+    pool, order, start, _, _ = _cache(32, [100], 2, 64)
+    t = _tables(order, start, [50], [50])
+    none = t._replace(pos0=ints([]), cu_seqlens=ints([0]), seq_len=ints([]), page_start=ints([0]))
+    for q, tables, its in ((torch.zeros(50, 4, 64), none, pool), (torch.zeros(50, 0, 64), t, pool), (torch.zeros(50, 4, 64), t, pool[:, :0].contiguous())):
+        for impl in ("auto", "plain", "rows", "read"):
+            with pytest.raises(KernelError, match="kv4_attention"):
+                ops.kv4_attention(q.to(BF).to(DEV), its, tables, 50, 100, 0.1, impl=impl)

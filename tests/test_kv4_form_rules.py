@@ -46,3 +46,8 @@ def test_pieces_of_unequal_steps():
                 for hd in (64, 128):
                     n, tiles = pieces(T, B, max_new, 100000, 1, 1, hd)
                     assert n >= 1 and n * B <= 65535 and n * tiles >= 100000 // 64 + 1
+
+
+@pytest.mark.parametrize("B,Hq,Hkv", [(0, 32, 8), (1, 0, 8), (1, 8, 0), (0, 0, 0), (1, 4, 8)])
+def test_a_step_without_sequences_or_heads_is_no_division_by_0(B, Hq, Hkv):
+    assert ops._ask("attention_kv4", "qwb_kv4_plan", 100, 50, 0, 2, B, Hq, Hkv, 64, 50, 3) & 7 == 4
