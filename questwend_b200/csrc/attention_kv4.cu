@@ -199,7 +199,7 @@ __device__ __forceinline__ void kd_cluster_sync() {
 }
 
 // NT: tiles of 8 columns of a block.  CLUSTER: the runs of a tile are the blocks of a cluster.  part: [rows, max_runs, HD] outputs, then [rows, max_runs, 2] maxima (of scores times log2 e) and sums
-// of the runs of sequences that have more than one; a row is (token, query head).
+// of the runs of sequences that have more than one; a row is (token, query head), of the key/value heads from kv0 on that the launch has blocks for.
 // ROOM: blocks an SM that registers leave room for.  With 8 columns 7, as many as shared memory does: 32 x 16,384 tokens 113 us, 116 with 8, 120 with 6.  With
 // 16 columns 5 (168 registers, some of them spilled), and 4 where no more are launched than so fit at once: 4 new tokens of one sequence of 8,192
 // 15.6 us instead of 17.7, of four sequences, 1,000 blocks, 33.4 instead of 30.1.
@@ -208,7 +208,7 @@ __global__ void __launch_bounds__(KD_WARPS * 32, ROOM)
 kv4_attn_rows_kernel(const bf16* __restrict__ q, const unsigned char* __restrict__ pool, const int* __restrict__ page_table,
                      const int* __restrict__ cu_seqlens, const int* __restrict__ pos0, bf16* __restrict__ out, float* __restrict__ part_o,
                      float* __restrict__ part_ml, int T, int B, int pool_pages, int G, int Hkv, int table_width, float scale_log2, int window,
-                     int tiles, int max_runs) {
+                     int tiles, int max_runs, int kv0) {
     pdl_wait();
     pdl_launch_dependents();
     using Tile = KdTile<HD>;
@@ -223,13 +223,13 @@ kv4_attn_rows_kernel(const bf16* __restrict__ q, const unsigned char* __restrict
         run = tiles == 1 ? blockIdx.x : blockIdx.x / tiles;
         tile = blockIdx.x - run * tiles;
     }
-    const int kvh = blockIdx.y, b = blockIdx.z;
+    const int kvh = kv0 + blockIdx.y, b = blockIdx.z;
     const int Hq = Hkv * G;
     const float one_in_g = 1.f / (float)G;
     auto by_g = [&](int x) { return (int)(((float)x + 0.5f) * one_in_g); };             // x / G: exact for x below 2^20 (the launcher's bound)
     const int t0 = cu_seqlens[b], t1 = cu_seqlens[b + 1], p0 = pos0[b], used = max(cu_seqlens[B], 0);
     if (used < T) {                                         // tokens behind the last sequence's: zeros
-        const long long me = (((long long)b * gridDim.y + kvh) * gridDim.x + blockIdx.x) * (KD_WARPS * 32) + threadIdx.x;
+        const long long me = (((long long)b * gridDim.y + blockIdx.y) * gridDim.x + blockIdx.x) * (KD_WARPS * 32) + threadIdx.x;
         const long long all = (long long)gridDim.x * gridDim.y * gridDim.z * (KD_WARPS * 32), end = (long long)T * Hq * (HD / 8);
         for (long long i = (long long)used * Hq * (HD / 8) + me; i < end; i += all) reinterpret_cast<uint4*>(out)[i] = make_uint4(0, 0, 0, 0);
     }
@@ -539,10 +539,11 @@ kv4_attn_rows_kernel(const bf16* __restrict__ q, const unsigned char* __restrict
                 out[row * HD + d] = from_f32<bf16>(total == 0.f ? 0.f : y[e] / total);
             }
         } else {
-            float* dst = CLUSTER ? done_o + col * Smem::COL + lane * E : part_o + (row * max_runs + run) * HD + lane * E;
+            const size_t part = ((size_t)(t0 + tok) * gridDim.y + blockIdx.y) * G + col0 + col - tok * G;         // the row among those of the heads of this launch
+            float* dst = CLUSTER ? done_o + col * Smem::COL + lane * E : part_o + (part * max_runs + run) * HD + lane * E;
             if constexpr (E == 4) *reinterpret_cast<float4*>(dst) = make_float4(y[0], y[1], y[2], y[3]);
             else *reinterpret_cast<float2*>(dst) = make_float2(y[0], y[1]);
-            if (lane == 0) *reinterpret_cast<float2*>(CLUSTER ? done_ml + 2 * col : part_ml + (row * max_runs + run) * 2) = make_float2(top, total);
+            if (lane == 0) *reinterpret_cast<float2*>(CLUSTER ? done_ml + 2 * col : part_ml + (part * max_runs + run) * 2) = make_float2(top, total);
         }
     }
     if (CLUSTER && max_runs > 1) {
@@ -581,10 +582,10 @@ kv4_attn_rows_kernel(const bf16* __restrict__ q, const unsigned char* __restrict
 template <int HD>
 __global__ void __launch_bounds__(KJ_WARPS * 32)
 kv4_attn_join_kernel(const float* part_o, const float* part_ml, const int* cu_seqlens, const int* pos0, const int* tok_seq, bf16* __restrict__ out, int T, int B,
-                     int Hq, int table_width, int window, int max_runs) {
+                     int Hq, int head0, int heads, int table_width, int window, int max_runs) {
     __shared__ float join_o[KJ_WARPS][HD], join_l[KJ_WARPS];
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, t = blockIdx.x / Hq;
-    const size_t row = blockIdx.x;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, t = blockIdx.x / heads;
+    const size_t row = blockIdx.x, to = (size_t)t * Hq + head0 + (blockIdx.x - t * heads);
     const int b = __ldcg(tok_seq + t);
     int runs = 0;
     if (b >= 0 && b < B) {
@@ -622,7 +623,7 @@ kv4_attn_join_kernel(const float* part_o, const float* part_ml, const int* cu_se
         const float l[4] = {join_l[0], join_l[1], join_l[2], join_l[3]}, o[4] = {join_o[0][at], join_o[1][at], join_o[2][at], join_o[3][at]};
         const float total = kd_four(l);
         const int mma = at / 16, half = (at >> 3) & 1, d = (at & 7) * (HD / 8) + 8 * (mma >> 2) + 4 * half + (mma & 3);
-        out[row * HD + d] = from_f32<bf16>(total == 0.f ? 0.f : kd_four(o) / total);
+        out[to * HD + d] = from_f32<bf16>(total == 0.f ? 0.f : kd_four(o) / total);
     }
 }
 
@@ -687,10 +688,10 @@ extern "C" int qwb_kv4_plan(int max_len, int max_new, int window, int table_widt
 template <int HD, int NT>
 static int kv4_launch_rows(const bf16* q, const unsigned char* pool, const int* page_table, const int* cu, const int* pos0, const int* tok_seq, bf16* out,
                            float* scratch, int T, int B, int pool_pages, int max_new, int Hq, int Hkv, int table_width, float scale, int window, int max_runs,
-                           cudaStream_t stream) {
+                           int heads, cudaStream_t stream) {
     using Smem = KdSmem<HD, NT>;
     static_assert(Smem::BYTES <= 48 * 1024, "more needs an attribute of the kernel");
-    const long long tiles = ((long long)max_new * (Hq / Hkv) + 8 * NT - 1) / (8 * NT), rows = (long long)T * Hq;
+    const long long tiles = ((long long)max_new * (Hq / Hkv) + 8 * NT - 1) / (8 * NT);
     if (kv4_rows_refuse(T, B, max_new, Hq, Hkv, max_runs))
         return qwb_fail(QWB_ERR_ARG, "kv4_attention: %d sequences of up to %d new tokens, %d heads: too many blocks as rows", B, max_new, Hq);
     const float log2_scale = scale * 1.4426950408889634f;
@@ -719,24 +720,30 @@ static int kv4_launch_rows(const bf16* q, const unsigned char* pool, const int* 
         cfg.attrs = attr;
         cfg.numAttrs = 1;
         const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, q, pool, page_table, cu, pos0, out, (float*)nullptr, (float*)nullptr, T, B, pool_pages, Hq / Hkv, Hkv,
-                                                 table_width, log2_scale, window, (int)tiles, size);
+                                                 table_width, log2_scale, window, (int)tiles, size, 0);
         if (e != cudaSuccess) return qwb_fail(QWB_ERR_CUDA, "kv4_attention: %s", cudaGetErrorString(e));
         return qwb_check_launch("kv4_attention");
     }
-    float* part_ml = scratch + (size_t)rows * max_runs * HD;
+    const int G = Hq / Hkv;
+    float* part_ml = scratch + (size_t)T * heads * G * max_runs * HD;
     auto kernel = tiles * max_runs * Hkv * B <= 148 * 4 ? kv4_attn_rows_kernel<HD, NT, false, NT == 1 ? 7 : 4> : kv4_attn_rows_kernel<HD, NT, false, NT == 1 ? 7 : 5>;
-    qwb_launch(kernel, dim3((unsigned)(tiles * max_runs), Hkv, B), KD_WARPS * 32, Smem::BYTES, stream, q, pool, page_table, cu, pos0, out,
-               scratch, part_ml, T, B, pool_pages, Hq / Hkv, Hkv, table_width, log2_scale, window, (int)tiles, max_runs);
-    qwb_launch_early(kv4_attn_join_kernel<HD>, dim3((unsigned)rows), KJ_WARPS * 32, 0, stream, scratch, part_ml, cu, pos0, tok_seq, out, T, B, Hq, table_width, window,
-                     max_runs);
+    for (int kv0 = 0; kv0 < Hkv; kv0 += heads) {            // `heads` key/value heads at a time share the scratch memory
+        const int n = heads < Hkv - kv0 ? heads : Hkv - kv0;
+        qwb_launch(kernel, dim3((unsigned)(tiles * max_runs), n, B), KD_WARPS * 32, Smem::BYTES, stream, q, pool, page_table, cu, pos0, out,
+                   scratch, part_ml, T, B, pool_pages, G, Hkv, table_width, log2_scale, window, (int)tiles, max_runs, kv0);
+        qwb_launch_early(kv4_attn_join_kernel<HD>, dim3((unsigned)((long long)T * n * G)), KJ_WARPS * 32, 0, stream, scratch, part_ml, cu, pos0, tok_seq, out, T, B, Hq,
+                         kv0 * G, n * G, table_width, window, max_runs);
+    }
     return qwb_check_launch("kv4_attention");
 }
 
-// max_runs, and whether there is scratch memory, T * Hq * max_runs * (hd + 2) floats: as qwb_kv4_plan says, or with scratch memory anyway
+// max_runs, and whether there is scratch memory: as qwb_kv4_plan says, or with scratch memory anyway.  With it `heads` key/value heads go at a time (others: all
+// of them), and it holds T * heads * (Hq / Hkv) * max_runs * (hd + 2) floats.
 extern "C" int qwb_kv4_attn_rows(const void* q, const unsigned char* pool, const int* page_table, const int* cu, const int* pos0, const int* tok_seq,
                                  void* out, float* scratch, int T, int B, int pool_pages, int max_new, int Hq, int Hkv, int hd, int table_width, float scale,
-                                 int window, int max_runs, cudaStream_t stream) {
+                                 int window, int max_runs, int heads, cudaStream_t stream) {
     if (T <= 0) return 0;
+    if (heads <= 0 || heads > Hkv) return qwb_fail(QWB_ERR_ARG, "kv4_attention: %d of %d key/value heads at a time", heads, Hkv);
     if (Hkv <= 0 || Hq <= 0 || Hq % Hkv || (hd != 64 && hd != 128) || table_width <= 0 || window < 0 || max_new <= 0 || max_runs <= 0 || B <= 0 || !(scale > 0.f))
         return qwb_fail(QWB_ERR_ARG, "kv4_attention: heads of 64 or 128 only, a scale above 0: Hq=%d Hkv=%d hd=%d width=%d window=%d scale=%g", Hq, Hkv, hd, table_width, window,
                         (double)scale);
@@ -744,7 +751,7 @@ extern "C" int qwb_kv4_attn_rows(const void* q, const unsigned char* pool, const
     if ((uintptr_t)q % 16 || (uintptr_t)pool % 16) return qwb_fail(QWB_ERR_ARG, "kv4_attention: q and the pool must start at a multiple of 16 bytes");
     const int columns = kv4_columns(max_new, Hq / Hkv);
 #define KV4_ROWS(HD, NT) kv4_launch_rows<HD, NT>((const bf16*)q, pool, page_table, cu, pos0, tok_seq, (bf16*)out, scratch, T, B, pool_pages, max_new, Hq, Hkv, \
-                                                 table_width, scale, window, max_runs, stream)
+                                                 table_width, scale, window, max_runs, heads, stream)
     if (hd == 128) return columns == 16 ? KV4_ROWS(128, 2) : KV4_ROWS(128, 1);
     return columns == 16 ? KV4_ROWS(64, 2) : KV4_ROWS(64, 1);
 #undef KV4_ROWS

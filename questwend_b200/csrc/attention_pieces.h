@@ -8,7 +8,7 @@
 
 struct AtPieces { int pieces, tiles; double us; };
 
-static inline AtPieces at_pieces(long long T, int B, int max_new, int max_len, int Hq, int Hkv, int hd, int window) {
+static inline AtPieces at_pieces(long long T, int B, int max_new, int max_len, int Hq, int Hkv, int hd, int window, int most = 64) {
     const int G = Hq / Hkv, tok = G <= 128 ? 128 / G : 1;
     // blocks with rows: of equal sequences B times the longest one's; of unequal ones (a prompt beside single tokens) no more than all tokens fill, and one each
     const double longest_each = (double)B * ((max_new + tok - 1) / tok), filled = (double)T / tok + B;
@@ -24,7 +24,7 @@ static inline AtPieces at_pieces(long long T, int B, int max_new, int max_len, i
     };
     AtPieces best = {1, (int)tiles, takes(blocks, (double)tiles)};
     if (blocks < 4 * 296) {
-        for (int s = 2; s <= 64 && s <= tiles && (long long)s * B <= 65535; ++s) {       // (the grid's bound)
+        for (int s = 2; s <= most && s <= tiles && (long long)s * B <= 65535; ++s) {       // (the grid's bound)
             const long long p = (tiles + s - 1) / s;
             const double us = takes(blocks * s, (double)p) + 4.0 + (double)T * Hq * s * hd * 8 / 5e6;
             if (us < 0.98 * best.us) best = {s, (int)p, us};

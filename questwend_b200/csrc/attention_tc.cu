@@ -50,7 +50,7 @@ struct AtSmem {
 // HD, VD: key and value sizes filled up to 64 or 128; vd: the value size itself.
 // SHAPED: the softmax also takes a distance bias per head and a sink (else the kernel is as it was).
 // PIECES: a block takes `piece_tiles` tiles of its rows' keys and leaves its sums, maximum (of scores times log2 e) and denominator to
-// attn_tc_join_kernel, in part_o [T * Hq, pieces, VD] and part_ml [T * Hq, pieces, 2] (with few rows and long contexts a block a row's tile
+// attn_tc_join_kernel, in part_o [T * Hkv * G, pieces, VD] and part_ml [T * Hkv * G, pieces, 2] (with few rows and long contexts a block a row's tile
 // would walk over all keys by itself while most SMs stand idle).
 // GAPS: the table may hold pages that are not there (below 0); their keys are not seen.
 template <int HD, int VD, bool SHAPED, bool GAPS = false, bool PIECES = false>
@@ -340,7 +340,7 @@ attn_tc_prefill_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
             // a sink: one more term of the denominator, exp(sink), relative to the row's reference
             if (SHAPED && sinks && row_ok) l += at_exp2(sinks[head] * 1.4426950408889634f - (m_ref == -INFINITY ? 0.f : m_ref * sl2));
             if constexpr (PIECES) {
-                const size_t at = ((size_t)(t0 + tok) * Hq + head) * pieces + piece;
+                const size_t at = ((size_t)(t0 + tok) * (Hkv * G) + head) * pieces + piece;
                 float* part = part_o + at * VD;
 #pragma unroll 1
                 for (int c = 0; c < VD; c += 32) {
@@ -387,17 +387,17 @@ attn_tc_prefill_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
 template <int VD>
 __global__ void __launch_bounds__(256)
 attn_tc_join_kernel(const float* __restrict__ part_o, const float* __restrict__ part_ml, const int* __restrict__ tok_seq, const int* __restrict__ cu_seqlens,
-                    const int* __restrict__ pos0, bf16* __restrict__ out, int rows, int B, int Hq, int tok_per_block, int window, int table_width, int pieces,
-                    int piece_tiles) {
+                    const int* __restrict__ pos0, bf16* __restrict__ out, int rows, int B, int Hq, int heads, int tok_per_block, int window, int table_width,
+                    int pieces, int piece_tiles) {
     pdl_wait();
     pdl_launch_dependents();
     const int lane = threadIdx.x & 31;
     const long long row = (long long)blockIdx.x * 8 + (threadIdx.x >> 5);
     if (row >= rows) return;
-    const int t = (int)(row / Hq), b = tok_seq[t];
+    const int t = (int)(row / heads), b = tok_seq[t];
     if (b < 0 || b >= B) return;
     // the tiles that the row's block went over, as it found them
-    const int t0 = cu_seqlens[b], n_new = min(cu_seqlens[b + 1], rows / Hq) - t0, q0 = (t - t0) / tok_per_block * tok_per_block, p0 = pos0[b];
+    const int t0 = cu_seqlens[b], n_new = min(cu_seqlens[b + 1], rows / heads) - t0, q0 = (t - t0) / tok_per_block * tok_per_block, p0 = pos0[b];
     const int first = (window > 0 ? max(0, p0 + q0 - window + 1) : 0) / AT_KEYS, last = min((p0 + min(n_new, q0 + tok_per_block) - 1) / AT_KEYS, table_width - 1);
     const int count = last < first ? 0 : min((last - first) / piece_tiles + 1, pieces);
     const float* ml = part_ml + row * pieces * 2;
@@ -424,8 +424,9 @@ attn_tc_join_kernel(const float* __restrict__ part_o, const float* __restrict__ 
     __nv_bfloat162 p[E / 2];
 #pragma unroll
     for (int e = 0; e < E / 2; ++e) p[e] = __floats2bfloat162_rn(y[2 * e] * inv, y[2 * e + 1] * inv);
-    if constexpr (E == 4) *reinterpret_cast<uint2*>(out + row * VD + lane * E) = *reinterpret_cast<uint2*>(p);
-    else *reinterpret_cast<__nv_bfloat162*>(out + row * VD + lane * E) = p[0];
+    bf16* dst = out + ((long long)t * Hq + (row - (long long)t * heads)) * VD + lane * E;
+    if constexpr (E == 4) *reinterpret_cast<uint2*>(dst) = *reinterpret_cast<uint2*>(p);
+    else *reinterpret_cast<__nv_bfloat162*>(dst) = p[0];
 }
 
 // ------------------------------------------------------------------------------------------- host side
@@ -433,13 +434,13 @@ template <int HD, int VD>
 static int launch_attn_tc(const void* q, const void* k_pool, const void* v_pool, const int* page_table, const int* cu_seqlens,
                           const int* pos0, void* out, int B, int T, int max_new, int n_pages, int Hq, int Hkv, int hd, int vd, int table_width,
                           float scale, int window, int chunk, int* error, const float* slopes, const float* sinks, cudaStream_t stream,
-                          int pieces = 1, int piece_tiles = 0, float* scratch = nullptr, const int* tok_seq = nullptr, bool early = false) {
+                          int pieces = 1, int piece_tiles = 0, float* scratch = nullptr, const int* tok_seq = nullptr, bool early = false, int G = 0) {
     AtEncodeFn enc = at_encode();
     if (!enc) return qwb_fail(QWB_ERR_CUDA, "attn_tc_prefill: cuTensorMapEncodeTiled is not available from this driver");
-    const int G = Hq / Hkv;
+    if (!G) G = Hq / Hkv;                                   // else Hkv * G of q's Hq heads, from the pointers on
     CUtensorMap map_q, map_k, map_v;
     {   // q [T, Hq, hd]: boxes of [128 / G tokens][G heads][64 d]
-        cuuint64_t dims[3] = {(cuuint64_t)hd, (cuuint64_t)Hq, (cuuint64_t)T};
+        cuuint64_t dims[3] = {(cuuint64_t)hd, (cuuint64_t)Hkv * G, (cuuint64_t)T};
         cuuint64_t strides[2] = {(cuuint64_t)hd * 2, (cuuint64_t)Hq * hd * 2};
         cuuint32_t box[3] = {64, (cuuint32_t)G, (cuuint32_t)(AT_ROWS / G)};
         cuuint32_t elem[3] = {1, 1, 1};
@@ -464,7 +465,8 @@ static int launch_attn_tc(const void* q, const void* k_pool, const void* v_pool,
     const size_t smem = AtSmem<HD, VD>::BYTES;
     const int tok_per_block = AT_ROWS / G;
     dim3 grid(Hkv, (max_new + tok_per_block - 1) / tok_per_block, B * pieces);
-    float* part_ml = scratch ? scratch + (size_t)T * Hq * pieces * VD : nullptr;
+    const long long rows = (long long)T * Hkv * G;
+    float* part_ml = scratch ? scratch + (size_t)rows * pieces * VD : nullptr;
     auto go = [&](auto kernel) -> int {
         cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
         if (e != cudaSuccess) return qwb_fail(QWB_ERR_CUDA, "attn_tc_prefill: %s", cudaGetErrorString(e));
@@ -476,8 +478,8 @@ static int launch_attn_tc(const void* q, const void* k_pool, const void* v_pool,
     if (pieces > 1) {
         if constexpr (HD == VD) {
             if (int rc = go(attn_tc_prefill_kernel<HD, VD, false, true, true>)) return rc;
-            qwb_launch(attn_tc_join_kernel<VD>, dim3((unsigned)(((long long)T * Hq + 7) / 8)), 256, 0, stream, scratch, part_ml, tok_seq, cu_seqlens, pos0, (bf16*)out,
-                       T * Hq, B, Hq, tok_per_block, window, table_width, pieces, piece_tiles);
+            qwb_launch(attn_tc_join_kernel<VD>, dim3((unsigned)((rows + 7) / 8)), 256, 0, stream, scratch, part_ml, tok_seq, cu_seqlens, pos0, (bf16*)out,
+                       (int)rows, B, Hq, Hkv * G, tok_per_block, window, table_width, pieces, piece_tiles);
             return qwb_check_launch("attn_tc_prefill_pieces");
         }
     }
@@ -526,10 +528,10 @@ extern "C" int qwb_attn_tc_prefill(const void* q, const void* k_pool, const void
 #undef QWB_AT_LAUNCH
 }
 
-// The pieces that a step's keys are best cut into, and the tiles of 64 keys of each: 2^32 tiles + pieces.  32 query and 8 key heads of 128, over pages
+// The pieces that a step's keys are best cut into, up to `most`, and the tiles of 64 keys of each: 2^32 tiles + pieces.  32 query and 8 key heads of 128, over pages
 // read from a cache in 4 bits, that included: 64 new tokens of a sequence of 60,000 999 us whole, 143 in 17 pieces; of 8,192 143 and 40.
-extern "C" long long qwb_attn_tc_pieces(int T, int B, int max_new, int max_len, int Hq, int Hkv, int hd, int window) {
-    const AtPieces p = at_pieces(T, B, max_new, max_len, Hq, Hkv, hd, window);
+extern "C" long long qwb_attn_tc_pieces(int T, int B, int max_new, int max_len, int Hq, int Hkv, int hd, int window, int most) {
+    const AtPieces p = at_pieces(T, B, max_new, max_len, Hq, Hkv, hd, window, most);
     return ((long long)p.tiles << 32) + p.pieces;
 }
 
@@ -537,22 +539,22 @@ extern "C" long long qwb_attn_tc_pieces(int T, int B, int max_new, int max_len, 
 // whose tail it is launched: what it reads before that kernel has ended, or through the read-only path (cu_seqlens, pos0), has to be older than it; pages
 // and their table (a page below 0: its keys are not seen) are what that kernel writes, and are read behind the wait and at L2.  A prompt of 128 tokens 9.0 -> 7.8 us with
 // it, three of 900 behind 5,000 95 -> 90.  The keys are cut into `pieces` of `piece_tiles` tiles of 64; with more than one tok_seq [T] says each token's
-// sequence, or -1, and scratch holds T * Hq * pieces * (hd + 2) floats.
+// sequence, or -1, and scratch holds T * Hkv * G * pieces * (hd + 2) floats.  q and out have Hq heads a token, of which the call takes Hkv * G from the
+// pointers on; the pages hold their Hkv.
 extern "C" int qwb_attn_tc_prefill_pieces(const void* q, const void* k_pool, const void* v_pool, const int* page_table, const int* cu_seqlens,
                                           const int* pos0, const int* tok_seq, void* out, float* scratch, int B, int T, int max_new, int n_pages, int Hq, int Hkv,
-                                          int hd, int table_width, float scale, int window, int pieces, int piece_tiles, int* error, cudaStream_t stream) {
+                                          int G, int hd, int table_width, float scale, int window, int pieces, int piece_tiles, int* error, cudaStream_t stream) {
     if (B <= 0 || max_new <= 0 || T <= 0) return 0;
-    if ((hd != 64 && hd != 128) || Hq <= 0 || Hkv <= 0 || Hq % Hkv || Hq / Hkv > AT_ROWS / 2 || window < 0 || pieces < 1 || !error || !(scale > 0.f) ||
+    if ((hd != 64 && hd != 128) || Hq <= 0 || Hkv <= 0 || G <= 0 || (long long)Hkv * G > Hq || G > AT_ROWS / 2 || window < 0 || pieces < 1 || !error || !(scale > 0.f) ||
         (pieces > 1 && (piece_tiles < 1 || !scratch || !tok_seq)))
-        return qwb_fail(QWB_ERR_ARG, "attn_tc_prefill_pieces: %d heads of 64 or 128 (not %d) over %d, %d pieces of %d tiles, a scale above 0 (not %g)", Hq, hd, Hkv,
+        return qwb_fail(QWB_ERR_ARG, "attn_tc_prefill_pieces: %d heads of 64 or 128 (not %d), %d groups of them, %d pieces of %d tiles, a scale above 0 (not %g)", Hq, hd, Hkv,
                         pieces, piece_tiles, (double)scale);
-    const int G = Hq / Hkv;
     if ((long long)B * pieces > 65535 || (max_new + AT_ROWS / G - 1) / (AT_ROWS / G) > 65535 || (long long)T * Hq > 2147483647ll)
         return qwb_fail(QWB_ERR_ARG, "attn_tc_prefill_pieces: batch %d in %d pieces or %d new tokens of a sequence are more than the grid takes", B, pieces, max_new);
     if ((uintptr_t)q % 16 || (uintptr_t)k_pool % 16 || (uintptr_t)v_pool % 16 || (uintptr_t)out % 16 || (uintptr_t)scratch % 16)
         return qwb_fail(QWB_ERR_ARG, "attn_tc_prefill_pieces: operands must be 16-byte aligned");
     return hd == 64 ? launch_attn_tc<64, 64>(q, k_pool, v_pool, page_table, cu_seqlens, pos0, out, B, T, max_new, n_pages, Hq, Hkv, hd, hd, table_width, scale, window, 0,
-                                             error, nullptr, nullptr, stream, pieces, piece_tiles, scratch, tok_seq, true)
+                                             error, nullptr, nullptr, stream, pieces, piece_tiles, scratch, tok_seq, true, G)
                     : launch_attn_tc<128, 128>(q, k_pool, v_pool, page_table, cu_seqlens, pos0, out, B, T, max_new, n_pages, Hq, Hkv, hd, hd, table_width, scale, window, 0,
-                                               error, nullptr, nullptr, stream, pieces, piece_tiles, scratch, tok_seq, true);
+                                               error, nullptr, nullptr, stream, pieces, piece_tiles, scratch, tok_seq, true, G);
 }

@@ -391,7 +391,7 @@ extern "C" int qwb_kv4_store(const float* qkv, const float* q_weight, const floa
     return qwb_check_launch("kv4_store");
 }
 
-// Pages of a step's sequences, one after the other, as plain pages [P, Hkv, 64, hd] of keys and of values; rows behind a
+// Pages of a step's sequences, one after the other, as plain pages [P, heads, 64, hd] of keys and of values (of the pool's heads from head0 on); rows behind a
 // sequence's last token are zeros.  A block takes a (page, head), a thread 8 numbers at a time (one 32-bit word of codes).
 // `marked`: a token one of whose values is not finite has values of zero and keys of NaN here, so that a kernel that multiplies
 // what a query does not see by 0 gives NaN to the queries that see it only.
@@ -403,12 +403,12 @@ struct Kv4ReadArgs {
     const int *pages, *page_start, *seq_len, *rows_used;
     int* table;
     uint4* rows_out;
-    int B, width, pool_pages, Hkv, hd, marked, rows, row_bytes;
+    int B, width, pool_pages, Hkv, head0, hd, marked, rows, row_bytes;
 };
 // The table and the rows; then what this block's page holds: its bytes of this head, and how many rows of it live.
 __device__ __forceinline__ const unsigned char* kv4_read_begin(const Kv4ReadArgs& a, int hd, int& live) {
-    const int entry = blockIdx.x, head = blockIdx.y;
-    const long long me = ((long long)head * gridDim.x + entry) * blockDim.x + threadIdx.x, all = (long long)gridDim.x * gridDim.y * blockDim.x;
+    const int entry = blockIdx.x, head = a.head0 + blockIdx.y;
+    const long long me = ((long long)blockIdx.y * gridDim.x + entry) * blockDim.x + threadIdx.x, all = (long long)gridDim.x * gridDim.y * blockDim.x;
     for (long long i = me; i < (long long)a.B * a.width; i += all) {
         const int b = (int)(i / a.width), j = (int)(i - (long long)b * a.width), at = a.page_start[b] + j;
         const bool listed = at >= 0 && at < a.page_start[b + 1] && at < (int)gridDim.x;
@@ -444,7 +444,7 @@ kv4_read_kernel(const Kv4ReadArgs a, T* __restrict__ k_out, T* __restrict__ v_ou
     int live;
     const int hd = a.hd, words = hd / 8, groups = hd / KV4_GROUP;
     const unsigned char* base = kv4_read_begin(a, hd, live);
-    const size_t out0 = ((size_t)blockIdx.x * a.Hkv + blockIdx.y) * KV4_PAGE * hd;
+    const size_t out0 = ((size_t)blockIdx.x * gridDim.y + blockIdx.y) * KV4_PAGE * hd;
     const uint16_t* v_words = reinterpret_cast<const uint16_t*>(base + kv4_half_bytes(hd) + kv4_code_bytes(hd));
     for (int i = threadIdx.x; i < 2 * KV4_PAGE * words; i += 256) {
         const bool is_v = i >= KV4_PAGE * words;
@@ -470,8 +470,9 @@ kv4_read_kernel(const Kv4ReadArgs a, T* __restrict__ k_out, T* __restrict__ v_ou
 // bfloat16, heads of 64 and 128: a thread takes the same 8 numbers of every 16th (32nd) row, all its loads on their way before the first
 // is used, and two codes at a time, all of it exact: c s - z s.  What bounds it: 32 KB written a page and head of 128 for 9 KB read; 7,500 of them
 // 54 us, 5.8 TB/s (one word and its address at a time 82).
+// Registers for 8 blocks an SM with heads of 64: with the 39 that it takes by itself three chunks of 900 over it 93.8 us instead of 91.5.
 template <int HD>
-__global__ void __launch_bounds__(256)
+__global__ void __launch_bounds__(256, HD == 64 ? 8 : 4)
 kv4_read_fast_kernel(const Kv4ReadArgs a, bf16* __restrict__ k_out, bf16* __restrict__ v_out) {
     pdl_wait();
     pdl_launch_dependents();
@@ -495,7 +496,7 @@ kv4_read_fast_kernel(const Kv4ReadArgs a, bf16* __restrict__ k_out, bf16* __rest
                 else words[p][i].x = reinterpret_cast<const uint32_t*>(base + p * HALF + CODES)[row];
             }
         }
-    const size_t out0 = ((size_t)blockIdx.x * a.Hkv + blockIdx.y) * KV4_PAGE * HD;
+    const size_t out0 = ((size_t)blockIdx.x * gridDim.y + blockIdx.y) * KV4_PAGE * HD;
 #pragma unroll
     for (int i = 0; i < PASSES; ++i) {
         const uint2 v = words[1][i];
@@ -520,17 +521,17 @@ kv4_read_fast_kernel(const Kv4ReadArgs a, bf16* __restrict__ k_out, bf16* __rest
 }
 
 extern "C" int qwb_kv4_read(const unsigned char* pool, const int* pages, const int* page_start, const int* seq_len, void* k_out,
-                            void* v_out, int dtype, int* table, int P, int B, int width, int pool_pages, int Hkv, int hd,
-                            int marked, void* rows_out, const int* rows_used, int rows, int row_bytes, cudaStream_t stream) {
+                            void* v_out, int dtype, int* table, int P, int B, int width, int pool_pages, int Hkv, int head0,
+                            int heads, int hd, int marked, void* rows_out, const int* rows_used, int rows, int row_bytes, cudaStream_t stream) {
     if (P <= 0) return 0;
-    if (B <= 0 || width <= 0 || Hkv <= 0 || Hkv > 65535 || hd <= 0 || hd % KV4_GROUP || hd > KV4_MAX_DIM || pool_pages <= 0)
-        return qwb_fail(QWB_ERR_ARG, "kv4_read: bad sizes B=%d width=%d Hkv=%d hd=%d pages=%d", B, width, Hkv, hd, pool_pages);
+    if (B <= 0 || width <= 0 || Hkv <= 0 || Hkv > 65535 || head0 < 0 || heads <= 0 || heads > Hkv - head0 || hd <= 0 || hd % KV4_GROUP || hd > KV4_MAX_DIM || pool_pages <= 0)
+        return qwb_fail(QWB_ERR_ARG, "kv4_read: bad sizes B=%d width=%d Hkv=%d (%d from %d on) hd=%d pages=%d", B, width, Hkv, heads, head0, hd, pool_pages);
     if ((uintptr_t)pool % 16 || (uintptr_t)k_out % 16 || (uintptr_t)v_out % 16)
         return qwb_fail(QWB_ERR_ARG, "kv4_read: pool and outputs must start at a multiple of 16 bytes");
     if (rows_out && ((uintptr_t)rows_out % 16 || row_bytes % 16 || !rows_used))
         return qwb_fail(QWB_ERR_ARG, "kv4_read: rows of %d bytes", row_bytes);
-    const Kv4ReadArgs args = {pool, pages, page_start, seq_len, rows_used, table, (uint4*)rows_out, B, width, pool_pages, Hkv, hd, marked, rows, row_bytes};
-    const dim3 grid(P, Hkv);
+    const Kv4ReadArgs args = {pool, pages, page_start, seq_len, rows_used, table, (uint4*)rows_out, B, width, pool_pages, Hkv, head0, hd, marked, rows, row_bytes};
+    const dim3 grid(P, heads);
     // early: its blocks wait at their beginning, its launch does not; one token's write and read 4.7 -> 4.1 us
     if (dtype == QWB_DT_F32) qwb_launch_early(kv4_read_kernel<float>, grid, 256, 0, stream, args, (float*)k_out, (float*)v_out);
     else if (dtype != QWB_DT_BF16) return qwb_fail(QWB_ERR_ARG, "kv4_read: unknown dtype %d", dtype);

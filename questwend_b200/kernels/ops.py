@@ -15,7 +15,7 @@ from typing import NamedTuple
 import torch
 
 from .build import host_calls, host_calls_built, load_module
-from .limits import KV4_GROUP, kv4_refusal, kv4_scale_refusal
+from .limits import KV4_GROUP, KV4_SCALE, kv4_refusal, kv4_scale_refusal
 
 DT_F32, DT_BF16 = 0, 1
 PAGE_SIZE = 64          # tokens per cache page
@@ -2254,13 +2254,13 @@ def kv4_store(qkv: torch.Tensor, q_weight, k_weight, cos, sin, slot_map: torch.T
 
 
 def kv4_read(pool: torch.Tensor, pages: torch.Tensor, page_start: torch.Tensor, seq_len: torch.Tensor, max_len: int, head_dim: int,
-             dtype: torch.dtype, marked: bool = False, rest: tuple | None = None) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+             dtype: torch.dtype, marked: bool = False, rest: tuple | None = None, heads: tuple[int, int] | None = None) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
     """What the 4-bit cache holds for a step's sequences, as plain pages: keys and values [P, Hkv, 64, hd] in ``dtype`` of the P
     entries of ``pages`` (``StepTables``), zeros behind a sequence's last token, and the page table [B, pages of ``max_len``] that names
     them (0 where a sequence has no page).  Both types hold the numbers exactly.  ``marked``: a token with a value that is not finite has
     values of 0 and keys of NaN instead (what a kernel needs that multiplies unseen values by 0), and the table has -1 where a sequence has no page or
     the pool does not have it.  ``rest`` (rows [n, bytes a multiple of
-    16], one int32 on the device): the rows from that number on are set to zero."""
+    16], one int32 on the device): the rows from that number on are set to zero.  ``heads`` (first, count): of these key/value heads only."""
     if not _ready(pool, torch.uint8, 3, pages, torch.int32, 1, page_start, torch.int32, 1, seq_len, torch.int32, 1):
         _need(pool, "pool", torch.uint8, 3)
         for name, t in (("pages", pages), ("page_start", page_start), ("seq_len", seq_len)):
@@ -2275,14 +2275,30 @@ def kv4_read(pool: torch.Tensor, pages: torch.Tensor, page_start: torch.Tensor, 
         _need(rows, "rest", ndim=2)
         _need(used, "rest", torch.int32)
         _here("kv4_read", rows, used)
+    first, count = (0, Hkv) if heads is None else heads
+    if first < 0 or count < 1 or first + count > Hkv:
+        raise KernelError(f"kv4_read: {count} heads from {first} on of {Hkv}")
     width = -(-max_len // PAGE_SIZE)
-    shape = (P, Hkv, PAGE_SIZE, head_dim)
+    shape = (P, count, PAGE_SIZE, head_dim)
     k, v, table = _pieces(pool, dtype, shape, dtype, shape, torch.int32, (B, width))
     if not P:
         table.zero_()
-    _run("kv4_cache", "qwb_kv4_read", pool, pages, page_start, seq_len, k, v, _dt(dtype), table, P, B, width, n_pages, Hkv, head_dim, 1 if marked else 0, rows,
+    _run("kv4_cache", "qwb_kv4_read", pool, pages, page_start, seq_len, k, v, _dt(dtype), table, P, B, width, n_pages, Hkv, first, count, head_dim, 1 if marked else 0, rows,
          used, 0 if rows is None else rows.shape[0], 0 if rows is None else rows.shape[1] * rows.element_size(), _stream())
     return k, v, table
+
+
+# The most memory, in bytes, that a call of kv4_attention takes beside its output: it goes over the key/value heads a few at a time where all of them at once
+# would take more (one head at the least).  262,144 tokens with heads of 128 read back are 134 MB a head.
+KV4_WORK_BYTES = 1 << 29
+
+
+def _heads_at_once(heads: int, each: int) -> int:
+    """How many heads go at a time that take so many bytes each."""
+    if heads * each <= KV4_WORK_BYTES:
+        return heads
+    times = -(-heads // max(1, KV4_WORK_BYTES // each))
+    return -(-heads // times)
 
 
 def kv4_attention(q: torch.Tensor, pool: torch.Tensor, tables: StepTables, max_new: int, max_len: int, scale: float, window: int = 0,
@@ -2295,7 +2311,12 @@ def kv4_attention(q: torch.Tensor, pool: torch.Tensor, tables: StepTables, max_n
 
     ``impl``: "rows" (bfloat16, heads of 64 or 128: codes to tensor-core fragments, a sequence's keys cut into runs; for few new tokens), "read"
     (the same sizes, groups of up to 64 heads, ``tables.pages`` given: the step's pages as bfloat16 once, then the tcgen05 prompt kernel), "plain"
-    (every size and type), or "auto": the fastest that takes the case (rows take up to 2^20 / group new tokens of a sequence)."""
+    (every size and type), or "auto": the fastest that takes the case (rows take up to 2^20 / group new tokens of a sequence) and as rows with all of a
+    head's runs within ``KV4_WORK_BYTES``.
+
+    Memory beside the output: as rows T * Hq * runs * (hd + 2) * 4 bytes where a sequence's runs (of up to 8 pages) are joined by a second kernel; read back
+    256 * hd bytes for each listed page and head, and up to as much again as ``KV4_WORK_BYTES`` for pieces; the heads go a few at a time where this would be more
+    than ``KV4_WORK_BYTES``.  Plainly none."""
     table, tok_seq, tok_pos, cu, pos0 = tables.page_table, tables.tok_seq, tables.tok_pos, tables.cu_seqlens, tables.pos0
     whole = torch.int32
     if not _ready(q, None, 3, pool, torch.uint8, 3, table, whole, 2, tok_seq, whole, 1, tok_pos, whole, 1, cu, whole, 1, pos0, whole, 1):
@@ -2314,7 +2335,7 @@ def kv4_attention(q: torch.Tensor, pool: torch.Tensor, tables: StepTables, max_n
     if max_new < 1 or max_len < 1 or width < 1 or window < 0:
         raise KernelError(f"kv4_attention: up to {max_new} new tokens of sequences of up to {max_len}, window {window}, a page table of "
                           f"{width} columns")
-    if kv4_scale_refusal(scale):
+    if not KV4_SCALE[0] <= scale <= KV4_SCALE[1]:
         raise KernelError(f"kv4_attention: {kv4_scale_refusal(scale)}")
     max_len = min(max_len, width * PAGE_SIZE)
     if impl not in ("auto", "plain", "rows", "read"):
@@ -2323,7 +2344,7 @@ def kv4_attention(q: torch.Tensor, pool: torch.Tensor, tables: StepTables, max_n
     fits = dtype == torch.bfloat16 and hd in (64, 128)
     listed = tables.pages.numel() if fits and group <= 64 and tables.pages is not None and tables.page_start is not None else 0
     reads = listed > 0
-    if reads and (tables.seq_len is None or tables.seq_len.numel() != B or tables.page_start.numel() != B + 1):
+    if listed and (tables.seq_len is None or tables.seq_len.numel() != B or tables.page_start.numel() != B + 1):
         raise KernelError(f"kv4_attention: a list of pages goes with lengths and page starts of all {B} sequences")
     if reads and max_new > 65535 * (128 // group):         # more blocks than the prompt kernel's grid takes
         listed, reads = 0, False
@@ -2331,7 +2352,8 @@ def kv4_attention(q: torch.Tensor, pool: torch.Tensor, tables: StepTables, max_n
     if fits and impl != "plain":
         plan = _ask("attention_kv4", "qwb_kv4_plan", max_len, max_new, window, width, B, Hq, Hkv, hd, T, listed)
     if impl == "auto":
-        impl = "plain" if not fits else "read" if reads and plan & 5 else "plain" if plan & 4 else "rows"
+        rows_too_large = plan & 4 or (plan & 2 and T * group * (plan >> 3) * (hd + 2) * 4 > KV4_WORK_BYTES)
+        impl = "plain" if not fits else "read" if reads and (plan & 1 or rows_too_large) else "plain" if rows_too_large else "rows"
     if (impl == "rows" and not fits) or (impl == "read" and not reads):
         raise KernelError(f"kv4_attention: form '{impl}' does not take {q.dtype} queries of {hd}, groups of {group}"
                           f"{'' if reads else ' (or has no list of pages, or too many tokens of a sequence)'}")
@@ -2340,18 +2362,31 @@ def kv4_attention(q: torch.Tensor, pool: torch.Tensor, tables: StepTables, max_n
     out = _empty((T, Hq * hd), dtype=dtype, device=q.device)
     if impl == "rows":
         max_runs = plan >> 3
-        scratch = _empty((T * Hq * max_runs * (hd + 2),), dtype=torch.float32, device=q.device) if plan & 2 else None
+        scratch, heads, times = None, Hkv, 1
+        if plan & 2:
+            each = T * group * max_runs * (hd + 2)
+            heads = _heads_at_once(Hkv, 4 * each)
+            scratch, times = _empty((heads * each,), dtype=torch.float32, device=q.device), 2 * -(-Hkv // heads)
         _run("attention_kv4", "qwb_kv4_attn_rows", q, pool, table, cu, pos0, tok_seq, out, scratch, T, B, n_pages, max_new, Hq, Hkv, hd, width, float(scale), window,
-             max_runs, _stream(), kernels=1 if scratch is None else 2)
+             max_runs, heads, _stream(), kernels=times)
         return out
     if impl == "read":
-        k, v, compact = kv4_read(pool, tables.pages, tables.page_start, tables.seq_len, max_len, hd, q.dtype, marked=True, rest=(out, cu[B:]))
         cut = _lookup("attention_tc", "qwb_attn_tc_pieces")[1]
         cut.restype = ctypes.c_longlong
-        tiles, pieces = divmod(cut(T, B, operator.index(max_new), operator.index(max_len), Hq, Hkv, hd, operator.index(window)), 2 ** 32)
-        scratch = _empty((T * Hq * pieces * (hd + 2),), dtype=torch.float32, device=q.device) if pieces > 1 else None
-        _run("attention_tc", "qwb_attn_tc_prefill_pieces", q, k, v, compact, cu, pos0, tok_seq, out, scratch, B, T, max_new, k.shape[0], Hq, Hkv, hd,
-             compact.shape[1], float(scale), window, pieces, tiles, gemm_tc_error_word(q.device), _stream(), kernels=1 if scratch is None else 2)
+        heads = _heads_at_once(Hkv, listed * PAGE_SIZE * hd * 4)
+        for first in range(0, Hkv, heads):
+            n = min(heads, Hkv - first)
+            its_q, its_out = (q, out) if n == Hkv else (q[:, first * group:], out[:, first * group * hd:])
+            k, v, compact = kv4_read(pool, tables.pages, tables.page_start, tables.seq_len, max_len, hd, dtype, marked=True,
+                                     rest=None if first else (out, cu[B:]), heads=(first, n))
+            each = T * n * group * (hd + 2)                # of a piece
+            tiles, pieces = divmod(cut(T, B, operator.index(max_new), operator.index(max_len), n * group, n, hd, operator.index(window),
+                                       max(1, min(64, KV4_WORK_BYTES // max(1, 4 * each)))), 2 ** 32)
+            scratch = _empty((each * pieces,), dtype=torch.float32, device=q.device) if pieces > 1 else None
+            _run("attention_tc", "qwb_attn_tc_prefill_pieces", its_q, k, v, compact, cu, pos0, tok_seq, its_out, scratch, B, T, max_new, listed, Hq, n, group, hd,
+                 compact.shape[1], float(scale), window, pieces, tiles, gemm_tc_error_word(q.device), _stream(), kernels=1 if scratch is None else 2)
+            if n < Hkv:
+                del k, v, compact, scratch                 # the next heads' take their place
         return out
     _run("attention_kv4", "qwb_kv4_attn_plain", q, pool, table, tok_seq, tok_pos, out, _dt(dtype), T, B, n_pages, Hq, Hkv, hd, width, float(scale), window, _stream())
     return out

@@ -216,3 +216,56 @@ def test_steps_without_sequences_or_heads_are_refused():
         for impl in ("auto", "plain", "rows", "read"):
             with pytest.raises(KernelError, match="kv4_attention"):
                 ops.kv4_attention(q.to(BF).to(DEV), its, tables, 50, 100, 0.1, impl=impl)
+
+
+def _peak(call):
+    """The result and the bytes that the call took beside it."""
+    torch.cuda.synchronize()
+    torch.cuda.reset_peak_memory_stats()
+    before = torch.cuda.memory_allocated()
+    out = call()
+    torch.cuda.synchronize()
+    return out, torch.cuda.max_memory_allocated() - before - out.numel() * out.element_size()
+
+
+@pytest.mark.parametrize("Hq,Hkv,hd", [(16, 8, 128), (15, 5, 64), (6, 3, 128)])
+@pytest.mark.parametrize("lens,n_new", [([2500, 300], [1, 1]), ([2500, 300, 1500], [5, 40, 1]), ([700, 500], [400, 60])])
+def test_heads_a_few_at_a_time(Hq, Hkv, hd, lens, n_new, monkeypatch):
+    """Where all heads at once would take more memory than a call may: the same results, as rows bit for bit, in that much less memory."""
+    pool, order, start, seqs, rng = _cache(33, lens, Hkv, hd)
+    pos0, behind = [a - b for a, b in zip(lens, n_new)], 3
+    q = torch.from_numpy(rng.standard_normal((sum(n_new) + behind, Hq, hd))).to(BF).to(DEV)
+    wide = _tables(order, start, pos0, n_new, behind=behind, width=200)           # a table of 200 pages: runs joined by scratch memory
+    t = _tables(order, start, pos0, n_new, behind=behind)
+    run = lambda impl, t, most: _peak(lambda: ops.kv4_attention(q, pool, t, max(n_new), most, hd ** -0.5, impl=impl))
+    rows, rows_bytes = run("rows", wide, 200 * 64)
+    read, read_bytes = run("read", t, max(lens))
+    each_rows, each_read = q.shape[0] * (Hq // Hkv) * 25 * (hd + 2) * 4, start[-1] * 64 * hd * 4
+    assert rows_bytes >= Hkv * each_rows and read_bytes >= Hkv * each_read
+    for heads in {1, 2, 3} - {Hkv}:
+        monkeypatch.setattr(ops, "KV4_WORK_BYTES", heads * each_rows)
+        before = ops.LAUNCHES[0]
+        got, took = run("rows", wide, 200 * 64)
+        assert torch.equal(got, rows) and took <= heads * each_rows + 1024 and ops.LAUNCHES[0] - before == 2 * -(-Hkv // ops._heads_at_once(Hkv, each_rows))
+        monkeypatch.setattr(ops, "KV4_WORK_BYTES", heads * each_read)
+        got, took = run("read", t, max(lens))
+        assert (got.float() - read.float()).abs().max() <= 2.0 ** -7 * read.float().abs().max() and took <= 2 * heads * each_read + 4096
+        _check(pool, t, seqs, q, pos0, n_new, max(lens), hd ** -0.5, 0)
+    monkeypatch.setattr(ops, "KV4_WORK_BYTES", 1)                                   # a head's runs are too much: not as rows by itself
+    _check(pool, wide, seqs, q, pos0, n_new, 200 * 64, hd ** -0.5, 0)
+    got, took = run("auto", wide._replace(pages=None, page_start=None), 200 * 64)
+    assert torch.equal(got, ops.kv4_attention(q, pool, wide, max(n_new), 200 * 64, hd ** -0.5, impl="plain")) and took <= 1024
+
+
+def test_pages_of_some_heads():
+    pool, order, start, _, _ = _cache(34, [200, 70], 5, 64)
+    args = (pool, ints(order), ints(start), ints([200, 70]), 200, 64, BF)
+    k, v, table = ops.kv4_read(*args)
+    for first, n in ((0, 5), (0, 2), (2, 3), (4, 1)):
+        its = ops.kv4_read(*args, heads=(first, n))
+        assert torch.equal(its[0], k[:, first:first + n]) and torch.equal(its[1], v[:, first:first + n]) and torch.equal(its[2], table)
+    plain = ops.kv4_read(*args[:-1], F32, heads=(3, 2))
+    assert torch.equal(plain[0], k[:, 3:].float()) and torch.equal(plain[1], v[:, 3:].float())
+    for heads in ((-1, 2), (0, 0), (4, 2), (5, 1)):
+        with pytest.raises(KernelError, match="heads from"):
+            ops.kv4_read(*args, heads=heads)

@@ -29,10 +29,10 @@ def test_a_step_goes_by_the_tokens_that_it_has(held, new, read):
     assert bool(plan(held, new) & 1) is read
 
 
-def pieces(T, B, max_new, max_len, Hq, Hkv, hd, window=0):
+def pieces(T, B, max_new, max_len, Hq, Hkv, hd, window=0, most=64):
     ask = ops._lookup("attention_tc", "qwb_attn_tc_pieces")[1]
     ask.restype = ctypes.c_longlong
-    tiles, n = divmod(ask(T, B, max_new, max_len, Hq, Hkv, hd, window), 2 ** 32)
+    tiles, n = divmod(ask(T, B, max_new, max_len, Hq, Hkv, hd, window, most), 2 ** 32)
     return n, tiles
 
 
@@ -51,3 +51,10 @@ def test_pieces_of_unequal_steps():
 @pytest.mark.parametrize("B,Hq,Hkv", [(0, 32, 8), (1, 0, 8), (1, 8, 0), (0, 0, 0), (1, 4, 8)])
 def test_a_step_without_sequences_or_heads_is_no_division_by_0(B, Hq, Hkv):
     assert ops._ask("attention_kv4", "qwb_kv4_plan", 100, 50, 0, 2, B, Hq, Hkv, 64, 50, 3) & 7 == 4
+
+
+def test_heads_go_a_few_at_a_time_where_memory_is_bounded(monkeypatch):
+    monkeypatch.setattr(ops, "KV4_WORK_BYTES", 1000)
+    assert [ops._heads_at_once(8, each) for each in (1, 125, 126, 250, 251, 333, 334, 500, 501, 1000, 1001, 10 ** 12)] == [8, 8, 4, 4, 3, 3, 2, 2, 1, 1, 1, 1]
+    assert ops._heads_at_once(1, 10 ** 12) == 1 and ops._heads_at_once(7, 0) == 7
+    assert pieces(64, 1, 64, 60000, 32, 8, 128, most=4)[0] <= 4 and pieces(64, 1, 64, 60000, 32, 8, 128, most=1)[0] == 1

@@ -52,4 +52,4 @@ def test_a_block_of_the_prompt_kernel_that_has_nothing_to_do_waits_all_the_same(
 def test_the_prompt_kernel_writes_no_row_behind_the_tokens_that_there_are():
     for name in ("attn_tc_prefill_kernel", "attn_tc_join_kernel"):
         _, body = kernel("attention_tc.cu", name)
-        assert re.search(r"n_new = min\(cu_seqlens\[b \+ 1\], (T|rows / Hq)\) - t0", body), name
+        assert re.search(r"n_new = min\(cu_seqlens\[b \+ 1\], (T|rows / heads)\) - t0", body), name
