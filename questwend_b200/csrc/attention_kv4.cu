@@ -82,9 +82,14 @@ kv4_attn_plain_kernel(const T* __restrict__ q, const unsigned char* __restrict__
             m = m_new;
         }
     }
+    bool broken = false;                    // a value that is not finite makes all of the head NaN
 #pragma unroll
     for (int g = 0; g < KV4_MAX_DIM / 32; ++g)
-        if (g < groups) part[warp][g * 32 + lane] = acc[g];
+        if (g < groups) {
+            part[warp][g * 32 + lane] = acc[g];
+            broken |= acc[g] != acc[g];
+        }
+    if (__any_sync(0xffffffffu, broken)) l = __uint_as_float(0x7fffffffu);
     if (lane == 0) { part[warp][KV4_MAX_DIM] = m; part[warp][KV4_MAX_DIM + 1] = l; }
     __syncthreads();
     float top = -INFINITY, total = 0.f, f[KP_WARPS];
@@ -530,6 +535,11 @@ kv4_attn_rows_kernel(const bf16* __restrict__ q, const unsigned char* __restrict
                 for (int e = 0; e < E; ++e) y[e] += f * src[e];
             }
         }
+        // a value that is not finite makes all of the head NaN, wherever in its page it lies (masked tiles have it so by the score)
+        bool broken = false;
+#pragma unroll
+        for (int e = 0; e < E; ++e) broken |= y[e] != y[e];
+        if (__any_sync(0xffffffffu, broken)) total = __uint_as_float(0x7fffffffu);
         const int tok = by_g(col0 + col);
         const size_t row = (size_t)(t0 + tok) * Hq + kvh * G + col0 + col - tok * G;
         if (CLUSTER ? max_runs == 1 : runs <= 1) {

@@ -8,8 +8,8 @@
 // makes it 2 % larger or smaller on average, and the codes' own rounding, half a step at most, with it; the largest numbers may then lie up to
 // 15/16 of a step beyond the last code instead of half a step.)
 // A group of zeros, or whose step would lie under 2^-126, has step 0 and stands for zeros.  A group that holds a number that
-// is not finite, or whose step would be 2^120 or more (so that 128 s is a number), stands for NaN: what sees the token is NaN and nothing
-// is lost silently.
+// is not finite, or whose step would be 2^120 or more (so that 128 s is a number), stands for NaN: whoever sees the token gets NaN for all numbers
+// of the head, in every form of the attention, and nothing is lost silently.
 //
 // A page of 64 tokens and one head: 64 rows of key codes (hd / 2 bytes, the lower half of a byte first), 64 rows of the
 // keys' words (hd / 32 of 16 bits: the bits of s as a bfloat16, whose lowest 4 are zero, with z in them), then the values' codes

@@ -2306,8 +2306,8 @@ def kv4_attention(q: torch.Tensor, pool: torch.Tensor, tables: StepTables, max_n
     """Causal attention of a step's tokens over the cache in 4 bits (their own rows written before).  ``q`` [T, Hq, hd] float32
     or bfloat16; ``max_new`` and ``max_len`` bound what a sequence brings and holds; with ``window`` > 0 a query sees the last ``window``
     keys, its own among them; ``scale`` is above 0.  A key behind what the page table's columns name, or of a page
-    that the pool does not have, is not seen (of a sequence that holds more than ``max_len``, whether
-    keys behind that are is left open).  Returns [T, Hq * hd] in q's type, zeros for a token of no sequence.
+    that the pool does not have, is not seen (of a sequence that holds more than ``max_len``, whether keys behind that are is left open).  A key or value
+    with a number that is not finite makes all numbers of its head NaN for the queries that see it.  Returns [T, Hq * hd] in q's type, zeros for a token of no sequence.
 
     ``impl``: "rows" (bfloat16, heads of 64 or 128: codes to tensor-core fragments, a sequence's keys cut into runs; for few new tokens), "read"
     (the same sizes, groups of up to 64 heads, ``tables.pages`` given: the step's pages as bfloat16 once, then the tcgen05 prompt kernel), "plain"

@@ -269,3 +269,25 @@ def test_pages_of_some_heads():
     for heads in ((-1, 2), (0, 0), (4, 2), (5, 1)):
         with pytest.raises(KernelError, match="heads from"):
             ops.kv4_read(*args, heads=heads)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF])
+@pytest.mark.parametrize("hd,L,n_new", [(128, 200, 4), (128, 200, 90), (64, 1100, 1), (64, 1100, 30), (96, 200, 5)])
+@pytest.mark.parametrize("window", [0, 70])
+def test_what_is_not_finite_makes_all_of_its_head_nan_wherever_it_lies(dtype, hd, L, n_new, window):
+    """A key's or a value's group, in pages that are seen wholly, in the last one and at a window's edge: the same in every form."""
+    pool, order, start, seqs, rng = _cache(35, [L], 2, hd)
+    t = _tables(order, start, [L - n_new], [n_new])
+    q = torch.from_numpy(rng.standard_normal((n_new, 4, hd))).to(dtype).to(DEV)
+    clean = {f: ops.kv4_attention(q, pool, t, n_new, L, 0.1, window=window, impl=f).view(n_new, 4, hd) for f in forms(q)}
+    for at in (3, 64, L - n_new - 60, L - n_new, L - 2):
+        for part in (0, 1):
+            group = at % (hd // 32)
+            broken = pool.clone()
+            word = part * 64 * (hd // 2 + hd // 16) + 64 * hd // 2 + (at % 64) * (hd // 16) + 2 * group
+            broken[order[at // 64], 1, word:word + 2] = torch.tensor([0xC0, 0x7F], dtype=torch.uint8, device=DEV)
+            sees = torch.tensor([at <= p and (not window or at > p - window) for p in range(L - n_new, L)], device=DEV)
+            for f in forms(q):
+                got = ops.kv4_attention(q, broken, t, n_new, L, 0.1, window=window, impl=f).view(n_new, 4, hd)
+                assert torch.equal(got[:, :2], clean[f][:, :2]) and torch.equal(got[~sees], clean[f][~sees]), (f, at, part)
+                assert got[sees][:, 2:].isnan().all(), (f, at, part)
