@@ -205,7 +205,7 @@ __device__ __forceinline__ void kd_cluster_sync() {
 
 // NT: tiles of 8 columns of a block.  CLUSTER: the runs of a tile are the blocks of a cluster.  part: [rows, max_runs, HD] outputs, then [rows, max_runs, 2] maxima (of scores times log2 e) and sums
 // of the runs of sequences that have more than one; a row is (token, query head), of the key/value heads from kv0 on that the launch has blocks for.
-// ROOM: blocks an SM that registers leave room for.  With 8 columns 7, as many as shared memory does: 32 x 16,384 tokens 113 us, 116 with 8, 120 with 6.  With
+// ROOM: blocks an SM that registers leave room for.  With 8 columns 7, as many as shared memory does: 32 x 16,384 tokens 114 us, 116 with 8, 120 with 6.  With
 // 16 columns 5 (168 registers, some of them spilled), and 4 where no more are launched than so fit at once: 4 new tokens of one sequence of 8,192
 // 15.6 us instead of 17.7, of four sequences, 1,000 blocks, 33.4 instead of 30.1.
 template <int HD, int NT, bool CLUSTER, int ROOM>
@@ -252,7 +252,7 @@ kv4_attn_rows_kernel(const bf16* __restrict__ q, const unsigned char* __restrict
 
     unsigned char* ring = smem + (size_t)warp * KD_STAGES * Tile::BYTES;
     int slot_in = 0, slot_out = 0;
-    auto ask = [&](int i) {                                 // the warp's 16 keys of the run's i-th page
+    auto ask = [&](int i) {                                 // the warp's 32 keys of the run's i-th page
         const int page = __shfl_sync(0xffffffffu, my_page, i & 31);
         if (i < n_pages && page >= 0) {
             unsigned char* dst = ring + slot_in * Tile::BYTES;

@@ -206,7 +206,7 @@ attn_tc_prefill_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
             if (ok && n_tiles > 1) ok = issue_s(1);
             for (int j = 0; j < n_tiles && ok; ++j) {
                 const int s = j % AT_KV_STAGES;
-                ok = at_wait(&v_full[s], (j / AT_KV_STAGES) & 1) && at_wait(p_full, j & 1);   // V has landed; P is in shared memory
+                ok = at_wait(&v_full[s], (j / AT_KV_STAGES) & 1) && at_wait(p_full, j & 1);   // V has landed; P is in tensor memory
                 if (!ok) break;
                 at_fence_after();
                 const unsigned char* vt = v_tiles + (size_t)s * V_BYTES;
