@@ -219,13 +219,14 @@ def test_steps_without_sequences_or_heads_are_refused():
 
 
 def _peak(call):
-    """The result and the bytes that the call took beside it."""
+    """The result and the bytes that the call asked for beside it at most.  (Asked for: a cached block that is given may be up to 1 MB larger.)"""
     torch.cuda.synchronize()
     torch.cuda.reset_peak_memory_stats()
-    before = torch.cuda.memory_allocated()
+    asked = lambda which: torch.cuda.memory_stats()[f"requested_bytes.all.{which}"]
+    before = asked("current")
     out = call()
     torch.cuda.synchronize()
-    return out, torch.cuda.max_memory_allocated() - before - out.numel() * out.element_size()
+    return out, asked("peak") - before - out.numel() * out.element_size()
 
 
 @pytest.mark.parametrize("Hq,Hkv,hd", [(16, 8, 128), (15, 5, 64), (6, 3, 128)])
